@@ -44,6 +44,137 @@ int gpu_deltanet_step_gated(gpu_context *ctx, gpu_buffer *state, const gpu_buffe
 int gpu_kv_cache_append(gpu_context *ctx, gpu_buffer *K_cache, gpu_buffer *V_cache,
                         const gpu_buffer *K_new, const gpu_buffer *V_new, int pos, int head_dim);
 
+/* ---------------------------------------------------------------------------
+ * The attention side of a decode step over a paged key-value cache: rotary
+ * positions of several axes, the append, the attention of one new token per
+ * sequence, and the eviction that bounds the cache.  The reference keeps one
+ * contiguous fp32 cache of 256 positions (inference.c:15) and attends one head
+ * at a time; these calls take a batch of sequences, query heads that share kv
+ * heads, and narrower cache types.
+ *
+ * Activations are fp32, lengths, positions, slots and page numbers int32, all
+ * in buffers of the context.  Calls return 0 or a negative status, run on the
+ * context's stream and are synchronous unless ORN_KV_ASYNC is given.
+ *
+ * Numbers in device buffers are checked by the kernels: a page number outside
+ * [0, n_pages), a slot past the pages or a length outside its bounds is left
+ * out (its keys take no part, its token or row is not stored; a length is
+ * clamped), nothing outside the buffers is touched, and the call returns
+ * ORN_EINVAL.  After ORN_KV_ASYNC calls the next synchronous one of this group,
+ * or gpu_kv_check, reports it.
+ * ------------------------------------------------------------------------- */
+#define ORN_KV_ASYNC 1u
+
+enum {
+    ORN_KV_F32 = 0,
+    ORN_KV_F16 = 1,
+    ORN_KV_BF16 = 2,
+    ORN_KV_E4M3 = 3 /* 8 bits, largest value 448, no infinities */
+};
+
+/* One layer's cache: two buffers [n_pages][n_kv_heads][page_size][head_dim] of
+ * `type`.  Slot page * page_size + i is place i of a page.  A sequence's
+ * tokens lie in the pages of its row of a table [n_seqs][max_pages], token t in
+ * page table[t / page_size]; entries past a sequence's length are not read.
+ * Sequences may share pages that only the attention reads. */
+typedef struct {
+    gpu_buffer *K, *V;
+    int type;      /* ORN_KV_* */
+    int n_pages;
+    int page_size; /* a power of two, 8 to 1024; n_pages * page_size < 2^31 */
+    int n_kv_heads;
+    int head_dim;  /* 1 to 256 */
+    /* ORN_KV_E4M3: a stored value c stands for c * scale (0: 1).  Values beyond
+     * 448 * scale are stored as that; a NaN stays one. */
+    float k_scale, v_scale;
+} ornith_kv_pages;
+
+/* Rotary positions of up to four axes (time, height, width, ...).  Axis a turns
+ * pairs[a] pairs of dimensions; with R pairs in all, pair p turns by
+ * position[axis of p] * base^(-p / R), as gpu_rope does on one axis.
+ * interleaved = 0: the axes' pairs follow each other; 1: they are dealt out in
+ * turn (p = 0 axis 0, 1 axis 1, ...), an axis that has its pairs being passed
+ * over.  halves = 0: pair p is (x[2p], x[2p+1]), as in gpu_rope; 1: (x[p],
+ * x[p+R]).  Dimensions past 2R stay as they are. */
+#define ORN_ROPE_MAX_AXES 4
+#define ORN_ROPE_MAX_PAIRS 256
+typedef struct {
+    int n_axes; /* 1 to 4 */
+    int pairs[ORN_ROPE_MAX_AXES]; /* >= 0, at most ORN_ROPE_MAX_PAIRS in all */
+    int interleaved, halves;
+    double base; /* > 0 */
+} ornith_rope_axes;
+
+/* q_out = Q [n_tokens][n_heads][head_dim] and k_out = K [n_tokens]
+ * [n_kv_heads][head_dim] rotated; positions [n_axes][n_tokens].  Angles are
+ * formed in 64 bits, so that far positions keep their digits.  q_out may be Q
+ * and k_out may be K; a pair of NULLs with 0 heads leaves one side out. */
+int gpu_rope_axes(gpu_context *ctx, gpu_buffer *q_out, gpu_buffer *k_out, const gpu_buffer *Q,
+                  const gpu_buffer *K, int n_tokens, int n_heads, int n_kv_heads, int head_dim,
+                  const gpu_buffer *positions, const ornith_rope_axes *rope, unsigned flags);
+
+/* K, V [n_tokens][n_kv_heads][head_dim] rounded to the cache's type (to nearest)
+ * and stored at slots[n_tokens]; a token of slot -1 (padding) is not stored.
+ * Slots of one call differ.  With `rope`, K is rotated first, and so is Q
+ * [n_tokens][n_heads][head_dim] into q_out (which may be Q; NULL, NULL, 0: no
+ * queries), the padding's too.  rope NULL: nothing is rotated, and Q, q_out and
+ * positions are NULL. */
+int gpu_kv_append(gpu_context *ctx, const ornith_kv_pages *kv, const gpu_buffer *K,
+                  const gpu_buffer *V, int n_tokens, const gpu_buffer *slots, gpu_buffer *q_out,
+                  const gpu_buffer *Q, int n_heads, const gpu_buffer *positions,
+                  const ornith_rope_axes *rope, unsigned flags);
+
+/* out [n_seqs][n_heads][head_dim]: the attention of one query per sequence, Q
+ * [n_seqs][n_heads][head_dim], over the first lens[b] tokens of its row of the
+ * table, w = softmax(scale * q.k); n_heads is a multiple of n_kv_heads, head j
+ * reads kv head j / (n_heads / n_kv_heads).  A sequence of length 0 (a row of a
+ * padded batch) gives zeros.  out is not Q.
+ *
+ * score_out (may be NULL) [n_seqs][n_kv_heads][score_stride]: for the tokens
+ * t < lens[b], decay * score_in[b][h][t] (score_in NULL: 0) + the sum of w over
+ * kv head h's query heads; entries past a length stay as they are.  score_in may
+ * be score_out. */
+typedef struct {
+    float scale;  /* 0: 1 / sqrt(head_dim) */
+    int max_len;  /* no length is larger; 0: the table's width.  Sizes the workspace. */
+    unsigned flags;
+    const gpu_buffer *score_in;
+    gpu_buffer *score_out;
+    int score_stride; /* >= max_len */
+    float decay;
+} ornith_attend_opts;
+int gpu_kv_attend(gpu_context *ctx, const ornith_kv_pages *kv, gpu_buffer *out,
+                  const gpu_buffer *Q, int n_seqs, int n_heads, const gpu_buffer *table,
+                  int max_pages, const gpu_buffer *lens, const ornith_attend_opts *opts);
+
+/* Every kv head of every sequence keeps at most opts->keep of its tokens: the
+ * first `sink`, the last `recent`, and of those between the ones of the highest
+ * score (score [n_seqs][n_kv_heads][score_stride]; ties: the lowest token; a NaN
+ * is the lowest).  The kept tokens move, in order, to the front of the pages of
+ * dst_table [n_seqs][dst_pages], as do their scores (dst_score, may be NULL,
+ * [n_seqs][n_kv_heads][dst_stride]); dst_lens[b] = min(lens[b], keep), and kept
+ * [n_seqs][n_kv_heads][keep] says which they were (-1 past dst_lens).
+ *
+ * dst_table == table (then dst_pages == max_pages) moves them within their own
+ * pages, which no other sequence may share then; else no page of dst_table is
+ * read as one of table.  dst_lens may be lens, dst_score may be score (with
+ * dst_stride == score_stride). */
+typedef struct {
+    int keep;         /* >= 1, >= sink + recent */
+    int sink, recent; /* >= 0 */
+    int max_len;      /* no length is larger; 0: the table's width */
+    unsigned flags;
+} ornith_evict_opts;
+int gpu_kv_evict(gpu_context *ctx, const ornith_kv_pages *kv, int n_seqs, const gpu_buffer *table,
+                 int max_pages, const gpu_buffer *lens, const gpu_buffer *score, int score_stride,
+                 const gpu_buffer *dst_table, int dst_pages, gpu_buffer *dst_lens,
+                 gpu_buffer *dst_score, int dst_stride, gpu_buffer *kept,
+                 const ornith_evict_opts *opts);
+
+/* Waits for the context's stream; ORN_EINVAL (once) if a call of this group met
+ * a number out of range since the last report. */
+int gpu_kv_check(gpu_context *ctx);
+
 /* Device address of a buffer (for interop and tests). */
 void *gpu_device_ptr(gpu_context *ctx, gpu_buffer *buf);
 

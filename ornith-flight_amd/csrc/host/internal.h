@@ -15,6 +15,7 @@
 
 #define ORN_PROF_MAX_NAMES 32
 #define ORN_PROF_MAX_PENDING 8192
+#define ORN_CTL_KV 32 /* of 64 words */
 
 typedef struct {
     int name_id;
@@ -40,6 +41,9 @@ struct gpu_context {
     size_t used_memory;
     char err[256];
     orn_workspace ws;
+    /* the same for the paged cache's calls: apart, because the MoE forward's
+     * logits and counters stay readable in `ws` and its graphs record it */
+    orn_workspace kv_ws;
     /* this device's fixed scratch, resolved by the first
      * gpu_moe_forward_noalloc call on the context (NULL until then) */
     void *scratch;
@@ -49,7 +53,8 @@ struct gpu_context {
      * workspace is shared with other ops and is reallocated as it grows. */
     int *sync;
     /* device counters read back after a forward */
-    int *ctl_host; /* pinned mirror of the last forward's counters */
+    int *ctl_host; /* pinned mirror of the last forward's counters; from
+                      ORN_CTL_KV on the paged cache kernels' error words */
     int *last_ctl; /* device counters of the last forward (inside the workspace) */
     float *last_logits; /* [last_T][last_E] router logits of the last forward */
     int last_T, last_E;
@@ -99,6 +104,7 @@ void orn_cache_stats(orn_cache *c, ornith_moe_cache_stats *out, int reset);
 
 /* workspace (moe.c) */
 void *orn_ws_get(gpu_context *ctx, size_t bytes);
+void *orn_kv_ws_get(gpu_context *ctx, size_t bytes);
 void orn_ws_release(gpu_context *ctx);
 
 #endif /* ORNITH_HOST_INTERNAL_H */

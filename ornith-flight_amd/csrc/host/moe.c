@@ -129,6 +129,9 @@ void orn_ws_release(gpu_context *ctx)
     if (ctx->ws.base) hipFree(ctx->ws.base);
     ctx->ws.base = NULL;
     ctx->ws.bytes = 0;
+    if (ctx->kv_ws.base) hipFree(ctx->kv_ws.base);
+    ctx->kv_ws.base = NULL;
+    ctx->kv_ws.bytes = 0;
 }
 
 /* ---------------------------------------------------------------------------

@@ -61,6 +61,57 @@ int ornk_deltanet_step(float *state, const float *Q, const float *K, const float
 int ornk_kv_append(float *Kc, float *Vc, const float *Kn, const float *Vn, int pos, int hd,
                    hipStream_t s);
 
+/* ---- paged key-value cache (kv.hip, kv_attend.hip, kv_evict.hip) ------------ */
+/* The caller's pages, their sizes checked; `err` are host words (device-mapped)
+ * that a kernel sets to 1 + the token or sequence whose number is out of range. */
+#define ORNK_KV_ERR_PAGE 0
+#define ORNK_KV_ERR_SLOT 1
+#define ORNK_KV_ERR_LEN 2
+#define ORNK_KV_ERR_WORDS 3
+typedef struct {
+    void *k, *v;
+    int type, n_pages, page, page_log2, kv, hd;
+    float k_scale, v_scale;
+    int *err;
+} ornk_kv_pages;
+
+typedef struct {
+    const float *q, *k, *v; /* q or k may be NULL, v is with slots */
+    float *q_out, *k_out;   /* k_out: rotated K of gpu_rope_axes */
+    const int *pos;         /* [n_axes][T] */
+    const int *slots;       /* NULL: nothing is stored */
+    int T, heads, kv, hd, R, halves;
+    double turns[256];      /* per pair, revolutions per position */
+    uint8_t axis[256];
+} ornk_rope_args;
+int ornk_rope_append(const ornk_kv_pages *p, const ornk_rope_args *a, hipStream_t s);
+
+typedef struct {
+    const float *q;
+    float *out;
+    const int *table, *lens;
+    int n_seqs, heads, max_pages, max_len;
+    float scale;
+    const float *score_in;
+    float *score_out;
+    size_t score_stride;
+    float decay;
+    void *ws;
+} ornk_attend_args;
+size_t ornk_kv_attend_ws(const ornk_kv_pages *p, const ornk_attend_args *a);
+int ornk_kv_attend(const ornk_kv_pages *p, const ornk_attend_args *a, hipStream_t s);
+
+typedef struct {
+    const int *table, *lens, *dst_table;
+    const float *score;
+    float *dst_score;
+    size_t score_stride, dst_stride;
+    int *dst_lens, *kept;
+    int n_seqs, max_pages, dst_pages, max_len, keep, sink, recent, in_place;
+    int *counts; /* [n_seqs] work buffer */
+} ornk_evict_args;
+int ornk_kv_evict(const ornk_kv_pages *p, const ornk_evict_args *a, hipStream_t s);
+
 /* ---- fixed scratch of the forward that allocates nothing (scratch.hip) ---- */
 /* Size of the per-device scratch array; equals ORN_NOALLOC_SCRATCH_BYTES of
  * ornith_hip.h. */

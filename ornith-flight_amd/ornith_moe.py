@@ -25,6 +25,8 @@ MOE_EXACT_LOGITS = 64
 SYN_GATE, SYN_UP, SYN_DOWN, SYN_ROUTER, SYN_ACT, SYN_ZIPF = 1, 2, 3, 4, 5, 6
 GPU_BUF_DEFAULT, GPU_BUF_SHARED, GPU_BUF_CONSTANT = 0, 1, 2
 Q4K_BYTES, Q6K_BYTES = 144, 210
+KV_ASYNC = 1
+KV_TYPES = {"f32": 0, "f16": 1, "bf16": 2, "e4m3": 3}
 
 # Every symbol the public headers declare (include/ornith/gpu.h, ornith_hip.h).
 EXPORTED = [
@@ -55,6 +57,7 @@ EXPORTED = [
     "gpu_dequantize_tensor_gguf", "gpu_dequantize_expert_slice_gguf", "gpu_moe_store_load_gguf",
     "gpu_deltanet_step_gated", "gpu_kv_cache_append",
     "gpu_moe_store_prefetch", "gpu_moe_store_pin", "gpu_moe_store_cache_stats",
+    "gpu_rope_axes", "gpu_kv_append", "gpu_kv_attend", "gpu_kv_evict", "gpu_kv_check",
 ]
 
 
@@ -105,6 +108,32 @@ class CacheStats(C.Structure):
 class MoEOpts(C.Structure):
     _fields_ = [("route_mode", C.c_int), ("flags", C.c_uint), ("ep_first", C.c_int),
                 ("ep_count", C.c_int)]
+
+
+class KVPages(C.Structure):
+    """ornith_kv_pages: one layer's paged key-value cache."""
+    _fields_ = [("K", C.c_void_p), ("V", C.c_void_p), ("type", C.c_int), ("n_pages", C.c_int),
+                ("page_size", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("k_scale", C.c_float), ("v_scale", C.c_float)]
+
+
+class RopeAxes(C.Structure):
+    """ornith_rope_axes: rotary positions of up to four axes."""
+    _fields_ = [("n_axes", C.c_int), ("pairs", C.c_int * 4), ("interleaved", C.c_int),
+                ("halves", C.c_int), ("base", C.c_double)]
+
+
+class AttendOpts(C.Structure):
+    """ornith_attend_opts."""
+    _fields_ = [("scale", C.c_float), ("max_len", C.c_int), ("flags", C.c_uint),
+                ("score_in", C.c_void_p), ("score_out", C.c_void_p), ("score_stride", C.c_int),
+                ("decay", C.c_float)]
+
+
+class EvictOpts(C.Structure):
+    """ornith_evict_opts."""
+    _fields_ = [("keep", C.c_int), ("sink", C.c_int), ("recent", C.c_int), ("max_len", C.c_int),
+                ("flags", C.c_uint)]
 
 
 _lib = None
@@ -190,6 +219,14 @@ def lib():
         "gpu_moe_store_prefetch": (i, [vp, vp, i, vp, i]),
         "gpu_moe_store_pin": (i, [vp, vp, i, vp, i, i]),
         "gpu_moe_store_cache_stats": (i, [vp, vp, C.POINTER(CacheStats), i]),
+        "gpu_rope_axes": (i, [vp, vp, vp, vp, vp, i, i, i, i, vp, C.POINTER(RopeAxes), C.c_uint]),
+        "gpu_kv_append": (i, [vp, C.POINTER(KVPages), vp, vp, i, vp, vp, vp, i, vp,
+                              C.POINTER(RopeAxes), C.c_uint]),
+        "gpu_kv_attend": (i, [vp, C.POINTER(KVPages), vp, vp, i, i, vp, i, vp,
+                              C.POINTER(AttendOpts)]),
+        "gpu_kv_evict": (i, [vp, C.POINTER(KVPages), i, vp, i, vp, vp, i, vp, i, vp, vp, i, vp,
+                             C.POINTER(EvictOpts)]),
+        "gpu_kv_check": (i, [vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -452,6 +489,63 @@ class Store:
         if self.ptr:
             lib().gpu_moe_store_destroy(self.ctx.ptr, self.ptr)
             self.ptr = None
+
+
+# ---------------------------------------------------------------- paged key-value cache
+def _ptr(buf):
+    return buf.ptr if buf else None
+
+
+def kv_pages(K, V, type, n_pages, page_size, n_kv_heads, head_dim, k_scale=0.0, v_scale=0.0):
+    """The description of a cache in the buffers K and V (type: "f32", "f16", "bf16", "e4m3")."""
+    p = KVPages(K.ptr, V.ptr, KV_TYPES[type], n_pages, page_size, n_kv_heads, head_dim, k_scale,
+                v_scale)
+    p.buffers = (K, V)  # live as long as the description
+    return p
+
+
+def rope_axes(pairs, base, halves=False, interleaved=False):
+    """pairs: the rotated pairs of each axis."""
+    return RopeAxes(len(pairs), (C.c_int * 4)(*pairs), int(interleaved), int(halves), base)
+
+
+def rope_axes_apply(ctx, q_out, k_out, Q, K, T, heads, kv_heads, head_dim, positions, rope, flags=0):
+    ctx.check(lib().gpu_rope_axes(ctx.ptr, _ptr(q_out), _ptr(k_out), _ptr(Q), _ptr(K), T, heads,
+                                  kv_heads, head_dim, positions.ptr, C.byref(rope), flags),
+              "gpu_rope_axes")
+
+
+def kv_append(ctx, pages, K, V, T, slots, q_out=None, Q=None, heads=0, positions=None, rope=None,
+              flags=0):
+    ctx.check(lib().gpu_kv_append(ctx.ptr, C.byref(pages), K.ptr, V.ptr, T, slots.ptr, _ptr(q_out),
+                                  _ptr(Q), heads, _ptr(positions),
+                                  C.byref(rope) if rope is not None else None, flags),
+              "gpu_kv_append")
+
+
+def attend_opts(scale=0.0, max_len=0, flags=0, score_in=None, score_out=None, score_stride=0,
+                decay=1.0):
+    o = AttendOpts(scale, max_len, flags, _ptr(score_in), _ptr(score_out), score_stride, decay)
+    o.buffers = (score_in, score_out)
+    return o
+
+
+def kv_attend(ctx, pages, out, Q, n_seqs, heads, table, max_pages, lens, opts=None):
+    ctx.check(lib().gpu_kv_attend(ctx.ptr, C.byref(pages), out.ptr, Q.ptr, n_seqs, heads, table.ptr,
+                                  max_pages, lens.ptr, C.byref(opts) if opts is not None else None),
+              "gpu_kv_attend")
+
+
+def evict_opts(keep, sink=0, recent=0, max_len=0, flags=0):
+    return EvictOpts(keep, sink, recent, max_len, flags)
+
+
+def kv_evict(ctx, pages, n_seqs, table, max_pages, lens, score, score_stride, dst_table, dst_pages,
+             dst_lens, dst_score, dst_stride, kept, opts):
+    ctx.check(lib().gpu_kv_evict(ctx.ptr, C.byref(pages), n_seqs, table.ptr, max_pages, lens.ptr,
+                                 score.ptr, score_stride, dst_table.ptr, dst_pages, dst_lens.ptr,
+                                 _ptr(dst_score), dst_stride, kept.ptr, C.byref(opts)),
+              "gpu_kv_evict")
 
 
 def profile(ctx: Context):
