@@ -3,119 +3,824 @@
 // Attention of one new token per sequence over the paged key-value cache
 // (ornith_hip.h): out = sum_t w_t V[t], w = softmax(scale * q . K[t]), the sums
 // over the sequence's tokens, query heads sharing kv heads.
+//
+// Work: the tokens of every sequence, kv head and tile of 16 of its query
+// heads ("pair") in units of 128, one after the other on a line.  W work groups
+// take equal stretches of the line, whatever the lengths are; a pair that one
+// group covers is finished there, of the others the groups leave O, m and l of
+// their part, which k_kv_join puts together:
+//   M = max m_i, L = sum l_i 2^(m_i - M), out = sum O_i 2^(m_i - M) / L.
+// (Exponents are base 2: log2 e is in the query's scale.)
 #include "kv.h"
 
 namespace {
 
-constexpr int WAVES = 4;
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+constexpr int WAVES = 4, UNIT = 128;  // waves of a work group, tokens of a unit
+constexpr int GROUPS = 512;           // work groups: two per CU
 
 struct AttendWs {
-    float *s;   // [n_seqs][heads][max_len] scores (only where the weights are asked for)
-    float2 *ml; // [n_seqs][heads] maximum and sum
+    long long *cum;  // [n_seqs + 1] units before each sequence, per pair of it
+    float2 *part_ml; // [2 W][16] of the parts: a group's first stretch, its last
+    float *part_o;   // [2 W][16][row]
+    int W, row;      // groups launched; floats of a row of part_o
+    float2 *ml;      // [n_seqs][heads] and scores [n_seqs][heads][s_len], for the weights
+    float *s;
+    size_t s_len;
 };
 
-// One work group per sequence and query head.
-template <int TYPE>
-__global__ void __launch_bounds__(64 * WAVES) k_kv_attend(ornk_kv_pages p, ornk_attend_args a,
-                                                          AttendWs w)
+// The line of units: `first` of a group's stretch.
+__device__ __forceinline__ long long line_at(long long T, int W, int w)
 {
-    typedef KvElem<TYPE> E;
-    __shared__ float so[WAVES][256], sm[WAVES], sl[WAVES];
-    const int b = blockIdx.x, head = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int h = head / (a.heads / p.kv), hd = p.hd;
-    const int len = kv_len(p, a.lens, b, a.max_len);
-    const float *q = a.q + ((size_t)b * a.heads + head) * hd;
-    float qr[4], o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    return T * w / W;
+}
+
+struct Seg {  // part of one pair
+    int b, h, j0, rows;  // sequence, kv head, first query head, query heads
+    int len, k0, k1;     // the sequence's tokens; this part's
+    size_t score;        // first score of query head j0
+};
+
+__device__ __forceinline__ uint32_t top16(float hi, float lo)
+{
+    return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+__device__ __forceinline__ float rest16(float x)
+{
+    return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+}
+__device__ __forceinline__ v8b as_v8b(u4 x) { return __builtin_bit_cast(v8b, x); }
+
+// N bytes (4, 8, 16) into words.
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t *w, const uint8_t *p)
+{
+    typedef uint32_t vec __attribute__((ext_vector_type(N / 4)));
+    const vec v = *reinterpret_cast<const vec *>(p);
+    if constexpr (N == 4) w[0] = v[0];
+    else
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        qr[j] = lane + 64 * j < hd ? q[lane + 64 * j] * a.scale * p.k_scale : 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    for (int t = wave; t < len; t += WAVES) {
-        const int page = kv_page(p, a.table[(size_t)b * a.max_pages + (t >> p.page_log2)], b);
-        float sc = -INFINITY;
-        const size_t at = page < 0 ? 0 : kv_at(p, page, h, t & (p.page - 1));
-        if (page >= 0) {
-            const typename E::T *k = static_cast<const typename E::T *>(p.k) + at;
-            sc = 0.0f;
+        for (int i = 0; i < N / 4; ++i) w[i] = v[i];
+}
+
+template <int TYPE>
+constexpr int elem_size = (int)sizeof(typename KvElem<TYPE>::T);
+
+// Four consecutive elements in words -> fp32.
+template <int TYPE>
+__device__ __forceinline__ void unpack4(float *f, const uint32_t *w)
+{
+    if constexpr (TYPE == ORN_KV_F32) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (lane + 64 * j < hd) sc = fmaf(qr[j], E::get(k[lane + 64 * j]), sc);
-            sc = orn_wave_sum(sc);
+        for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(w[i]);
+    } else if constexpr (TYPE == ORN_KV_BF16) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
         }
-        if (w.s && lane == 0) w.s[((size_t)b * a.heads + head) * a.max_len + t] = sc;
-        if (page < 0) continue;
-        const float mn = fmaxf(m, sc);
-        const bool none = mn == -INFINITY;
-        const float corr = none ? 1.0f : expf(m - mn), pr = none ? 0.0f : expf(sc - mn);
-        l = l * corr + pr;
-        m = mn;
-        const typename E::T *v = static_cast<const typename E::T *>(p.v) + at;
+    } else if constexpr (TYPE == ORN_KV_F16) {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (lane + 64 * j < hd) o[j] = fmaf(pr, E::get(v[lane + 64 * j]), o[j] * corr);
+        for (int i = 0; i < 2; ++i) {
+            const h2 h = __builtin_bit_cast(h2, w[i]);
+            f[2 * i] = (float)h[0];
+            f[2 * i + 1] = (float)h[1];
+        }
+    } else {
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[0], false);
+        const f2 b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[0], true);
+        f[0] = a[0], f[1] = a[1], f[2] = b[0], f[3] = b[1];
     }
+}
+
+// ---------------------------------------------------------------------------
+// A wave's tile: KT keys by the 16 query heads of the pair.  Scores are formed
+// transposed, S^T = K Q^T, so that lane (g = lane / 16, n = lane % 16) holds the
+// scores of query head n for keys 16 i + 4 g + r: the row maximum and sum are
+// two exchanges away, and the weights are the A operand of O = P V as they
+// are.  Both paths read K and V from memory straight into operand registers.
+// ---------------------------------------------------------------------------
+
+// fp32 operands (v_mfma_f32_16x16x4_f32): what 32-bit arithmetic gives, with
+// infinities and NaN where it has them.  The path of the fp32 cache; of heads
+// whose rows are not whole 16-byte words (VEC = false); and of what the path
+// of the narrower types cannot give (see there).  16 keys per tile.
+template <int TYPE, int HD, bool VEC, bool FULL>
+struct Exact {
+    static constexpr int KT = 16, NJ = HD / 16, NV = HD / 64, NO = HD / 16;
+    static constexpr int ES = elem_size<TYPE>;
+    static constexpr size_t Q_BYTES = 16 * HD * 4;
+    static constexpr bool full = FULL, exact = true, ahead = TYPE == ORN_KV_F32 && VEC;
+    float k[NJ][4], v[4][NV][4];
+
+    static __device__ __forceinline__ void load4(float *f, const uint8_t *p, int c, int hd)
+    {
+        if constexpr (VEC) {
+            uint32_t w[ES];
+            load_words<4 * ES>(w, p + (FULL || c < hd ? c : 0) * ES);
+            unpack4<TYPE>(f, w);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) so[wave][lane + 64 * j] = o[j];
-    if (lane == 0) {
-        sm[wave] = m;
-        sl[wave] = l;
+            for (int i = 0; i < 4; ++i) f[i] = FULL || c < hd ? f[i] : 0.0f;
+        } else {
+            const typename KvElem<TYPE>::T *e = reinterpret_cast<const typename KvElem<TYPE>::T *>(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = c + i < hd ? KvElem<TYPE>::get(e[c + i]) : 0.0f;
+        }
+    }
+    // row: this lane's key of each 16
+    __device__ __forceinline__ void load_k(const uint8_t *const *row, int g, int hd)
+    {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) load4(k[j], row[0], 16 * j + 4 * g, hd);
+    }
+    // row: this lane's four keys of each 16
+    __device__ __forceinline__ void load_v(const uint8_t *const *row, int n, int hd)
+    {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < NV; ++j) load4(v[r][j], row[r], 64 * j + 4 * n, hd);
+    }
+    static __device__ void put_q(void *lds, int n, int d, float q)
+    {
+        // [16 j][n][4 g + i]: a lane's four steps are one word
+        static_cast<float *>(lds)[(d / 16) * 256 + n * 16 + d % 16] = q;
+    }
+    __device__ __forceinline__ void scores(float *s, const void *lds, int lane) const
+    {
+        const int g = lane >> 4, n = lane & 15;
+        const v4f *q = reinterpret_cast<const v4f *>(static_cast<const float *>(lds) + n * 16 + 4 * g);
+        v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const v4f b = q[64 * j];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                acc = __builtin_amdgcn_mfma_f32_16x16x4f32(k[j][i], b[i], acc, 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[r] = acc[r];
+    }
+    // A key that is left out has the weight 0, and 0 times an infinity is none:
+    // its values count as zeros.
+    __device__ __forceinline__ void pv(v4f *o, const float *p, const bool *on)
+    {
+        if (__any(!(on[0] && on[1] && on[2] && on[3]))) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[r][j][i] = on[r] ? v[r][j][i] : 0.0f;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    o[4 * j + i] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[r], v[r][j][i], o[4 * j + i],
+                                                                        0, 0, 0);
+    }
+    // column of o[c] in lane n; four at a time are consecutive
+    static __device__ __forceinline__ int col(int c, int n) { return 64 * (c / 4) + 4 * n + c % 4; }
+};
+
+// bf16 operands (v_mfma_f32_16x16x32_bf16) for the caches of 16 and 8 bits.  A
+// cached value is one bf16 part (bf16, e4m3) or two (f16: 8 and 3 bits), a query
+// or a weight three: the top 8 bits, of the rest the top 8, and the rest.  Each
+// part has fp32's exponents, so 24 bits stay at every size, and the sums are
+// fp32.  Of the f16 products the smallest, second part by third, is left out
+// (2^-24 of the whole).  Parts of an infinity are no numbers: a segment whose
+// sums are not finite is done again by Exact.  32 keys per tile.
+//
+// Reduction indexes are permuted alike in both operands: a lane's 16 bytes of a
+// K row are its dimensions of one step (of two, for e4m3), and key 16 i + 4 g + r
+// is place 8 g + 4 i + r of the reduction over keys, so that the weights stay
+// where they are.  V's 8 rows by CW columns in a lane's registers are turned
+// into CW operands of 8 keys there (v_perm_b32).
+template <int TYPE, int HD, bool FULL>
+struct Parts {
+    static constexpr int KT = 32, ES = elem_size<TYPE>, NS = HD / 32, NO = HD / 16;
+    static constexpr int DL = 16 / ES, NL = HD / (4 * DL);             // K: dimensions of a load, loads
+    static constexpr int CW = HD / 16 < DL ? HD / 16 : DL, NH = HD / (16 * CW);  // V: columns, loads of a row
+    static constexpr int VW = CW * ES / 4;
+    static constexpr int NP = TYPE == ORN_KV_F16 ? 2 : 1;
+    static constexpr size_t Q_BYTES = 3 * 16 * HD * 2;
+    static constexpr bool full = FULL, exact = false, ahead = true;
+    uint32_t k[2][NL][4], v[8][NH][VW];
+
+    __device__ __forceinline__ void load_k(const uint8_t *const *row, int g, int hd)
+    {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < NL; ++j) {
+                // past the row: its start, which meets zeros of the query
+                const int c = (4 * j + g) * DL;
+                load_words<16>(k[i][j], row[i] + (FULL || c < hd ? c : 0) * ES);
+            }
+    }
+    __device__ __forceinline__ void load_v(const uint8_t *const *row, int n, int hd)
+    {
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+#pragma unroll
+            for (int j = 0; j < NH; ++j) {
+                const int c = CW * (16 * j + n);  // past the row: a column that is not stored
+                load_words<4 * VW>(v[r][j], row[r] + (FULL || c < hd ? c : 0) * ES);
+            }
+    }
+    // [part][step][lane][8]; dimension d of the queries
+    static __device__ void put_q(void *lds, int n, int d, float q)
+    {
+        const int j = d / (4 * DL), g = d / DL % 4, e = d % DL;
+        const int step = j * (DL / 8) + e / 8;
+        uint16_t *at = static_cast<uint16_t *>(lds) + ((step * 64 + 16 * g + n) * 8 + e % 8);
+#pragma unroll
+        for (int part = 0; part < 3; ++part) {
+            at[part * NS * 512] = (uint16_t)(__float_as_uint(q) >> 16);
+            q = rest16(q);
+        }
+    }
+    // operand of step `st`, keys of half i
+    __device__ __forceinline__ void k_parts(v8b *out, int i, int st) const
+    {
+        if constexpr (TYPE == ORN_KV_BF16) {
+            out[0] = as_v8b((u4){k[i][st][0], k[i][st][1], k[i][st][2], k[i][st][3]});
+        } else if constexpr (TYPE == ORN_KV_F16) {
+            u4 hi, lo;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                float f[4];
+                unpack4<TYPE>(f, &k[i][st][2 * w]);
+                hi[2 * w] = top16(f[1], f[0]), hi[2 * w + 1] = top16(f[3], f[2]);
+                lo[2 * w] = top16(rest16(f[1]), rest16(f[0]));
+                lo[2 * w + 1] = top16(rest16(f[3]), rest16(f[2]));
+            }
+            out[0] = as_v8b(hi), out[1] = as_v8b(lo);
+        } else {
+            u4 hi;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                float f[4];
+                unpack4<TYPE>(f, &k[i][st / 2][2 * (st % 2) + w]);
+                hi[2 * w] = top16(f[1], f[0]), hi[2 * w + 1] = top16(f[3], f[2]);
+            }
+            out[0] = as_v8b(hi);
+        }
+    }
+    static __device__ __forceinline__ v4f mma(v8b a, v8b b, v4f c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    __device__ __forceinline__ void scores(float *s, const void *lds, int lane) const
+    {
+        const v8b *q = static_cast<const v8b *>(lds) + lane;
+        v4f a0 = {0.0f, 0.0f, 0.0f, 0.0f}, a1 = a0, b0 = a0, b1 = a0;
+#pragma unroll
+        for (int st = 0; st < NS; ++st) {
+            v8b k0[NP], k1[NP];
+            k_parts(k0, 0, st);
+            k_parts(k1, 1, st);
+            const v8b q0 = q[64 * st], q1 = q[64 * (NS + st)], q2 = q[64 * (2 * NS + st)];
+            a0 = mma(k0[0], q0, a0);
+            a1 = mma(k1[0], q0, a1);
+            b0 = mma(k0[0], q2, b0);
+            b1 = mma(k1[0], q2, b1);
+            b0 = mma(k0[0], q1, b0);
+            b1 = mma(k1[0], q1, b1);
+            if constexpr (NP == 2) {
+                b0 = mma(k0[1], q1, b0);
+                b1 = mma(k1[1], q1, b1);
+                b0 = mma(k0[1], q0, b0);
+                b1 = mma(k1[1], q0, b1);
+            }
+        }
+        a0 += b0;
+        a1 += b1;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[r] = a0[r], s[4 + r] = a1[r];
+    }
+    __device__ __forceinline__ void pv(v4f *o, const float *p, const bool *)
+    {
+        v8b pp[3];
+        {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = p[e];
+#pragma unroll
+            for (int part = 0; part < 3; ++part) {
+                u4 w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = top16(x[2 * e + 1], x[2 * e]);
+                pp[part] = as_v8b(w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = rest16(x[e]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NH; ++j) {
+            if constexpr (TYPE == ORN_KV_BF16) {
+#pragma unroll
+                for (int c = 0; c < CW; ++c) {
+                    u4 w;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        w[e] = __builtin_amdgcn_perm(v[2 * e + 1][j][c / 2], v[2 * e][j][c / 2],
+                                                     c % 2 ? 0x07060302u : 0x05040100u);
+                    const v8b b = as_v8b(w);
+                    v4f &x = o[j * CW + c];
+                    x = mma(pp[2], b, x);
+                    x = mma(pp[1], b, x);
+                    x = mma(pp[0], b, x);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < CW; c += 4) {
+                    float f[8][4];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) unpack4<TYPE>(f[e], &v[e][j][c * ES / 4]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        u4 hi, lo;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            hi[e] = top16(f[2 * e + 1][i], f[2 * e][i]);
+                            if constexpr (NP == 2)
+                                lo[e] = top16(rest16(f[2 * e + 1][i]), rest16(f[2 * e][i]));
+                        }
+                        v4f &x = o[j * CW + c + i];
+                        x = mma(pp[2], as_v8b(hi), x);
+                        if constexpr (NP == 2) x = mma(pp[1], as_v8b(lo), x);
+                        x = mma(pp[1], as_v8b(hi), x);
+                        if constexpr (NP == 2) x = mma(pp[0], as_v8b(lo), x);
+                        x = mma(pp[0], as_v8b(hi), x);
+                    }
+                }
+            }
+        }
+    }
+    static __device__ __forceinline__ int col(int c, int n) { return CW * (16 * (c / CW) + n) + c % CW; }
+};
+
+// ---------------------------------------------------------------------------
+template <int TYPE, int HD, class Path>
+__device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a, const AttendWs &w,
+                               const Seg &sg, uint8_t *lds, int slot)
+{
+    constexpr int KT = Path::KT, NI = KT / 16, NO = Path::NO, ES = elem_size<TYPE>;
+    __shared__ float sm[WAVES][16], sl[WAVES][16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, n = lane & 15;
+    const int hd = p.hd;
+
+    // the query heads, scaled; those past the last are zeros
+    __syncthreads();
+    {
+        const float f = a.scale * p.k_scale * 1.44269504088896341f;
+        const float *q = a.q + ((size_t)sg.b * a.heads + sg.j0) * hd;
+        for (int i = tid; i < 16 * HD; i += 64 * WAVES) {
+            const int row = i / HD, d = i % HD;
+            Path::put_q(lds, row, d, row < sg.rows && d < hd ? q[(size_t)row * hd + d] * f : 0.0f);
+        }
     }
     __syncthreads();
-    float M = -INFINITY, L = 0.0f;
-    for (int i = 0; i < WAVES; ++i) M = fmaxf(M, sm[i]);
-    float acc = 0.0f;
-    for (int i = 0; i < WAVES; ++i) {
-        const float f = sm[i] == -INFINITY ? 0.0f : expf(sm[i] - M);
-        L += sl[i] * f;
-        acc += so[i][tid] * f;
+
+    const int *table = a.table + (size_t)sg.b * a.max_pages;
+    const uint8_t *kp = static_cast<const uint8_t *>(p.k), *vp = static_cast<const uint8_t *>(p.v);
+    const int last_page = (sg.len - 1) >> p.page_log2;
+    int page0 = -64, ids = -1;  // lane i holds the page of place page0 + i
+    const int row_bytes = hd * ES;
+    // the row of token t < sg.len, through its page (page 0 for one that is none)
+    auto place = [&](int t, bool &on) {
+        const int id = __shfl(ids, (t >> p.page_log2) - page0, 64);
+        on = id >= 0;
+        return kv_at(p, id < 0 ? 0 : id, sg.h, t & (p.page - 1)) * ES;
+    };
+    auto pages_for = [&](int t) {
+        const int want = (t >> p.page_log2) & ~63;
+        if (want == page0) return;
+        page0 = want;
+        const int i = want + lane;
+        ids = i <= last_page ? kv_page(p, table[i], sg.b) : -1;
+    };
+
+    Path x;
+    v4f o[NO];
+#pragma unroll
+    for (int c = 0; c < NO; ++c) o[c] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+    bool von[4 * NI];  // whether this lane's keys count
+    auto load_k = [&](int t) {  // rows past the sequence's last: that one again
+        const uint8_t *row[NI];
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            bool on;
+            row[i] = kp + place(min(t + 16 * i + n, sg.len - 1), on);
+        }
+        x.load_k(row, g, hd);
+    };
+    auto load_v = [&](int t) {
+        const uint8_t *row[4 * NI];
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int t0 = t + 16 * i + 4 * g, at = min(t0, (sg.len - 1) & ~3);  // four of one page
+            bool on;
+            const uint8_t *first = vp + place(at, on);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                row[4 * i + r] = first + min(r, sg.len - 1 - at) * row_bytes;
+                von[4 * i + r] = on && t0 + r < sg.len;
+            }
+        }
+        x.load_v(row, n, hd);
+    };
+
+    int t = sg.k0 + KT * wave;
+    if (Path::ahead && t < sg.k1) {
+        pages_for(t);
+        load_k(t);
+        load_v(t);
     }
-    if (tid < hd)
-        a.out[((size_t)b * a.heads + head) * hd + tid] = L != 0.0f ? acc / L * p.v_scale : 0.0f;
-    if (w.s && tid == 0) w.ml[(size_t)b * a.heads + head] = make_float2(M, L);
+    for (; t < sg.k1; t += KT * WAVES) {
+        asm volatile("" ::: "memory");  // the queries are read from LDS in every tile
+        if (!Path::ahead) {
+            pages_for(t);
+            load_k(t);
+            load_v(t);
+        }
+        float s[4 * NI];
+        x.scores(s, lds, lane);
+        const int nt = t + KT * WAVES;
+        const bool more = Path::ahead && nt < sg.k1;
+        if (more) {
+            pages_for(nt);
+            load_k(nt);
+        }
+        float tm = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4 * NI; ++i) {
+            s[i] = von[i] ? s[i] : -INFINITY;
+            tm = fmaxf(tm, s[i]);
+        }
+        if (w.s && n < sg.rows) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const v4f v = {s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
+                *reinterpret_cast<v4f *>(w.s + sg.score + n * w.s_len + t + 16 * i + 4 * g) = v;
+            }
+        }
+        tm = fmaxf(tm, __shfl_xor(tm, 16, 64));
+        tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
+        // the reference moves only when the maximum has passed it by a factor
+        // of 2^6 (weights up to that stay): O is left alone in most tiles
+        const float mn = tm > m + 6.0f ? tm : m;
+        if (__any(mn != m)) {
+            const float corr = mn == -INFINITY ? 1.0f : exp2f(m - mn);
+            l *= corr;
+            float cr[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) cr[r] = __shfl(corr, 4 * g + r, 64);
+#pragma unroll
+            for (int c = 0; c < NO; ++c)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[c][r] *= cr[r];
+            m = mn;
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * NI; ++i) {
+            s[i] = mn == -INFINITY ? 0.0f : exp2f(s[i] - mn);
+            l += s[i];
+        }
+        x.pv(o, s, von);
+        if (more) load_v(nt);
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+
+    if constexpr (!Path::exact) {  // anything that is not finite: not this path's to say
+        float z = l * 0.0f;
+#pragma unroll
+        for (int c = 0; c < NO; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) z = fmaf(o[c][r], 0.0f, z);
+        if (__syncthreads_or(z != 0.0f)) return false;
+    } else {
+        __syncthreads();  // the queries are consumed
+    }
+    if (g == 0) {
+        sm[wave][n] = m;
+        sl[wave][n] = l;
+    }
+    float *ob = reinterpret_cast<float *>(lds);  // [wave][rows][HD]
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int row = 4 * g + r;
+        if (row >= sg.rows) continue;
+#pragma unroll
+        for (int c = 0; c < NO; c += 4) {
+            const v4f v = {o[c][r], o[c + 1][r], o[c + 2][r], o[c + 3][r]};
+            *reinterpret_cast<v4f *>(ob + ((size_t)wave * sg.rows + row) * HD + Path::col(c, n)) = v;
+        }
+    }
+    __syncthreads();
+    const bool whole = slot < 0;
+    for (int i = tid; i < sg.rows * (HD / 4); i += 64 * WAVES) {
+        const int row = i / (HD / 4), c = 4 * (i % (HD / 4));
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) M = fmaxf(M, sm[v][row]);
+        v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) {
+            const float f = sm[v][row] == -INFINITY ? 0.0f : exp2f(sm[v][row] - M);
+            // (a wave without tokens: zeros, and its factor)
+            L += sl[v][row] * f;
+            const v4f x4 = *reinterpret_cast<const v4f *>(ob + ((size_t)v * sg.rows + row) * HD + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = sm[v][row] == -INFINITY ? acc[e] : fmaf(x4[e], f, acc[e]);
+        }
+        if (whole) {
+            const float f = L != 0.0f ? p.v_scale / L : 0.0f;
+            float *out = a.out + ((size_t)sg.b * a.heads + sg.j0 + row) * hd + c;
+            if (hd % 4 == 0) {
+                if (c < hd) *reinterpret_cast<v4f *>(out) = acc * f;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c + e < hd) out[e] = acc[e] * f;
+            }
+            if (w.ml && c == 0) w.ml[(size_t)sg.b * a.heads + sg.j0 + row] = make_float2(M, L);
+        } else {
+            if (c < w.row)
+                *reinterpret_cast<v4f *>(w.part_o + ((size_t)slot * 16 + row) * w.row + c) = acc;
+            if (c == 0) w.part_ml[(size_t)slot * 16 + row] = make_float2(M, L);
+        }
+    }
+    return true;
+}
+
+// cum[i] = units of a pair before sequence c0 + i, of the 64 * WAVES from c0 on;
+// returns those before the next stretch.
+__device__ long long scan_lens(const ornk_kv_pages &p, const ornk_attend_args &a, int c0,
+                               long long before, long long *cum)
+{
+    __shared__ long long tot[WAVES];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int b = c0 + tid;
+    const long long u = b < a.n_seqs ? (kv_len(p, a.lens, b, a.max_len) + UNIT - 1) / UNIT : 0;
+    long long x = u;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const long long y = __shfl_up(x, d, 64);
+        if (lane >= d) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) tot[wave] = x;
+    __syncthreads();
+    long long all = before;
+#pragma unroll
+    for (int v = 0; v < WAVES; ++v) {
+        if (v < wave) x += tot[v];
+        all += tot[v];
+    }
+    cum[tid] = before + x - u;
+    if (tid == 0) cum[64 * WAVES] = all;
+    __syncthreads();
+    return all;
+}
+
+template <int TYPE, int HD, class Path>
+__global__ void __launch_bounds__(64 * WAVES, 2) k_kv_attend(ornk_kv_pages p, ornk_attend_args a,
+                                                             AttendWs w)
+{
+    extern __shared__ __align__(16) uint8_t lds[];
+    constexpr int CH = 64 * WAVES;
+    __shared__ long long cum[CH + 1];
+    const int G = a.heads / p.kv, HT = (G + 15) / 16;
+    const long long per = (long long)p.kv * HT;  // pairs of a sequence
+    long long units = 0;
+    int c0 = 0;
+    for (int c = 0; c < a.n_seqs; c += CH) {
+        units = scan_lens(p, a, c, units, cum);
+        c0 = c;
+        if (blockIdx.x == 0) {
+            if (c + threadIdx.x < a.n_seqs) w.cum[c + threadIdx.x] = cum[threadIdx.x];
+            if (threadIdx.x == 0 && c + CH >= a.n_seqs) w.cum[a.n_seqs] = units;
+        }
+    }
+    const long long T = units * per;
+    const int W = (int)min((long long)w.W, T);
+    if ((int)blockIdx.x >= W) return;
+    const long long lo = line_at(T, W, blockIdx.x), hi = line_at(T, W, blockIdx.x + 1);
+    if (lo < cum[0] * per) {  // an earlier stretch of sequences
+        long long before = 0;
+        for (c0 = 0;; c0 += CH) {
+            before = scan_lens(p, a, c0, before, cum);
+            if (lo < before * per) break;
+        }
+    }
+    for (long long u = lo; u < hi;) {
+        while (u >= cum[CH] * per) {
+            c0 += CH;
+            scan_lens(p, a, c0, cum[CH], cum);
+        }
+        int i = 0;  // the last sequence that starts at or before u
+#pragma unroll
+        for (int d = CH / 2; d; d >>= 1)
+            if (cum[i + d] * per <= u) i += d;
+        const int n = (int)(cum[i + 1] - cum[i]);
+        const long long off = u - cum[i] * per;
+        const int pair = (int)(off / n), k = (int)(off - (long long)pair * n);
+        const int cnt = (int)min((long long)(n - k), hi - u);
+        Seg sg;
+        sg.b = c0 + i;
+        sg.h = pair / HT;
+        const int j = 16 * (pair % HT);
+        sg.j0 = sg.h * G + j;
+        sg.rows = min(16, G - j);
+        sg.len = min(max(a.lens[sg.b], 0), a.max_len);
+        sg.k0 = k * UNIT;
+        sg.k1 = min(sg.len, (k + cnt) * UNIT);
+        sg.score = ((size_t)sg.b * a.heads + sg.j0) * w.s_len;
+        const int slot = cnt == n ? -1 : 2 * (int)blockIdx.x + (u == lo ? 0 : 1);
+        const bool done = attend_segment<TYPE, HD, Path>(p, a, w, sg, lds, slot);
+        if constexpr (!Path::exact) {
+            if (!done) attend_segment<TYPE, HD, Exact<TYPE, HD, true, Path::full>>(p, a, w, sg, lds, slot);
+        }
+        u += cnt;
+    }
+}
+
+// One work group per sequence and query head: the parts of its pair put
+// together; zeros for a sequence without tokens.
+constexpr int JT = 256;
+__global__ void __launch_bounds__(JT) k_kv_join(ornk_kv_pages p, ornk_attend_args a, AttendWs w)
+{
+    __shared__ float f[GROUPS], red[JT / 64];
+    __shared__ __align__(16) float acc[JT * 4];
+    const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int G = a.heads / p.kv, HT = (G + 15) / 16, hd = p.hd;
+    const long long per = (long long)p.kv * HT, T = w.cum[a.n_seqs] * per;
+    const long long c0 = w.cum[b], n = w.cum[b + 1] - c0;
+    float *out = a.out + ((size_t)b * a.heads + head) * hd;
+    if (n == 0) {
+        for (int i = tid; i < hd; i += JT) out[i] = 0.0f;
+        return;
+    }
+    const int pair = head / G * HT + head % G / 16, row = head % G % 16;
+    const int W = (int)min((long long)w.W, T);
+    const long long s = c0 * per + pair * n, e = s + n;
+    const int w0 = (int)(((s + 1) * W - 1) / T), w1 = (int)((e * W - 1) / T);
+    if (w0 == w1) return;  // finished by one group
+    const int nseg = w1 - w0 + 1, first = 2 * w0 + (line_at(T, W, w0) == s ? 0 : 1);
+    auto slot = [&](int i) { return (size_t)(i ? 2 * (w0 + i) : first) * 16 + row; };
+    auto all = [&](float v, bool mx) {
+#pragma unroll
+        for (int d = 32; d; d >>= 1) {
+            const float y = __shfl_xor(v, d, 64);
+            v = mx ? fmaxf(v, y) : v + y;
+        }
+        __syncthreads();
+        if (lane == 0) red[wave] = v;
+        __syncthreads();
+        v = red[0];
+        for (int i = 1; i < JT / 64; ++i) v = mx ? fmaxf(v, red[i]) : v + red[i];
+        return v;
+    };
+    float M = -INFINITY, L = 0.0f;
+    for (int i = tid; i < nseg; i += JT) M = fmaxf(M, w.part_ml[slot(i)].x);
+    M = all(M, true);
+    for (int i = tid; i < nseg; i += JT) {
+        const float2 ml = w.part_ml[slot(i)];
+        f[i] = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
+        L += ml.y * f[i];
+    }
+    L = all(L, false);
+    const int q4 = w.row / 4, ng = JT / q4, c = tid % q4, sub = tid / q4;
+    v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (sub < ng)
+        for (int i = sub; i < nseg; i += ng) {
+            const v4f x = *reinterpret_cast<const v4f *>(w.part_o + slot(i) * w.row + 4 * c);
+            const float fi = f[i];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = fi == 0.0f ? o[k] : fmaf(x[k], fi, o[k]);
+        }
+    *reinterpret_cast<v4f *>(acc + 4 * tid) = o;
+    __syncthreads();
+    const float inv = L != 0.0f ? p.v_scale / L : 0.0f;
+    for (int i = tid; i < hd; i += JT) {
+        float v = 0.0f;
+        for (int k = 0; k < ng; ++k) v += acc[k * w.row + i];
+        out[i] = v * inv;
+    }
+    if (w.ml && tid == 0) w.ml[(size_t)b * a.heads + head] = make_float2(M, L);
 }
 
 // The weights each token got, summed over a kv head's query heads.
 __global__ void k_kv_score(ornk_kv_pages p, ornk_attend_args a, AttendWs w)
 {
     const int t = blockIdx.x * blockDim.x + threadIdx.x, h = blockIdx.y, b = blockIdx.z;
-    if (t >= kv_len(p, a.lens, b, a.max_len)) return;
+    if (t >= min(max(a.lens[b], 0), a.max_len)) return;
     const int G = a.heads / p.kv;
     float sum = 0.0f;
     for (int g = 0; g < G; ++g) {
         const size_t row = (size_t)b * a.heads + h * G + g;
         const float2 ml = w.ml[row];
-        const float s = w.s[row * a.max_len + t];
-        sum += s == -INFINITY ? 0.0f : expf(s - ml.x) / ml.y;
+        const float s = w.s[row * w.s_len + t];
+        sum += s == -INFINITY ? 0.0f : exp2f(s - ml.x) / ml.y;
     }
     const size_t i = ((size_t)b * p.kv + h) * a.score_stride + t;
     a.score_out[i] = a.score_in ? fmaf(a.decay, a.score_in[i], sum) : sum;
+}
+
+size_t attend_ws(const ornk_kv_pages *p, const ornk_attend_args *a, AttendWs *w)
+{
+    size_t off = 0;
+    uint8_t *base = static_cast<uint8_t *>(a->ws);
+    auto take = [&](size_t n) {
+        uint8_t *at = base + off;
+        off += (n + 255) & ~(size_t)255;
+        return at;
+    };
+    w->W = GROUPS;
+    w->row = (p->hd + 3) & ~3;
+    w->cum = reinterpret_cast<long long *>(take(((size_t)a->n_seqs + 1) * 8));
+    w->part_ml = reinterpret_cast<float2 *>(take((size_t)2 * w->W * 16 * 8));
+    w->part_o = reinterpret_cast<float *>(take((size_t)2 * w->W * 16 * w->row * 4));
+    w->ml = nullptr;
+    w->s = nullptr;
+    w->s_len = 0;
+    if (a->score_out) {
+        const size_t rows = (size_t)a->n_seqs * a->heads;
+        w->s_len = ((size_t)a->max_len + UNIT - 1) / UNIT * UNIT;
+        w->ml = reinterpret_cast<float2 *>(take(rows * 8));
+        w->s = reinterpret_cast<float *>(take(rows * w->s_len * 4));
+    }
+    return off;
+}
+
+template <int TYPE, int HD, class Path>
+int launch_hd(const ornk_kv_pages *p, const ornk_attend_args *a, const AttendWs &w, hipStream_t s)
+{
+    // the queries as the path takes them, then O of the waves; at most 64 KB
+    const int G = a->heads / p->kv, rows = G < 16 ? G : 16;
+    size_t lds = (size_t)WAVES * rows * HD * 4;
+    if (lds < Path::Q_BYTES) lds = Path::Q_BYTES;
+    if (lds < Exact<TYPE, HD, true, true>::Q_BYTES) lds = Exact<TYPE, HD, true, true>::Q_BYTES;
+    hipLaunchKernelGGL((k_kv_attend<TYPE, HD, Path>), dim3(w.W), dim3(64 * WAVES), lds, s, *p, *a, w);
+    return hipGetLastError();
+}
+
+template <int TYPE, int HD, bool FULL>
+int launch_full(const ornk_kv_pages *p, const ornk_attend_args *a, const AttendWs &w, hipStream_t s)
+{
+    if constexpr (TYPE == ORN_KV_F32) return launch_hd<TYPE, HD, Exact<TYPE, HD, true, FULL>>(p, a, w, s);
+    else return launch_hd<TYPE, HD, Parts<TYPE, HD, FULL>>(p, a, w, s);
+}
+
+template <int TYPE, int HD>
+int launch_type(const ornk_kv_pages *p, const ornk_attend_args *a, const AttendWs &w, hipStream_t s)
+{
+    return p->hd == HD ? launch_full<TYPE, HD, true>(p, a, w, s)
+           : p->hd * elem_size<TYPE> % 16 == 0
+               ? launch_full<TYPE, HD, false>(p, a, w, s)
+               : launch_hd<TYPE, HD, Exact<TYPE, HD, false, false>>(p, a, w, s);
+}
+
+template <int TYPE>
+int launch_type(const ornk_kv_pages *p, const ornk_attend_args *a, const AttendWs &w, hipStream_t s)
+{
+    return p->hd <= 64    ? launch_type<TYPE, 64>(p, a, w, s)
+           : p->hd <= 128 ? launch_type<TYPE, 128>(p, a, w, s)
+                          : launch_type<TYPE, 256>(p, a, w, s);
 }
 
 }  // namespace
 
 extern "C" size_t ornk_kv_attend_ws(const ornk_kv_pages *p, const ornk_attend_args *a)
 {
-    if (!a->score_out) return 0;
-    const size_t rows = (size_t)a->n_seqs * a->heads;
-    return rows * 8 + rows * a->max_len * 4;
+    AttendWs w;
+    return attend_ws(p, a, &w);
 }
 
 extern "C" int ornk_kv_attend(const ornk_kv_pages *p, const ornk_attend_args *a, hipStream_t s)
 {
-    AttendWs w = {};
-    if (a->score_out) {
-        w.ml = static_cast<float2 *>(a->ws);
-        w.s = reinterpret_cast<float *>(w.ml + (size_t)a->n_seqs * a->heads);
-    }
-    const dim3 grid(a->n_seqs, a->heads), block(64 * WAVES);
-    switch (p->type) {
-    case ORN_KV_F32: hipLaunchKernelGGL(k_kv_attend<ORN_KV_F32>, grid, block, 0, s, *p, *a, w); break;
-    case ORN_KV_F16: hipLaunchKernelGGL(k_kv_attend<ORN_KV_F16>, grid, block, 0, s, *p, *a, w); break;
-    case ORN_KV_BF16: hipLaunchKernelGGL(k_kv_attend<ORN_KV_BF16>, grid, block, 0, s, *p, *a, w); break;
-    default: hipLaunchKernelGGL(k_kv_attend<ORN_KV_E4M3>, grid, block, 0, s, *p, *a, w); break;
-    }
+    AttendWs w;
+    attend_ws(p, a, &w);
+    if (a->n_seqs > 65535) return hipErrorInvalidValue;
+    int rc = p->type == ORN_KV_F32    ? launch_type<ORN_KV_F32>(p, a, w, s)
+             : p->type == ORN_KV_F16  ? launch_type<ORN_KV_F16>(p, a, w, s)
+             : p->type == ORN_KV_BF16 ? launch_type<ORN_KV_BF16>(p, a, w, s)
+                                      : launch_type<ORN_KV_E4M3>(p, a, w, s);
+    if (rc != hipSuccess) return rc;
+    hipLaunchKernelGGL(k_kv_join, dim3(a->heads, a->n_seqs), dim3(JT), 0, s, *p, *a, w);
     if (a->score_out && a->max_len)
-        hipLaunchKernelGGL(k_kv_score, dim3((a->max_len + 255) / 256, p->kv, a->n_seqs), dim3(256),
-                           0, s, *p, *a, w);
+        hipLaunchKernelGGL(k_kv_score, dim3((a->max_len + 255) / 256, p->kv, a->n_seqs), dim3(256), 0,
+                           s, *p, *a, w);
     return hipGetLastError();
 }
