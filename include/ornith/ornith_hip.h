@@ -53,7 +53,8 @@ int gpu_kv_cache_append(gpu_context *ctx, gpu_buffer *K_cache, gpu_buffer *V_cac
  * heads, and narrower cache types.
  *
  * Activations are fp32, lengths, positions, slots and page numbers int32, all
- * in buffers of the context.  Calls return 0 or a negative status, run on the
+ * in buffers of the context; a call takes up to 65535 sequences and as many
+ * heads.  Calls return 0 or a negative status, run on the
  * context's stream and are synchronous unless ORN_KV_ASYNC is given.
  *
  * Numbers in device buffers are checked by the kernels: a page number outside
@@ -82,8 +83,8 @@ typedef struct {
     int type;      /* ORN_KV_* */
     int n_pages;
     int page_size; /* a power of two, 8 to 1024; n_pages * page_size < 2^31 */
-    int n_kv_heads;
-    int head_dim;  /* 1 to 256 */
+    int n_kv_heads; /* at most 32767 */
+    int head_dim;   /* 1 to 256 */
     /* ORN_KV_E4M3: a stored value c stands for c * scale (0: 1).  Values beyond
      * 448 * scale are stored as that; a NaN stays one. */
     float k_scale, v_scale;

@@ -111,7 +111,7 @@ static int pages_ok(gpu_context *ctx, const ornith_kv_pages *kv, ornk_kv_pages *
         return orn_set_err(ctx, ORN_EUNSUPPORTED,
                            "%s: page_size %d is not a power of two from 8 to 1024", who,
                            kv->page_size);
-    if (kv->n_pages < 1 || kv->n_kv_heads < 1 || kv->n_kv_heads > 65535 ||
+    if (kv->n_pages < 1 || kv->n_kv_heads < 1 || kv->n_kv_heads > 32767 ||
         (long long)kv->n_pages * kv->page_size > 0x7fffffffll)
         return orn_set_err(ctx, ORN_EINVAL, "%s: %d pages of %d slots, %d kv heads", who,
                            kv->n_pages, kv->page_size, kv->n_kv_heads);
@@ -268,6 +268,8 @@ static int seqs_ok(gpu_context *ctx, const ornk_kv_pages *p, int n_seqs, const g
 {
     if (!table || !lens || n_seqs < 0 || max_pages < 0 || max_len < 0)
         return orn_set_err(ctx, ORN_EINVAL, "%s: bad arguments", who);
+    if (n_seqs > 65535)
+        return orn_set_err(ctx, ORN_EUNSUPPORTED, "%s: %d sequences (at most 65535)", who, n_seqs);
     const long long width = (long long)max_pages * p->page;
     if (width > 0x7fffffffll || max_len > width)
         return orn_set_err(ctx, ORN_EINVAL, "%s: max_len %d, and %d pages of %d in the table", who,

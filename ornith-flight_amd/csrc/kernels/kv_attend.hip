@@ -812,7 +812,6 @@ extern "C" int ornk_kv_attend(const ornk_kv_pages *p, const ornk_attend_args *a,
 {
     AttendWs w;
     attend_ws(p, a, &w);
-    if (a->n_seqs > 65535) return hipErrorInvalidValue;
     int rc = p->type == ORN_KV_F32    ? launch_type<ORN_KV_F32>(p, a, w, s)
              : p->type == ORN_KV_F16  ? launch_type<ORN_KV_F16>(p, a, w, s)
              : p->type == ORN_KV_BF16 ? launch_type<ORN_KV_BF16>(p, a, w, s)

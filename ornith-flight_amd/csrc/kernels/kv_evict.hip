@@ -8,7 +8,8 @@
 
 namespace {
 
-constexpr int CT = 1024;  // threads of the choosing work group
+constexpr int CT = 1024, PER = 16;  // threads of the choosing work group, scores of a thread
+constexpr int BINS = 2048;
 
 // Order of the scores as unsigned integers: a NaN is 0, -0 counts as +0.
 __device__ __forceinline__ uint32_t order_key(float f)
@@ -18,13 +19,14 @@ __device__ __forceinline__ uint32_t order_key(float f)
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// One work group per kv head and sequence.  Where the tokens are more than
-// `keep`, four rounds of eight bits find the key of the lowest score that
-// stays and how many of its equals do; a last pass numbers the kept tokens in
-// order.
+// One work group per kv head and sequence; a thread holds PER consecutive
+// scores of a stretch.  Where the tokens are more than `keep`, three rounds of
+// counting (11, 11 and 10 bits of the keys, from the top) find the lowest key
+// that stays and how many of its equals do; then one scan numbers the kept
+// tokens in order.  Longer sequences read their scores again in every round.
 __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict_args a)
 {
-    __shared__ int hist[256], wsum[CT / 64], sh[2];
+    __shared__ int hist[BINS], wsum[CT / 64], sh[2];
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int len = kv_len(p, a.lens, b, a.max_len), n = min(len, a.keep);
     const float *score = a.score + ((size_t)b * p.kv + h) * a.score_stride;
@@ -32,104 +34,183 @@ __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict
     int *kept = a.kept + ((size_t)b * p.kv + h) * a.keep;
     if (h == 0 && tid == 0) a.counts[b] = n;
     const int lo = a.sink, hi = len - a.recent;  // the tokens that the scores decide on
-    uint32_t key = 0;                            // the lowest key that stays
-    int ties = 0;                                // and how many tokens of that key
+    const bool one = len <= CT * PER;
+    float f[PER];
+    auto load = [&](int i0) {
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            const int i = i0 + PER * tid + e;
+            f[e] = i < len ? score[i] : 0.0f;
+        }
+    };
+    // the sum of the later threads' v, of the threads' of one work group
+    auto later = [&](int v) {
+        int x = v;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int y = __shfl_down(x, d, 64);
+            if (lane + d < 64) x += y;
+        }
+        if (lane == 0) wsum[wave] = x;
+        __syncthreads();
+        x -= v;
+        for (int w = wave + 1; w < CT / 64; ++w) x += wsum[w];
+        __syncthreads();
+        return x;
+    };
+
+    uint32_t key = 0;  // the lowest key that stays
+    int ties = 0;      // and how many tokens of that key
+    if (one) load(0);
     if (len > a.keep) {
         int left = a.keep - a.sink - a.recent;
-        if (left == 0) {
-            key = 0xffffffffu;  // above every key
-        } else {
-            for (int shift = 24; shift >= 0; shift -= 8) {
-                for (int i = tid; i < 256; i += CT) hist[i] = 0;
-                __syncthreads();
-                for (int i = lo + tid; i < hi; i += CT) {
-                    const uint32_t k = order_key(score[i]);
-                    if (shift == 24 || k >> (shift + 8) == key >> (shift + 8))
-                        atomicAdd(&hist[(k >> shift) & 255], 1);
+        if (left == 0) key = 0xffffffffu;  // above every key
+        for (int round = 0; round < 3 && left; ++round) {
+            const int shift = round == 0 ? 21 : round == 1 ? 10 : 0;
+            const uint32_t mask = round == 2 ? 1023u : 2047u;
+            const uint32_t fixed = round == 0 ? 0u : round == 1 ? ~0u << 21 : ~0u << 10;
+            for (int i = tid; i < BINS; i += CT) hist[i] = 0;
+            __syncthreads();
+            for (int i0 = 0; i0 < len; i0 += CT * PER) {
+                if (!one) load(i0);
+#pragma unroll
+                for (int e = 0; e < PER; ++e) {
+                    const int i = i0 + PER * tid + e;
+                    const uint32_t k = order_key(f[e]);
+                    if (i >= lo && i < hi && (k & fixed) == key) atomicAdd(&hist[(k >> shift) & mask], 1);
                 }
-                __syncthreads();
-                if (tid == 0) {
-                    int d = 255, above = 0;
-                    while (d > 0 && above + hist[d] < left) above += hist[d--];
-                    sh[0] = d;
-                    sh[1] = above;
-                }
-                __syncthreads();
-                key |= (uint32_t)sh[0] << shift;
-                left -= sh[1];
-                __syncthreads();
             }
-            ties = left;
+            __syncthreads();
+            const int c0 = hist[2 * tid], c1 = hist[2 * tid + 1];
+            const int above = later(c0 + c1);
+            if (above < left && left <= above + c1) sh[0] = 2 * tid + 1, sh[1] = above;
+            else if (above + c1 < left && left <= above + c1 + c0) sh[0] = 2 * tid, sh[1] = above + c1;
+            __syncthreads();
+            key |= (uint32_t)sh[0] << shift;
+            left -= sh[1];
+            __syncthreads();
         }
+        ties = left;
     }
     int base = 0, eq_base = 0;  // kept for certain, and ties, before this stretch
-    for (int i0 = 0; i0 < len; i0 += CT) {
-        const int i = i0 + tid;
-        const float f = i < len ? score[i] : 0.0f;
-        bool sure = false, tie = false;
-        if (i < len) {
-            const uint32_t k = order_key(f);
-            sure = len <= a.keep || i < lo || i >= hi || k > key;
-            tie = !sure && ties && k == key;
+    for (int i0 = 0; i0 < len; i0 += CT * PER) {
+        if (!one) load(i0);
+        uint32_t sure = 0, tie = 0;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            const int i = i0 + PER * tid + e;
+            if (i >= len) continue;
+            const uint32_t k = order_key(f[e]);
+            if (len <= a.keep || i < lo || i >= hi || k > key) sure |= 1u << e;
+            else if (k == key) tie |= 1u << e;
         }
-        const uint64_t bs = __ballot(sure), bt = __ballot(tie);
-        if (lane == 0) wsum[wave] = __popcll(bs) | __popcll(bt) << 16;
-        __syncthreads();
-        int before = 0, all = 0;
-        for (int w = 0; w < CT / 64; ++w) {
-            if (w < wave) before += wsum[w];
-            all += wsum[w];
+        // both counts in one word: a stretch has CT * PER = 2^14 tokens
+        const int mine = __popc(sure) | __popc(tie) << 16;
+        const int after = later(mine);
+        if (tid == 0) sh[0] = mine + after;
+        __syncthreads();  // also: every score of this stretch has been read
+        const int before = sh[0] - after - mine;
+        int at = base + (before & 0xffff), eq = eq_base + (before >> 16);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            const bool t = tie >> e & 1;
+            if ((sure >> e & 1) || (t && eq < ties)) {
+                const int j = at + min(eq, ties);
+                kept[j] = i0 + PER * tid + e;
+                if (ds) ds[j] = f[e];
+                at += sure >> e & 1;
+            }
+            eq += t;
         }
-        const uint64_t mask = ((uint64_t)1 << lane) - 1;
-        const int eq = eq_base + (before >> 16) + __popcll(bt & mask);
-        const int at = base + (before & 0xffff) + __popcll(bs & mask) + min(eq, ties);
-        // every score of this stretch has been read: an earlier place may be written
-        if (sure || (tie && eq < ties)) {
-            kept[at] = i;
-            if (ds) ds[at] = f;
-        }
-        base += all & 0xffff;
-        eq_base += all >> 16;
+        base += sh[0] & 0xffff;
+        eq_base += sh[0] >> 16;
         __syncthreads();
     }
     for (int i = n + tid; i < a.keep; i += CT) kept[i] = -1;
 }
 
-// One work group per kv head, sequence and K or V.  Within a sequence's own
-// pages a row moves towards the front or stays, so a stretch of rows is read
-// before any of it is written and nothing that a later stretch reads is.
-__global__ void __launch_bounds__(256) k_evict_move(ornk_kv_pages p, ornk_evict_args a, int row_bytes)
+// The kept rows to their new places, in words of WORD bytes.  A work group takes
+// rows of one kv head, sequence and K or V, MR at a time: their addresses go
+// through LDS, then every thread copies its words.
+//
+// Into other pages, each group takes one stretch of MR rows whole.  Within a
+// sequence's own pages (IN_PLACE) a row moves towards the front or stays: a
+// group takes every row, one stretch after the other, of SLICE bytes of the
+// columns; a stretch is read whole before any of it is written, and no later
+// stretch reads what it writes.
+constexpr int MT = 256, MR = 64, SLICE = 64;
+
+template <class WORD, bool IN_PLACE>
+__global__ void __launch_bounds__(MT) k_evict_move(ornk_kv_pages p, ornk_evict_args a, int row_bytes)
 {
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+    __shared__ const uint8_t *from[MR];
+    __shared__ uint8_t *to[MR];
+    constexpr int WB = sizeof(WORD), NW = IN_PLACE ? MR * (SLICE / WB) / MT : 4;
+    const int h = blockIdx.y % p.kv, b = blockIdx.z, tid = threadIdx.x;
     const int n = a.counts[b];
     const int *kept = a.kept + ((size_t)b * p.kv + h) * a.keep;
-    uint8_t *pool = static_cast<uint8_t *>(blockIdx.z ? p.v : p.k);
-    if (h == 0 && blockIdx.z == 0 && tid == 0) a.dst_lens[b] = n;
-    const size_t es = row_bytes / p.hd;
-    auto row = [&](const int *table, int pages, int i) {
-        const int page = kv_page(p, table[(size_t)b * pages + (i >> p.page_log2)], b);
-        return page < 0 ? nullptr : pool + kv_at(p, page, h, i & (p.page - 1)) * es;
-    };
-    for (int j = 0; j < n; ++j) {
-        const uint8_t *from = row(a.table, a.max_pages, kept[j]);
-        uint8_t *to = row(a.dst_table, a.dst_pages, j);
-        uint8_t v[4];
-        if (from && to)
-            for (int i = tid, k = 0; i < row_bytes; i += 256, ++k) v[k] = from[i];
+    uint8_t *pool = static_cast<uint8_t *>(blockIdx.y >= p.kv ? p.v : p.k);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) a.dst_lens[b] = n;
+    const int es = row_bytes / p.hd;
+    const int c0 = IN_PLACE ? blockIdx.x * SLICE : 0;
+    const int words = (IN_PLACE ? min(SLICE, row_bytes - c0) : row_bytes) / WB;
+    for (int j0 = IN_PLACE ? 0 : blockIdx.x * MR; j0 < n; j0 += MR) {
+        const int rows = min(MR, n - j0);
+        if (tid < rows) {
+            const int j = j0 + tid, i = kept[j];
+            const int pf = kv_page(p, a.table[(size_t)b * a.max_pages + (i >> p.page_log2)], b);
+            const int pt = kv_page(p, a.dst_table[(size_t)b * a.dst_pages + (j >> p.page_log2)], b);
+            const bool on = pf >= 0 && pt >= 0 && !(IN_PLACE && i == j);
+            from[tid] = on ? pool + kv_at(p, pf, h, i & (p.page - 1)) * es + c0 : nullptr;
+            to[tid] = on ? pool + kv_at(p, pt, h, j & (p.page - 1)) * es + c0 : nullptr;
+        }
         __syncthreads();
-        if (from && to)
-            for (int i = tid, k = 0; i < row_bytes; i += 256, ++k) to[i] = v[k];
+        for (int w0 = 0; w0 < rows * words; w0 += NW * MT) {
+            WORD v[NW];
+#pragma unroll
+            for (int k = 0; k < NW; ++k) {
+                const int w = w0 + k * MT + tid, r = w / words;
+                if (w < rows * words && from[r])
+                    v[k] = *reinterpret_cast<const WORD *>(from[r] + (size_t)(w - r * words) * WB);
+            }
+            if (IN_PLACE) {  // one pass: NW * MT words hold a stretch
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();
+            }
+#pragma unroll
+            for (int k = 0; k < NW; ++k) {
+                const int w = w0 + k * MT + tid, r = w / words;
+                if (w < rows * words && to[r])
+                    *reinterpret_cast<WORD *>(to[r] + (size_t)(w - r * words) * WB) = v[k];
+            }
+        }
+        if (!IN_PLACE) break;
         __syncthreads();
     }
+}
+
+template <class WORD>
+void move(const ornk_kv_pages &p, const ornk_evict_args &a, int row_bytes, hipStream_t s)
+{
+    const int most = a.keep < a.max_len ? a.keep : a.max_len;
+    const unsigned y = 2 * p.kv, z = a.n_seqs;
+    if (a.in_place)
+        hipLaunchKernelGGL((k_evict_move<WORD, true>), dim3((row_bytes + SLICE - 1) / SLICE, y, z),
+                           dim3(MT), 0, s, p, a, row_bytes);
+    else
+        hipLaunchKernelGGL((k_evict_move<WORD, false>), dim3(most ? (most + MR - 1) / MR : 1, y, z),
+                           dim3(MT), 0, s, p, a, row_bytes);
 }
 
 }  // namespace
 
 extern "C" int ornk_kv_evict(const ornk_kv_pages *p, const ornk_evict_args *a, hipStream_t s)
 {
-    if (a->n_seqs > 65535) return hipErrorInvalidValue;
-    const int es = p->type == ORN_KV_F32 ? 4 : p->type == ORN_KV_E4M3 ? 1 : 2;
+    const int rb = p->hd * (p->type == ORN_KV_F32 ? 4 : p->type == ORN_KV_E4M3 ? 1 : 2);
     hipLaunchKernelGGL(k_evict_choose, dim3(p->kv, a->n_seqs), dim3(CT), 0, s, *p, *a);
-    hipLaunchKernelGGL(k_evict_move, dim3(p->kv, a->n_seqs, 2), dim3(256), 0, s, *p, *a, es * p->hd);
+    if (rb % 16 == 0) move<uint4>(*p, *a, rb, s);
+    else if (rb % 4 == 0) move<uint32_t>(*p, *a, rb, s);
+    else if (rb % 2 == 0) move<uint16_t>(*p, *a, rb, s);
+    else move<uint8_t>(*p, *a, rb, s);
     return hipGetLastError();
 }
