@@ -107,8 +107,9 @@ typedef struct {
 } ornith_rope_axes;
 
 /* q_out = Q [n_tokens][n_heads][head_dim] and k_out = K [n_tokens]
- * [n_kv_heads][head_dim] rotated; positions [n_axes][n_tokens].  Angles are
- * formed in 64 bits, so that far positions keep their digits.  q_out may be Q
+ * [n_kv_heads][head_dim] rotated (head_dim up to 4096); positions
+ * [n_axes][n_tokens].  Angles are formed in 64 bits, so that far positions keep
+ * their digits.  q_out may be Q
  * and k_out may be K; a pair of NULLs with 0 heads leaves one side out. */
 int gpu_rope_axes(gpu_context *ctx, gpu_buffer *q_out, gpu_buffer *k_out, const gpu_buffer *Q,
                   const gpu_buffer *K, int n_tokens, int n_heads, int n_kv_heads, int head_dim,

@@ -189,6 +189,8 @@ int gpu_rope_axes(gpu_context *ctx, gpu_buffer *q_out, gpu_buffer *k_out, const 
         n_kv_heads > 65535 || head_dim < 1 || !Q != !n_heads || !q_out != !n_heads ||
         !K != !n_kv_heads || !k_out != !n_kv_heads)
         return orn_set_err(ctx, ORN_EINVAL, "%s: bad arguments", who);
+    if (head_dim > 4096)
+        return orn_set_err(ctx, ORN_EUNSUPPORTED, "%s: head_dim %d > 4096", who, head_dim);
     ornk_rope_args a;
     memset(&a, 0, sizeof a);
     int rc = rope_ok(ctx, rope, head_dim, &a, who);

@@ -73,3 +73,12 @@ __device__ __forceinline__ size_t kv_at(const ornk_kv_pages &p, int page, int h,
 {
     return ((((size_t)page * p.kv + h) << p.page_log2) + i) * p.hd;
 }
+
+// Token t's slot, -1 where it is not stored.
+__device__ __forceinline__ int kv_slot(const ornk_kv_pages &p, const int *slots, int t)
+{
+    const int slot = slots[t];
+    if (slot >= 0 && slot < p.n_pages * p.page) return slot;
+    if (slot != -1) kv_error(p, ORNK_KV_ERR_SLOT, t);
+    return -1;
+}
