@@ -115,6 +115,8 @@ static int pages_ok(gpu_context *ctx, const ornith_kv_pages *kv, ornk_kv_pages *
         (long long)kv->n_pages * kv->page_size > 0x7fffffffll)
         return orn_set_err(ctx, ORN_EINVAL, "%s: %d pages of %d slots, %d kv heads", who,
                            kv->n_pages, kv->page_size, kv->n_kv_heads);
+    if (span(kv->n_kv_heads, kv->page_size, kv->head_dim, 1, elem_bytes(kv->type)) > UINT32_MAX)
+        return orn_set_err(ctx, ORN_EUNSUPPORTED, "%s: a page of 4 GB or more", who);
     const size_t n = span(kv->n_pages, kv->n_kv_heads, kv->page_size, kv->head_dim,
                           elem_bytes(kv->type));
     if (!holds(kv->K, n) || !holds(kv->V, n))

@@ -19,7 +19,11 @@ typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int WAVES = 4, UNIT = 128;  // waves of a work group, tokens of a unit
-constexpr int GROUPS = 512;           // work groups: two per CU
+// Work groups per CU: the registers of 256 columns (K, V and O of a tile, 64
+// each, beside their addresses) leave room for one wave per SIMD.
+template <int HD>
+constexpr int per_cu = HD == 256 ? 1 : 2;
+constexpr int CUS = 256, GROUPS = 2 * CUS;  // the most that are launched
 
 struct AttendWs {
     long long *cum;  // [n_seqs + 1] units before each sequence, per pair of it
@@ -42,6 +46,9 @@ struct Seg {  // part of one pair
     int len, k0, k1;     // the sequence's tokens; this part's
     size_t score;        // first score of query head j0
 };
+
+// 2^x (results below 2^-126: zero)
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 __device__ __forceinline__ uint32_t top16(float hi, float lo)
 {
@@ -145,10 +152,11 @@ struct Exact {
 #pragma unroll
             for (int j = 0; j < NV; ++j) load4(v[r][j], row[r], 64 * j + 4 * n, hd);
     }
-    static __device__ void put_q(void *lds, int n, int d, float q)
+    // dimensions d .. d + 3 of query n: [16 j][n][4 g + i], so that a lane's four
+    // steps are one word
+    static __device__ __forceinline__ void put_q(void *lds, int n, int d, v4f q)
     {
-        // [16 j][n][4 g + i]: a lane's four steps are one word
-        static_cast<float *>(lds)[(d / 16) * 256 + n * 16 + d % 16] = q;
+        *reinterpret_cast<v4f *>(static_cast<float *>(lds) + (d / 16) * 256 + n * 16 + d % 16) = q;
     }
     __device__ __forceinline__ void scores(float *s, const void *lds, int lane) const
     {
@@ -166,17 +174,16 @@ struct Exact {
         for (int r = 0; r < 4; ++r) s[r] = acc[r];
     }
     // A key that is left out has the weight 0, and 0 times an infinity is none:
-    // its values count as zeros.
-    __device__ __forceinline__ void pv(v4f *o, const float *p, const bool *on)
+    // its values count as zeros.  (Parts: such a segment comes to Exact.)
+    __device__ __forceinline__ void leave_out(int r)
     {
-        if (__any(!(on[0] && on[1] && on[2] && on[3]))) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+        for (int j = 0; j < NV; ++j)
 #pragma unroll
-                for (int j = 0; j < NV; ++j)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[r][j][i] = on[r] ? v[r][j][i] : 0.0f;
-        }
+            for (int i = 0; i < 4; ++i) v[r][j][i] = 0.0f;
+    }
+    __device__ __forceinline__ void pv(v4f *o, const float *p) const
+    {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -235,16 +242,17 @@ struct Parts {
                 load_words<4 * VW>(v[r][j], row[r] + (FULL || c < hd ? c : 0) * ES);
             }
     }
-    // [part][step][lane][8]; dimension d of the queries
-    static __device__ void put_q(void *lds, int n, int d, float q)
+    // dimensions d .. d + 3 of query n: [part][step][lane][8]
+    static __device__ __forceinline__ void put_q(void *lds, int n, int d, v4f q)
     {
         const int j = d / (4 * DL), g = d / DL % 4, e = d % DL;
         const int step = j * (DL / 8) + e / 8;
-        uint16_t *at = static_cast<uint16_t *>(lds) + ((step * 64 + 16 * g + n) * 8 + e % 8);
+        uint8_t *at = static_cast<uint8_t *>(lds) + (step * 64 + 16 * g + n) * 16 + e % 8 * 2;
 #pragma unroll
         for (int part = 0; part < 3; ++part) {
-            at[part * NS * 512] = (uint16_t)(__float_as_uint(q) >> 16);
-            q = rest16(q);
+            *reinterpret_cast<uint2 *>(at + part * NS * 1024) = make_uint2(top16(q[1], q[0]), top16(q[3], q[2]));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[i] = rest16(q[i]);
         }
     }
     // operand of step `st`, keys of half i
@@ -306,7 +314,8 @@ struct Parts {
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[r] = a0[r], s[4 + r] = a1[r];
     }
-    __device__ __forceinline__ void pv(v4f *o, const float *p, const bool *)
+    __device__ __forceinline__ void leave_out(int) {}
+    __device__ __forceinline__ void pv(v4f *o, const float *p) const
     {
         v8b pp[3];
         {
@@ -327,17 +336,25 @@ struct Parts {
         for (int j = 0; j < NH; ++j) {
             if constexpr (TYPE == ORN_KV_BF16) {
 #pragma unroll
-                for (int c = 0; c < CW; ++c) {
-                    u4 w;
+                for (int c = 0; c < CW; c += 4) {
+                    v8b b[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        w[e] = __builtin_amdgcn_perm(v[2 * e + 1][j][c / 2], v[2 * e][j][c / 2],
-                                                     c % 2 ? 0x07060302u : 0x05040100u);
-                    const v8b b = as_v8b(w);
-                    v4f &x = o[j * CW + c];
-                    x = mma(pp[2], b, x);
-                    x = mma(pp[1], b, x);
-                    x = mma(pp[0], b, x);
+                    for (int i = 0; i < 4; ++i) {
+                        u4 w;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            w[e] = __builtin_amdgcn_perm(v[2 * e + 1][j][(c + i) / 2],
+                                                         v[2 * e][j][(c + i) / 2],
+                                                         i % 2 ? 0x07060302u : 0x05040100u);
+                        b[i] = as_v8b(w);
+                    }
+#pragma unroll
+                    for (int part = 2; part >= 0; --part)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            v4f &x = o[j * CW + c + i];
+                            x = mma(pp[part], b[i], x);
+                        }
                 }
             } else {
 #pragma unroll
@@ -345,22 +362,30 @@ struct Parts {
                     float f[8][4];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) unpack4<TYPE>(f[e], &v[e][j][c * ES / 4]);
+                    v8b hi[4], lo[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        u4 hi, lo;
+                        u4 w;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            hi[e] = top16(f[2 * e + 1][i], f[2 * e][i]);
-                            if constexpr (NP == 2)
-                                lo[e] = top16(rest16(f[2 * e + 1][i]), rest16(f[2 * e][i]));
+                        for (int e = 0; e < 4; ++e) w[e] = top16(f[2 * e + 1][i], f[2 * e][i]);
+                        hi[i] = as_v8b(w);
+                        if constexpr (NP == 2) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                w[e] = top16(rest16(f[2 * e + 1][i]), rest16(f[2 * e][i]));
+                            lo[i] = as_v8b(w);
                         }
-                        v4f &x = o[j * CW + c + i];
-                        x = mma(pp[2], as_v8b(hi), x);
-                        if constexpr (NP == 2) x = mma(pp[1], as_v8b(lo), x);
-                        x = mma(pp[1], as_v8b(hi), x);
-                        if constexpr (NP == 2) x = mma(pp[0], as_v8b(lo), x);
-                        x = mma(pp[0], as_v8b(hi), x);
                     }
+                    v4f *x = o + j * CW + c;
+                    auto add = [&](int part, const v8b *b) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) x[i] = mma(pp[part], b[i], x[i]);
+                    };
+                    add(2, hi);
+                    if constexpr (NP == 2) add(1, lo);
+                    add(1, hi);
+                    if constexpr (NP == 2) add(0, lo);
+                    add(0, hi);
                 }
             }
         }
@@ -375,97 +400,108 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
 {
     constexpr int KT = Path::KT, NI = KT / 16, NO = Path::NO, ES = elem_size<TYPE>;
     __shared__ float sm[WAVES][16], sl[WAVES][16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, n = lane & 15;
-    const int hd = p.hd;
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, n = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int hd = p.hd, len = sg.len;
 
-    // the query heads, scaled; those past the last are zeros
-    __syncthreads();
-    {
-        const float f = a.scale * p.k_scale * 1.44269504088896341f;
-        const float *q = a.q + ((size_t)sg.b * a.heads + sg.j0) * hd;
-        for (int i = tid; i < 16 * HD; i += 64 * WAVES) {
-            const int row = i / HD, d = i % HD;
-            Path::put_q(lds, row, d, row < sg.rows && d < hd ? q[(size_t)row * hd + d] * f : 0.0f);
-        }
-    }
-    __syncthreads();
-
+    // Pages: lane i holds the page of place page0 + i of the table.  A tile's
+    // tokens are in places of one such 64 (their first is a multiple of KT).
     const int *table = a.table + (size_t)sg.b * a.max_pages;
-    const uint8_t *kp = static_cast<const uint8_t *>(p.k), *vp = static_cast<const uint8_t *>(p.v);
-    const int last_page = (sg.len - 1) >> p.page_log2;
-    int page0 = -64, ids = -1;  // lane i holds the page of place page0 + i
-    const int row_bytes = hd * ES;
-    // the row of token t < sg.len, through its page (page 0 for one that is none)
-    auto place = [&](int t, bool &on) {
-        const int id = __shfl(ids, (t >> p.page_log2) - page0, 64);
-        on = id >= 0;
-        return kv_at(p, id < 0 ? 0 : id, sg.h, t & (p.page - 1)) * ES;
-    };
+    const uint32_t row_bytes = hd * ES, page_bytes = (row_bytes << p.page_log2) * p.kv;
+    const size_t head = (size_t)(row_bytes << p.page_log2) * sg.h;
+    const uint8_t *kp = static_cast<const uint8_t *>(p.k) + head;
+    const uint8_t *vp = static_cast<const uint8_t *>(p.v) + head;
+    int page0 = -1, ids = 0;
     auto pages_for = [&](int t) {
         const int want = (t >> p.page_log2) & ~63;
         if (want == page0) return;
         page0 = want;
         const int i = want + lane;
-        ids = i <= last_page ? kv_page(p, table[i], sg.b) : -1;
+        ids = i <= (len - 1) >> p.page_log2 ? kv_page(p, table[i], sg.b) : -1;
+    };
+    // the row of token t, through its page (page 0 for one that is none)
+    auto place = [&](const uint8_t *base, int t, bool &ok) {
+        const int id = __builtin_amdgcn_ds_bpermute(4 * ((t >> p.page_log2) & 63), ids);
+        ok = id >= 0;
+        return base + (size_t)(uint32_t)max(id, 0) * page_bytes + (uint32_t)(t & (p.page - 1)) * row_bytes;
     };
 
     Path x;
-    v4f o[NO];
-#pragma unroll
-    for (int c = 0; c < NO; ++c) o[c] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -INFINITY, l = 0.0f;
-    bool von[4 * NI];  // whether this lane's keys count
-    auto load_k = [&](int t) {  // rows past the sequence's last: that one again
+    bool ok[NI];  // whether this lane's four tokens of each 16 have a page
+    auto load_k = [&](int t) {  // past the sequence's last token: that one again
         const uint8_t *row[NI];
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            bool on;
-            row[i] = kp + place(min(t + 16 * i + n, sg.len - 1), on);
+            bool any;
+            row[i] = place(kp, min(t + 16 * i + n, len - 1), any);
         }
         x.load_k(row, g, hd);
+        __builtin_amdgcn_sched_barrier(0);
     };
     auto load_v = [&](int t) {
         const uint8_t *row[4 * NI];
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const int t0 = t + 16 * i + 4 * g, at = min(t0, (sg.len - 1) & ~3);  // four of one page
-            bool on;
-            const uint8_t *first = vp + place(at, on);
+            const int at = min(t + 16 * i + 4 * g, (len - 1) & ~3);  // four of one page
+            const uint8_t *first = place(vp, at, ok[i]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                row[4 * i + r] = first + min(r, sg.len - 1 - at) * row_bytes;
-                von[4 * i + r] = on && t0 + r < sg.len;
-            }
+            for (int r = 0; r < 4; ++r) row[4 * i + r] = first + (uint32_t)min(r, len - 1 - at) * row_bytes;
         }
         x.load_v(row, n, hd);
+        __builtin_amdgcn_sched_barrier(0);
     };
 
+    // On their way together: the table, the queries, then the first K and V.
     int t = sg.k0 + KT * wave;
+    if (t < sg.k1) pages_for(t);
+    v4f q[HD / 64];
+    {
+        const float *src = a.q + ((size_t)sg.b * a.heads + sg.j0) * hd;
+#pragma unroll
+        for (int i = 0; i < HD / 64; ++i) {
+            const int at = tid + 64 * WAVES * i, row = at / (HD / 4), d = at % (HD / 4) * 4;
+            q[i] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};  // of heads past the last too
+            if (row >= sg.rows) continue;
+            if (hd % 4 == 0) {
+                if (d < hd) q[i] = *reinterpret_cast<const v4f *>(src + (size_t)row * hd + d);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (d + e < hd) q[i][e] = src[(size_t)row * hd + d + e];
+            }
+        }
+    }
     if (Path::ahead && t < sg.k1) {
-        pages_for(t);
         load_k(t);
         load_v(t);
     }
-    for (; t < sg.k1; t += KT * WAVES) {
-        asm volatile("" ::: "memory");  // the queries are read from LDS in every tile
-        if (!Path::ahead) {
-            pages_for(t);
-            load_k(t);
-            load_v(t);
-        }
-        float s[4 * NI];
-        x.scores(s, lds, lane);
-        const int nt = t + KT * WAVES;
-        const bool more = Path::ahead && nt < sg.k1;
-        if (more) {
-            pages_for(nt);
-            load_k(nt);
-        }
-        float tm = -INFINITY;
+    __syncthreads();  // what the last segment left in LDS is consumed
 #pragma unroll
-        for (int i = 0; i < 4 * NI; ++i) {
-            s[i] = von[i] ? s[i] : -INFINITY;
-            tm = fmaxf(tm, s[i]);
+    for (int i = 0; i < HD / 64; ++i) {
+        const int at = tid + 64 * WAVES * i;
+        Path::put_q(lds, at / (HD / 4), at % (HD / 4) * 4, q[i] * (a.scale * p.k_scale * 1.44269504088896341f));
+    }
+    __syncthreads();
+
+    v4f o[NO];
+#pragma unroll
+    for (int c = 0; c < NO; ++c) o[c] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+    float s[4 * NI];
+    // the softmax of a tile's scores, and its O
+    auto rest = [&](int t) {
+        bool all = t + KT <= len;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) all = all && ok[i];
+        if (__any(!all)) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (!ok[i] || t + 16 * i + 4 * g + r >= len) {
+                        s[4 * i + r] = -INFINITY;
+                        x.leave_out(4 * i + r);
+                    }
         }
         if (w.s && n < sg.rows) {
 #pragma unroll
@@ -474,13 +510,16 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
                 *reinterpret_cast<v4f *>(w.s + sg.score + n * w.s_len + t + 16 * i + 4 * g) = v;
             }
         }
+        float tm = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4 * NI; ++i) tm = fmaxf(tm, s[i]);
         tm = fmaxf(tm, __shfl_xor(tm, 16, 64));
         tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
         // the reference moves only when the maximum has passed it by a factor
         // of 2^6 (weights up to that stay): O is left alone in most tiles
         const float mn = tm > m + 6.0f ? tm : m;
         if (__any(mn != m)) {
-            const float corr = mn == -INFINITY ? 1.0f : exp2f(m - mn);
+            const float corr = mn == -INFINITY ? 1.0f : exp2_(m - mn);
             l *= corr;
             float cr[4];
 #pragma unroll
@@ -493,11 +532,34 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
         }
 #pragma unroll
         for (int i = 0; i < 4 * NI; ++i) {
-            s[i] = mn == -INFINITY ? 0.0f : exp2f(s[i] - mn);
+            s[i] = mn == -INFINITY ? 0.0f : exp2_(s[i] - mn);
             l += s[i];
         }
-        x.pv(o, s, von);
-        if (more) load_v(nt);
+        x.pv(o, s);
+    };
+    if constexpr (Path::ahead) {
+        // the next tile's K is on its way from the scores on, its V from O on
+        if (t < sg.k1) {
+            for (; t + KT * WAVES < sg.k1; t += KT * WAVES) {
+                asm volatile("" ::: "memory");  // the queries are read from LDS in every tile
+                x.scores(s, lds, lane);
+                pages_for(t + KT * WAVES);
+                load_k(t + KT * WAVES);
+                rest(t);
+                load_v(t + KT * WAVES);
+            }
+            x.scores(s, lds, lane);
+            rest(t);
+        }
+    } else {
+        for (; t < sg.k1; t += KT * WAVES) {
+            asm volatile("" ::: "memory");
+            pages_for(t);
+            load_k(t);
+            load_v(t);
+            x.scores(s, lds, lane);
+            rest(t);
+        }
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
@@ -537,7 +599,7 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
         v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int v = 0; v < WAVES; ++v) {
-            const float f = sm[v][row] == -INFINITY ? 0.0f : exp2f(sm[v][row] - M);
+            const float f = sm[v][row] == -INFINITY ? 0.0f : exp2_(sm[v][row] - M);
             // (a wave without tokens: zeros, and its factor)
             L += sl[v][row] * f;
             const v4f x4 = *reinterpret_cast<const v4f *>(ob + ((size_t)v * sg.rows + row) * HD + c);
@@ -595,7 +657,7 @@ __device__ long long scan_lens(const ornk_kv_pages &p, const ornk_attend_args &a
 }
 
 template <int TYPE, int HD, class Path>
-__global__ void __launch_bounds__(64 * WAVES, 2) k_kv_attend(ornk_kv_pages p, ornk_attend_args a,
+__global__ void __launch_bounds__(64 * WAVES, per_cu<HD>) k_kv_attend(ornk_kv_pages p, ornk_attend_args a,
                                                              AttendWs w)
 {
     extern __shared__ __align__(16) uint8_t lds[];
@@ -697,7 +759,7 @@ __global__ void __launch_bounds__(JT) k_kv_join(ornk_kv_pages p, ornk_attend_arg
     M = all(M, true);
     for (int i = tid; i < nseg; i += JT) {
         const float2 ml = w.part_ml[slot(i)];
-        f[i] = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
+        f[i] = ml.x == -INFINITY ? 0.0f : exp2_(ml.x - M);
         L += ml.y * f[i];
     }
     L = all(L, false);
@@ -732,7 +794,7 @@ __global__ void k_kv_score(ornk_kv_pages p, ornk_attend_args a, AttendWs w)
         const size_t row = (size_t)b * a.heads + h * G + g;
         const float2 ml = w.ml[row];
         const float s = w.s[row * w.s_len + t];
-        sum += s == -INFINITY ? 0.0f : exp2f(s - ml.x) / ml.y;
+        sum += s == -INFINITY ? 0.0f : exp2_(s - ml.x) / ml.y;
     }
     const size_t i = ((size_t)b * p.kv + h) * a.score_stride + t;
     a.score_out[i] = a.score_in ? fmaf(a.decay, a.score_in[i], sum) : sum;
@@ -747,7 +809,7 @@ size_t attend_ws(const ornk_kv_pages *p, const ornk_attend_args *a, AttendWs *w)
         off += (n + 255) & ~(size_t)255;
         return at;
     };
-    w->W = GROUPS;
+    w->W = p->hd > 128 ? per_cu<256> * CUS : GROUPS;
     w->row = (p->hd + 3) & ~3;
     w->cum = reinterpret_cast<long long *>(take(((size_t)a->n_seqs + 1) * 8));
     w->part_ml = reinterpret_cast<float2 *>(take((size_t)2 * w->W * 16 * 8));
