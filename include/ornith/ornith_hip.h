@@ -130,7 +130,9 @@ int gpu_kv_append(gpu_context *ctx, const ornith_kv_pages *kv, const gpu_buffer 
  * [n_seqs][n_heads][head_dim], over the first lens[b] tokens of its row of the
  * table, w = softmax(scale * q.k); n_heads is a multiple of n_kv_heads, head j
  * reads kv head j / (n_heads / n_kv_heads).  A sequence of length 0 (a row of a
- * padded batch) gives zeros.  out is not Q.
+ * padded batch) gives zeros.  out is not Q.  n_seqs * n_kv_heads, times
+ * ceil(n_heads / n_kv_heads / 16), is at most 2^21.  The arithmetic is that of
+ * 32 bits whatever the cache's type, infinities and NaN included.
  *
  * score_out (may be NULL) [n_seqs][n_kv_heads][score_stride]: for the tokens
  * t < lens[b], decay * score_in[b][h][t] (score_in NULL: 0) + the sum of w over

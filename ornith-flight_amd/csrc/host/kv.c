@@ -299,6 +299,8 @@ int gpu_kv_attend(gpu_context *ctx, const ornith_kv_pages *kv, gpu_buffer *out,
     if (!out || !Q || n_heads < 1 || n_heads > 65535 || n_heads % p.kv)
         return orn_set_err(ctx, ORN_EINVAL, "%s: bad arguments, or %d heads over %d kv heads", who,
                            n_heads, p.kv);
+    if ((size_t)n_seqs * p.kv * ((n_heads / p.kv + 15) / 16) > 1 << 21)
+        return orn_set_err(ctx, ORN_EUNSUPPORTED, "%s: %d sequences of %d kv heads", who, n_seqs, p.kv);
     if (!isfinite(o->scale)) return orn_set_err(ctx, ORN_EINVAL, "%s: scale", who);
     const size_t nq = span(n_seqs, n_heads, p.hd, 1, 4);
     if (!holds(Q, nq) || !holds(out, nq))

@@ -18,27 +18,35 @@ namespace {
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr int WAVES = 4, UNIT = 128;  // waves of a work group, tokens of a unit
+constexpr int WAVES = 4;
+// log2 of a unit's tokens: four tiles, or as many more as keep the line below
+// 2^22 units (32-bit products with a group's number).
+constexpr int UNIT_LOG2 = 7, LINE_LOG2 = 22;
 // Work groups per CU: the registers of 256 columns (K, V and O of a tile, 64
 // each, beside their addresses) leave room for one wave per SIMD.
 template <int HD>
 constexpr int per_cu = HD == 256 ? 1 : 2;
-constexpr int CUS = 256, GROUPS = 2 * CUS;  // the most that are launched
+constexpr int CUS_LOG2 = 8;
 
 struct AttendWs {
-    long long *cum;  // [n_seqs + 1] units before each sequence, per pair of it
+    uint32_t *cum;   // [n_seqs + 1] units before each sequence, per pair of it
     float2 *part_ml; // [2 W][16] of the parts: a group's first stretch, its last
     float *part_o;   // [2 W][16][row]
-    int W, row;      // groups launched; floats of a row of part_o
+    int w_log2, row, unit_log2;  // W; floats of a row of part_o; a unit
     float2 *ml;      // [n_seqs][heads] and scores [n_seqs][heads][s_len], for the weights
     float *s;
     size_t s_len;
 };
 
-// The line of units: `first` of a group's stretch.
-__device__ __forceinline__ long long line_at(long long T, int W, int w)
+// The line of T units: the first of group w's stretch, and the group of unit u.
+// A line shorter than the groups gives one unit to each of the first T.
+__device__ __forceinline__ uint32_t line_at(uint32_t T, int w_log2, uint32_t w)
 {
-    return T * w / W;
+    return T >> w_log2 ? T * w >> w_log2 : min(w, T);
+}
+__device__ __forceinline__ uint32_t line_group(uint32_t T, int w_log2, uint32_t u)
+{
+    return T >> w_log2 ? (((u + 1) << w_log2) - 1) / T : u;
 }
 
 struct Seg {  // part of one pair
@@ -49,6 +57,10 @@ struct Seg {  // part of one pair
 
 // 2^x (results below 2^-126: zero)
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The factor of sums relative to m in sums relative to M >= m: 1 also where
+// both are -inf (no weight yet; but a NaN's sum is one).
+__device__ __forceinline__ float weight_from(float m, float M) { return m == M ? 1.0f : exp2_(m - M); }
 
 __device__ __forceinline__ uint32_t top16(float hi, float lo)
 {
@@ -519,7 +531,7 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
         // of 2^6 (weights up to that stay): O is left alone in most tiles
         const float mn = tm > m + 6.0f ? tm : m;
         if (__any(mn != m)) {
-            const float corr = mn == -INFINITY ? 1.0f : exp2_(m - mn);
+            const float corr = weight_from(m, mn);
             l *= corr;
             float cr[4];
 #pragma unroll
@@ -532,7 +544,7 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
         }
 #pragma unroll
         for (int i = 0; i < 4 * NI; ++i) {
-            s[i] = mn == -INFINITY ? 0.0f : exp2_(s[i] - mn);
+            s[i] = s[i] == -INFINITY ? 0.0f : exp2_(s[i] - mn);
             l += s[i];
         }
         x.pv(o, s);
@@ -599,12 +611,11 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
         v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int v = 0; v < WAVES; ++v) {
-            const float f = sm[v][row] == -INFINITY ? 0.0f : exp2_(sm[v][row] - M);
-            // (a wave without tokens: zeros, and its factor)
+            const float f = weight_from(sm[v][row], M);  // (a wave without tokens holds zeros)
             L += sl[v][row] * f;
             const v4f x4 = *reinterpret_cast<const v4f *>(ob + ((size_t)v * sg.rows + row) * HD + c);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] = sm[v][row] == -INFINITY ? acc[e] : fmaf(x4[e], f, acc[e]);
+            for (int e = 0; e < 4; ++e) acc[e] = fmaf(x4[e], f, acc[e]);
         }
         if (whole) {
             const float f = L != 0.0f ? p.v_scale / L : 0.0f;
@@ -626,88 +637,86 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
     return true;
 }
 
-// cum[i] = units of a pair before sequence c0 + i, of the 64 * WAVES from c0 on;
-// returns those before the next stretch.
-__device__ long long scan_lens(const ornk_kv_pages &p, const ornk_attend_args &a, int c0,
-                               long long before, long long *cum)
+// Inclusive sum over the lanes of a wave.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x)
 {
-    __shared__ long long tot[WAVES];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int b = c0 + tid;
-    const long long u = b < a.n_seqs ? (kv_len(p, a.lens, b, a.max_len) + UNIT - 1) / UNIT : 0;
-    long long x = u;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const long long y = __shfl_up(x, d, 64);
-        if (lane >= d) x += y;
-    }
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
+    return x;
+}
+
+// A stretch of 64 * WAVES sequences; every thread holds one of them.
+struct Stretch {
+    int c0;             // the first
+    uint32_t end;       // units of a pair up to the last one's end
+    int len;            // the thread's: tokens, units, units before it
+    uint32_t units, before;
+};
+
+__device__ __forceinline__ Stretch scan_lens(const ornk_kv_pages &p, const ornk_attend_args &a,
+                                             const AttendWs &w, int c0, uint32_t before)
+{
+    __shared__ uint32_t tot[WAVES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = c0 + threadIdx.x;
+    Stretch s;
+    s.c0 = c0;
+    s.len = b < a.n_seqs ? kv_len(p, a.lens, b, a.max_len) : 0;
+    s.units = (uint32_t)(((long long)s.len + (1 << w.unit_log2) - 1) >> w.unit_log2);
+    uint32_t x = wave_scan(s.units);
     __syncthreads();
     if (lane == 63) tot[wave] = x;
     __syncthreads();
-    long long all = before;
+    s.end = before;
 #pragma unroll
     for (int v = 0; v < WAVES; ++v) {
         if (v < wave) x += tot[v];
-        all += tot[v];
+        s.end += tot[v];
     }
-    cum[tid] = before + x - u;
-    if (tid == 0) cum[64 * WAVES] = all;
-    __syncthreads();
-    return all;
+    s.before = before + x - s.units;
+    return s;
 }
 
 template <int TYPE, int HD, class Path>
 __global__ void __launch_bounds__(64 * WAVES, per_cu<HD>) k_kv_attend(ornk_kv_pages p, ornk_attend_args a,
-                                                             AttendWs w)
+                                                                      AttendWs w)
 {
     extern __shared__ __align__(16) uint8_t lds[];
-    constexpr int CH = 64 * WAVES;
-    __shared__ long long cum[CH + 1];
+    __shared__ int4 found;
     const int G = a.heads / p.kv, HT = (G + 15) / 16;
-    const long long per = (long long)p.kv * HT;  // pairs of a sequence
-    long long units = 0;
-    int c0 = 0;
-    for (int c = 0; c < a.n_seqs; c += CH) {
-        units = scan_lens(p, a, c, units, cum);
-        c0 = c;
+    const uint32_t per = p.kv * HT;  // pairs of a sequence
+    Stretch st;
+    for (int c = 0; c == 0 || c < a.n_seqs; c += 64 * WAVES) {
+        st = scan_lens(p, a, w, c, c ? st.end : 0);
         if (blockIdx.x == 0) {
-            if (c + threadIdx.x < a.n_seqs) w.cum[c + threadIdx.x] = cum[threadIdx.x];
-            if (threadIdx.x == 0 && c + CH >= a.n_seqs) w.cum[a.n_seqs] = units;
+            if (c + threadIdx.x < a.n_seqs) w.cum[c + threadIdx.x] = st.before;
+            if (threadIdx.x == 0) w.cum[min(c + 64 * WAVES, a.n_seqs)] = st.end;
         }
     }
-    const long long T = units * per;
-    const int W = (int)min((long long)w.W, T);
-    if ((int)blockIdx.x >= W) return;
-    const long long lo = line_at(T, W, blockIdx.x), hi = line_at(T, W, blockIdx.x + 1);
-    if (lo < cum[0] * per) {  // an earlier stretch of sequences
-        long long before = 0;
-        for (c0 = 0;; c0 += CH) {
-            before = scan_lens(p, a, c0, before, cum);
-            if (lo < before * per) break;
-        }
-    }
-    for (long long u = lo; u < hi;) {
-        while (u >= cum[CH] * per) {
-            c0 += CH;
-            scan_lens(p, a, c0, cum[CH], cum);
-        }
-        int i = 0;  // the last sequence that starts at or before u
-#pragma unroll
-        for (int d = CH / 2; d; d >>= 1)
-            if (cum[i + d] * per <= u) i += d;
-        const int n = (int)(cum[i + 1] - cum[i]);
-        const long long off = u - cum[i] * per;
-        const int pair = (int)(off / n), k = (int)(off - (long long)pair * n);
-        const int cnt = (int)min((long long)(n - k), hi - u);
+    const uint32_t T = st.end * per;
+    const uint32_t lo = line_at(T, w.w_log2, blockIdx.x), hi = line_at(T, w.w_log2, blockIdx.x + 1);
+    if (lo >= hi) return;
+    if (st.c0) st = scan_lens(p, a, w, 0, 0);
+    for (uint32_t u = lo; u < hi;) {
+        while (u >= st.end * per) st = scan_lens(p, a, w, st.c0 + 64 * WAVES, st.end);
+        if (u - st.before * per < st.units * per)  // this thread's sequence (else u is past it, or wraps)
+            found = make_int4(st.c0 + threadIdx.x, st.len, st.units, st.before * per);
+        __syncthreads();
         Seg sg;
-        sg.b = c0 + i;
-        sg.h = pair / HT;
+        sg.b = __builtin_amdgcn_readfirstlane(found.x);
+        sg.len = __builtin_amdgcn_readfirstlane(found.y);
+        const uint32_t n = __builtin_amdgcn_readfirstlane(found.z);
+        const uint32_t off = u - __builtin_amdgcn_readfirstlane(found.w);
+        const uint32_t pair = off / n, k = off - pair * n, cnt = min(n - k, hi - u);
         const int j = 16 * (pair % HT);
+        sg.h = pair / HT;
         sg.j0 = sg.h * G + j;
         sg.rows = min(16, G - j);
-        sg.len = min(max(a.lens[sg.b], 0), a.max_len);
-        sg.k0 = k * UNIT;
-        sg.k1 = min(sg.len, (k + cnt) * UNIT);
+        sg.k0 = k << w.unit_log2;
+        sg.k1 = (int)min((long long)sg.len, (long long)(k + cnt) << w.unit_log2);
         sg.score = ((size_t)sg.b * a.heads + sg.j0) * w.s_len;
         const int slot = cnt == n ? -1 : 2 * (int)blockIdx.x + (u == lo ? 0 : 1);
         const bool done = attend_segment<TYPE, HD, Path>(p, a, w, sg, lds, slot);
@@ -718,86 +727,88 @@ __global__ void __launch_bounds__(64 * WAVES, per_cu<HD>) k_kv_attend(ornk_kv_pa
     }
 }
 
-// One work group per sequence and query head: the parts of its pair put
-// together; zeros for a sequence without tokens.
-constexpr int JT = 256;
-__global__ void __launch_bounds__(JT) k_kv_join(ornk_kv_pages p, ornk_attend_args a, AttendWs w)
+// The parts of a pair put together, 32 float4s of its rows per work group by
+// eight shares of the parts; zeros for a sequence without tokens.
+constexpr int JC = 32, JS = 8;
+__global__ void __launch_bounds__(JC * JS) k_kv_join(ornk_kv_pages p, ornk_attend_args a, AttendWs w)
 {
-    __shared__ float f[GROUPS], red[JT / 64];
-    __shared__ __align__(16) float acc[JT * 4];
-    const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int G = a.heads / p.kv, HT = (G + 15) / 16, hd = p.hd;
-    const long long per = (long long)p.kv * HT, T = w.cum[a.n_seqs] * per;
-    const long long c0 = w.cum[b], n = w.cum[b + 1] - c0;
-    float *out = a.out + ((size_t)b * a.heads + head) * hd;
-    if (n == 0) {
-        for (int i = tid; i < hd; i += JT) out[i] = 0.0f;
-        return;
+    __shared__ float sm[JS][JC], sl[JS][JC];
+    __shared__ v4f so[JS][JC];
+    const int b = blockIdx.z, pair = blockIdx.y, G = a.heads / p.kv, HT = (G + 15) / 16, hd = p.hd;
+    const uint32_t per = p.kv * HT, before = w.cum[b], n = w.cum[b + 1] - before, T = w.cum[a.n_seqs] * per;
+    const uint32_t s = before * per + pair * n;
+    uint32_t w0 = 0, nseg = 0;
+    if (n) {
+        w0 = line_group(T, w.w_log2, s);
+        nseg = line_group(T, w.w_log2, s + n - 1) - w0 + 1;
+        if (nseg == 1) return;  // finished by one group
     }
-    const int pair = head / G * HT + head % G / 16, row = head % G % 16;
-    const int W = (int)min((long long)w.W, T);
-    const long long s = c0 * per + pair * n, e = s + n;
-    const int w0 = (int)(((s + 1) * W - 1) / T), w1 = (int)((e * W - 1) / T);
-    if (w0 == w1) return;  // finished by one group
-    const int nseg = w1 - w0 + 1, first = 2 * w0 + (line_at(T, W, w0) == s ? 0 : 1);
-    auto slot = [&](int i) { return (size_t)(i ? 2 * (w0 + i) : first) * 16 + row; };
-    auto all = [&](float v, bool mx) {
-#pragma unroll
-        for (int d = 32; d; d >>= 1) {
-            const float y = __shfl_xor(v, d, 64);
-            v = mx ? fmaxf(v, y) : v + y;
-        }
-        __syncthreads();
-        if (lane == 0) red[wave] = v;
-        __syncthreads();
-        v = red[0];
-        for (int i = 1; i < JT / 64; ++i) v = mx ? fmaxf(v, red[i]) : v + red[i];
-        return v;
-    };
-    float M = -INFINITY, L = 0.0f;
-    for (int i = tid; i < nseg; i += JT) M = fmaxf(M, w.part_ml[slot(i)].x);
-    M = all(M, true);
-    for (int i = tid; i < nseg; i += JT) {
-        const float2 ml = w.part_ml[slot(i)];
-        f[i] = ml.x == -INFINITY ? 0.0f : exp2_(ml.x - M);
-        L += ml.y * f[i];
-    }
-    L = all(L, false);
-    const int q4 = w.row / 4, ng = JT / q4, c = tid % q4, sub = tid / q4;
+    const int j = 16 * (pair % HT), rows = min(16, G - j), j0 = pair / HT * G + j;
+    const int x = threadIdx.x % JC, sub = threadIdx.x / JC, at = blockIdx.x * JC + x;
+    const int row = at / (w.row / 4), c = at % (w.row / 4) * 4;
+    const uint32_t first = 2 * w0 + (line_at(T, w.w_log2, w0) == s ? 0 : 1);
+    float m = -INFINITY, l = 0.0f;
     v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (sub < ng)
-        for (int i = sub; i < nseg; i += ng) {
-            const v4f x = *reinterpret_cast<const v4f *>(w.part_o + slot(i) * w.row + 4 * c);
-            const float fi = f[i];
+    auto add = [&](float m2, float l2, v4f o2) {
+        const float mn = fmaxf(m, m2), f = weight_from(m, mn), f2 = weight_from(m2, mn);
+        m = mn;
+        l = l * f + l2 * f2;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) o[k] = fi == 0.0f ? o[k] : fmaf(x[k], fi, o[k]);
+        for (int e = 0; e < 4; ++e) o[e] = o[e] * f + o2[e] * f2;
+    };
+    if (row < rows)
+#pragma unroll 4
+        for (uint32_t i = sub; i < nseg; i += JS) {
+            const size_t slot = (size_t)(i ? 2 * (w0 + i) : first) * 16 + row;
+            const float2 ml = w.part_ml[slot];
+            add(ml.x, ml.y, *reinterpret_cast<const v4f *>(w.part_o + slot * w.row + c));
         }
-    *reinterpret_cast<v4f *>(acc + 4 * tid) = o;
+    sm[sub][x] = m;
+    sl[sub][x] = l;
+    so[sub][x] = o;
     __syncthreads();
-    const float inv = L != 0.0f ? p.v_scale / L : 0.0f;
-    for (int i = tid; i < hd; i += JT) {
-        float v = 0.0f;
-        for (int k = 0; k < ng; ++k) v += acc[k * w.row + i];
-        out[i] = v * inv;
-    }
-    if (w.ml && tid == 0) w.ml[(size_t)b * a.heads + head] = make_float2(M, L);
+    if (sub || row >= rows) return;
+    for (int i = 1; i < JS; ++i) add(sm[i][x], sl[i][x], so[i][x]);
+    const float f = l != 0.0f ? p.v_scale / l : 0.0f;
+    float *out = a.out + ((size_t)b * a.heads + j0 + row) * hd + c;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (c + e < hd) out[e] = o[e] * f;
+    if (w.ml && c == 0 && n) w.ml[(size_t)b * a.heads + j0 + row] = make_float2(m, l);
 }
 
-// The weights each token got, summed over a kv head's query heads.
-__global__ void k_kv_score(ornk_kv_pages p, ornk_attend_args a, AttendWs w)
+// The weights each token got, summed over a kv head's query heads; four tokens
+// per thread.
+constexpr int ST = 256;
+__global__ void __launch_bounds__(ST) k_kv_score(ornk_kv_pages p, ornk_attend_args a, AttendWs w)
 {
-    const int t = blockIdx.x * blockDim.x + threadIdx.x, h = blockIdx.y, b = blockIdx.z;
-    if (t >= min(max(a.lens[b], 0), a.max_len)) return;
-    const int G = a.heads / p.kv;
-    float sum = 0.0f;
+    const int h = blockIdx.y, b = blockIdx.z, G = a.heads / p.kv;
+    const int len = min(max(a.lens[b], 0), a.max_len);
+    const long long t = ((long long)blockIdx.x * ST + threadIdx.x) * 4;
+    if (t >= len) return;
+    const size_t row = (size_t)b * a.heads + h * G;
+    v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
     for (int g = 0; g < G; ++g) {
-        const size_t row = (size_t)b * a.heads + h * G + g;
-        const float2 ml = w.ml[row];
-        const float s = w.s[row * w.s_len + t];
-        sum += s == -INFINITY ? 0.0f : exp2_(s - ml.x) / ml.y;
+        const float2 ml = w.ml[row + g];
+        const v4f s = *reinterpret_cast<const v4f *>(w.s + (row + g) * w.s_len + t);
+        const float f = 1.0f / ml.y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += s[e] == -INFINITY ? 0.0f : exp2_(s[e] - ml.x) * f;
     }
     const size_t i = ((size_t)b * p.kv + h) * a.score_stride + t;
-    a.score_out[i] = a.score_in ? fmaf(a.decay, a.score_in[i], sum) : sum;
+    if (a.score_stride % 4 == 0 && t + 4 <= len) {
+        if (a.score_in) {
+            const v4f x = *reinterpret_cast<const v4f *>(a.score_in + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] = fmaf(a.decay, x[e], sum[e]);
+        }
+        *reinterpret_cast<v4f *>(a.score_out + i) = sum;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (t + e < len) a.score_out[i + e] = a.score_in ? fmaf(a.decay, a.score_in[i + e], sum[e]) : sum[e];
 }
 
 size_t attend_ws(const ornk_kv_pages *p, const ornk_attend_args *a, AttendWs *w)
@@ -809,17 +820,21 @@ size_t attend_ws(const ornk_kv_pages *p, const ornk_attend_args *a, AttendWs *w)
         off += (n + 255) & ~(size_t)255;
         return at;
     };
-    w->W = p->hd > 128 ? per_cu<256> * CUS : GROUPS;
+    const int G = a->heads / p->kv, W = 1 << (CUS_LOG2 + (p->hd > 128 ? 0 : 1));
+    w->w_log2 = CUS_LOG2 + (p->hd > 128 ? 0 : 1);
     w->row = (p->hd + 3) & ~3;
-    w->cum = reinterpret_cast<long long *>(take(((size_t)a->n_seqs + 1) * 8));
-    w->part_ml = reinterpret_cast<float2 *>(take((size_t)2 * w->W * 16 * 8));
-    w->part_o = reinterpret_cast<float *>(take((size_t)2 * w->W * 16 * w->row * 4));
+    w->unit_log2 = UNIT_LOG2;
+    const size_t pairs = (size_t)a->n_seqs * p->kv * ((G + 15) / 16);
+    while (w->unit_log2 < 31 && pairs * (((size_t)a->max_len >> w->unit_log2) + 1) >> LINE_LOG2) ++w->unit_log2;
+    w->cum = reinterpret_cast<uint32_t *>(take(((size_t)a->n_seqs + 1) * 4));
+    w->part_ml = reinterpret_cast<float2 *>(take((size_t)2 * W * 16 * 8));
+    w->part_o = reinterpret_cast<float *>(take((size_t)2 * W * 16 * w->row * 4));
     w->ml = nullptr;
     w->s = nullptr;
     w->s_len = 0;
     if (a->score_out) {
         const size_t rows = (size_t)a->n_seqs * a->heads;
-        w->s_len = ((size_t)a->max_len + UNIT - 1) / UNIT * UNIT;
+        w->s_len = ((size_t)a->max_len + 31) / 32 * 32;  // whole tiles
         w->ml = reinterpret_cast<float2 *>(take(rows * 8));
         w->s = reinterpret_cast<float *>(take(rows * w->s_len * 4));
     }
@@ -834,7 +849,7 @@ int launch_hd(const ornk_kv_pages *p, const ornk_attend_args *a, const AttendWs 
     size_t lds = (size_t)WAVES * rows * HD * 4;
     if (lds < Path::Q_BYTES) lds = Path::Q_BYTES;
     if (lds < Exact<TYPE, HD, true, true>::Q_BYTES) lds = Exact<TYPE, HD, true, true>::Q_BYTES;
-    hipLaunchKernelGGL((k_kv_attend<TYPE, HD, Path>), dim3(w.W), dim3(64 * WAVES), lds, s, *p, *a, w);
+    hipLaunchKernelGGL((k_kv_attend<TYPE, HD, Path>), dim3(1 << w.w_log2), dim3(64 * WAVES), lds, s, *p, *a, w);
     return hipGetLastError();
 }
 
@@ -879,9 +894,11 @@ extern "C" int ornk_kv_attend(const ornk_kv_pages *p, const ornk_attend_args *a,
              : p->type == ORN_KV_BF16 ? launch_type<ORN_KV_BF16>(p, a, w, s)
                                       : launch_type<ORN_KV_E4M3>(p, a, w, s);
     if (rc != hipSuccess) return rc;
-    hipLaunchKernelGGL(k_kv_join, dim3(a->heads, a->n_seqs), dim3(JT), 0, s, *p, *a, w);
+    const int G = a->heads / p->kv, HT = (G + 15) / 16;
+    hipLaunchKernelGGL(k_kv_join, dim3(((G < 16 ? G : 16) * (w.row / 4) + JC - 1) / JC, p->kv * HT, a->n_seqs),
+                       dim3(JC * JS), 0, s, *p, *a, w);
     if (a->score_out && a->max_len)
-        hipLaunchKernelGGL(k_kv_score, dim3((a->max_len + 255) / 256, p->kv, a->n_seqs), dim3(256), 0,
-                           s, *p, *a, w);
+        hipLaunchKernelGGL(k_kv_score, dim3(((unsigned)a->max_len + 4 * ST - 1) / (4 * ST), p->kv, a->n_seqs),
+                           dim3(ST), 0, s, *p, *a, w);
     return hipGetLastError();
 }

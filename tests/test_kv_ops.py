@@ -701,6 +701,32 @@ def test_attend_values_that_are_not_finite(om, ctx, type, heads, D):
     c.free()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("type", list(DTYPE))
+@pytest.mark.parametrize("n,bad", [(1, 0), (40, 17), (300, 299), (5000, 3)])
+def test_attend_one_nan_key_makes_its_sequence_nan(om, ctx, type, n, bad):
+    """Also where every score is one, and in a part that another group joins; a key of -inf
+    alone leaves a sequence without weights: zeros."""
+    rng = np.random.default_rng(n)
+    lens = [n, n, 1]
+    n_pages = sum(-(-m // 16) for m in lens)
+    c = Cache(om, ctx, type, n_pages, 16, 1, 64, seed=2)
+    table = tables(rng, lens, 16, n_pages, -(-n // 16))
+    c.k[table[0, bad // 16], 0, bad % 16, 0] = math.nan
+    if type != "e4m3":
+        c.k[table[2, 0], 0, 0] = -math.inf
+    c.write()
+    q = np.abs(rng.standard_normal((3, 4, 64))).astype(np.float32) + 0.25
+    out = attend(om, ctx, c, q, lens, table)
+    assert np.isnan(out[0]).all()
+    k, v = c.rows(table[1], n)
+    want, _, tol, _ = attend64(q[1], k, v, 1 / 8)
+    assert np.abs(out[1] - want).max() <= tol
+    if type != "e4m3":
+        assert (out[2] == 0).all()
+    c.free()
+
+
 def attend64_cols(q, k, v, cols):
     out, w, tol, tw = attend64(q, k, np.where(np.isfinite(v), v, 0.0), 1 / math.sqrt(q.shape[1]))
     return out[:, cols], w, tol, tw
