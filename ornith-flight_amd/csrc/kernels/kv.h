@@ -51,10 +51,9 @@ __device__ __forceinline__ void kv_error(const ornk_kv_pages &p, int what, int a
     *(volatile int *)(p.err + what) = 1 + at;
 }
 
-// lens[b] within [0, max_len].
-__device__ __forceinline__ int kv_len(const ornk_kv_pages &p, const int *lens, int b, int max_len)
+// Sequence b's length within [0, max_len].
+__device__ __forceinline__ int kv_len(const ornk_kv_pages &p, int n, int b, int max_len)
 {
-    const int n = lens[b];
     if (n >= 0 && n <= max_len) return n;
     kv_error(p, ORNK_KV_ERR_LEN, b);
     return n < 0 ? 0 : max_len;

@@ -576,16 +576,9 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
 
-    if constexpr (!Path::exact) {  // anything that is not finite: not this path's to say
-        float z = l * 0.0f;
-#pragma unroll
-        for (int c = 0; c < NO; ++c)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) z = fmaf(o[c][r], 0.0f, z);
-        if (__syncthreads_or(z != 0.0f)) return false;
-    } else {
-        __syncthreads();  // the queries are consumed
-    }
+    __shared__ int odd;
+    if (!Path::exact && tid == 0) odd = 0;
+    __syncthreads();  // the queries are consumed
     if (g == 0) {
         sm[wave][n] = m;
         sl[wave][n] = l;
@@ -603,6 +596,7 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
     }
     __syncthreads();
     const bool whole = slot < 0;
+    float z = 0.0f;
     for (int i = tid; i < sg.rows * (HD / 4); i += 64 * WAVES) {
         const int row = i / (HD / 4), c = 4 * (i % (HD / 4));
         float M = -INFINITY, L = 0.0f;
@@ -617,6 +611,8 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[e] = fmaf(x4[e], f, acc[e]);
         }
+        if (!Path::exact)
+            z += L * 0.0f + (acc[0] * 0.0f + acc[1] * 0.0f) + (acc[2] * 0.0f + acc[3] * 0.0f);
         if (whole) {
             const float f = L != 0.0f ? p.v_scale / L : 0.0f;
             float *out = a.out + ((size_t)sg.b * a.heads + sg.j0 + row) * hd + c;
@@ -634,7 +630,11 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
             if (c == 0) w.part_ml[(size_t)slot * 16 + row] = make_float2(M, L);
         }
     }
-    return true;
+    if constexpr (Path::exact) return true;
+    // a sum that is not finite is not this path's to say
+    if (z != 0.0f) odd = 1;
+    __syncthreads();
+    return odd == 0;
 }
 
 // Inclusive sum over the lanes of a wave.
@@ -649,34 +649,37 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x)
     return x;
 }
 
-// A stretch of 64 * WAVES sequences; every thread holds one of them.
+// A stretch of 256 sequences, four to a lane; every wave has it for itself, so
+// that finding one's place on the line takes no barrier.
+constexpr int STRETCH = 256;
 struct Stretch {
-    int c0;             // the first
-    uint32_t end;       // units of a pair up to the last one's end
-    int len;            // the thread's: tokens, units, units before it
-    uint32_t units, before;
+    int c0;                          // the first
+    uint32_t end;                    // units of a pair up to the last one's end
+    int len[4];                      // the lane's: tokens, units, units before
+    uint32_t units[4], before[4];
 };
 
 __device__ __forceinline__ Stretch scan_lens(const ornk_kv_pages &p, const ornk_attend_args &a,
                                              const AttendWs &w, int c0, uint32_t before)
 {
-    __shared__ uint32_t tot[WAVES];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = c0 + threadIdx.x;
     Stretch s;
     s.c0 = c0;
-    s.len = b < a.n_seqs ? kv_len(p, a.lens, b, a.max_len) : 0;
-    s.units = (uint32_t)(((long long)s.len + (1 << w.unit_log2) - 1) >> w.unit_log2);
-    uint32_t x = wave_scan(s.units);
-    __syncthreads();
-    if (lane == 63) tot[wave] = x;
-    __syncthreads();
-    s.end = before;
+    const int b0 = c0 + 4 * (threadIdx.x & 63);
+    int at[4];
 #pragma unroll
-    for (int v = 0; v < WAVES; ++v) {
-        if (v < wave) x += tot[v];
-        s.end += tot[v];
+    for (int i = 0; i < 4; ++i) at[i] = a.lens[min(b0 + i, a.n_seqs - 1)];
+    uint32_t sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        s.len[i] = b0 + i < a.n_seqs ? kv_len(p, at[i], b0 + i, a.max_len) : 0;
+        s.units[i] = (uint32_t)(((long long)s.len[i] + (1 << w.unit_log2) - 1) >> w.unit_log2);
+        s.before[i] = sum;
+        sum += s.units[i];
     }
-    s.before = before + x - s.units;
+    const uint32_t x = wave_scan(sum);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s.before[i] += before + x - sum;
+    s.end = before + __builtin_amdgcn_readlane(x, 63);
     return s;
 }
 
@@ -685,34 +688,47 @@ __global__ void __launch_bounds__(64 * WAVES, per_cu<HD>) k_kv_attend(ornk_kv_pa
                                                                       AttendWs w)
 {
     extern __shared__ __align__(16) uint8_t lds[];
-    __shared__ int4 found;
     const int G = a.heads / p.kv, HT = (G + 15) / 16;
     const uint32_t per = p.kv * HT;  // pairs of a sequence
     Stretch st;
-    for (int c = 0; c == 0 || c < a.n_seqs; c += 64 * WAVES) {
+    for (int c = 0; c == 0 || c < a.n_seqs; c += STRETCH) {
         st = scan_lens(p, a, w, c, c ? st.end : 0);
-        if (blockIdx.x == 0) {
-            if (c + threadIdx.x < a.n_seqs) w.cum[c + threadIdx.x] = st.before;
-            if (threadIdx.x == 0) w.cum[min(c + 64 * WAVES, a.n_seqs)] = st.end;
+        if (blockIdx.x == 0 && threadIdx.x < 64) {
+            const int b = c + 4 * threadIdx.x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (b + i < a.n_seqs) w.cum[b + i] = st.before[i];
+            if (threadIdx.x == 0) w.cum[min(c + STRETCH, a.n_seqs)] = st.end;
         }
     }
     const uint32_t T = st.end * per;
     const uint32_t lo = line_at(T, w.w_log2, blockIdx.x), hi = line_at(T, w.w_log2, blockIdx.x + 1);
-    if (lo >= hi) return;
-    if (st.c0) st = scan_lens(p, a, w, 0, 0);
+    if (st.c0 && lo < hi) st = scan_lens(p, a, w, 0, 0);
     for (uint32_t u = lo; u < hi;) {
-        while (u >= st.end * per) st = scan_lens(p, a, w, st.c0 + 64 * WAVES, st.end);
-        if (u - st.before * per < st.units * per)  // this thread's sequence (else u is past it, or wraps)
-            found = make_int4(st.c0 + threadIdx.x, st.len, st.units, st.before * per);
-        __syncthreads();
+        while (u >= st.end * per) st = scan_lens(p, a, w, st.c0 + STRETCH, st.end);
+        int b = -1, len = 0;  // u's sequence, in its lane
+        uint32_t units = 0, start = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (u - st.before[i] * per < st.units[i] * per) {  // (wraps where u is before it)
+                b = st.c0 + 4 * (threadIdx.x & 63) + i;
+                len = st.len[i];
+                units = st.units[i];
+                start = st.before[i] * per;
+            }
+        const int from = __ffsll((unsigned long long)__ballot(b >= 0)) - 1;
         Seg sg;
-        sg.b = __builtin_amdgcn_readfirstlane(found.x);
-        sg.len = __builtin_amdgcn_readfirstlane(found.y);
-        const uint32_t n = __builtin_amdgcn_readfirstlane(found.z);
-        const uint32_t off = u - __builtin_amdgcn_readfirstlane(found.w);
-        const uint32_t pair = off / n, k = off - pair * n, cnt = min(n - k, hi - u);
-        const int j = 16 * (pair % HT);
-        sg.h = pair / HT;
+        sg.b = __builtin_amdgcn_readlane(b, from);
+        sg.len = __builtin_amdgcn_readlane(len, from);
+        const uint32_t n = __builtin_amdgcn_readlane(units, from);
+        const uint32_t off = u - __builtin_amdgcn_readlane(start, from);
+        // off / n of integers below 2^22: fp32's quotient is at most one off
+        uint32_t pair = (uint32_t)((float)off / (float)n);
+        if (pair * n > off) --pair;
+        else if (off - pair * n >= n) ++pair;
+        const uint32_t k = off - pair * n, cnt = min(n - k, hi - u);
+        const int tile = HT == 1 ? 0 : pair % HT, j = 16 * tile;
+        sg.h = HT == 1 ? pair : pair / HT;
         sg.j0 = sg.h * G + j;
         sg.rows = min(16, G - j);
         sg.k0 = k << w.unit_log2;
@@ -725,10 +741,16 @@ __global__ void __launch_bounds__(64 * WAVES, per_cu<HD>) k_kv_attend(ornk_kv_pa
         }
         u += cnt;
     }
+    // sequences without tokens: zeros
+    for (int b = blockIdx.x; b < a.n_seqs; b += gridDim.x) {
+        if (a.lens[b] > 0 && a.max_len > 0) continue;
+        float *out = a.out + (size_t)b * a.heads * p.hd;
+        for (size_t i = threadIdx.x; i < (size_t)a.heads * p.hd; i += 64 * WAVES) out[i] = 0.0f;
+    }
 }
 
-// The parts of a pair put together, 32 float4s of its rows per work group by
-// eight shares of the parts; zeros for a sequence without tokens.
+// The parts of a pair put together, JC float4s of its rows per work group by JS
+// shares of the parts.
 constexpr int JC = 32, JS = 8;
 __global__ void __launch_bounds__(JC * JS) k_kv_join(ornk_kv_pages p, ornk_attend_args a, AttendWs w)
 {
@@ -737,12 +759,9 @@ __global__ void __launch_bounds__(JC * JS) k_kv_join(ornk_kv_pages p, ornk_atten
     const int b = blockIdx.z, pair = blockIdx.y, G = a.heads / p.kv, HT = (G + 15) / 16, hd = p.hd;
     const uint32_t per = p.kv * HT, before = w.cum[b], n = w.cum[b + 1] - before, T = w.cum[a.n_seqs] * per;
     const uint32_t s = before * per + pair * n;
-    uint32_t w0 = 0, nseg = 0;
-    if (n) {
-        w0 = line_group(T, w.w_log2, s);
-        nseg = line_group(T, w.w_log2, s + n - 1) - w0 + 1;
-        if (nseg == 1) return;  // finished by one group
-    }
+    if (n < 2) return;  // no tokens, or one unit
+    const uint32_t w0 = line_group(T, w.w_log2, s), nseg = line_group(T, w.w_log2, s + n - 1) - w0 + 1;
+    if (nseg == 1) return;  // finished by one group
     const int j = 16 * (pair % HT), rows = min(16, G - j), j0 = pair / HT * G + j;
     const int x = threadIdx.x % JC, sub = threadIdx.x / JC, at = blockIdx.x * JC + x;
     const int row = at / (w.row / 4), c = at % (w.row / 4) * 4;
@@ -774,7 +793,7 @@ __global__ void __launch_bounds__(JC * JS) k_kv_join(ornk_kv_pages p, ornk_atten
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (c + e < hd) out[e] = o[e] * f;
-    if (w.ml && c == 0 && n) w.ml[(size_t)b * a.heads + j0 + row] = make_float2(m, l);
+    if (w.ml && c == 0) w.ml[(size_t)b * a.heads + j0 + row] = make_float2(m, l);
 }
 
 // The weights each token got, summed over a kv head's query heads; four tokens
@@ -895,8 +914,9 @@ extern "C" int ornk_kv_attend(const ornk_kv_pages *p, const ornk_attend_args *a,
                                       : launch_type<ORN_KV_E4M3>(p, a, w, s);
     if (rc != hipSuccess) return rc;
     const int G = a->heads / p->kv, HT = (G + 15) / 16;
-    hipLaunchKernelGGL(k_kv_join, dim3(((G < 16 ? G : 16) * (w.row / 4) + JC - 1) / JC, p->kv * HT, a->n_seqs),
-                       dim3(JC * JS), 0, s, *p, *a, w);
+    if (a->max_len > 1 << w.unit_log2)  // else every pair is one unit
+        hipLaunchKernelGGL(k_kv_join, dim3(((G < 16 ? G : 16) * (w.row / 4) + JC - 1) / JC, p->kv * HT, a->n_seqs),
+                           dim3(JC * JS), 0, s, *p, *a, w);
     if (a->score_out && a->max_len)
         hipLaunchKernelGGL(k_kv_score, dim3(((unsigned)a->max_len + 4 * ST - 1) / (4 * ST), p->kv, a->n_seqs),
                            dim3(ST), 0, s, *p, *a, w);

@@ -28,7 +28,7 @@ __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict
 {
     __shared__ int hist[BINS], wsum[CT / 64], sh[2];
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int len = kv_len(p, a.lens, b, a.max_len), n = min(len, a.keep);
+    const int len = kv_len(p, a.lens[b], b, a.max_len), n = min(len, a.keep);
     const float *score = a.score + ((size_t)b * p.kv + h) * a.score_stride;
     float *ds = a.dst_score ? a.dst_score + ((size_t)b * p.kv + h) * a.dst_stride : nullptr;
     int *kept = a.kept + ((size_t)b * p.kv + h) * a.keep;
