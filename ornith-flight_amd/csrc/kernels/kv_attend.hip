@@ -22,8 +22,10 @@ constexpr int WAVES = 4;
 // log2 of a unit's tokens: four tiles, or as many more as keep the line below
 // 2^22 units (32-bit products with a group's number).
 constexpr int UNIT_LOG2 = 7, LINE_LOG2 = 22;
-// Work groups per CU: the registers of 256 columns (K, V and O of a tile, 64
-// each, beside their addresses) leave room for one wave per SIMD.
+// Work groups per CU: one's start and end under the other's stream.  The
+// registers of 256 columns (K, V and O of a tile, 64 each, beside their
+// addresses) leave room for one wave per SIMD; with two and tiles of 16 keys,
+// 131,071 tokens of bf16 take 64 us instead of 52.
 template <int HD>
 constexpr int per_cu = HD == 256 ? 1 : 2;
 constexpr int CUS_LOG2 = 8;
@@ -224,19 +226,20 @@ struct Exact {
 // into CW operands of 8 keys there (v_perm_b32).
 template <int TYPE, int HD, bool FULL>
 struct Parts {
-    static constexpr int KT = 32, ES = elem_size<TYPE>, NS = HD / 32, NO = HD / 16;
+    static constexpr int KT = 32, NI = KT / 16;
+    static constexpr int ES = elem_size<TYPE>, NS = HD / 32, NO = HD / 16;
     static constexpr int DL = 16 / ES, NL = HD / (4 * DL);             // K: dimensions of a load, loads
     static constexpr int CW = HD / 16 < DL ? HD / 16 : DL, NH = HD / (16 * CW);  // V: columns, loads of a row
     static constexpr int VW = CW * ES / 4;
     static constexpr int NP = TYPE == ORN_KV_F16 ? 2 : 1;
     static constexpr size_t Q_BYTES = 3 * 16 * HD * 2;
     static constexpr bool full = FULL, exact = false, ahead = true;
-    uint32_t k[2][NL][4], v[8][NH][VW];
+    uint32_t k[NI][NL][4], v[4 * NI][NH][VW];
 
     __device__ __forceinline__ void load_k(const uint8_t *const *row, int g, int hd)
     {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < NI; ++i)
 #pragma unroll
             for (int j = 0; j < NL; ++j) {
                 // past the row: its start, which meets zeros of the query
@@ -247,7 +250,7 @@ struct Parts {
     __device__ __forceinline__ void load_v(const uint8_t *const *row, int n, int hd)
     {
 #pragma unroll
-        for (int r = 0; r < 8; ++r)
+        for (int r = 0; r < 4 * NI; ++r)
 #pragma unroll
             for (int j = 0; j < NH; ++j) {
                 const int c = CW * (16 * j + n);  // past the row: a column that is not stored
@@ -301,39 +304,41 @@ struct Parts {
     __device__ __forceinline__ void scores(float *s, const void *lds, int lane) const
     {
         const v8b *q = static_cast<const v8b *>(lds) + lane;
-        v4f a0 = {0.0f, 0.0f, 0.0f, 0.0f}, a1 = a0, b0 = a0, b1 = a0;
+        v4f x[NI], y[NI];  // the products of the first parts; the others
+#pragma unroll
+        for (int i = 0; i < NI; ++i) x[i] = y[i] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int st = 0; st < NS; ++st) {
-            v8b k0[NP], k1[NP];
-            k_parts(k0, 0, st);
-            k_parts(k1, 1, st);
-            const v8b q0 = q[64 * st], q1 = q[64 * (NS + st)], q2 = q[64 * (2 * NS + st)];
-            a0 = mma(k0[0], q0, a0);
-            a1 = mma(k1[0], q0, a1);
-            b0 = mma(k0[0], q2, b0);
-            b1 = mma(k1[0], q2, b1);
-            b0 = mma(k0[0], q1, b0);
-            b1 = mma(k1[0], q1, b1);
+            v8b kk[NI][NP], qq[3];
+#pragma unroll
+            for (int i = 0; i < NI; ++i) k_parts(kk[i], i, st);
+#pragma unroll
+            for (int part = 0; part < 3; ++part) qq[part] = q[64 * (part * NS + st)];
+            auto add = [&](v4f *z, int kp, int qp) {
+#pragma unroll
+                for (int i = 0; i < NI; ++i) z[i] = mma(kk[i][kp], qq[qp], z[i]);
+            };
+            add(x, 0, 0);
+            add(y, 0, 2);
+            add(y, 0, 1);
             if constexpr (NP == 2) {
-                b0 = mma(k0[1], q1, b0);
-                b1 = mma(k1[1], q1, b1);
-                b0 = mma(k0[1], q0, b0);
-                b1 = mma(k1[1], q0, b1);
+                add(y, 1, 1);
+                add(y, 1, 0);
             }
         }
-        a0 += b0;
-        a1 += b1;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[r] = a0[r], s[4 + r] = a1[r];
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[4 * i + r] = x[i][r] + y[i][r];
     }
     __device__ __forceinline__ void leave_out(int) {}
     __device__ __forceinline__ void pv(v4f *o, const float *p) const
     {
         v8b pp[3];
         {
-            float x[8];
+            float x[4 * NI];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = p[e];
+            for (int e = 0; e < 4 * NI; ++e) x[e] = p[e];
 #pragma unroll
             for (int part = 0; part < 3; ++part) {
                 u4 w;
@@ -341,66 +346,47 @@ struct Parts {
                 for (int e = 0; e < 4; ++e) w[e] = top16(x[2 * e + 1], x[2 * e]);
                 pp[part] = as_v8b(w);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = rest16(x[e]);
+                for (int e = 0; e < 4 * NI; ++e) x[e] = rest16(x[e]);
             }
         }
 #pragma unroll
-        for (int j = 0; j < NH; ++j) {
-            if constexpr (TYPE == ORN_KV_BF16) {
+        for (int j = 0; j < NH; ++j)
 #pragma unroll
-                for (int c = 0; c < CW; c += 4) {
-                    v8b b[4];
+            for (int c = 0; c < CW; c += 4) {
+                // four columns' operands: V's rows turned
+                u4 hi[4], lo[4];
+                if constexpr (TYPE == ORN_KV_BF16) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        u4 w;
+                    for (int i = 0; i < 4; ++i)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            w[e] = __builtin_amdgcn_perm(v[2 * e + 1][j][(c + i) / 2],
-                                                         v[2 * e][j][(c + i) / 2],
-                                                         i % 2 ? 0x07060302u : 0x05040100u);
-                        b[i] = as_v8b(w);
-                    }
+                            hi[i][e] = __builtin_amdgcn_perm(v[2 * e + 1][j][(c + i) / 2],
+                                                             v[2 * e][j][(c + i) / 2],
+                                                             i % 2 ? 0x07060302u : 0x05040100u);
+                } else {
+                    float f[4 * NI][4];
 #pragma unroll
-                    for (int part = 2; part >= 0; --part)
+                    for (int e = 0; e < 4 * NI; ++e) unpack4<TYPE>(f[e], &v[e][j][c * ES / 4]);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            v4f &x = o[j * CW + c + i];
-                            x = mma(pp[part], b[i], x);
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            hi[i][e] = top16(f[2 * e + 1][i], f[2 * e][i]);
+                            if constexpr (NP == 2)
+                                lo[i][e] = top16(rest16(f[2 * e + 1][i]), rest16(f[2 * e][i]));
                         }
                 }
-            } else {
+                v4f *x = o + j * CW + c;
+                auto add = [&](int part, const u4 *b) {
 #pragma unroll
-                for (int c = 0; c < CW; c += 4) {
-                    float f[8][4];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) unpack4<TYPE>(f[e], &v[e][j][c * ES / 4]);
-                    v8b hi[4], lo[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        u4 w;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = top16(f[2 * e + 1][i], f[2 * e][i]);
-                        hi[i] = as_v8b(w);
-                        if constexpr (NP == 2) {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                w[e] = top16(rest16(f[2 * e + 1][i]), rest16(f[2 * e][i]));
-                            lo[i] = as_v8b(w);
-                        }
-                    }
-                    v4f *x = o + j * CW + c;
-                    auto add = [&](int part, const v8b *b) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) x[i] = mma(pp[part], b[i], x[i]);
-                    };
-                    add(2, hi);
-                    if constexpr (NP == 2) add(1, lo);
-                    add(1, hi);
-                    if constexpr (NP == 2) add(0, lo);
-                    add(0, hi);
-                }
+                    for (int i = 0; i < 4; ++i) x[i] = mma(pp[part], as_v8b(b[i]), x[i]);
+                };
+                add(2, hi);
+                if constexpr (NP == 2) add(1, lo);
+                add(1, hi);
+                if constexpr (NP == 2) add(0, lo);
+                add(0, hi);
             }
-        }
     }
     static __device__ __forceinline__ int col(int c, int n) { return CW * (16 * (c / CW) + n) + c % CW; }
 };
@@ -500,6 +486,16 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
     for (int c = 0; c < NO; ++c) o[c] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
     float s[4 * NI];
+    v4f raw[NI];
+    // A tile's scores kept for the weights: after the next tile's loads, which
+    // would wait for a store before them (they are counted in order).
+    auto keep = [&](int t) {
+        if (w.s && n < sg.rows) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+                *reinterpret_cast<v4f *>(w.s + sg.score + n * w.s_len + t + 16 * i + 4 * g) = raw[i];
+        }
+    };
     // the softmax of a tile's scores, and its O
     auto rest = [&](int t) {
         bool all = t + KT <= len;
@@ -515,13 +511,8 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
                         x.leave_out(4 * i + r);
                     }
         }
-        if (w.s && n < sg.rows) {
 #pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                const v4f v = {s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
-                *reinterpret_cast<v4f *>(w.s + sg.score + n * w.s_len + t + 16 * i + 4 * g) = v;
-            }
-        }
+        for (int i = 0; i < NI; ++i) raw[i] = (v4f){s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
         float tm = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 4 * NI; ++i) tm = fmaxf(tm, s[i]);
@@ -559,9 +550,11 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
                 load_k(t + KT * WAVES);
                 rest(t);
                 load_v(t + KT * WAVES);
+                keep(t);
             }
             x.scores(s, lds, lane);
             rest(t);
+            keep(t);
         }
     } else {
         for (; t < sg.k1; t += KT * WAVES) {
@@ -571,6 +564,7 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
             load_v(t);
             x.scores(s, lds, lane);
             rest(t);
+            keep(t);
         }
     }
     l += __shfl_xor(l, 16, 64);
@@ -595,27 +589,36 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
         }
     }
     __syncthreads();
-    const bool whole = slot < 0;
+    const int c = 4 * (tid % (HD / 4));
     float z = 0.0f;
-    for (int i = tid; i < sg.rows * (HD / 4); i += 64 * WAVES) {
-        const int row = i / (HD / 4), c = 4 * (i % (HD / 4));
-        float M = -INFINITY, L = 0.0f;
 #pragma unroll
-        for (int v = 0; v < WAVES; ++v) M = fmaxf(M, sm[v][row]);
+    for (int row = tid / (HD / 4); row < 16; row += 64 * WAVES / (HD / 4)) {
+        if (row >= sg.rows) break;
+        v4f part[WAVES];
+        float pm[WAVES], pl[WAVES];
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) {
+            part[v] = *reinterpret_cast<const v4f *>(ob + (v * sg.rows + row) * HD + c);
+            pm[v] = sm[v][row];
+            pl[v] = sl[v][row];
+        }
+        const float M = fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]));
+        float L = 0.0f;
         v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int v = 0; v < WAVES; ++v) {
-            const float f = weight_from(sm[v][row], M);  // (a wave without tokens holds zeros)
-            L += sl[v][row] * f;
-            const v4f x4 = *reinterpret_cast<const v4f *>(ob + ((size_t)v * sg.rows + row) * HD + c);
+            const float f = weight_from(pm[v], M);  // (a wave without tokens holds zeros)
+            L += pl[v] * f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] = fmaf(x4[e], f, acc[e]);
+            for (int e = 0; e < 4; ++e) acc[e] = fmaf(part[v][e], f, acc[e]);
         }
         if (!Path::exact)
             z += L * 0.0f + (acc[0] * 0.0f + acc[1] * 0.0f) + (acc[2] * 0.0f + acc[3] * 0.0f);
-        if (whole) {
+        float2 *ml;
+        if (slot < 0) {  // the whole pair
+            const size_t at = (size_t)sg.b * a.heads + sg.j0 + row;
+            float *out = a.out + at * hd + c;
             const float f = L != 0.0f ? p.v_scale / L : 0.0f;
-            float *out = a.out + ((size_t)sg.b * a.heads + sg.j0 + row) * hd + c;
             if (hd % 4 == 0) {
                 if (c < hd) *reinterpret_cast<v4f *>(out) = acc * f;
             } else {
@@ -623,12 +626,13 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
                 for (int e = 0; e < 4; ++e)
                     if (c + e < hd) out[e] = acc[e] * f;
             }
-            if (w.ml && c == 0) w.ml[(size_t)sg.b * a.heads + sg.j0 + row] = make_float2(M, L);
+            ml = w.ml ? w.ml + at : nullptr;
         } else {
-            if (c < w.row)
-                *reinterpret_cast<v4f *>(w.part_o + ((size_t)slot * 16 + row) * w.row + c) = acc;
-            if (c == 0) w.part_ml[(size_t)slot * 16 + row] = make_float2(M, L);
+            const size_t at = (size_t)slot * 16 + row;
+            if (c < w.row) *reinterpret_cast<v4f *>(w.part_o + at * w.row + c) = acc;
+            ml = w.part_ml + at;
         }
+        if (c == 0 && ml) *ml = make_float2(M, L);
     }
     if constexpr (Path::exact) return true;
     // a sum that is not finite is not this path's to say
@@ -839,8 +843,8 @@ size_t attend_ws(const ornk_kv_pages *p, const ornk_attend_args *a, AttendWs *w)
         off += (n + 255) & ~(size_t)255;
         return at;
     };
-    const int G = a->heads / p->kv, W = 1 << (CUS_LOG2 + (p->hd > 128 ? 0 : 1));
     w->w_log2 = CUS_LOG2 + (p->hd > 128 ? 0 : 1);
+    const int G = a->heads / p->kv, W = 1 << w->w_log2;
     w->row = (p->hd + 3) & ~3;
     w->unit_log2 = UNIT_LOG2;
     const size_t pairs = (size_t)a->n_seqs * p->kv * ((G + 15) / 16);
