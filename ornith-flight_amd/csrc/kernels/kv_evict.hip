@@ -8,7 +8,7 @@
 
 namespace {
 
-constexpr int CT = 1024, PER = 16;  // threads of the choosing work group, scores of a thread
+constexpr int CT = 1024;  // threads of the choosing work group
 constexpr int BINS = 2048;
 
 // Order of the scores as unsigned integers: a NaN is 0, -0 counts as +0.
@@ -24,6 +24,7 @@ __device__ __forceinline__ uint32_t order_key(float f)
 // counting (11, 11 and 10 bits of the keys, from the top) find the lowest key
 // that stays and how many of its equals do; then one scan numbers the kept
 // tokens in order.  Longer sequences read their scores again in every round.
+template <int PER>
 __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict_args a)
 {
     __shared__ int hist[BINS], wsum[CT / 64], sh[2];
@@ -104,7 +105,7 @@ __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict
             if (len <= a.keep || i < lo || i >= hi || k > key) sure |= 1u << e;
             else if (k == key) tie |= 1u << e;
         }
-        // both counts in one word: a stretch has CT * PER = 2^14 tokens
+        // both counts in one word: a stretch has CT * PER <= 2^14 tokens
         const int mine = __popc(sure) | __popc(tie) << 16;
         const int after = later(mine);
         if (tid == 0) sh[0] = mine + after;
@@ -129,61 +130,75 @@ __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict
     for (int i = n + tid; i < a.keep; i += CT) kept[i] = -1;
 }
 
-// The kept rows to their new places, in words of WORD bytes.  A work group takes
-// rows of one kv head, sequence and K or V, MR at a time: their addresses go
-// through LDS, then every thread copies its words.
+// The kept rows to their new places, in words of WORD.  A work group takes rows
+// of one kv head, sequence and K or V, a stretch at a time: the rows' places go
+// through LDS, then every thread has up to MB words in flight.
 //
-// Into other pages, each group takes one stretch of MR rows whole.  Within a
+// Into other pages, each group takes one stretch of whole rows.  Within a
 // sequence's own pages (IN_PLACE) a row moves towards the front or stays: a
 // group takes every row, one stretch after the other, of SLICE bytes of the
 // columns; a stretch is read whole before any of it is written, and no later
 // stretch reads what it writes.
-constexpr int MT = 256, MR = 64, SLICE = 64;
+constexpr int MT = 256, MB = 4, SLICE = 64;
+
+// Rows of a stretch, of `words` words each (at most MT): MB for every thread.
+__host__ __device__ inline int stretch_rows(int words)
+{
+    const int n = MB * (MT / words);
+    return n < MT ? n : MT;
+}
 
 template <class WORD, bool IN_PLACE>
 __global__ void __launch_bounds__(MT) k_evict_move(ornk_kv_pages p, ornk_evict_args a, int row_bytes)
 {
-    __shared__ const uint8_t *from[MR];
-    __shared__ uint8_t *to[MR];
-    constexpr int WB = sizeof(WORD), NW = IN_PLACE ? MR * (SLICE / WB) / MT : 4;
+    constexpr int WB = sizeof(WORD);
+    __shared__ size_t from[MT], to[MT];  // bytes into the pages; NONE: the row stays where it is
+    constexpr size_t NONE = ~(size_t)0;
     const int h = blockIdx.y % p.kv, b = blockIdx.z, tid = threadIdx.x;
-    const int n = a.counts[b];
     const int *kept = a.kept + ((size_t)b * p.kv + h) * a.keep;
-    uint8_t *pool = static_cast<uint8_t *>(blockIdx.y >= p.kv ? p.v : p.k);
-    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) a.dst_lens[b] = n;
-    const int es = row_bytes / p.hd;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) a.dst_lens[b] = a.counts[b];
+    const int es = row_bytes / p.hd, most = min(a.keep, a.max_len);
     const int c0 = IN_PLACE ? blockIdx.x * SLICE : 0;
     const int words = (IN_PLACE ? min(SLICE, row_bytes - c0) : row_bytes) / WB;
-    for (int j0 = IN_PLACE ? 0 : blockIdx.x * MR; j0 < n; j0 += MR) {
-        const int rows = min(MR, n - j0);
+    const int pass = MT / words, mr = stretch_rows(words);
+    const int r0 = tid / words < pass ? tid / words : MT, col = tid % words * WB;
+    uint8_t *pool = static_cast<uint8_t *>(blockIdx.y >= p.kv ? p.v : p.k) + c0;
+    for (int j0 = IN_PLACE ? 0 : blockIdx.x * mr; j0 < most; j0 += mr) {
+        const int rows = min(mr, most - j0);
+        int some = 0;  // (kept is -1 past the sequence's last)
         if (tid < rows) {
             const int j = j0 + tid, i = kept[j];
-            const int pf = kv_page(p, a.table[(size_t)b * a.max_pages + (i >> p.page_log2)], b);
-            const int pt = kv_page(p, a.dst_table[(size_t)b * a.dst_pages + (j >> p.page_log2)], b);
-            const bool on = pf >= 0 && pt >= 0 && !(IN_PLACE && i == j);
-            from[tid] = on ? pool + kv_at(p, pf, h, i & (p.page - 1)) * es + c0 : nullptr;
-            to[tid] = on ? pool + kv_at(p, pt, h, j & (p.page - 1)) * es + c0 : nullptr;
+            some = i >= 0;
+            size_t f = NONE, t = NONE;
+            if (some && !(IN_PLACE && i == j)) {
+                const int pf = kv_page(p, a.table[(size_t)b * a.max_pages + (i >> p.page_log2)], b);
+                const int pt = kv_page(p, a.dst_table[(size_t)b * a.dst_pages + (j >> p.page_log2)], b);
+                if (pf >= 0 && pt >= 0) {
+                    f = kv_at(p, pf, h, i & (p.page - 1)) * es;
+                    t = kv_at(p, pt, h, j & (p.page - 1)) * es;
+                }
+            }
+            from[tid] = f;
+            to[tid] = t;
         }
-        __syncthreads();
-        for (int w0 = 0; w0 < rows * words; w0 += NW * MT) {
-            WORD v[NW];
+        if (!__syncthreads_or(some)) break;
+        WORD v[MB];
+        size_t f[MB];
 #pragma unroll
-            for (int k = 0; k < NW; ++k) {
-                const int w = w0 + k * MT + tid, r = w / words;
-                if (w < rows * words && from[r])
-                    v[k] = *reinterpret_cast<const WORD *>(from[r] + (size_t)(w - r * words) * WB);
-            }
-            if (IN_PLACE) {  // one pass: NW * MT words hold a stretch
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                __syncthreads();
-            }
-#pragma unroll
-            for (int k = 0; k < NW; ++k) {
-                const int w = w0 + k * MT + tid, r = w / words;
-                if (w < rows * words && to[r])
-                    *reinterpret_cast<WORD *>(to[r] + (size_t)(w - r * words) * WB) = v[k];
-            }
+        for (int k = 0; k < MB; ++k) {
+            const int r = r0 + k * pass;
+            f[k] = r < rows ? from[r] : NONE;
         }
+#pragma unroll
+        for (int k = 0; k < MB; ++k)
+            if (f[k] != NONE) v[k] = *reinterpret_cast<const WORD *>(pool + f[k] + col);
+        if (IN_PLACE) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+        }
+#pragma unroll
+        for (int k = 0; k < MB; ++k)
+            if (f[k] != NONE) *reinterpret_cast<WORD *>(pool + to[r0 + k * pass] + col) = v[k];
         if (!IN_PLACE) break;
         __syncthreads();
     }
@@ -194,12 +209,14 @@ void move(const ornk_kv_pages &p, const ornk_evict_args &a, int row_bytes, hipSt
 {
     const int most = a.keep < a.max_len ? a.keep : a.max_len;
     const unsigned y = 2 * p.kv, z = a.n_seqs;
-    if (a.in_place)
+    if (a.in_place) {
         hipLaunchKernelGGL((k_evict_move<WORD, true>), dim3((row_bytes + SLICE - 1) / SLICE, y, z),
                            dim3(MT), 0, s, p, a, row_bytes);
-    else
-        hipLaunchKernelGGL((k_evict_move<WORD, false>), dim3(most ? (most + MR - 1) / MR : 1, y, z),
-                           dim3(MT), 0, s, p, a, row_bytes);
+        return;
+    }
+    const int mr = stretch_rows(row_bytes / (int)sizeof(WORD));
+    hipLaunchKernelGGL((k_evict_move<WORD, false>), dim3(most ? (most + mr - 1) / mr : 1, y, z),
+                       dim3(MT), 0, s, p, a, row_bytes);
 }
 
 }  // namespace
@@ -207,8 +224,12 @@ void move(const ornk_kv_pages &p, const ornk_evict_args &a, int row_bytes, hipSt
 extern "C" int ornk_kv_evict(const ornk_kv_pages *p, const ornk_evict_args *a, hipStream_t s)
 {
     const int rb = p->hd * (p->type == ORN_KV_F32 ? 4 : p->type == ORN_KV_E4M3 ? 1 : 2);
-    hipLaunchKernelGGL(k_evict_choose, dim3(p->kv, a->n_seqs), dim3(CT), 0, s, *p, *a);
-    if (rb % 16 == 0) move<uint4>(*p, *a, rb, s);
+    if (a->max_len <= 4 * CT)
+        hipLaunchKernelGGL(k_evict_choose<4>, dim3(p->kv, a->n_seqs), dim3(CT), 0, s, *p, *a);
+    else
+        hipLaunchKernelGGL(k_evict_choose<16>, dim3(p->kv, a->n_seqs), dim3(CT), 0, s, *p, *a);
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    if (rb % 16 == 0) move<u4>(*p, *a, rb, s);
     else if (rb % 4 == 0) move<uint32_t>(*p, *a, rb, s);
     else if (rb % 2 == 0) move<uint16_t>(*p, *a, rb, s);
     else move<uint8_t>(*p, *a, rb, s);
