@@ -19,15 +19,18 @@ __device__ __forceinline__ uint32_t order_key(float f)
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// One work group per kv head and sequence; a thread holds PER consecutive
-// scores of a stretch.  Where the tokens are more than `keep`, three rounds of
-// counting (11, 11 and 10 bits of the keys, from the top) find the lowest key
-// that stays and how many of its equals do; then one scan numbers the kept
-// tokens in order.  Longer sequences read their scores again in every round.
+// One work group per kv head and sequence; a thread holds PER scores of a
+// stretch of CT * PER, every CT-th one.  Where the tokens are more than `keep`,
+// three rounds of counting (11, 11 and 10 bits of the keys, from the top) find
+// the lowest key that stays and how many of its equals do; then one scan over
+// the waves' counts numbers the kept tokens in order.  Sequences longer than
+// the largest stretch read their scores again in every round.
 template <int PER>
 __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict_args a)
 {
-    __shared__ int hist[BINS], wsum[CT / 64], sh[2];
+    constexpr int NW = CT / 64, NC = PER * NW;  // waves; counts of a stretch
+    __shared__ int hist[BINS], wsum[2][NW], sh[2];
+    __shared__ int2 count[NC];
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int len = kv_len(p, a.lens[b], b, a.max_len), n = min(len, a.keep);
     const float *score = a.score + ((size_t)b * p.kv + h) * a.score_stride;
@@ -37,26 +40,27 @@ __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict
     const int lo = a.sink, hi = len - a.recent;  // the tokens that the scores decide on
     const bool one = len <= CT * PER;
     float f[PER];
-    auto load = [&](int i0) {
+    auto load = [&](long long i0) {
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
-            const int i = i0 + PER * tid + e;
+            const long long i = i0 + e * CT + tid;
             f[e] = i < len ? score[i] : 0.0f;
         }
     };
-    // the sum of the later threads' v, of the threads' of one work group
-    auto later = [&](int v) {
+    // the sum over the work group's threads before this one, from the first
+    // (dir = 1) or from the last (-1)
+    auto before = [&](int v, int dir, int k) {
         int x = v;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
-            const int y = __shfl_down(x, d, 64);
-            if (lane + d < 64) x += y;
+            const int y = __shfl(x, lane - dir * d, 64);
+            if (dir > 0 ? lane >= d : lane + d < 64) x += y;
         }
-        if (lane == 0) wsum[wave] = x;
+        if (lane == (dir > 0 ? 63 : 0)) wsum[k][wave] = x;
         __syncthreads();
         x -= v;
-        for (int w = wave + 1; w < CT / 64; ++w) x += wsum[w];
-        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NW; ++w) x += (dir > 0 ? w < wave : w > wave) ? wsum[k][w] : 0;
         return x;
     };
 
@@ -70,61 +74,65 @@ __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict
             const int shift = round == 0 ? 21 : round == 1 ? 10 : 0;
             const uint32_t mask = round == 2 ? 1023u : 2047u;
             const uint32_t fixed = round == 0 ? 0u : round == 1 ? ~0u << 21 : ~0u << 10;
-            for (int i = tid; i < BINS; i += CT) hist[i] = 0;
+            hist[tid] = hist[tid + CT] = 0;
             __syncthreads();
-            for (int i0 = 0; i0 < len; i0 += CT * PER) {
+            for (long long i0 = 0; i0 < len; i0 += CT * PER) {
                 if (!one) load(i0);
 #pragma unroll
                 for (int e = 0; e < PER; ++e) {
-                    const int i = i0 + PER * tid + e;
+                    const long long i = i0 + e * CT + tid;
                     const uint32_t k = order_key(f[e]);
                     if (i >= lo && i < hi && (k & fixed) == key) atomicAdd(&hist[(k >> shift) & mask], 1);
                 }
             }
             __syncthreads();
             const int c0 = hist[2 * tid], c1 = hist[2 * tid + 1];
-            const int above = later(c0 + c1);
+            const int above = before(c0 + c1, -1, 0);
             if (above < left && left <= above + c1) sh[0] = 2 * tid + 1, sh[1] = above;
             else if (above + c1 < left && left <= above + c1 + c0) sh[0] = 2 * tid, sh[1] = above + c1;
             __syncthreads();
             key |= (uint32_t)sh[0] << shift;
             left -= sh[1];
-            __syncthreads();
         }
         ties = left;
     }
     int base = 0, eq_base = 0;  // kept for certain, and ties, before this stretch
-    for (int i0 = 0; i0 < len; i0 += CT * PER) {
+    for (long long i0 = 0; i0 < len; i0 += CT * PER) {
         if (!one) load(i0);
-        uint32_t sure = 0, tie = 0;
+        uint64_t sure = 0, tie = 0;  // bit e
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
-            const int i = i0 + PER * tid + e;
-            if (i >= len) continue;
+            const long long i = i0 + e * CT + tid;
             const uint32_t k = order_key(f[e]);
-            if (len <= a.keep || i < lo || i >= hi || k > key) sure |= 1u << e;
-            else if (k == key) tie |= 1u << e;
+            const bool s = i < len && (len <= a.keep || i < lo || i >= hi || k > key);
+            const bool t = i < len && !s && k == key;
+            const uint64_t bs = __ballot(s), bt = __ballot(t);
+            if (lane == 0) count[e * NW + wave] = make_int2(__popcll(bs), __popcll(bt));
+            sure |= (uint64_t)s << e;
+            tie |= (uint64_t)t << e;
         }
-        // both counts in one word: a stretch has CT * PER <= 2^14 tokens
-        const int mine = __popc(sure) | __popc(tie) << 16;
-        const int after = later(mine);
-        if (tid == 0) sh[0] = mine + after;
         __syncthreads();  // also: every score of this stretch has been read
-        const int before = sh[0] - after - mine;
-        int at = base + (before & 0xffff), eq = eq_base + (before >> 16);
+        const int2 c = tid < NC ? count[tid] : make_int2(0, 0);
+        const int cs = before(c.x, 1, 0), ct = before(c.y, 1, 1);
+        if (tid < NC) count[tid] = make_int2(cs, ct);
+        if (tid == CT - 1) sh[0] = cs + c.x, sh[1] = ct + c.y;
+        __syncthreads();
+        const uint64_t mine = ((uint64_t)1 << lane) - 1;
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
-            const bool t = tie >> e & 1;
-            if ((sure >> e & 1) || (t && eq < ties)) {
-                const int j = at + min(eq, ties);
-                kept[j] = i0 + PER * tid + e;
+            const bool s = sure >> e & 1, t = tie >> e & 1;
+            const uint64_t bs = __ballot(s), bt = __ballot(t);
+            if (!(bs | bt)) continue;
+            const int2 c = count[e * NW + wave];
+            const int eq = eq_base + c.y + __popcll(bt & mine);
+            if (s || (t && eq < ties)) {
+                const int j = base + c.x + __popcll(bs & mine) + min(eq, ties);
+                kept[j] = (int)(i0 + e * CT + tid);
                 if (ds) ds[j] = f[e];
-                at += sure >> e & 1;
             }
-            eq += t;
         }
-        base += sh[0] & 0xffff;
-        eq_base += sh[0] >> 16;
+        base += sh[0];
+        eq_base += sh[1];
         __syncthreads();
     }
     for (int i = n + tid; i < a.keep; i += CT) kept[i] = -1;
@@ -226,8 +234,10 @@ extern "C" int ornk_kv_evict(const ornk_kv_pages *p, const ornk_evict_args *a, h
     const int rb = p->hd * (p->type == ORN_KV_F32 ? 4 : p->type == ORN_KV_E4M3 ? 1 : 2);
     if (a->max_len <= 4 * CT)
         hipLaunchKernelGGL(k_evict_choose<4>, dim3(p->kv, a->n_seqs), dim3(CT), 0, s, *p, *a);
-    else
+    else if (a->max_len <= 16 * CT)
         hipLaunchKernelGGL(k_evict_choose<16>, dim3(p->kv, a->n_seqs), dim3(CT), 0, s, *p, *a);
+    else
+        hipLaunchKernelGGL(k_evict_choose<64>, dim3(p->kv, a->n_seqs), dim3(CT), 0, s, *p, *a);
     typedef uint32_t u4 __attribute__((ext_vector_type(4)));
     if (rb % 16 == 0) move<u4>(*p, *a, rb, s);
     else if (rb % 4 == 0) move<uint32_t>(*p, *a, rb, s);

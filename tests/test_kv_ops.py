@@ -895,7 +895,7 @@ EVICTS = [  # kv, D, page, lengths, keep, sink, recent
     (2, 64, 16, [100, 0, 20, 1, 21], 20, 4, 6), (1, 256, 16, [700], 350, 4, 64),
     (3, 33, 8, [90, 41], 40, 0, 0), (1, 1, 8, [50], 1, 0, 0), (2, 7, 16, [64, 65], 64, 64, 0),
     (1, 128, 32, [300, 299], 40, 0, 40), (4, 80, 64, [2500, 130, 1025], 1000, 10, 100),
-    (1, 8, 8, [5000], 4999, 1, 1), (2, 96, 16, [33], 500, 3, 3), (1, 4, 1024, [9000], 3001, 5, 7)]
+    (1, 8, 8, [5000], 4999, 1, 1), (2, 8, 64, [17000, 16384], 4000, 0, 9), (1, 4, 128, [70001], 20000, 2, 2), (2, 96, 16, [33], 500, 3, 3), (1, 4, 1024, [9000], 3001, 5, 7)]
 
 
 @pytest.mark.gpu
