@@ -84,11 +84,16 @@ __device__ __forceinline__ void put4(typename KvElem<TYPE>::T *c, v4f x, float i
 // HALVES two float4s of one (pairs p..p+3 lie R apart).  The first items are on
 // their way while the group forms the token's cosines and sines in LDS, once
 // for all its heads.
-constexpr int RT = 256, RI = 4;  // threads, items in flight of each
+//
+// Bound by memory: 4099 tokens of 32 + 8 heads of 128 move 168 MB in 33 us (5.0
+// TB/s), 8190 with the append to e4m3 352 MB in 68 us (5.2 TB/s; a copy 4.7).
+// One item per thread at a time and eight groups per CU: with two items (and
+// 64 registers) 39 and 83 us, with four and five groups 46 and 103 us.
+constexpr int RT = 256;
 constexpr int MAX_GROUPS = 1 << 20;  // of a launch; more tokens take turns
 
 template <int TYPE, bool HALVES>
-__global__ void __launch_bounds__(RT) k_rope_append(ornk_kv_pages p, ornk_rope_args a)
+__global__ void __launch_bounds__(RT, 8) k_rope_append(ornk_kv_pages p, ornk_rope_args a)
 {
     __shared__ __align__(16) float2 cs[ORN_ROPE_MAX_PAIRS];
     const int tid = threadIdx.x, hd = a.hd, R = a.R;
@@ -125,14 +130,13 @@ __global__ void __launch_bounds__(RT) k_rope_append(ornk_kv_pages p, ornk_rope_a
     const float k_inv = 1.0f / p.k_scale, v_inv = 1.0f / p.v_scale;
     for (long long at = blockIdx.x; at < a.T; at += gridDim.x) {
         const int t = (int)at;
-        Item it[RI];
-#pragma unroll
-        for (int k = 0; k < RI; ++k)
-            if (i0 + tid + k * RT < i1) load(it[k], t, i0 + tid + k * RT);
+        Item it;
+        if (i0 + tid < i1) load(it, t, i0 + tid);
         for (int i = tid; i < R; i += RT) cs[i] = rope_cs(a, t, i);
         const int slot = a.slots ? kv_slot(p, a.slots, t) : -1;
         __syncthreads();
-        auto store = [&](const Item &it) {
+        for (int i = i0 + tid; i < i1; i += RT) {
+            if (i != i0 + tid) load(it, t, i);
             const int kvh = it.row - a.heads;  // key heads, then value heads
             v4f x = it.x, y = it.y;
             if (kvh < a.kv) {
@@ -169,16 +173,6 @@ __global__ void __launch_bounds__(RT) k_rope_append(ornk_kv_pages p, ornk_rope_a
                 put4<TYPE>(c, x, key ? k_inv : v_inv);
                 if (it.two) put4<TYPE>(c + R, y, k_inv);
             }
-        };
-        for (int i = i0 + tid;;) {
-#pragma unroll
-            for (int k = 0; k < RI; ++k)
-                if (i + k * RT < i1) store(it[k]);
-            i += RI * RT;
-            if (i >= i1) break;
-#pragma unroll
-            for (int k = 0; k < RI; ++k)
-                if (i + k * RT < i1) load(it[k], t, i + k * RT);
         }
         __syncthreads();  // the token's angles are consumed
     }
