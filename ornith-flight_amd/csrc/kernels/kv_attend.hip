@@ -8,7 +8,7 @@
 // heads ("pair") in units of 128, one after the other on a line.  W work groups
 // take equal stretches of the line, whatever the lengths are; a pair that one
 // group covers is finished there, of the others the groups leave O, m and l of
-// their part, which k_kv_join puts together:
+// their part, which k_kv_finish puts together:
 //   M = max m_i, L = sum l_i 2^(m_i - M), out = sum O_i 2^(m_i - M) / L.
 // (Exponents are base 2: log2 e is in the query's scale.)
 #include "kv.h"
@@ -753,23 +753,40 @@ __global__ void __launch_bounds__(64 * WAVES, per_cu<HD>) k_kv_attend(ornk_kv_pa
     }
 }
 
-// The parts of a pair put together, JC float4s of its rows per work group by JS
-// shares of the parts.
-constexpr int JC = 32, JS = 8;
-__global__ void __launch_bounds__(JC * JS) k_kv_join(ornk_kv_pages p, ornk_attend_args a, AttendWs w)
+// The parts of a pair: the first one's slot, the others' follow (2 (w0 + i)).
+struct PairParts {
+    uint32_t n, w0, first;  // 1: a group has finished the pair
+    __device__ __forceinline__ size_t slot(uint32_t i) const { return i ? 2 * (w0 + i) : first; }
+};
+__device__ __forceinline__ PairParts parts_of(const AttendWs &w, uint32_t per, int n_seqs, int b, int pair)
+{
+    const uint32_t before = w.cum[b], n = w.cum[b + 1] - before, T = w.cum[n_seqs] * per;
+    const uint32_t s = before * per + pair * n;
+    PairParts r = {n, 0, 0};
+    if (n < 2) return r;  // no tokens, or one unit
+    r.w0 = line_group(T, w.w_log2, s);
+    r.n = line_group(T, w.w_log2, s + n - 1) - r.w0 + 1;
+    r.first = 2 * r.w0 + (line_at(T, w.w_log2, r.w0) == s ? 0 : 1);
+    return r;
+}
+
+// What is left after the groups, in one launch.  Work groups blockIdx.x < jx:
+// the parts of a pair put together, JC float4s of its rows by JS shares of the
+// parts.  The others, where the weights are asked for: what 4 FT tokens got,
+// summed over a kv head's query heads; they put the parts' maxima and sums
+// together for themselves.
+constexpr int JC = 32, JS = 8, FT = JC * JS;
+
+__device__ __forceinline__ void join_pair(const ornk_kv_pages &p, const ornk_attend_args &a, const AttendWs &w)
 {
     __shared__ float sm[JS][JC], sl[JS][JC];
     __shared__ v4f so[JS][JC];
     const int b = blockIdx.z, pair = blockIdx.y, G = a.heads / p.kv, HT = (G + 15) / 16, hd = p.hd;
-    const uint32_t per = p.kv * HT, before = w.cum[b], n = w.cum[b + 1] - before, T = w.cum[a.n_seqs] * per;
-    const uint32_t s = before * per + pair * n;
-    if (n < 2) return;  // no tokens, or one unit
-    const uint32_t w0 = line_group(T, w.w_log2, s), nseg = line_group(T, w.w_log2, s + n - 1) - w0 + 1;
-    if (nseg == 1) return;  // finished by one group
+    const PairParts seg = parts_of(w, p.kv * HT, a.n_seqs, b, pair);
+    if (seg.n < 2) return;
     const int j = 16 * (pair % HT), rows = min(16, G - j), j0 = pair / HT * G + j;
     const int x = threadIdx.x % JC, sub = threadIdx.x / JC, at = blockIdx.x * JC + x;
     const int row = at / (w.row / 4), c = at % (w.row / 4) * 4;
-    const uint32_t first = 2 * w0 + (line_at(T, w.w_log2, w0) == s ? 0 : 1);
     float m = -INFINITY, l = 0.0f;
     v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
     auto add = [&](float m2, float l2, v4f o2) {
@@ -781,8 +798,8 @@ __global__ void __launch_bounds__(JC * JS) k_kv_join(ornk_kv_pages p, ornk_atten
     };
     if (row < rows)
 #pragma unroll 4
-        for (uint32_t i = sub; i < nseg; i += JS) {
-            const size_t slot = (size_t)(i ? 2 * (w0 + i) : first) * 16 + row;
+        for (uint32_t i = sub; i < seg.n; i += JS) {
+            const size_t slot = seg.slot(i) * 16 + row;
             const float2 ml = w.part_ml[slot];
             add(ml.x, ml.y, *reinterpret_cast<const v4f *>(w.part_o + slot * w.row + c));
         }
@@ -797,28 +814,54 @@ __global__ void __launch_bounds__(JC * JS) k_kv_join(ornk_kv_pages p, ornk_atten
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (c + e < hd) out[e] = o[e] * f;
-    if (w.ml && c == 0) w.ml[(size_t)b * a.heads + j0 + row] = make_float2(m, l);
 }
 
-// The weights each token got, summed over a kv head's query heads; four tokens
-// per thread.
-constexpr int ST = 256;
-__global__ void __launch_bounds__(ST) k_kv_score(ornk_kv_pages p, ornk_attend_args a, AttendWs w)
+__device__ __forceinline__ void sum_weights(const ornk_kv_pages &p, const ornk_attend_args &a,
+                                            const AttendWs &w, int chunk)
 {
-    const int h = blockIdx.y, b = blockIdx.z, G = a.heads / p.kv;
+    __shared__ float2 mi[16];  // of a tile's query heads: maximum, 1 / sum
+    const int b = blockIdx.z, G = a.heads / p.kv, HT = (G + 15) / 16, h = blockIdx.y / HT;
     const int len = min(max(a.lens[b], 0), a.max_len);
-    const long long t = ((long long)blockIdx.x * ST + threadIdx.x) * 4;
-    if (t >= len) return;
-    const size_t row = (size_t)b * a.heads + h * G;
+    const long long t0 = (long long)chunk * FT * 4, t = t0 + threadIdx.x * 4;
+    if (blockIdx.y % HT || t0 >= len) return;
     v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int tile = 0; tile < HT; ++tile) {
+        const size_t j0 = (size_t)b * a.heads + h * G + 16 * tile;
+        const int rows = min(16, G - 16 * tile), row = threadIdx.x / 16, share = threadIdx.x % 16;
+        const PairParts seg = parts_of(w, p.kv * HT, a.n_seqs, b, h * HT + tile);
+        float m = -INFINITY, l = 0.0f;
+        auto add = [&](float m2, float l2) {
+            const float mn = fmaxf(m, m2);
+            l = l * weight_from(m, mn) + l2 * weight_from(m2, mn);
+            m = mn;
+        };
+        if (row < rows) {
+            if (seg.n < 2) {
+                const float2 ml = w.ml[j0 + row];
+                m = ml.x, l = share ? 0.0f : ml.y;
+            } else {
 #pragma unroll 4
-    for (int g = 0; g < G; ++g) {
-        const float2 ml = w.ml[row + g];
-        const v4f s = *reinterpret_cast<const v4f *>(w.s + (row + g) * w.s_len + t);
-        const float f = 1.0f / ml.y;
+                for (uint32_t i = share; i < seg.n; i += 16) {
+                    const float2 ml = w.part_ml[seg.slot(i) * 16 + row];
+                    add(ml.x, ml.y);
+                }
+            }
+        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum[e] += s[e] == -INFINITY ? 0.0f : exp2_(s[e] - ml.x) * f;
+        for (int d = 8; d; d >>= 1) add(__shfl_xor(m, d, 16), __shfl_xor(l, d, 16));
+        __syncthreads();  // the last tile's are consumed
+        if (share == 0) mi[row] = make_float2(m, 1.0f / l);
+        __syncthreads();
+        if (t >= len) continue;
+#pragma unroll 4
+        for (int g = 0; g < rows; ++g) {
+            const v4f s = *reinterpret_cast<const v4f *>(w.s + (j0 + g) * w.s_len + t);
+            const float2 ml = mi[g];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] += s[e] == -INFINITY ? 0.0f : exp2_(s[e] - ml.x) * ml.y;
+        }
     }
+    if (t >= len) return;
     const size_t i = ((size_t)b * p.kv + h) * a.score_stride + t;
     if (a.score_stride % 4 == 0 && t + 4 <= len) {
         if (a.score_in) {
@@ -832,6 +875,12 @@ __global__ void __launch_bounds__(ST) k_kv_score(ornk_kv_pages p, ornk_attend_ar
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (t + e < len) a.score_out[i + e] = a.score_in ? fmaf(a.decay, a.score_in[i + e], sum[e]) : sum[e];
+}
+
+__global__ void __launch_bounds__(FT) k_kv_finish(ornk_kv_pages p, ornk_attend_args a, AttendWs w, int jx)
+{
+    if ((int)blockIdx.x < jx) join_pair(p, a, w);
+    else sum_weights(p, a, w, blockIdx.x - jx);
 }
 
 size_t attend_ws(const ornk_kv_pages *p, const ornk_attend_args *a, AttendWs *w)
@@ -918,11 +967,10 @@ extern "C" int ornk_kv_attend(const ornk_kv_pages *p, const ornk_attend_args *a,
                                       : launch_type<ORN_KV_E4M3>(p, a, w, s);
     if (rc != hipSuccess) return rc;
     const int G = a->heads / p->kv, HT = (G + 15) / 16;
-    if (a->max_len > 1 << w.unit_log2)  // else every pair is one unit
-        hipLaunchKernelGGL(k_kv_join, dim3(((G < 16 ? G : 16) * (w.row / 4) + JC - 1) / JC, p->kv * HT, a->n_seqs),
-                           dim3(JC * JS), 0, s, *p, *a, w);
-    if (a->score_out && a->max_len)
-        hipLaunchKernelGGL(k_kv_score, dim3(((unsigned)a->max_len + 4 * ST - 1) / (4 * ST), p->kv, a->n_seqs),
-                           dim3(ST), 0, s, *p, *a, w);
+    const int jx = a->max_len > 1 << w.unit_log2  // else every pair is one unit
+                       ? ((G < 16 ? G : 16) * (w.row / 4) + JC - 1) / JC : 0;
+    const int sx = a->score_out ? (int)(((long long)a->max_len + 4 * FT - 1) / (4 * FT)) : 0;
+    if (jx + sx)
+        hipLaunchKernelGGL(k_kv_finish, dim3(jx + sx, p->kv * HT, a->n_seqs), dim3(FT), 0, s, *p, *a, w, jx);
     return hipGetLastError();
 }
