@@ -54,7 +54,7 @@ int gpu_kv_cache_append(gpu_context *ctx, gpu_buffer *K_cache, gpu_buffer *V_cac
  *
  * Activations are fp32, lengths, positions, slots and page numbers int32, all
  * in buffers of the context; a call takes up to 65535 sequences and as many
- * heads.  Calls return 0 or a negative status, run on the
+ * heads, of at most 2^31 - 2^16 tokens (max_pages * page_size).  Calls return 0 or a negative status, run on the
  * context's stream and are synchronous unless ORN_KV_ASYNC is given.
  *
  * Numbers in device buffers are checked by the kernels: a page number outside

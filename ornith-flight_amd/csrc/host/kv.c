@@ -275,7 +275,7 @@ static int seqs_ok(gpu_context *ctx, const ornk_kv_pages *p, int n_seqs, const g
     if (n_seqs > 65535)
         return orn_set_err(ctx, ORN_EUNSUPPORTED, "%s: %d sequences (at most 65535)", who, n_seqs);
     const long long width = (long long)max_pages * p->page;
-    if (width > 0x7fffffffll || max_len > width)
+    if (width > 0x7fff0000ll || max_len > width)  /* indexes a stretch past a length fit an int */
         return orn_set_err(ctx, ORN_EINVAL, "%s: max_len %d, and %d pages of %d in the table", who,
                            max_len, max_pages, p->page);
     if (!holds(table, span(n_seqs, max_pages, 1, 1, 4)) || !holds(lens, span(n_seqs, 1, 1, 1, 4)))

@@ -81,3 +81,15 @@ __device__ __forceinline__ int kv_slot(const ornk_kv_pages &p, const int *slots,
     if (slot != -1) kv_error(p, ORNK_KV_ERR_SLOT, t);
     return -1;
 }
+
+// Inclusive sum over the lanes of a wave.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x)
+{
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
+    return x;
+}

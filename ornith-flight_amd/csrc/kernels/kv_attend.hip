@@ -641,18 +641,6 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
     return odd == 0;
 }
 
-// Inclusive sum over the lanes of a wave.
-__device__ __forceinline__ uint32_t wave_scan(uint32_t x)
-{
-    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
-    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
-    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
-    return x;
-}
-
 // A stretch of 256 sequences, four to a lane; every wave has it for itself, so
 // that finding one's place on the line takes no barrier.
 constexpr int STRETCH = 256;

@@ -21,16 +21,16 @@ __device__ __forceinline__ uint32_t order_key(float f)
 
 // One work group per kv head and sequence; a thread holds PER scores of a
 // stretch of CT * PER, every CT-th one.  Where the tokens are more than `keep`,
-// three rounds of counting (11, 11 and 10 bits of the keys, from the top) find
-// the lowest key that stays and how many of its equals do; then one scan over
+// up to three rounds of counting (11, 11 and 10 bits of the keys, from the top)
+// find the lowest key that stays and how many of its equals do; then one scan over
 // the waves' counts numbers the kept tokens in order.  Sequences longer than
 // the largest stretch read their scores again in every round.
 template <int PER>
 __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict_args a)
 {
     constexpr int NW = CT / 64, NC = PER * NW;  // waves; counts of a stretch
-    __shared__ int hist[BINS], wsum[2][NW], sh[2];
-    __shared__ int2 count[NC];
+    __shared__ uint32_t hist[3][BINS], wsum[2][NW], sh[3];
+    __shared__ uint2 count[NC];
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int len = kv_len(p, a.lens[b], b, a.max_len), n = min(len, a.keep);
     const float *score = a.score + ((size_t)b * p.kv + h) * a.score_stride;
@@ -40,81 +40,89 @@ __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict
     const int lo = a.sink, hi = len - a.recent;  // the tokens that the scores decide on
     const bool one = len <= CT * PER;
     float f[PER];
-    auto load = [&](long long i0) {
+    auto load = [&](int i0) {  // (lengths leave room for a stretch below 2^31)
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
-            const long long i = i0 + e * CT + tid;
+            const int i = i0 + e * CT + tid;
             f[e] = i < len ? score[i] : 0.0f;
         }
     };
-    // the sum over the work group's threads before this one, from the first
-    // (dir = 1) or from the last (-1)
-    auto before = [&](int v, int dir, int k) {
-        int x = v;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int y = __shfl(x, lane - dir * d, 64);
-            if (dir > 0 ? lane >= d : lane + d < 64) x += y;
-        }
-        if (lane == (dir > 0 ? 63 : 0)) wsum[k][wave] = x;
+    // the sums of x and y over the work group's threads before this one
+    auto before = [&](uint32_t &x, uint32_t &y) {
+        const uint32_t sx = wave_scan(x), sy = wave_scan(y);
+        if (lane == 63) wsum[0][wave] = sx, wsum[1][wave] = sy;
         __syncthreads();
-        x -= v;
+        x = sx - x;
+        y = sy - y;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) x += (dir > 0 ? w < wave : w > wave) ? wsum[k][w] : 0;
-        return x;
+        for (int w = 0; w < NW; ++w) {
+            x += w < wave ? wsum[0][w] : 0;
+            y += w < wave ? wsum[1][w] : 0;
+        }
     };
 
     uint32_t key = 0;  // the lowest key that stays
     int ties = 0;      // and how many tokens of that key
     if (one) load(0);
     if (len > a.keep) {
+        for (int i = tid; i < 3 * BINS; i += CT) hist[0][i] = 0;
+        __syncthreads();
         int left = a.keep - a.sink - a.recent;
         if (left == 0) key = 0xffffffffu;  // above every key
         for (int round = 0; round < 3 && left; ++round) {
             const int shift = round == 0 ? 21 : round == 1 ? 10 : 0;
             const uint32_t mask = round == 2 ? 1023u : 2047u;
             const uint32_t fixed = round == 0 ? 0u : round == 1 ? ~0u << 21 : ~0u << 10;
-            hist[tid] = hist[tid + CT] = 0;
-            __syncthreads();
-            for (long long i0 = 0; i0 < len; i0 += CT * PER) {
+            uint32_t *bins = hist[round];
+            for (int i0 = 0; i0 < len; i0 += CT * PER) {
                 if (!one) load(i0);
 #pragma unroll
                 for (int e = 0; e < PER; ++e) {
-                    const long long i = i0 + e * CT + tid;
+                    if (i0 + e * CT >= len) break;
+                    const int i = i0 + e * CT + tid;
                     const uint32_t k = order_key(f[e]);
-                    if (i >= lo && i < hi && (k & fixed) == key) atomicAdd(&hist[(k >> shift) & mask], 1);
+                    if (i >= lo && i < hi && (k & fixed) == key) atomicAdd(&bins[(k >> shift) & mask], 1u);
                 }
             }
             __syncthreads();
-            const int c0 = hist[2 * tid], c1 = hist[2 * tid + 1];
-            const int above = before(c0 + c1, -1, 0);
-            if (above < left && left <= above + c1) sh[0] = 2 * tid + 1, sh[1] = above;
-            else if (above + c1 < left && left <= above + c1 + c0) sh[0] = 2 * tid, sh[1] = above + c1;
+            // two bins a thread, from the highest down: one holds the key that is `left` from the top
+            const int d = BINS - 2 - 2 * tid;
+            const int c0 = bins[d], c1 = bins[d + 1];
+            uint32_t sum = c0 + c1, none = 0;
+            before(sum, none);
+            const int above = sum;
+            if (above < left && left <= above + c1) sh[0] = d + 1, sh[1] = above, sh[2] = c1;
+            else if (above + c1 < left && left <= above + c1 + c0) sh[0] = d, sh[1] = above + c1, sh[2] = c0;
             __syncthreads();
-            key |= (uint32_t)sh[0] << shift;
+            key |= sh[0] << shift;
             left -= sh[1];
+            if ((int)sh[2] == left) {  // every one of this bin stays: those above the key before it
+                key -= 1;
+                left = 0;
+            }
         }
         ties = left;
     }
     int base = 0, eq_base = 0;  // kept for certain, and ties, before this stretch
-    for (long long i0 = 0; i0 < len; i0 += CT * PER) {
+    for (int i0 = 0; i0 < len; i0 += CT * PER) {
         if (!one) load(i0);
         uint64_t sure = 0, tie = 0;  // bit e
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
-            const long long i = i0 + e * CT + tid;
+            const int i = i0 + e * CT + tid;
             const uint32_t k = order_key(f[e]);
             const bool s = i < len && (len <= a.keep || i < lo || i >= hi || k > key);
             const bool t = i < len && !s && k == key;
             const uint64_t bs = __ballot(s), bt = __ballot(t);
-            if (lane == 0) count[e * NW + wave] = make_int2(__popcll(bs), __popcll(bt));
+            if (lane == 0) count[e * NW + wave] = make_uint2(__popcll(bs), __popcll(bt));
             sure |= (uint64_t)s << e;
             tie |= (uint64_t)t << e;
         }
         __syncthreads();  // also: every score of this stretch has been read
-        const int2 c = tid < NC ? count[tid] : make_int2(0, 0);
-        const int cs = before(c.x, 1, 0), ct = before(c.y, 1, 1);
-        if (tid < NC) count[tid] = make_int2(cs, ct);
+        const uint2 c = tid < NC ? count[tid] : make_uint2(0, 0);
+        uint32_t cs = c.x, ct = c.y;
+        before(cs, ct);
+        if (tid < NC) count[tid] = make_uint2(cs, ct);
         if (tid == CT - 1) sh[0] = cs + c.x, sh[1] = ct + c.y;
         __syncthreads();
         const uint64_t mine = ((uint64_t)1 << lane) - 1;
@@ -123,11 +131,11 @@ __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict
             const bool s = sure >> e & 1, t = tie >> e & 1;
             const uint64_t bs = __ballot(s), bt = __ballot(t);
             if (!(bs | bt)) continue;
-            const int2 c = count[e * NW + wave];
-            const int eq = eq_base + c.y + __popcll(bt & mine);
+            const uint2 c = count[e * NW + wave];
+            const int eq = eq_base + (int)c.y + __popcll(bt & mine);
             if (s || (t && eq < ties)) {
-                const int j = base + c.x + __popcll(bs & mine) + min(eq, ties);
-                kept[j] = (int)(i0 + e * CT + tid);
+                const int j = base + (int)c.x + __popcll(bs & mine) + min(eq, ties);
+                kept[j] = i0 + e * CT + tid;
                 if (ds) ds[j] = f[e];
             }
         }
@@ -237,7 +245,7 @@ extern "C" int ornk_kv_evict(const ornk_kv_pages *p, const ornk_evict_args *a, h
     else if (a->max_len <= 16 * CT)
         hipLaunchKernelGGL(k_evict_choose<16>, dim3(p->kv, a->n_seqs), dim3(CT), 0, s, *p, *a);
     else
-        hipLaunchKernelGGL(k_evict_choose<64>, dim3(p->kv, a->n_seqs), dim3(CT), 0, s, *p, *a);
+        hipLaunchKernelGGL(k_evict_choose<32>, dim3(p->kv, a->n_seqs), dim3(CT), 0, s, *p, *a);
     typedef uint32_t u4 __attribute__((ext_vector_type(4)));
     if (rb % 16 == 0) move<u4>(*p, *a, rb, s);
     else if (rb % 4 == 0) move<uint32_t>(*p, *a, rb, s);
