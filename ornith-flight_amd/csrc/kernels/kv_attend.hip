@@ -5,7 +5,7 @@
 // over the sequence's tokens, query heads sharing kv heads.
 //
 // Work: the tokens of every sequence, kv head and tile of 16 of its query
-// heads ("pair") in units of 128, one after the other on a line.  W work groups
+// heads ("pair") in units of 128 or 256, one after the other on a line.  W work groups
 // take equal stretches of the line, whatever the lengths are; a pair that one
 // group covers is finished there, of the others the groups leave O, m and l of
 // their part, which k_kv_finish puts together:
@@ -19,15 +19,19 @@ typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int WAVES = 4;
-// log2 of a unit's tokens: four tiles, or as many more as keep the line below
-// 2^22 units (32-bit products with a group's number).
-constexpr int UNIT_LOG2 = 7, LINE_LOG2 = 22;
-// Work groups per CU: one's start and end under the other's stream.  The
-// registers of 256 columns (K, V and O of a tile, 64 each, beside their
-// addresses) leave room for one wave per SIMD; with two and tiles of 16 keys,
-// 131,071 tokens of bf16 take 64 us instead of 52.
-template <int HD>
-constexpr int per_cu = HD == 256 ? 1 : 2;
+// A unit is the waves' tiles, or as many more tokens as keep the line below 2^22
+// units (32-bit products with a group's number).
+constexpr int LINE_LOG2 = 22;
+// Work groups per CU, as log2: one's start and end under another's stream.  What
+// registers allow: K, V and O of a tile and their addresses take all of one
+// wave's per SIMD at 256 columns (two groups with tiles of 16 keys: 131,071
+// tokens of bf16 64 us instead of 52), and two waves' at 128 (four spill: 209 ->
+// 393 us); the fp32 path of 64 columns leaves room for four (5 x 2047 tokens of
+// 12 kv heads 20.0 -> 18.2 us), the others of 64 do not (126 -> 144 us).
+constexpr int groups_log2(int type, int HD)
+{
+    return HD == 256 ? 0 : HD == 64 && type == ORN_KV_F32 ? 2 : 1;
+}
 constexpr int CUS_LOG2 = 8;
 
 struct AttendWs {
@@ -217,17 +221,23 @@ struct Exact {
 // part has fp32's exponents, so 24 bits stay at every size, and the sums are
 // fp32.  Of the f16 products the smallest, second part by third, is left out
 // (2^-24 of the whole).  Parts of an infinity are no numbers: a segment whose
-// sums are not finite is done again by Exact.  32 keys per tile.
+// sums are not finite is done again by Exact.  32 or
+// 64 keys per tile.
 //
 // Reduction indexes are permuted alike in both operands: a lane's 16 bytes of a
 // K row are its dimensions of one step (of two, for e4m3), and key 16 i + 4 g + r
 // is place 8 g + 4 i + r of the reduction over keys, so that the weights stay
 // where they are.  V's 8 rows by CW columns in a lane's registers are turned
 // into CW operands of 8 keys there (v_perm_b32).
+// Keys of a tile: more bytes on their way for every wave where short rows leave
+// registers for them (98 sequences of 10,699, e4m3, 64 columns: 126 us with 32
+// keys, 117 with 64; 128 columns of e4m3 70 and 74 us).
+constexpr int parts_keys(int HD) { return HD == 64 ? 64 : 32; }
+
 template <int TYPE, int HD, bool FULL>
 struct Parts {
-    static constexpr int KT = 32, NI = KT / 16;
-    static constexpr int ES = elem_size<TYPE>, NS = HD / 32, NO = HD / 16;
+    static constexpr int ES = elem_size<TYPE>, KT = parts_keys(HD), NI = KT / 16, NG = KT / 32;
+    static constexpr int NS = HD / 32, NO = HD / 16;
     static constexpr int DL = 16 / ES, NL = HD / (4 * DL);             // K: dimensions of a load, loads
     static constexpr int CW = HD / 16 < DL ? HD / 16 : DL, NH = HD / (16 * CW);  // V: columns, loads of a row
     static constexpr int VW = CW * ES / 4;
@@ -334,11 +344,12 @@ struct Parts {
     __device__ __forceinline__ void leave_out(int) {}
     __device__ __forceinline__ void pv(v4f *o, const float *p) const
     {
-        v8b pp[3];
-        {
-            float x[4 * NI];
 #pragma unroll
-            for (int e = 0; e < 4 * NI; ++e) x[e] = p[e];
+        for (int gr = 0; gr < NG; ++gr) {
+            v8b pp[3];
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = p[8 * gr + e];
 #pragma unroll
             for (int part = 0; part < 3; ++part) {
                 u4 w;
@@ -346,47 +357,47 @@ struct Parts {
                 for (int e = 0; e < 4; ++e) w[e] = top16(x[2 * e + 1], x[2 * e]);
                 pp[part] = as_v8b(w);
 #pragma unroll
-                for (int e = 0; e < 4 * NI; ++e) x[e] = rest16(x[e]);
+                for (int e = 0; e < 8; ++e) x[e] = rest16(x[e]);
             }
+#pragma unroll
+            for (int j = 0; j < NH; ++j)
+#pragma unroll
+                for (int c = 0; c < CW; c += 4) pv4(o + j * CW + c, pp, v + 8 * gr, j, c);
         }
+    }
+    // Four columns of O: their operands are V's rows turned.
+    static __device__ __forceinline__ void pv4(v4f *o, const v8b *pp, const uint32_t (*v)[NH][VW], int j,
+                                               int c)
+    {
+        u4 hi[4], lo[4];
+        if constexpr (TYPE == ORN_KV_BF16) {
 #pragma unroll
-        for (int j = 0; j < NH; ++j)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int c = 0; c < CW; c += 4) {
-                // four columns' operands: V's rows turned
-                u4 hi[4], lo[4];
-                if constexpr (TYPE == ORN_KV_BF16) {
+                for (int e = 0; e < 4; ++e)
+                    hi[i][e] = __builtin_amdgcn_perm(v[2 * e + 1][j][(c + i) / 2], v[2 * e][j][(c + i) / 2],
+                                                     i % 2 ? 0x07060302u : 0x05040100u);
+        } else {
+            float f[8][4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+            for (int e = 0; e < 8; ++e) unpack4<TYPE>(f[e], &v[e][j][c * ES / 4]);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            hi[i][e] = __builtin_amdgcn_perm(v[2 * e + 1][j][(c + i) / 2],
-                                                             v[2 * e][j][(c + i) / 2],
-                                                             i % 2 ? 0x07060302u : 0x05040100u);
-                } else {
-                    float f[4 * NI][4];
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4 * NI; ++e) unpack4<TYPE>(f[e], &v[e][j][c * ES / 4]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            hi[i][e] = top16(f[2 * e + 1][i], f[2 * e][i]);
-                            if constexpr (NP == 2)
-                                lo[i][e] = top16(rest16(f[2 * e + 1][i]), rest16(f[2 * e][i]));
-                        }
+                for (int e = 0; e < 4; ++e) {
+                    hi[i][e] = top16(f[2 * e + 1][i], f[2 * e][i]);
+                    if constexpr (NP == 2) lo[i][e] = top16(rest16(f[2 * e + 1][i]), rest16(f[2 * e][i]));
                 }
-                v4f *x = o + j * CW + c;
-                auto add = [&](int part, const u4 *b) {
+        }
+        auto add = [&](int part, const u4 *b) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[i] = mma(pp[part], as_v8b(b[i]), x[i]);
-                };
-                add(2, hi);
-                if constexpr (NP == 2) add(1, lo);
-                add(1, hi);
-                if constexpr (NP == 2) add(0, lo);
-                add(0, hi);
-            }
+            for (int i = 0; i < 4; ++i) o[i] = mma(pp[part], as_v8b(b[i]), o[i]);
+        };
+        add(2, hi);
+        if constexpr (NP == 2) add(1, lo);
+        add(1, hi);
+        if constexpr (NP == 2) add(0, lo);
+        add(0, hi);
     }
     static __device__ __forceinline__ int col(int c, int n) { return CW * (16 * (c / CW) + n) + c % CW; }
 };
@@ -676,7 +687,7 @@ __device__ __forceinline__ Stretch scan_lens(const ornk_kv_pages &p, const ornk_
 }
 
 template <int TYPE, int HD, class Path>
-__global__ void __launch_bounds__(64 * WAVES, per_cu<HD>) k_kv_attend(ornk_kv_pages p, ornk_attend_args a,
+__global__ void __launch_bounds__(64 * WAVES, (1 << groups_log2(TYPE, HD))) k_kv_attend(ornk_kv_pages p, ornk_attend_args a,
                                                                       AttendWs w)
 {
     extern __shared__ __align__(16) uint8_t lds[];
@@ -880,10 +891,11 @@ size_t attend_ws(const ornk_kv_pages *p, const ornk_attend_args *a, AttendWs *w)
         off += (n + 255) & ~(size_t)255;
         return at;
     };
-    w->w_log2 = CUS_LOG2 + (p->hd > 128 ? 0 : 1);
+    const int HD = p->hd <= 64 ? 64 : p->hd <= 128 ? 128 : 256;
+    w->w_log2 = CUS_LOG2 + groups_log2(p->type, HD);
     const int G = a->heads / p->kv, W = 1 << w->w_log2;
     w->row = (p->hd + 3) & ~3;
-    w->unit_log2 = UNIT_LOG2;
+    w->unit_log2 = parts_keys(HD) == 64 ? 8 : 7;
     const size_t pairs = (size_t)a->n_seqs * p->kv * ((G + 15) / 16);
     while (w->unit_log2 < 31 && pairs * (((size_t)a->max_len >> w->unit_log2) + 1) >> LINE_LOG2) ++w->unit_log2;
     w->cum = reinterpret_cast<uint32_t *>(take(((size_t)a->n_seqs + 1) * 4));
@@ -894,7 +906,7 @@ size_t attend_ws(const ornk_kv_pages *p, const ornk_attend_args *a, AttendWs *w)
     w->s_len = 0;
     if (a->score_out) {
         const size_t rows = (size_t)a->n_seqs * a->heads;
-        w->s_len = ((size_t)a->max_len + 31) / 32 * 32;  // whole tiles
+        w->s_len = ((size_t)a->max_len + 63) / 64 * 64;  // whole tiles
         w->ml = reinterpret_cast<float2 *>(take(rows * 8));
         w->s = reinterpret_cast<float *>(take(rows * w->s_len * 4));
     }
