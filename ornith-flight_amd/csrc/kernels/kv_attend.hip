@@ -675,7 +675,7 @@ __device__ __forceinline__ Stretch scan_lens(const ornk_kv_pages &p, const ornk_
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         s.len[i] = b0 + i < a.n_seqs ? kv_len(p, at[i], b0 + i, a.max_len) : 0;
-        s.units[i] = (uint32_t)(((long long)s.len[i] + (1 << w.unit_log2) - 1) >> w.unit_log2);
+        s.units[i] = (uint32_t)((s.len[i] + (1ll << w.unit_log2) - 1) >> w.unit_log2);
         s.before[i] = sum;
         sum += s.units[i];
     }
@@ -967,7 +967,7 @@ extern "C" int ornk_kv_attend(const ornk_kv_pages *p, const ornk_attend_args *a,
                                       : launch_type<ORN_KV_E4M3>(p, a, w, s);
     if (rc != hipSuccess) return rc;
     const int G = a->heads / p->kv, HT = (G + 15) / 16;
-    const int jx = a->max_len > 1 << w.unit_log2  // else every pair is one unit
+    const int jx = a->max_len > 1ll << w.unit_log2  // else every pair is one unit
                        ? ((G < 16 ? G : 16) * (w.row / 4) + JC - 1) / JC : 0;
     const int sx = a->score_out ? (int)(((long long)a->max_len + 4 * FT - 1) / (4 * FT)) : 0;
     if (jx + sx)

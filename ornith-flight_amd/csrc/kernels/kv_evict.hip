@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict
     int ties = 0;      // and how many tokens of that key
     if (one) load(0);
     if (len > a.keep) {
-        for (int i = tid; i < 3 * BINS; i += CT) hist[0][i] = 0;
+        for (int i = tid; i < 3 * BINS; i += CT) hist[i / BINS][i % BINS] = 0;
         __syncthreads();
         int left = a.keep - a.sink - a.recent;
         if (left == 0) key = 0xffffffffu;  // above every key
@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict
         eq_base += sh[1];
         __syncthreads();
     }
-    for (int i = n + tid; i < a.keep; i += CT) kept[i] = -1;
+    for (long long i = n + tid; i < a.keep; i += CT) kept[i] = -1;
 }
 
 // The kept rows to their new places, in words of WORD.  A work group takes rows

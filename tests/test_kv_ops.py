@@ -775,6 +775,101 @@ def test_attend_large_and_growing_scores(om, ctx, type):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,kv,G,pages", [(700, 2, 4, 30), (3000, 4, 2, 64)])
+def test_attend_many_rows(om, ctx, n, kv, G, pages):
+    """More rows than are looked at together; at 3000 x 4 heads over a table of 65,536 tokens
+    the units of the work are larger, too.  Rows share pages and have junk behind their last."""
+    rng = np.random.default_rng(n)
+    c = Cache(om, ctx, "bf16", 9, 1024, kv, 64, seed=n)
+    lens = [int(x) for x in rng.integers(0, 700, n)]
+    lens[5], lens[n - 1], lens[n // 2] = 5000, 0, 9000
+    table = np.full((n, pages), -1, np.int32)
+    table[:, 0] = rng.integers(0, 9, n)
+    for b in (5, n // 2):
+        table[b, :9] = rng.permutation(9)
+    q = rng.standard_normal((n, kv * G, 64)).astype(np.float32)
+    score = rng.uniform(0, 1, (n, kv, 9001)).astype(np.float32) if n < 1000 else None
+    got = attend(om, ctx, c, q, lens, table, score=score, max_len=9000 if n < 1000 else 0)
+    out = got[0] if score is not None else got
+    for b in [0, 1, 5, 6, 255, 256, 257, 511, 512, n // 2, n - 2, n - 1] + list(range(20, n, 97)):
+        k, v = c.rows(table[b], lens[b]) if lens[b] else (np.zeros((kv, 0, 64)),) * 2
+        want, w, tol, tw = attend64(q[b], k, v, 1 / 8)
+        assert np.abs(out[b] - want).max() <= tol, (b, lens[b])
+        if score is not None:
+            add = w.reshape(kv, G, -1).sum(1)
+            ws = score[b, :, :lens[b]] + add
+            assert (np.abs(got[1][b, :, :lens[b]] - ws) <= (tw + EPS * G) * add + 4 * EPS * np.abs(ws)).all()
+            assert (got[1][b, :, lens[b]:] == -9.0).all()
+    c.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type,n_pages", [("f32", 600), ("bf16", 1200), ("e4m3", 2200)])
+def test_pages_past_4_gb(om, ctx, type, n_pages):
+    """Append, attention and eviction in the last pages of a cache of over 4 GB."""
+    rng = np.random.default_rng(3)
+    kv, D, page = 8, 256, 1024
+    nbytes = n_pages * kv * page * D * DTYPE[type].itemsize
+    assert nbytes > 1 << 32
+    K, V = ctx.alloc(nbytes), ctx.alloc(nbytes)
+    pages = om.kv_pages(K, V, type, n_pages, page, kv, D)
+    n, far = 1500, n_pages - 3
+    table = i32([[n_pages - 1, far]])
+    k, v = (rng.standard_normal((n, kv, D)).astype(np.float32) for _ in range(2))
+    slots = i32([table[0, t // page] * page + t % page for t in range(n)])
+    q = rng.standard_normal((1, 16, D)).astype(np.float32)
+    bufs = [ctx.upload(x) for x in (k, v, slots, q, np.zeros_like(q), table, i32([n]),
+                                    np.zeros((1, kv, 2048), np.float32), i32([[n_pages - 2]]), i32([0]),
+                                    np.zeros((1, kv, 400), np.int32))]
+    kb, vb, sb, qb, ob, tb, lb, scb, dt, dl, kept = bufs
+    om.kv_append(ctx, pages, kb, vb, n, sb)
+    om.kv_attend(ctx, pages, ob, qb, 1, 16, tb, 2, lb,
+                 om.attend_opts(score_out=scb, score_stride=2048))
+    kk, vv = (value(stored(x, type)).transpose(1, 0, 2) for x in (k, v))
+    want, w, tol, tw = attend64(q[0], kk, vv, 1 / 16)
+    assert np.abs(ctx.download(ob, np.float32, q.shape)[0] - want).max() <= tol
+    score = ctx.download(scb, np.float32, (1, kv, 2048))
+    om.kv_evict(ctx, pages, 1, tb, 2, lb, scb, 2048, dt, 1, dl, None, 0, kept, om.evict_opts(400, 4, 50))
+    ids = ctx.download(kept, np.int32, (1, kv, 400))
+    om.kv_attend(ctx, pages, ob, qb, 1, 16, dt, 1, dl)
+    for h in range(kv):
+        assert ids[0, h].tolist() == choose(score[0, h], n, 400, 4, 50)
+    k2, v2 = (np.stack([x[h][ids[0, h]] for h in range(kv)]) for x in (kk, vv))
+    want, _, tol, _ = attend64(q[0], k2, v2, 1 / 16)
+    assert np.abs(ctx.download(ob, np.float32, q.shape)[0] - want).max() <= tol
+    for b in bufs + [K, V]:
+        b.free()
+
+
+@pytest.mark.gpu
+def test_two_contexts_at_once(om):
+    """Asynchronous calls of two contexts, each with its stream and workspace, on pages that
+    both read."""
+    rng = np.random.default_rng(31)
+    one, two = om.Context(), om.Context()
+    c = Cache(om, one, "bf16", 300, 16, 2, 128, seed=10)
+    table = tables(rng, [4000], 16, 300, 250)
+    q = rng.standard_normal((2, 1, 8, 128)).astype(np.float32)
+    s = rng.uniform(0, 1, (1, 2, 4000)).astype(np.float32)
+    alone = [attend(om, one, c, q[i], [4000], table, score=s) for i in (0, 1)]
+    jobs = []
+    for x, i in ((one, 0), (two, 1)):
+        b = [x.upload(y) for y in (q[i], np.zeros_like(q[i]), table, i32([4000]), s, np.zeros_like(s))]
+        jobs.append((x, b, om.attend_opts(flags=om.KV_ASYNC, score_in=b[4], score_out=b[5],
+                                          score_stride=4000)))
+    for _ in range(5):
+        for x, b, o in jobs:
+            om.kv_attend(x, c.pages, b[1], b[0], 1, 8, b[2], 250, b[3], o)
+    for i, (x, b, _) in enumerate(jobs):
+        assert om.lib().gpu_kv_check(x.ptr) == 0
+        assert np.array_equal(x.download(b[1], np.float32, q[i].shape), alone[i][0])
+        assert np.array_equal(x.download(b[5], np.float32, s.shape), alone[i][1])
+    two.close()
+    c.free()
+    one.close()
+
+
+@pytest.mark.gpu
 def test_attend_scale_zero_is_the_default_and_uniform_weights(om, ctx):
     """Equal keys: every token has the weight 1 / n, and the scores of a kv head add up to its
     query heads."""
