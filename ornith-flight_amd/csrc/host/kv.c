@@ -244,7 +244,7 @@ int gpu_kv_append(gpu_context *ctx, const ornith_kv_pages *kv, const gpu_buffer 
         return orn_set_err(ctx, ORN_EINVAL, "%s: buffer too small", who);
     const gpu_buffer *in[] = {K, V, Q, slots, positions};
     for (int i = 0; i < 5; ++i)
-        if (in[i] && (in[i] == kv->K || in[i] == kv->V || (in[i] == q_out && in[i] != Q)))
+        if (in[i] && (in[i] == kv->K || in[i] == kv->V || (in[i] == q_out && i != 2)))
             return orn_set_err(ctx, ORN_EINVAL, "%s: an output aliases another argument", who);
     if (q_out && (q_out == kv->K || q_out == kv->V))
         return orn_set_err(ctx, ORN_EINVAL, "%s: q_out is the cache", who);

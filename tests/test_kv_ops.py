@@ -196,6 +196,17 @@ def test_host_refuses_aliases(host, what, out, others):
         assert c() in [(-1, 0)], (out, o)
 
 
+def test_host_refuses_rotated_queries_over_rows_still_to_be_read(host):
+    """q_out may be Q, but not where K or V is that buffer, too."""
+    for o in ("K", "V"):
+        c = Call(host, "append")
+        c.args["q_out"] = c.args["Q"] = c.args[o] = host.buf(1 << 20)
+        assert c() == (-1, 0), o
+    c = Call(host, "rope")
+    c.args["q_out"] = c.args["Q"] = c.args["K"] = host.buf(1 << 20)
+    assert c() == (-1, 0)
+
+
 def test_host_takes_in_place_calls(host):
     c = Call(host, "rope")
     c.args["q_out"], c.args["k_out"] = c.args["Q"], c.args["K"]
