@@ -54,8 +54,9 @@ int gpu_kv_cache_append(gpu_context *ctx, gpu_buffer *K_cache, gpu_buffer *V_cac
  *
  * Activations are fp32, lengths, positions, slots and page numbers int32, all
  * in buffers of the context; a call takes up to 65535 sequences and as many
- * heads, of at most 2^31 - 2^16 tokens (max_pages * page_size).  Calls return 0 or a negative status, run on the
- * context's stream and are synchronous unless ORN_KV_ASYNC is given.
+ * heads, of at most 2^31 - 2^16 tokens (max_pages * page_size).  Calls return 0
+ * or a negative status, run on the context's stream and are synchronous unless
+ * ORN_KV_ASYNC is given.
  *
  * Numbers in device buffers are checked by the kernels: a page number outside
  * [0, n_pages), a slot past the pages or a length outside its bounds is left
@@ -83,7 +84,7 @@ typedef struct {
     int type;      /* ORN_KV_* */
     int n_pages;
     int page_size; /* a power of two, 8 to 1024; n_pages * page_size < 2^31 */
-    int n_kv_heads; /* at most 32767 */
+    int n_kv_heads; /* at most 32767; a page of all heads is below 4 GB */
     int head_dim;   /* 1 to 256 */
     /* ORN_KV_E4M3: a stored value c stands for c * scale (0: 1).  Values beyond
      * 448 * scale are stored as that; a NaN stays one. */
@@ -103,14 +104,14 @@ typedef struct {
     int n_axes; /* 1 to 4 */
     int pairs[ORN_ROPE_MAX_AXES]; /* >= 0, at most ORN_ROPE_MAX_PAIRS in all */
     int interleaved, halves;
-    double base; /* > 0 */
+    double base; /* > 0; every angle is finite */
 } ornith_rope_axes;
 
 /* q_out = Q [n_tokens][n_heads][head_dim] and k_out = K [n_tokens]
  * [n_kv_heads][head_dim] rotated (head_dim up to 4096); positions
  * [n_axes][n_tokens].  Angles are formed in 64 bits, so that far positions keep
- * their digits.  q_out may be Q
- * and k_out may be K; a pair of NULLs with 0 heads leaves one side out. */
+ * their digits.  q_out may be Q and k_out may be K; a pair of NULLs with 0 heads
+ * leaves one side out. */
 int gpu_rope_axes(gpu_context *ctx, gpu_buffer *q_out, gpu_buffer *k_out, const gpu_buffer *Q,
                   const gpu_buffer *K, int n_tokens, int n_heads, int n_kv_heads, int head_dim,
                   const gpu_buffer *positions, const ornith_rope_axes *rope, unsigned flags);
@@ -130,9 +131,10 @@ int gpu_kv_append(gpu_context *ctx, const ornith_kv_pages *kv, const gpu_buffer 
  * [n_seqs][n_heads][head_dim], over the first lens[b] tokens of its row of the
  * table, w = softmax(scale * q.k); n_heads is a multiple of n_kv_heads, head j
  * reads kv head j / (n_heads / n_kv_heads).  A sequence of length 0 (a row of a
- * padded batch) gives zeros.  out is not Q.  n_seqs * n_kv_heads, times
- * ceil(n_heads / n_kv_heads / 16), is at most 2^21.  The arithmetic is that of
- * 32 bits whatever the cache's type, infinities and NaN included.
+ * padded batch) gives zeros, as does a head whose scores are all -infinity.  out
+ * is not Q.  n_seqs * n_kv_heads, times ceil(n_heads / n_kv_heads / 16), is at
+ * most 2^21.  The arithmetic is that of 32 bits whatever the cache's type,
+ * infinities and NaN included.
  *
  * score_out (may be NULL) [n_seqs][n_kv_heads][score_stride]: for the tokens
  * t < lens[b], decay * score_in[b][h][t] (score_in NULL: 0) + the sum of w over
@@ -160,11 +162,11 @@ int gpu_kv_attend(gpu_context *ctx, const ornith_kv_pages *kv, gpu_buffer *out,
  * [n_seqs][n_kv_heads][keep] says which they were (-1 past dst_lens).
  *
  * dst_table == table (then dst_pages == max_pages) moves them within their own
- * pages, which no other sequence may share then; else no page of dst_table is
- * read as one of table.  dst_lens may be lens, dst_score may be score (with
+ * pages, each of which is then one sequence's, once; else no page of dst_table is
+ * read as one of table, and none is listed twice.  dst_lens may be lens, dst_score may be score (with
  * dst_stride == score_stride). */
 typedef struct {
-    int keep;         /* >= 1, >= sink + recent */
+    int keep;         /* >= 1, >= sink + recent; at most 2^27, or max_len is */
     int sink, recent; /* >= 0 */
     int max_len;      /* no length is larger; 0: the table's width */
     unsigned flags;

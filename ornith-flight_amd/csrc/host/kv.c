@@ -175,7 +175,11 @@ static int rope_ok(gpu_context *ctx, const ornith_rope_axes *r, int hd, ornk_rop
     }
     const double step = R ? pow(r->base, -1.0 / R) : 1.0;
     double f = 0.15915494309189533577; /* 1 / 2 pi */
-    for (int p = 0; p < R; ++p, f *= step) a->turns[p] = f;
+    for (int p = 0; p < R; ++p, f *= step) {
+        if (!(f * 2147483648.0 < INFINITY)) /* no angle at the farthest position */
+            return orn_set_err(ctx, ORN_EINVAL, "%s: base %g", who, r->base);
+        a->turns[p] = f;
+    }
     a->R = R;
     a->halves = r->halves != 0;
     return ORN_OK;
@@ -365,6 +369,8 @@ int gpu_kv_evict(gpu_context *ctx, const ornith_kv_pages *kv, int n_seqs, const 
     if (!score || !dst_table || !dst_lens || !kept || dst_pages < 0)
         return orn_set_err(ctx, ORN_EINVAL, "%s: bad arguments", who);
     const int most = opts->keep < bound ? opts->keep : bound; /* the longest result */
+    if (most > 1 << 27) /* work groups of 256 threads to 16 rows or more, 2^32 threads a launch */
+        return orn_set_err(ctx, ORN_EUNSUPPORTED, "%s: %d tokens kept (at most 2^27)", who, most);
     if ((long long)dst_pages * p.page < most || !holds(dst_table, span(n_seqs, dst_pages, 1, 1, 4)))
         return orn_set_err(ctx, ORN_EINVAL, "%s: dst_table has no room for %d tokens", who, most);
     if (score_stride < bound || !holds(score, span(n_seqs, p.kv, score_stride, 1, 4)) ||

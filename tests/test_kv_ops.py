@@ -247,7 +247,8 @@ def test_host_leaves_sides_out(host):
 @pytest.mark.parametrize("change", [
     dict(n_axes=0), dict(n_axes=5), dict(base=0.0), dict(base=-1.0), dict(base=math.inf),
     dict(base=math.nan), dict(pairs=(4, -1, 2, 0)), dict(pairs=(6, 6, 5, 0)),
-    dict(pairs=(1 << 30, 1 << 30, 1 << 30, 0)), dict(n_axes=4)])
+    dict(pairs=(1 << 30, 1 << 30, 1 << 30, 0)), dict(n_axes=4),
+    dict(base=5e-324, pairs=(16, 0, 0, 0))])
 def test_host_refuses_rotations(host, change):
     for what in ("rope", "append"):
         c = Call(host, what)
@@ -275,6 +276,43 @@ def test_host_refuses_evict_options(host, change):
     for k, v in change.items():
         setattr(c.opts, k, v)
     assert c() == (-1, 0)
+
+
+def test_host_refuses_what_passes_its_limits(host):
+    """Calls whose buffers would hold what they ask for."""
+    def big(what, pages=(), args=(), opts=()):
+        c = Call(host, what)
+        for k, v in c.args.items():
+            if isinstance(v, int) and v > 1 << 30:  # a buffer's handle
+                c.args[k] = host.buf(1 << 60)
+        c.pages.K, c.pages.V = host.buf(1 << 60), host.buf(1 << 60)
+        c.args.update(args)
+        for k, v in dict(pages).items():
+            setattr(c.pages, k, v)
+        for k, v in dict(opts).items():
+            setattr(c.opts, k, v)
+        return c()
+    att = dict(score_in=None, score_out=None)
+    assert big("attend", opts=att) == (0, 1)
+    assert big("attend", args=dict(B=65535), opts=att) == (0, 1)
+    assert big("attend", args=dict(B=65536), opts=att) == (-4, 0)
+    assert big("attend", dict(n_kv_heads=32), dict(B=65535, heads=32), att) == (0, 1)
+    assert big("attend", dict(n_kv_heads=33), dict(B=65535, heads=33), att) == (-4, 0)
+    assert big("attend", dict(n_kv_heads=32), dict(B=65535, heads=32 * 17), att) == (-4, 0)
+    assert big("attend", args=dict(heads=65536), opts=att)[0] < 0
+    wide = dict(page_size=1024)
+    assert big("attend", wide, dict(width=2 ** 21 - 64), dict(att, max_len=0)) == (0, 1)
+    assert big("attend", wide, dict(width=2 ** 21 - 63), dict(att, max_len=0)) == (-1, 0)
+    page = dict(page_size=1024, head_dim=256, type=0)
+    assert big("append", dict(page, n_kv_heads=4095)) == (0, 1)
+    assert big("append", dict(page, n_kv_heads=4096)) == (-4, 0)
+    assert big("rope", args=dict(D=4096)) == (0, 1)
+    assert big("rope", args=dict(D=4097)) == (-4, 0)
+    assert big("rope", args=dict(heads=65536))[0] < 0
+    far = dict(width=2 ** 18, stride=2 ** 28, dst_pages=2 ** 18, dst_stride=2 ** 28)
+    assert big("evict", wide, far, dict(keep=1 << 27, max_len=0)) == (0, 1)
+    assert big("evict", wide, far, dict(keep=(1 << 27) + 1, max_len=0)) == (-4, 0)
+    assert big("evict", wide, far, dict(keep=2 ** 31 - 1, max_len=1 << 27)) == (0, 1)
 
 
 def test_host_no_context(host):
