@@ -4,8 +4,8 @@
 // (ornith_hip.h): out = sum_t w_t V[t], w = softmax(scale * q . K[t]), the sums
 // over the sequence's tokens, query heads sharing kv heads.
 //
-// Work: the tokens of every sequence, kv head and tile of 16 of its query
-// heads ("pair") in units of 128 or 256, one after the other on a line.  W work groups
+// Work: the tokens of every sequence, kv head and tile of 16 of its query heads
+// ("pair") in units of 128 or 256, one after the other on a line.  W work groups
 // take equal stretches of the line, whatever the lengths are; a pair that one
 // group covers is finished there, of the others the groups leave O, m and l of
 // their part, which k_kv_finish puts together:
@@ -36,7 +36,7 @@ constexpr int CUS_LOG2 = 8;
 
 struct AttendWs {
     uint32_t *cum;   // [n_seqs + 1] units before each sequence, per pair of it
-    float2 *part_ml; // [2 W][16] of the parts: a group's first stretch, its last
+    float2 *part_ml; // [2 W][16] of the parts: of the pair a group goes on with, of the one it begins
     float *part_o;   // [2 W][16][row]
     int w_log2, row, unit_log2;  // W; floats of a row of part_o; a unit
     float2 *ml;      // [n_seqs][heads] and scores [n_seqs][heads][s_len], for the weights
@@ -53,6 +53,18 @@ __device__ __forceinline__ uint32_t line_at(uint32_t T, int w_log2, uint32_t w)
 __device__ __forceinline__ uint32_t line_group(uint32_t T, int w_log2, uint32_t u)
 {
     return T >> w_log2 ? (((u + 1) << w_log2) - 1) / T : u;
+}
+
+// Pairs of up to so many units are not cut: a bound of a group's stretch that
+// falls into one moves to its nearer end.  Up to a group's share of the line, as
+// parts of two pairs take a group about twice as long as a whole one (70 sequences
+// of 246 tokens, 4 kv heads of 128 in f16: 25.9 -> 18.1 us; 256 of up to 300, 8
+// heads of bf16: 59.3 -> 55.9; 100 of up to 600, 2 heads: 20.1 -> 21.0); at most
+// 4, since a group waits for the longest (8: the same times).
+__device__ __forceinline__ uint32_t line_whole(uint32_t T, int w_log2)
+{
+    const uint32_t share = T >> w_log2;
+    return share ? min(share + 1, 4u) : 1;
 }
 
 struct Seg {  // part of one pair
@@ -707,6 +719,7 @@ __global__ void __launch_bounds__(64 * WAVES, (1 << groups_log2(TYPE, HD))) k_kv
     const uint32_t T = st.end * per;
     const uint32_t lo = line_at(T, w.w_log2, blockIdx.x), hi = line_at(T, w.w_log2, blockIdx.x + 1);
     if (st.c0 && lo < hi) st = scan_lens(p, a, w, 0, 0);
+    const uint32_t whole = line_whole(T, w.w_log2);
     for (uint32_t u = lo; u < hi;) {
         while (u >= st.end * per) st = scan_lens(p, a, w, st.c0 + STRETCH, st.end);
         int b = -1, len = 0;  // u's sequence, in its lane
@@ -729,7 +742,16 @@ __global__ void __launch_bounds__(64 * WAVES, (1 << groups_log2(TYPE, HD))) k_kv
         uint32_t pair = (uint32_t)((float)off / (float)n);
         if (pair * n > off) --pair;
         else if (off - pair * n >= n) ++pair;
-        const uint32_t k = off - pair * n, cnt = min(n - k, hi - u);
+        uint32_t k = off - pair * n, cnt = min(n - k, hi - u);
+        if (n <= whole) {  // a bound within it moves to its nearer end
+            if (k && 2 * k >= n) {
+                u += n - k;
+                continue;
+            }
+            u -= k;
+            if (hi - u < n && 2 * (hi - u) < n) break;
+            k = 0, cnt = n;
+        }
         const int tile = HT == 1 ? 0 : pair % HT, j = 16 * tile;
         sg.h = HT == 1 ? pair : pair / HT;
         sg.j0 = sg.h * G + j;
@@ -737,7 +759,7 @@ __global__ void __launch_bounds__(64 * WAVES, (1 << groups_log2(TYPE, HD))) k_kv
         sg.k0 = k << w.unit_log2;
         sg.k1 = (int)min((long long)sg.len, (long long)(k + cnt) << w.unit_log2);
         sg.score = ((size_t)sg.b * a.heads + sg.j0) * w.s_len;
-        const int slot = cnt == n ? -1 : 2 * (int)blockIdx.x + (u == lo ? 0 : 1);
+        const int slot = cnt == n ? -1 : 2 * (int)blockIdx.x + (k ? 0 : 1);
         const bool done = attend_segment<TYPE, HD, Path>(p, a, w, sg, lds, slot);
         if constexpr (!Path::exact) {
             if (!done) attend_segment<TYPE, HD, Exact<TYPE, HD, true, Path::full>>(p, a, w, sg, lds, slot);
@@ -752,20 +774,19 @@ __global__ void __launch_bounds__(64 * WAVES, (1 << groups_log2(TYPE, HD))) k_kv
     }
 }
 
-// The parts of a pair: the first one's slot, the others' follow (2 (w0 + i)).
+// The n parts of a pair (below 2: nothing is left to do), from group w0 on.
 struct PairParts {
-    uint32_t n, w0, first;  // 1: a group has finished the pair
-    __device__ __forceinline__ size_t slot(uint32_t i) const { return i ? 2 * (w0 + i) : first; }
+    uint32_t n, w0;
+    __device__ __forceinline__ size_t slot(uint32_t i) const { return 2 * (w0 + i) + (i ? 0 : 1); }
 };
 __device__ __forceinline__ PairParts parts_of(const AttendWs &w, uint32_t per, int n_seqs, int b, int pair)
 {
     const uint32_t before = w.cum[b], n = w.cum[b + 1] - before, T = w.cum[n_seqs] * per;
     const uint32_t s = before * per + pair * n;
-    PairParts r = {n, 0, 0};
-    if (n < 2) return r;  // no tokens, or one unit
+    PairParts r = {1, 0};
+    if (n <= line_whole(T, w.w_log2)) return r;
     r.w0 = line_group(T, w.w_log2, s);
     r.n = line_group(T, w.w_log2, s + n - 1) - r.w0 + 1;
-    r.first = 2 * r.w0 + (line_at(T, w.w_log2, r.w0) == s ? 0 : 1);
     return r;
 }
 
