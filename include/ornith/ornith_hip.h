@@ -142,7 +142,8 @@ int gpu_kv_append(gpu_context *ctx, const ornith_kv_pages *kv, const gpu_buffer 
  * be score_out. */
 typedef struct {
     float scale;  /* 0: 1 / sqrt(head_dim) */
-    int max_len;  /* no length is larger; 0: the table's width.  Sizes the workspace. */
+    int max_len;  /* no length is larger; 0: the table's width.  Sizes the workspace and
+                   * the launches: a near bound is faster than a far one. */
     unsigned flags;
     const gpu_buffer *score_in;
     gpu_buffer *score_out;

@@ -39,6 +39,7 @@ struct AttendWs {
     float2 *part_ml; // [2 W][16] of the parts: of the pair a group goes on with, of the one it begins
     float *part_o;   // [2 W][16][row]
     int w_log2, row, unit_log2;  // W; floats of a row of part_o; a unit
+    uint32_t whole;  // units of a pair that is not cut, at least
     float2 *ml;      // [n_seqs][heads] and scores [n_seqs][heads][s_len], for the weights
     float *s;
     size_t s_len;
@@ -57,14 +58,17 @@ __device__ __forceinline__ uint32_t line_group(uint32_t T, int w_log2, uint32_t 
 
 // Pairs of up to so many units are not cut: a bound of a group's stretch that
 // falls into one moves to its nearer end.  Up to a group's share of the line, as
-// parts of two pairs take a group about twice as long as a whole one (70 sequences
-// of 246 tokens, 4 kv heads of 128 in f16: 25.9 -> 18.1 us; 256 of up to 300, 8
-// heads of bf16: 59.3 -> 55.9; 100 of up to 600, 2 heads: 20.1 -> 21.0); at most
-// 4, since a group waits for the longest (8: the same times).
-__device__ __forceinline__ uint32_t line_whole(uint32_t T, int w_log2)
+// parts of two pairs take a group about twice as long as a whole one (256 rows of
+// up to 300 tokens, 8 kv heads of 128 in bf16: 59.3 -> 55.9 us; 100 of up to 600,
+// 2 heads: 20.1 -> 21.0); at most 4, since a group waits for the longest (8: the
+// same times).  `least`: all of them, where max_len alone says that they are
+// short; then there is nothing to join either.  Pairs of 2 units always (one row
+// of 250 tokens, 8 heads of 128: 10.8 -> 8.9 us), pairs of 8 where there are half
+// as many as groups (200 rows of up to 1000: 103 -> 91; 8 rows: 13.2 -> 18.3).
+__device__ __forceinline__ uint32_t line_whole(uint32_t T, int w_log2, uint32_t least)
 {
     const uint32_t share = T >> w_log2;
-    return share ? min(share + 1, 4u) : 1;
+    return max(least, share ? min(share + 1, 4u) : 1);
 }
 
 struct Seg {  // part of one pair
@@ -719,7 +723,7 @@ __global__ void __launch_bounds__(64 * WAVES, (1 << groups_log2(TYPE, HD))) k_kv
     const uint32_t T = st.end * per;
     const uint32_t lo = line_at(T, w.w_log2, blockIdx.x), hi = line_at(T, w.w_log2, blockIdx.x + 1);
     if (st.c0 && lo < hi) st = scan_lens(p, a, w, 0, 0);
-    const uint32_t whole = line_whole(T, w.w_log2);
+    const uint32_t whole = line_whole(T, w.w_log2, w.whole);
     for (uint32_t u = lo; u < hi;) {
         while (u >= st.end * per) st = scan_lens(p, a, w, st.c0 + STRETCH, st.end);
         int b = -1, len = 0;  // u's sequence, in its lane
@@ -784,7 +788,7 @@ __device__ __forceinline__ PairParts parts_of(const AttendWs &w, uint32_t per, i
     const uint32_t before = w.cum[b], n = w.cum[b + 1] - before, T = w.cum[n_seqs] * per;
     const uint32_t s = before * per + pair * n;
     PairParts r = {1, 0};
-    if (n <= line_whole(T, w.w_log2)) return r;
+    if (n <= line_whole(T, w.w_log2, w.whole)) return r;
     r.w0 = line_group(T, w.w_log2, s);
     r.n = line_group(T, w.w_log2, s + n - 1) - r.w0 + 1;
     return r;
@@ -919,6 +923,8 @@ size_t attend_ws(const ornk_kv_pages *p, const ornk_attend_args *a, AttendWs *w)
     w->unit_log2 = parts_keys(HD) == 64 ? 8 : 7;
     const size_t pairs = (size_t)a->n_seqs * p->kv * ((G + 15) / 16);
     while (w->unit_log2 < 31 && pairs * (((size_t)a->max_len >> w->unit_log2) + 1) >> LINE_LOG2) ++w->unit_log2;
+    const size_t longest = ((size_t)a->max_len + ((size_t)1 << w->unit_log2) - 1) >> w->unit_log2;
+    w->whole = longest <= 2 || (longest <= 8 && pairs >= (size_t)W / 2) ? (uint32_t)longest : 1;
     w->cum = reinterpret_cast<uint32_t *>(take(((size_t)a->n_seqs + 1) * 4));
     w->part_ml = reinterpret_cast<float2 *>(take((size_t)2 * W * 16 * 8));
     w->part_o = reinterpret_cast<float *>(take((size_t)2 * W * 16 * w->row * 4));
@@ -988,7 +994,7 @@ extern "C" int ornk_kv_attend(const ornk_kv_pages *p, const ornk_attend_args *a,
                                       : launch_type<ORN_KV_E4M3>(p, a, w, s);
     if (rc != hipSuccess) return rc;
     const int G = a->heads / p->kv, HT = (G + 15) / 16;
-    const int jx = a->max_len > 1ll << w.unit_log2  // else every pair is one unit
+    const int jx = a->max_len > (long long)w.whole << w.unit_log2  // else no pair is cut
                        ? ((G < 16 ? G : 16) * (w.row / 4) + JC - 1) / JC : 0;
     const int sx = a->score_out ? (int)(((long long)a->max_len + 4 * FT - 1) / (4 * FT)) : 0;
     if (jx + sx)
