@@ -10,7 +10,17 @@
 // group covers is finished there, of the others the groups leave O, m and l of
 // their part, which k_kv_finish puts together:
 //   M = max m_i, L = sum l_i 2^(m_i - M), out = sum O_i 2^(m_i - M) / L.
-// (Exponents are base 2: log2 e is in the query's scale.)
+// (Exponents are base 2: log2 e is in the query's scale.)  The parts' places and
+// the order of their sums depend on the lengths alone: equal calls give equal bits.
+//
+// Bound by the reading of K and V where the cache is large: 64 sequences of up to
+// 8192 tokens, 32 heads over 8 of 128, 1.1 GB of bf16 in 202 us (5.5 TB/s; a
+// streaming read 6.3, a copy 4.7), of f16 in 220; one of 131,071, 16 heads over 2 of
+// 256 in bf16, 268 MB in 52 us and 6 more for the joining; 32 of up to 16,384, 64
+// heads over 4 of 128 in e4m3, 280 MB in 61 + 6 us (of a CU's cycles vector
+// instructions take half there, mostly unpacking, and MFMA a fifth; in f16 44% and
+// 17%).  Short calls are bound by latency: lengths, table, K and V, the waves'
+// joining, 8 us for 37 tokens.
 #include "kv.h"
 
 namespace {

@@ -14,17 +14,22 @@ constexpr int BINS = 2048;
 // Order of the scores as unsigned integers: a NaN is 0, -0 counts as +0.
 __device__ __forceinline__ uint32_t order_key(float f)
 {
-    if (f != f) return 0u;
     const uint32_t u = __float_as_uint(f + 0.0f);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+    return f != f ? 0u : u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
-
 // One work group per kv head and sequence; a thread holds PER scores of a
 // stretch of CT * PER, every CT-th one.  Where the tokens are more than `keep`,
 // up to three rounds of counting (11, 11 and 10 bits of the keys, from the top)
 // find the lowest key that stays and how many of its equals do; then one scan over
-// the waves' counts numbers the kept tokens in order.  Sequences longer than
-// the largest stretch read their scores again in every round.
+// the waves' counts numbers the kept tokens in order.  Sequences longer than a
+// stretch read their scores (from L2) again in every round.
+//
+// Up to 4096 tokens bound by latency: lengths, scores, then a dozen barriers, 7 us
+// for one sequence or 64; beyond by the instructions of one CU, about 30 per score
+// and round (one sequence, with the move of few tokens: 4096 11 us, 8192 14, 16,384
+// 20, 32,768 33, 131,072 97).  PER 4 up to 4096 tokens (8: 12 us) and 8 beyond (4:
+// 8192 15 us; 16 and 32 hold longer sequences, for 19.5 and 31.5 us at 16,384 and
+// 32,768, but take 16 and 21 us at 8192, as what is unrolled is run).
 template <int PER>
 __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict_args a)
 {
@@ -37,15 +42,14 @@ __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict
     float *ds = a.dst_score ? a.dst_score + ((size_t)b * p.kv + h) * a.dst_stride : nullptr;
     int *kept = a.kept + ((size_t)b * p.kv + h) * a.keep;
     if (h == 0 && tid == 0) a.counts[b] = n;
-    const int lo = a.sink, hi = len - a.recent;  // the tokens that the scores decide on
+    // the tokens that the scores decide on: `some` from `lo` on
+    const int lo = a.sink;
+    const uint32_t some = len > a.keep ? len - a.recent - lo : 0;
     const bool one = len <= CT * PER;
     float f[PER];
     auto load = [&](int i0) {  // (lengths leave room for a stretch below 2^31)
 #pragma unroll
-        for (int e = 0; e < PER; ++e) {
-            const int i = i0 + e * CT + tid;
-            f[e] = i < len ? score[i] : 0.0f;
-        }
+        for (int e = 0; e < PER; ++e) f[e] = score[min(i0 + e * CT + tid, len - 1)];
     };
     // the sums of x and y over the work group's threads before this one
     auto before = [&](uint32_t &x, uint32_t &y) {
@@ -63,25 +67,26 @@ __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict
 
     uint32_t key = 0;  // the lowest key that stays
     int ties = 0;      // and how many tokens of that key
-    if (one) load(0);
-    if (len > a.keep) {
+    if (one && len) load(0);
+    if (some) {
         for (int i = tid; i < 3 * BINS; i += CT) hist[i / BINS][i % BINS] = 0;
         __syncthreads();
         int left = a.keep - a.sink - a.recent;
         if (left == 0) key = 0xffffffffu;  // above every key
+#pragma unroll 1
         for (int round = 0; round < 3 && left; ++round) {
             const int shift = round == 0 ? 21 : round == 1 ? 10 : 0;
             const uint32_t mask = round == 2 ? 1023u : 2047u;
-            const uint32_t fixed = round == 0 ? 0u : round == 1 ? ~0u << 21 : ~0u << 10;
+            const uint32_t width = round == 0 ? ~0u : round == 1 ? (1u << 21) - 1 : 1023u;
             uint32_t *bins = hist[round];
             for (int i0 = 0; i0 < len; i0 += CT * PER) {
                 if (!one) load(i0);
 #pragma unroll
                 for (int e = 0; e < PER; ++e) {
                     if (i0 + e * CT >= len) break;
-                    const int i = i0 + e * CT + tid;
                     const uint32_t k = order_key(f[e]);
-                    if (i >= lo && i < hi && (k & fixed) == key) atomicAdd(&bins[(k >> shift) & mask], 1u);
+                    if ((uint32_t)(i0 + e * CT + tid - lo) < some && k - key <= width)
+                        atomicAdd(&bins[(k >> shift) & mask], 1u);
                 }
             }
             __syncthreads();
@@ -111,8 +116,9 @@ __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict
         for (int e = 0; e < PER; ++e) {
             const int i = i0 + e * CT + tid;
             const uint32_t k = order_key(f[e]);
-            const bool s = i < len && (len <= a.keep || i < lo || i >= hi || k > key);
-            const bool t = i < len && !s && k == key;
+            const bool open = (uint32_t)(i - lo) < some;
+            const bool s = i < len && (!open || k > key);
+            const bool t = open && k == key;
             const uint64_t bs = __ballot(s), bt = __ballot(t);
             if (lane == 0) count[e * NW + wave] = make_uint2(__popcll(bs), __popcll(bt));
             sure |= (uint64_t)s << e;
@@ -155,6 +161,12 @@ __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict
 // group takes every row, one stretch after the other, of SLICE bytes of the
 // columns; a stretch is read whole before any of it is written, and no later
 // stretch reads what it writes.
+//
+// Bound by memory: 32 sequences' up to 4096 rows of 8 kv heads of 128 in f16, 0.94
+// GB read and written, take 198 us (4.75 TB/s; a copy 4.72); 2048 rows of 2 heads
+// of 256 in bf16, 8.4 MB, 4.4 us, most of them the start and the chain of kept,
+// table and row.  The words are a vector type of the compiler: a struct of four
+// was put into LDS with a wait after each load (17 us).
 constexpr int MT = 256, MB = 4, SLICE = 64;
 
 // Rows of a stretch, of `words` words each (at most MT): MB for every thread.
@@ -242,10 +254,8 @@ extern "C" int ornk_kv_evict(const ornk_kv_pages *p, const ornk_evict_args *a, h
     const int rb = p->hd * (p->type == ORN_KV_F32 ? 4 : p->type == ORN_KV_E4M3 ? 1 : 2);
     if (a->max_len <= 4 * CT)
         hipLaunchKernelGGL(k_evict_choose<4>, dim3(p->kv, a->n_seqs), dim3(CT), 0, s, *p, *a);
-    else if (a->max_len <= 16 * CT)
-        hipLaunchKernelGGL(k_evict_choose<16>, dim3(p->kv, a->n_seqs), dim3(CT), 0, s, *p, *a);
     else
-        hipLaunchKernelGGL(k_evict_choose<32>, dim3(p->kv, a->n_seqs), dim3(CT), 0, s, *p, *a);
+        hipLaunchKernelGGL(k_evict_choose<8>, dim3(p->kv, a->n_seqs), dim3(CT), 0, s, *p, *a);
     typedef uint32_t u4 __attribute__((ext_vector_type(4)));
     if (rb % 16 == 0) move<u4>(*p, *a, rb, s);
     else if (rb % 4 == 0) move<uint32_t>(*p, *a, rb, s);
