@@ -139,7 +139,9 @@ int gpu_kv_append(gpu_context *ctx, const ornith_kv_pages *kv, const gpu_buffer 
  * score_out (may be NULL) [n_seqs][n_kv_heads][score_stride]: for the tokens
  * t < lens[b], decay * score_in[b][h][t] (score_in NULL: 0) + the sum of w over
  * kv head h's query heads; entries past a length stay as they are.  score_in may
- * be score_out. */
+ * be score_out.  The last score_new tokens of every sequence (1 in a step that
+ * appends one) have no score before this call: their score_in counts as 0,
+ * whatever it holds. */
 typedef struct {
     float scale;  /* 0: 1 / sqrt(head_dim) */
     int max_len;  /* no length is larger; 0: the table's width.  Sizes the workspace and
@@ -149,6 +151,7 @@ typedef struct {
     gpu_buffer *score_out;
     int score_stride; /* >= max_len */
     float decay;
+    int score_new; /* >= 0 */
 } ornith_attend_opts;
 int gpu_kv_attend(gpu_context *ctx, const ornith_kv_pages *kv, gpu_buffer *out,
                   const gpu_buffer *Q, int n_seqs, int n_heads, const gpu_buffer *table,

@@ -311,6 +311,7 @@ int gpu_kv_attend(gpu_context *ctx, const ornith_kv_pages *kv, gpu_buffer *out,
         return orn_set_err(ctx, ORN_EINVAL, "%s: Q or out too small", who);
     if (o->score_in && !o->score_out)
         return orn_set_err(ctx, ORN_EINVAL, "%s: score_in without score_out", who);
+    if (o->score_new < 0) return orn_set_err(ctx, ORN_EINVAL, "%s: score_new", who);
     if (o->score_out) {
         const size_t ns = o->score_stride < 0 ? SIZE_MAX
                                               : span(n_seqs, p.kv, o->score_stride, 1, 4);
@@ -340,6 +341,7 @@ int gpu_kv_attend(gpu_context *ctx, const ornith_kv_pages *kv, gpu_buffer *out,
     a.score_out = o->score_out ? (float *)o->score_out->dev : NULL;
     a.score_stride = (size_t)o->score_stride;
     a.decay = o->decay;
+    a.score_new = o->score_new;
     int prev;
     if ((rc = enter(ctx, &prev))) return rc;
     if (!(rc = err_words(ctx, &p.err))) {

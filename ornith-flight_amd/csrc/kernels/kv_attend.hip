@@ -897,18 +897,19 @@ __device__ __forceinline__ void sum_weights(const ornk_kv_pages &p, const ornk_a
     }
     if (t >= len) return;
     const size_t i = ((size_t)b * p.kv + h) * a.score_stride + t;
+    const int old = a.score_in ? max(len - a.score_new, 0) : 0;  // tokens that have a score
     if (a.score_stride % 4 == 0 && t + 4 <= len) {
         if (a.score_in) {
             const v4f x = *reinterpret_cast<const v4f *>(a.score_in + i);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum[e] = fmaf(a.decay, x[e], sum[e]);
+            for (int e = 0; e < 4; ++e) sum[e] = t + e < old ? fmaf(a.decay, x[e], sum[e]) : sum[e];
         }
         *reinterpret_cast<v4f *>(a.score_out + i) = sum;
         return;
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        if (t + e < len) a.score_out[i + e] = a.score_in ? fmaf(a.decay, a.score_in[i + e], sum[e]) : sum[e];
+        if (t + e < len) a.score_out[i + e] = t + e < old ? fmaf(a.decay, a.score_in[i + e], sum[e]) : sum[e];
 }
 
 __global__ void __launch_bounds__(FT) k_kv_finish(ornk_kv_pages p, ornk_attend_args a, AttendWs w, int jx)

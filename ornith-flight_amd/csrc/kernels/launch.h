@@ -96,6 +96,7 @@ typedef struct {
     float *score_out;
     size_t score_stride;
     float decay;
+    int score_new;
     void *ws;
 } ornk_attend_args;
 size_t ornk_kv_attend_ws(const ornk_kv_pages *p, const ornk_attend_args *a);

@@ -127,7 +127,7 @@ class AttendOpts(C.Structure):
     """ornith_attend_opts."""
     _fields_ = [("scale", C.c_float), ("max_len", C.c_int), ("flags", C.c_uint),
                 ("score_in", C.c_void_p), ("score_out", C.c_void_p), ("score_stride", C.c_int),
-                ("decay", C.c_float)]
+                ("decay", C.c_float), ("score_new", C.c_int)]
 
 
 class EvictOpts(C.Structure):
@@ -524,8 +524,9 @@ def kv_append(ctx, pages, K, V, T, slots, q_out=None, Q=None, heads=0, positions
 
 
 def attend_opts(scale=0.0, max_len=0, flags=0, score_in=None, score_out=None, score_stride=0,
-                decay=1.0):
-    o = AttendOpts(scale, max_len, flags, _ptr(score_in), _ptr(score_out), score_stride, decay)
+                decay=1.0, score_new=0):
+    o = AttendOpts(scale, max_len, flags, _ptr(score_in), _ptr(score_out), score_stride, decay,
+                   score_new)
     o.buffers = (score_in, score_out)
     return o
 

@@ -260,7 +260,7 @@ def test_host_refuses_rotations(host, change):
 @pytest.mark.parametrize("change", [
     dict(scale=math.nan), dict(scale=math.inf), dict(max_len=49), dict(max_len=-1), dict(max_len=41),
     dict(max_len=0), dict(score_stride=39), dict(score_stride=41), dict(score_stride=-1),
-    dict(score_out=None)])
+    dict(score_out=None), dict(score_new=-1)])
 def test_host_refuses_attend_options(host, change):
     c = Call(host, "attend")
     for k, v in change.items():
@@ -890,6 +890,99 @@ def test_pages_past_4_gb(om, ctx, type, n_pages):
     assert np.abs(ctx.download(ob, np.float32, q.shape)[0] - want).max() <= tol
     for b in bufs + [K, V]:
         b.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("stride", [64, 67])
+@pytest.mark.parametrize("fresh", [0, 1, 3, 50, 2 ** 31 - 1])
+def test_attend_tokens_without_a_score(om, ctx, fresh, stride):
+    """The last tokens' score_in holds anything, also a NaN."""
+    rng = np.random.default_rng(fresh % 97)
+    lens = [1, 2, 40, 61, 0]
+    c = Cache(om, ctx, "bf16", 20, 16, 2, 64, seed=4)
+    table = tables(rng, lens, 16, 20, 4)
+    q = rng.standard_normal((5, 4, 64)).astype(np.float32)
+    score = rng.uniform(0, 1, (5, 2, stride)).astype(np.float32)
+    for b, n in enumerate(lens):
+        score[b, :, max(n - fresh, 0):n] = np.nan
+    bufs = [ctx.upload(x) for x in (q, np.zeros_like(q), table, i32(lens), score)]
+    om.kv_attend(ctx, c.pages, bufs[1], bufs[0], 5, 4, bufs[2], 4, bufs[3],
+                 om.attend_opts(score_in=bufs[4], score_out=bufs[4], score_stride=stride, decay=0.5,
+                                score_new=fresh))
+    got = ctx.download(bufs[4], np.float32, score.shape)
+    for b, n in enumerate(lens):
+        k, v = c.rows(table[b], n) if n else (np.zeros((2, 0, 64)),) * 2
+        _, w, _, tw = attend64(q[b], k, v, 1 / 8)
+        add = w.reshape(2, 2, n).sum(1)
+        ws = add + 0.5 * np.nan_to_num(score[b, :, :n].astype(np.float64))
+        assert (np.abs(got[b, :, :n] - ws) <= (tw + EPS * 2) * add + 4 * EPS * np.abs(ws)).all()
+        assert same(torch.tensor(got[b, :, n:]), torch.tensor(score[b, :, n:]))
+    for b in bufs:
+        b.free()
+    c.free()
+
+
+@pytest.mark.gpu
+def test_decode_loop_without_the_host(om, ctx):
+    """Lengths, slots and positions of all steps are there beforehand; nothing is read back
+    until the end, and the scores live on the device only."""
+    rng = np.random.default_rng(41)
+    B, H, kv, D, page, width, steps = 2, 4, 2, 64, 16, 3, 40
+    keep, full = 20, 30
+    c = Cache(om, ctx, "f32", B * width, page, kv, D, seed=1)
+    table = i32(rng.permutation(B * width).reshape(B, width))
+    tb, junk = ctx.upload(table), np.full((B, kv, width * page), np.nan, np.float32)
+    sb, kept = ctx.upload(junk), ctx.upload(np.zeros((B, kv, keep), np.int32))
+    rope = om.rope_axes([D // 2], 1e4)
+    lens, outs, bufs = [0, 0], [], []
+    cache = [[[] for _ in range(kv)] for _ in range(B)]  # key, value, score, its tolerance
+    for step in range(steps):
+        q = rng.standard_normal((B, H, D)).astype(np.float32)
+        k, v = (rng.standard_normal((B, kv, D)).astype(np.float32) for _ in range(2))
+        slots = i32([table[b, lens[b] // page] * page + lens[b] % page for b in range(B)])
+        lens = [n + 1 for n in lens]
+        x = [ctx.upload(y) for y in (q, k, v, slots, i32([step] * B), i32(lens), np.zeros_like(q))]
+        bufs += x
+        om.kv_append(ctx, c.pages, x[1], x[2], B, x[3], x[0], x[0], H, x[4], rope, flags=om.KV_ASYNC)
+        om.kv_attend(ctx, c.pages, x[6], x[0], B, H, tb, width, x[5],
+                     om.attend_opts(flags=om.KV_ASYNC, score_in=sb, score_out=sb, score_new=1,
+                                    score_stride=width * page))
+        q64, k64 = (rope64(y, np.array([[step] * B]), [D // 2], 1e4, 0, 0)[0] for y in (q, k))
+        want, tol = np.zeros((B, H, D)), 0.0
+        for b in range(B):
+            for h in range(kv):
+                cache[b][h].append([k64[b, h], v[b, h].astype(np.float64), 0.0, 0.0])
+                kk, vv = (np.stack([t[i] for t in cache[b][h]])[None] for i in (0, 1))
+                g = slice(h * H // kv, (h + 1) * H // kv)
+                want[b, g], w, t1, tw = attend64(q64[b, g], kk, vv, 1 / 8)
+                # the rotations of q and k are off by 6 e (|u| + |v|) each
+                extra = 24 * EPS * np.abs(kk).max() * np.abs(q64[b, g]).max() * D / 8
+                tol = max(tol, t1 + 2 * extra * np.abs(vv).max())
+                for t, add in zip(cache[b][h], w.sum(0)):
+                    t[2] += add
+                    t[3] += (tw + 2 * extra + 2 * EPS) * add + 2 * EPS * t[2]
+        outs.append((x[6], want, tol))
+        if lens[0] == full:
+            om.kv_evict(ctx, c.pages, B, tb, width, x[5], sb, width * page, tb, width, x[5], sb,
+                        width * page, kept, om.evict_opts(keep, 2, 6, flags=om.KV_ASYNC))
+            for b in range(B):
+                for h in range(kv):
+                    s = np.array([t[2] for t in cache[b][h]])
+                    mid = np.sort(s[2:full - 6])[::-1]
+                    off = max(t[3] for t in cache[b][h])
+                    assert mid[keep - 9] - mid[keep - 8] > 2 * off  # rounding does not choose
+                    cache[b][h] = [cache[b][h][i] for i in choose(s.astype(np.float32), full, keep, 2, 6)]
+            lens = [keep] * B
+    assert om.lib().gpu_kv_check(ctx.ptr) == 0
+    for o, want, tol in outs:
+        assert np.abs(ctx.download(o, np.float32, want.shape) - want).max() <= tol
+    got = ctx.download(sb, np.float32, junk.shape)
+    for b in range(B):
+        for h in range(kv):
+            assert (np.abs(got[b, h, :lens[b]] - [t[2] for t in cache[b][h]]) <= [t[3] for t in cache[b][h]]).all()
+    for b in bufs + [tb, sb, kept]:
+        b.free()
+    c.free()
 
 
 @pytest.mark.gpu
