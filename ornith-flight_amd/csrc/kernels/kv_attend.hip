@@ -5,7 +5,7 @@
 // over the sequence's tokens, query heads sharing kv heads.
 //
 // Work: the tokens of every sequence, kv head and tile of 16 of its query heads
-// ("pair") in units of 128 or 256, one after the other on a line.  W work groups
+// ("pair") in units of 64 to 256, one after the other on a line.  W work groups
 // take equal stretches of the line, whatever the lengths are; a pair that one
 // group covers is finished there, of the others the groups leave O, m and l of
 // their part, which k_kv_finish puts together:
@@ -29,8 +29,8 @@ typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int WAVES = 4;
-// A unit is the waves' tiles, or as many more tokens as keep the line below 2^22
-// units (32-bit products with a group's number).
+// A unit has more tokens than below where that keeps the line below 2^22 units
+// (32-bit products with a group's number).
 constexpr int LINE_LOG2 = 22;
 // Work groups per CU, as log2: one's start and end under another's stream.  What
 // registers allow: K, V and O of a tile and their addresses take all of one
@@ -43,6 +43,15 @@ constexpr int groups_log2(int type, int HD)
     return HD == 256 ? 0 : HD == 64 && type == ORN_KV_F32 ? 2 : 1;
 }
 constexpr int CUS_LOG2 = 8;
+// Tokens of a unit, as log2: a tile for each wave; of the fp32 cache, whose tiles
+// are 16 keys, two at 64 columns (four: 32 sequences of up to 8000 tokens, 4 heads,
+// 66.3 instead of 60.9 us; 5 of 2047, 12 heads, 17.0 and 17.9) and one beyond (two:
+// 100 of up to 600, 2 heads of 128, 27.7 instead of 22.7 us; 5 of 2047, 4 heads of
+// 256, 31.9 and 27.6; one of 4000, 8 heads of 128, 14.1 and 16.5: more parts).
+constexpr int unit_log2(int type, int HD)
+{
+    return type == ORN_KV_F32 ? HD == 64 ? 7 : 6 : HD == 64 ? 8 : 7;
+}
 
 struct AttendWs {
     uint32_t *cum;   // [n_seqs + 1] units before each sequence, per pair of it
@@ -931,7 +940,7 @@ size_t attend_ws(const ornk_kv_pages *p, const ornk_attend_args *a, AttendWs *w)
     w->w_log2 = CUS_LOG2 + groups_log2(p->type, HD);
     const int G = a->heads / p->kv, W = 1 << w->w_log2;
     w->row = (p->hd + 3) & ~3;
-    w->unit_log2 = parts_keys(HD) == 64 ? 8 : 7;
+    w->unit_log2 = unit_log2(p->type, HD);
     const size_t pairs = (size_t)a->n_seqs * p->kv * ((G + 15) / 16);
     while (w->unit_log2 < 31 && pairs * (((size_t)a->max_len >> w->unit_log2) + 1) >> LINE_LOG2) ++w->unit_log2;
     const size_t longest = ((size_t)a->max_len + ((size_t)1 << w->unit_log2) - 1) >> w->unit_log2;
