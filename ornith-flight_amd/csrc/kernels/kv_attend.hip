@@ -32,6 +32,7 @@ constexpr int WAVES = 4;
 // A unit has more tokens than below where that keeps the line below 2^22 units
 // (32-bit products with a group's number).
 constexpr int LINE_LOG2 = 22;
+constexpr int MAX_SEGMENTS = (1 << (LINE_LOG2 - 8)) + 32;  // of one of 2^8 groups or more
 // Work groups per CU, as log2: one's start and end under another's stream.  What
 // registers allow: K, V and O of a tile and their addresses take all of one
 // wave's per SIMD at 256 columns (two groups with tiles of 16 keys: 131,071
@@ -167,14 +168,14 @@ __device__ __forceinline__ void unpack4(float *f, const uint32_t *w)
 
 // fp32 operands (v_mfma_f32_16x16x4_f32): what 32-bit arithmetic gives, with
 // infinities and NaN where it has them.  The path of the fp32 cache; of heads
-// whose rows are not whole 16-byte words (VEC = false); and of what the path
-// of the narrower types cannot give (see there).  16 keys per tile.
+// whose rows are not whole 16-byte words (VEC = false); and, as Shares, of what
+// neither path gives.  16 keys per tile.
 template <int TYPE, int HD, bool VEC, bool FULL>
 struct Exact {
     static constexpr int KT = 16, NJ = HD / 16, NV = HD / 64, NO = HD / 16;
     static constexpr int ES = elem_size<TYPE>;
     static constexpr size_t Q_BYTES = 16 * HD * 4;
-    static constexpr bool full = FULL, exact = true, ahead = TYPE == ORN_KV_F32 && VEC;
+    static constexpr bool full = FULL, vec = VEC, shares = false, ahead = TYPE == ORN_KV_F32 && VEC;
     float k[NJ][4], v[4][NV][4];
 
     // Past the row: any of its elements.  Of V they are columns that are not
@@ -231,7 +232,7 @@ struct Exact {
         for (int r = 0; r < 4; ++r) s[r] = acc[r];
     }
     // A key that is left out has the weight 0, and 0 times an infinity is none:
-    // its values count as zeros.  (Parts: such a segment comes to Exact.)
+    // its values count as zeros.  (Parts: such a segment comes to Shares.)
     __device__ __forceinline__ void leave_out(int r)
     {
 #pragma unroll
@@ -254,14 +255,23 @@ struct Exact {
     static __device__ __forceinline__ int col(int c, int n) { return 64 * (c / 4) + 4 * n + c % 4; }
 };
 
+// A segment whose sums were not finite, once more.  There are two reasons: an
+// infinity or a NaN, which Parts' operands cannot be; and weights relative to a
+// maximum that still grows, up to 2^6 each, whose sums with values near the largest
+// number pass it though the mean does not.  So the maximum and the sum are found
+// first (the scores are formed twice), and O is the sum of shares of it.
+template <int TYPE, int HD, bool VEC, bool FULL>
+struct Shares : Exact<TYPE, HD, VEC, FULL> {
+    static constexpr bool shares = true, ahead = false;
+};
+
 // bf16 operands (v_mfma_f32_16x16x32_bf16) for the caches of 16 and 8 bits.  A
 // cached value is one bf16 part (bf16, e4m3) or two (f16: 8 and 3 bits), a query
 // or a weight three: the top 8 bits, of the rest the top 8, and the rest.  Each
 // part has fp32's exponents, so 24 bits stay at every size, and the sums are
 // fp32.  Of the f16 products the smallest, second part by third, is left out
 // (2^-24 of the whole).  Parts of an infinity are no numbers: a segment whose
-// sums are not finite is done again by Exact.  32 or
-// 64 keys per tile.
+// sums are not finite is left to Shares.  32 or 64 keys per tile.
 //
 // Reduction indexes are permuted alike in both operands: a lane's 16 bytes of a
 // K row are its dimensions of one step (of two, for e4m3), and key 16 i + 4 g + r
@@ -282,7 +292,7 @@ struct Parts {
     static constexpr int VW = CW * ES / 4;
     static constexpr int NP = TYPE == ORN_KV_F16 ? 2 : 1;
     static constexpr size_t Q_BYTES = 3 * 16 * HD * 2;
-    static constexpr bool full = FULL, exact = false, ahead = true;
+    static constexpr bool full = FULL, vec = true, shares = false, ahead = true;
     uint32_t k[NI][NL][4], v[4 * NI][NH][VW];
 
     __device__ __forceinline__ void load_k(const uint8_t *const *row, int g, int hd)
@@ -442,13 +452,14 @@ struct Parts {
 };
 
 // ---------------------------------------------------------------------------
+// Returns whether one of this thread's sums is not finite.
 template <int TYPE, int HD, class Path>
 __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a, const AttendWs &w,
-                               const Seg &sg, uint8_t *lds, int slot)
+                               const Seg &sg, uint8_t *lds, int slot, int tid)
 {
     constexpr int KT = Path::KT, NI = KT / 16, NO = Path::NO, ES = elem_size<TYPE>;
     __shared__ float sm[WAVES][16], sl[WAVES][16];
-    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, n = lane & 15;
+    const int lane = tid & 63, g = lane >> 4, n = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hd = p.hd, len = sg.len;
 
@@ -546,8 +557,8 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
                 *reinterpret_cast<v4f *>(w.s + sg.score + n * w.s_len + t + 16 * i + 4 * g) = raw[i];
         }
     };
-    // the softmax of a tile's scores, and its O
-    auto rest = [&](int t) {
+    // a tile's scores without the keys that are left out
+    auto mask = [&](int t) {
         bool all = t + KT <= len;
 #pragma unroll
         for (int i = 0; i < NI; ++i) all = all && ok[i];
@@ -563,11 +574,19 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
         }
 #pragma unroll
         for (int i = 0; i < NI; ++i) raw[i] = (v4f){s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
+    };
+    auto tile_max = [&]() {
         float tm = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 4 * NI; ++i) tm = fmaxf(tm, s[i]);
         tm = fmaxf(tm, __shfl_xor(tm, 16, 64));
         tm = fmaxf(tm, __shfl_xor(tm, 32, 64));
+        return tm;
+    };
+    // the softmax of a tile's scores, and its O
+    auto rest = [&](int t) {
+        mask(t);
+        const float tm = tile_max();
         // the reference moves only when the maximum has passed it by a factor
         // of 2^6 (weights up to that stay): O is left alone in most tiles
         const float mn = tm > m + 6.0f ? tm : m;
@@ -590,7 +609,46 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
         }
         x.pv(o, s);
     };
-    if constexpr (Path::ahead) {
+    if constexpr (Path::shares) {
+        auto tile = [&](int t) {
+            asm volatile("" ::: "memory");
+            pages_for(t);
+            load_k(t);
+            load_v(t);
+            x.scores(s, lds, lane, hd);
+            mask(t);
+        };
+        auto weight = [&](float v) { return v == -INFINITY ? 0.0f : exp2_(v - m); };
+        for (int u = t; u < sg.k1; u += KT * WAVES) {
+            tile(u);
+            const float mn = fmaxf(m, tile_max());
+            l *= weight_from(m, mn);
+            m = mn;
+#pragma unroll
+            for (int i = 0; i < 4 * NI; ++i) l += weight(s[i]);
+        }
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        if (g == 0) {
+            sm[wave][n] = m;
+            sl[wave][n] = l;
+        }
+        __syncthreads();
+        const float M = fmaxf(fmaxf(sm[0][n], sm[1][n]), fmaxf(sm[2][n], sm[3][n]));
+        float L = 0.0f;
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) L += sl[v][n] * weight_from(sm[v][n], M);
+        l *= weight_from(m, M);
+        m = M;
+        const float share = L != 0.0f ? 1.0f / L : 0.0f;
+        for (; t < sg.k1; t += KT * WAVES) {
+            tile(t);
+#pragma unroll
+            for (int i = 0; i < 4 * NI; ++i) s[i] = weight(s[i]) * share;
+            x.pv(o, s);
+            keep(t);
+        }
+    } else if constexpr (Path::ahead) {
         // the next tile's K is on its way from the scores on, its V from O on
         if (t < sg.k1) {
             for (; t + KT * WAVES < sg.k1; t += KT * WAVES) {
@@ -617,11 +675,11 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
             keep(t);
         }
     }
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+    if constexpr (!Path::shares) {
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+    }
 
-    __shared__ int odd;
-    if (!Path::exact && tid == 0) odd = 0;
     __syncthreads();  // the queries are consumed
     if (g == 0) {
         sm[wave][n] = m;
@@ -662,13 +720,12 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[e] = fmaf(part[v][e], f, acc[e]);
         }
-        if (!Path::exact)
-            z += L * 0.0f + (acc[0] * 0.0f + acc[1] * 0.0f) + (acc[2] * 0.0f + acc[3] * 0.0f);
+        z += L * 0.0f + (acc[0] * 0.0f + acc[1] * 0.0f) + (acc[2] * 0.0f + acc[3] * 0.0f);
         float2 *ml;
         if (slot < 0) {  // the whole pair
             const size_t at = (size_t)sg.b * a.heads + sg.j0 + row;
             float *out = a.out + at * hd + c;
-            const float f = L != 0.0f ? p.v_scale / L : 0.0f;
+            const float f = Path::shares ? p.v_scale : L != 0.0f ? p.v_scale / L : 0.0f;
             if (hd % 4 == 0) {
                 if (c < hd) *reinterpret_cast<v4f *>(out) = acc * f;
             } else {
@@ -682,13 +739,10 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
             if (c < w.row) *reinterpret_cast<v4f *>(w.part_o + at * w.row + c) = acc;
             ml = w.part_ml + at;
         }
-        if (c == 0 && ml) *ml = make_float2(M, L);
+        // of a part, L below zero: O is the sum of shares
+        if (c == 0 && ml) *ml = make_float2(M, Path::shares && slot >= 0 ? -L : L);
     }
-    if constexpr (Path::exact) return true;
-    // a sum that is not finite is not this path's to say
-    if (z != 0.0f) odd = 1;
-    __syncthreads();
-    return odd == 0;
+    return z != 0.0f;
 }
 
 // A stretch of 256 sequences, four to a lane; every wave has it for itself, so
@@ -702,11 +756,11 @@ struct Stretch {
 };
 
 __device__ __forceinline__ Stretch scan_lens(const ornk_kv_pages &p, const ornk_attend_args &a,
-                                             const AttendWs &w, int c0, uint32_t before)
+                                             const AttendWs &w, int c0, uint32_t before, int lane)
 {
     Stretch s;
     s.c0 = c0;
-    const int b0 = c0 + 4 * (threadIdx.x & 63);
+    const int b0 = c0 + 4 * lane;
     int at[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) at[i] = a.lens[min(b0 + i, a.n_seqs - 1)];
@@ -725,36 +779,45 @@ __device__ __forceinline__ Stretch scan_lens(const ornk_kv_pages &p, const ornk_
     return s;
 }
 
-template <int TYPE, int HD, class Path>
-__global__ void __launch_bounds__(64 * WAVES, (1 << groups_log2(TYPE, HD))) k_kv_attend(ornk_kv_pages p, ornk_attend_args a,
-                                                                      AttendWs w)
+struct AttendCall {
+    ornk_kv_pages p;
+    ornk_attend_args a;
+    AttendWs w;
+};
+
+// The segments of this group's stretch of the line, in order.
+template <class F>
+__device__ __forceinline__ void walk(const AttendCall &call, int tid, F segment)
 {
-    extern __shared__ __align__(16) uint8_t lds[];
+    const ornk_kv_pages &p = call.p;
+    const ornk_attend_args &a = call.a;
+    const AttendWs &w = call.w;
     const int G = a.heads / p.kv, HT = (G + 15) / 16;
     const uint32_t per = p.kv * HT;  // pairs of a sequence
+    const int lane = tid & 63;
     Stretch st;
     for (int c = 0; c == 0 || c < a.n_seqs; c += STRETCH) {
-        st = scan_lens(p, a, w, c, c ? st.end : 0);
-        if (blockIdx.x == 0 && threadIdx.x < 64) {
-            const int b = c + 4 * threadIdx.x;
+        st = scan_lens(p, a, w, c, c ? st.end : 0, lane);
+        if (blockIdx.x == 0 && tid < 64) {
+            const int b = c + 4 * tid;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (b + i < a.n_seqs) w.cum[b + i] = st.before[i];
-            if (threadIdx.x == 0) w.cum[min(c + STRETCH, a.n_seqs)] = st.end;
+            if (tid == 0) w.cum[min(c + STRETCH, a.n_seqs)] = st.end;
         }
     }
     const uint32_t T = st.end * per;
     const uint32_t lo = line_at(T, w.w_log2, blockIdx.x), hi = line_at(T, w.w_log2, blockIdx.x + 1);
-    if (st.c0 && lo < hi) st = scan_lens(p, a, w, 0, 0);
+    if (st.c0 && lo < hi) st = scan_lens(p, a, w, 0, 0, lane);
     const uint32_t whole = line_whole(T, w.w_log2, w.whole);
     for (uint32_t u = lo; u < hi;) {
-        while (u >= st.end * per) st = scan_lens(p, a, w, st.c0 + STRETCH, st.end);
+        while (u >= st.end * per) st = scan_lens(p, a, w, st.c0 + STRETCH, st.end, lane);
         int b = -1, len = 0;  // u's sequence, in its lane
         uint32_t units = 0, start = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (u - st.before[i] * per < st.units[i] * per) {  // (wraps where u is before it)
-                b = st.c0 + 4 * (threadIdx.x & 63) + i;
+                b = st.c0 + 4 * lane + i;
                 len = st.len[i];
                 units = st.units[i];
                 start = st.before[i] * per;
@@ -787,18 +850,48 @@ __global__ void __launch_bounds__(64 * WAVES, (1 << groups_log2(TYPE, HD))) k_kv
         sg.k1 = (int)min((long long)sg.len, (long long)(k + cnt) << w.unit_log2);
         sg.score = ((size_t)sg.b * a.heads + sg.j0) * w.s_len;
         const int slot = cnt == n ? -1 : 2 * (int)blockIdx.x + (k ? 0 : 1);
-        const bool done = attend_segment<TYPE, HD, Path>(p, a, w, sg, lds, slot);
-        if constexpr (!Path::exact) {
-            if (!done) attend_segment<TYPE, HD, Exact<TYPE, HD, true, Path::full>>(p, a, w, sg, lds, slot);
-        }
+        segment(sg, slot);
         u += cnt;
     }
+}
+
+template <int TYPE, int HD, class Path>
+__global__ void __launch_bounds__(64 * WAVES, (1 << groups_log2(TYPE, HD))) k_kv_attend(AttendCall call)
+{
+    extern __shared__ __align__(16) uint8_t lds[];
+    __shared__ uint32_t odd[MAX_SEGMENTS / 32 + 1];  // a bit each; whether there is one
+    for (int i = threadIdx.x; i <= MAX_SEGMENTS / 32; i += 64 * WAVES) odd[i] = 0;
+    uint32_t at = 0;
+    walk(call, threadIdx.x, [&](const Seg &sg, int slot) {
+        if (attend_segment<TYPE, HD, Path>(call.p, call.a, call.w, sg, lds, slot, threadIdx.x)) {
+            atomicOr(&odd[at / 32], 1u << at % 32);
+            odd[MAX_SEGMENTS / 32] = 1;
+        }
+        ++at;
+    });
     // sequences without tokens: zeros
+    const ornk_attend_args &a = call.a;
     for (int b = blockIdx.x; b < a.n_seqs; b += gridDim.x) {
         if (a.lens[b] > 0 && a.max_len > 0) continue;
-        float *out = a.out + (size_t)b * a.heads * p.hd;
-        for (size_t i = threadIdx.x; i < (size_t)a.heads * p.hd; i += 64 * WAVES) out[i] = 0.0f;
+        float *out = a.out + (size_t)b * a.heads * call.p.hd;
+        for (size_t i = threadIdx.x; i < (size_t)a.heads * call.p.hd; i += 64 * WAVES) out[i] = 0.0f;
     }
+    __syncthreads();
+    if (!odd[MAX_SEGMENTS / 32]) return;
+    // Segments whose sums were not finite.  Nothing that the first walk has formed is
+    // held in registers for them (5 x 2047 tokens of 12 kv heads of 64 in fp32: 19.2
+    // instead of 17.4 us): the call is read anew.
+    auto args = __builtin_amdgcn_kernarg_segment_ptr();
+    int tid = threadIdx.x;
+    asm volatile("" : "+s"(args), "+v"(tid));
+    const AttendCall again = *(const AttendCall *)args;
+    at = 0;
+    walk(again, tid, [&](const Seg &sg, int slot) {
+        if (odd[at / 32] >> at % 32 & 1)
+            attend_segment<TYPE, HD, Shares<TYPE, HD, Path::vec, Path::full>>(again.p, again.a, again.w, sg, lds,
+                                                                              slot, tid);
+        ++at;
+    });
 }
 
 // The n parts of a pair (below 2: nothing is left to do), from group w0 on.
@@ -848,7 +941,8 @@ __device__ __forceinline__ void join_pair(const ornk_kv_pages &p, const ornk_att
         for (uint32_t i = sub; i < seg.n; i += JS) {
             const size_t slot = seg.slot(i) * 16 + row;
             const float2 ml = w.part_ml[slot];
-            add(ml.x, ml.y, *reinterpret_cast<const v4f *>(w.part_o + slot * w.row + c));
+            const v4f part = *reinterpret_cast<const v4f *>(w.part_o + slot * w.row + c);
+            add(ml.x, fabsf(ml.y), ml.y < 0.0f ? part * -ml.y : part);
         }
     sm[sub][x] = m;
     sl[sub][x] = l;
@@ -857,10 +951,28 @@ __device__ __forceinline__ void join_pair(const ornk_kv_pages &p, const ornk_att
     if (sub || row >= rows) return;
     for (int i = 1; i < JS; ++i) add(sm[i][x], sl[i][x], so[i][x]);
     const float f = l != 0.0f ? p.v_scale / l : 0.0f;
+    o *= f;
+    if (o[0] * 0.0f + o[1] * 0.0f + o[2] * 0.0f + o[3] * 0.0f != 0.0f) {
+        // not finite, or past the largest number on the way: every part by its share
+        m = -INFINITY, l = 0.0f;
+        for (uint32_t i = 0; i < seg.n; ++i) m = fmaxf(m, w.part_ml[seg.slot(i) * 16 + row].x);
+        for (uint32_t i = 0; i < seg.n; ++i) {
+            const float2 ml = w.part_ml[seg.slot(i) * 16 + row];
+            l += fabsf(ml.y) * weight_from(ml.x, m);
+        }
+        o = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t i = 0; i < seg.n; ++i) {
+            const size_t slot = seg.slot(i) * 16 + row;
+            const float2 ml = w.part_ml[slot];
+            const float share = (ml.y < 0.0f ? -ml.y : 1.0f) * weight_from(ml.x, m) / l;
+            o += *reinterpret_cast<const v4f *>(w.part_o + slot * w.row + c) * share;
+        }
+        o *= p.v_scale;
+    }
     float *out = a.out + ((size_t)b * a.heads + j0 + row) * hd + c;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        if (c + e < hd) out[e] = o[e] * f;
+        if (c + e < hd) out[e] = o[e];
 }
 
 __device__ __forceinline__ void sum_weights(const ornk_kv_pages &p, const ornk_attend_args &a,
@@ -890,7 +1002,7 @@ __device__ __forceinline__ void sum_weights(const ornk_kv_pages &p, const ornk_a
 #pragma unroll 4
                 for (uint32_t i = share; i < seg.n; i += 16) {
                     const float2 ml = w.part_ml[seg.slot(i) * 16 + row];
-                    add(ml.x, ml.y);
+                    add(ml.x, fabsf(ml.y));
                 }
             }
         }
@@ -972,7 +1084,8 @@ int launch_hd(const ornk_kv_pages *p, const ornk_attend_args *a, const AttendWs 
     size_t lds = (size_t)WAVES * rows * HD * 4;
     if (lds < Path::Q_BYTES) lds = Path::Q_BYTES;
     if (lds < Exact<TYPE, HD, true, true>::Q_BYTES) lds = Exact<TYPE, HD, true, true>::Q_BYTES;
-    hipLaunchKernelGGL((k_kv_attend<TYPE, HD, Path>), dim3(1 << w.w_log2), dim3(64 * WAVES), lds, s, *p, *a, w);
+    const AttendCall call = {*p, *a, w};
+    hipLaunchKernelGGL((k_kv_attend<TYPE, HD, Path>), dim3(1 << w.w_log2), dim3(64 * WAVES), lds, s, call);
     return hipGetLastError();
 }
 

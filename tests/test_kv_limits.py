@@ -1,0 +1,98 @@
+"""The paged key-value cache's calls where numbers end: values near the largest
+of 32 bits, scales of the 8-bit type, sizes of a launch, bits of a product, a
+workspace that grows.  Definitions and tolerances are those of test_kv_ops.py.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from test_kv_ops import (Cache, attend, attend64, ctx, i32, om, tables)  # noqa: F401
+
+
+# ------------------------------------------------------------ values near the largest
+def large_values(c, biggest, seed):
+    """Every value of V between half of +-biggest and all of it, one sign per dimension."""
+    g = torch.Generator().manual_seed(seed)
+    sign = torch.where(torch.rand(c.v.shape[3], generator=g) < 0.5, -1.0, 1.0)
+    x = (0.5 + 0.5 * torch.rand(c.v.shape, generator=g)) * sign * biggest
+    c.v.copy_(x.to(c.v.dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv,D,page,lens", [
+    (8, 2, 64, 16, [700, 0, 3]), (4, 1, 128, 64, [9000, 5]), (3, 3, 33, 8, [300]), (3, 1, 33, 64, [6000]),
+    (20, 4, 80, 16, [500, 3]), (16, 2, 256, 64, [4100]), (2, 1, 250, 64, [2500]), (40, 1, 192, 64, [1500])])
+def test_attend_values_near_the_largest(om, ctx, type, heads, kv, D, page, lens):
+    """A mean of finite values is finite, however many they are: a pair in one group, and cut
+    between groups."""
+    rng = np.random.default_rng(D)
+    n_pages = sum(-(-n // page) for n in lens)
+    c = Cache(om, ctx, type, n_pages, page, kv, D, seed=D)
+    large_values(c, 3e38, D)
+    c.write()
+    table = tables(rng, lens, page, n_pages, -(-max(lens) // page))
+    q = rng.standard_normal((len(lens), heads, D)).astype(np.float32)
+    score = rng.uniform(0, 2, (len(lens), kv, max(lens))).astype(np.float32)
+    for factor in (1.0, 0.0):  # 0: every weight is 1 / n
+        out, sc = attend(om, ctx, c, q * factor, lens, table, score=score, max_len=max(lens))
+        assert np.isfinite(out).sum() == out.size
+        for b, n in enumerate(lens):
+            k, v = c.rows(table[b], n) if n else (np.zeros((kv, 0, D)),) * 2
+            want, w, tol, tw = attend64((q * factor)[b], k, v, 1 / math.sqrt(D))
+            assert np.abs(out[b] - want).max() <= tol, (b, factor)
+            add = w.reshape(kv, heads // kv, n).sum(1)
+            ws = score[b, :, :n].astype(np.float64) + add
+            assert (np.abs(sc[b, :, :n] - ws) <= (tw + 2.0 ** -24 * heads // kv) * add +
+                    4 * 2.0 ** -24 * np.abs(ws)).all(), (b, factor)
+    c.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [64, 100, 128, 256])
+def test_attend_large_values_behind_a_growing_score(om, ctx, type, D):
+    """Scores that step up and down by less than a factor of 2^6 within a stretch of one group:
+    a weight relative to an earlier maximum is up to 64, and 64 such values are past 32 bits."""
+    B, n, page = 150, 4096, 1024
+    c = Cache(om, ctx, type, 4, page, 1, D, seed=D)
+    large_values(c, 3e37, D)
+    c.k[:] = 0.0
+    step = torch.arange(n).reshape(4, 1, page) // 256 % 2 == 1
+    c.k[..., 0] = torch.where(step, 4.0625, 0.0).to(c.k.dtype)  # 4.0625 log2 e = 5.86
+    c.write()
+    q = np.zeros((B, 4, D), np.float32)
+    q[..., 0] = 1.0
+    table = i32(np.tile(np.arange(4), (B, 1)))
+    out = attend(om, ctx, c, q, [n] * B, table, scale=1.0)
+    k, v = c.rows(table[0], n)
+    want, _, tol, _ = attend64(q[0], k, v, 1.0)
+    assert np.isfinite(out).sum() == out.size
+    assert np.abs(out - want).max() <= tol
+    c.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("D,n", [(64, 9000), (128, 200), (33, 700)])
+def test_attend_large_values_beside_what_is_not_finite(om, ctx, type, D, n):
+    """An infinite value makes its dimension infinite, and the others stay what they are: large
+    ones, and ones that would end below the smallest if they were scaled down."""
+    rng = np.random.default_rng(n)
+    n_pages = -(-n // 64)
+    c = Cache(om, ctx, type, n_pages, 64, 1, D, seed=D)
+    large_values(c, 3e38, D)
+    c.v[..., 3] = (torch.rand(c.v.shape[:3], generator=torch.Generator().manual_seed(1)) * 1e-36).to(c.v.dtype)
+    table = tables(rng, [n], 64, n_pages, n_pages)
+    c.v[table[0, (n // 2) // 64], 0, n // 2 % 64, 4] = math.inf
+    c.write()
+    q = rng.standard_normal((1, 4, D)).astype(np.float32)
+    out = attend(om, ctx, c, q, [n], table)
+    k, v = c.rows(table[0], n)
+    assert np.isposinf(out[0][:, 4]).sum() == 4
+    for d in [d for d in range(D) if d != 4]:  # every dimension by its own size
+        want, _, tol, _ = attend64(q[0], k, v[..., d:d + 1], 1 / math.sqrt(D))
+        assert np.abs(out[0][:, d:d + 1] - want).max() <= tol, d
+    c.free()
