@@ -726,6 +726,7 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
             const size_t at = (size_t)sg.b * a.heads + sg.j0 + row;
             float *out = a.out + at * hd + c;
             const float f = Path::shares ? p.v_scale : L != 0.0f ? p.v_scale / L : 0.0f;
+            if (L == 0.0f) acc = (v4f){0.0f, 0.0f, 0.0f, 0.0f};  // no weight, also of an infinity
             if (hd % 4 == 0) {
                 if (c < hd) *reinterpret_cast<v4f *>(out) = acc * f;
             } else {
@@ -952,7 +953,9 @@ __device__ __forceinline__ void join_pair(const ornk_kv_pages &p, const ornk_att
     for (int i = 1; i < JS; ++i) add(sm[i][x], sl[i][x], so[i][x]);
     const float f = l != 0.0f ? p.v_scale / l : 0.0f;
     o *= f;
-    if (o[0] * 0.0f + o[1] * 0.0f + o[2] * 0.0f + o[3] * 0.0f != 0.0f) {
+    if (l == 0.0f) {
+        o = (v4f){0.0f, 0.0f, 0.0f, 0.0f};  // no weight, also of an infinity
+    } else if (o[0] * 0.0f + o[1] * 0.0f + o[2] * 0.0f + o[3] * 0.0f != 0.0f) {
         // not finite, or past the largest number on the way: every part by its share
         m = -INFINITY, l = 0.0f;
         for (uint32_t i = 0; i < seg.n; ++i) m = fmaxf(m, w.part_ml[seg.slot(i) * 16 + row].x);

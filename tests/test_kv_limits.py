@@ -96,3 +96,27 @@ def test_attend_large_values_beside_what_is_not_finite(om, ctx, type, D, n):
         want, _, tol, _ = attend64(q[0], k, v[..., d:d + 1], 1 / math.sqrt(D))
         assert np.abs(out[0][:, d:d + 1] - want).max() <= tol, d
     c.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D,n", [(64, 1), (64, 40), (128, 6000), (33, 40), (33, 6000)])
+def test_attend_no_weight_at_all_is_zero(om, ctx, type, D, n):
+    """A head whose scores are all -infinity gives zeros, whatever the values are; the sequence
+    beside it is as ever."""
+    rng = np.random.default_rng(n)
+    n_pages = 2 * -(-n // 64)
+    c = Cache(om, ctx, type, n_pages, 64, 1, D, seed=D)
+    table = tables(rng, [n, n], 64, n_pages, n_pages // 2)
+    dead = torch.as_tensor(table[0].astype(np.int64))
+    c.k[dead] = -math.inf
+    c.v[dead[::2]] = math.inf
+    c.v[dead[0], 0, 0, 1] = math.nan
+    c.write()
+    q = np.abs(rng.standard_normal((2, 4, D))).astype(np.float32) + 0.25
+    out = attend(om, ctx, c, q, [n, n], table)
+    assert (out[0] == 0).sum() == out[0].size
+    k, v = c.rows(table[1], n)
+    want, _, tol, _ = attend64(q[1], k, v, 1 / math.sqrt(D))
+    assert np.abs(out[1] - want).max() <= tol
+    c.free()
