@@ -86,7 +86,8 @@ typedef struct {
     int page_size; /* a power of two, 8 to 1024; n_pages * page_size < 2^31 */
     int n_kv_heads; /* at most 32767; a page of all heads is below 4 GB */
     int head_dim;   /* 1 to 256 */
-    /* ORN_KV_E4M3: a stored value c stands for c * scale (0: 1).  Values beyond
+    /* ORN_KV_E4M3: a stored value c stands for c * scale (0: 1), of 2^-126 to 2^126;
+     * x is stored as the fp32 quotient x / scale, rounded to nearest.  Values beyond
      * 448 * scale are stored as that; a NaN stays one. */
     float k_scale, v_scale;
 } ornith_kv_pages;
@@ -134,7 +135,8 @@ int gpu_kv_append(gpu_context *ctx, const ornith_kv_pages *kv, const gpu_buffer 
  * padded batch) gives zeros, as does a head whose scores are all -infinity.  out
  * is not Q.  n_seqs * n_kv_heads, times ceil(n_heads / n_kv_heads / 16), is at
  * most 2^21.  The arithmetic is that of 32 bits whatever the cache's type,
- * infinities and NaN included.
+ * infinities and NaN included; scale and k_scale multiply the query first, v_scale
+ * the result.
  *
  * score_out (may be NULL) [n_seqs][n_kv_heads][score_stride]: for the tokens
  * t < lens[b], decay * score_in[b][h][t] (score_in NULL: 0) + the sum of w over

@@ -124,8 +124,10 @@ static int pages_ok(gpu_context *ctx, const ornith_kv_pages *kv, ornk_kv_pages *
     if (kv->K == kv->V) return orn_set_err(ctx, ORN_EINVAL, "%s: K is V", who);
     const float ks = kv->k_scale == 0.0f ? 1.0f : kv->k_scale;
     const float vs = kv->v_scale == 0.0f ? 1.0f : kv->v_scale;
-    if (kv->type == ORN_KV_E4M3 && !(ks > 0.0f && ks < INFINITY && vs > 0.0f && vs < INFINITY))
-        return orn_set_err(ctx, ORN_EINVAL, "%s: k_scale and v_scale are positive", who);
+    /* below, a scale is subnormal and has fewer digits; above, hardly a stored value is finite */
+    if (kv->type == ORN_KV_E4M3 &&
+        !(ks >= 0x1p-126f && ks <= 0x1p126f && vs >= 0x1p-126f && vs <= 0x1p126f))
+        return orn_set_err(ctx, ORN_EINVAL, "%s: k_scale and v_scale are from 2^-126 to 2^126", who);
     memset(p, 0, sizeof *p);
     p->k = kv->K->dev;
     p->v = kv->V->dev;

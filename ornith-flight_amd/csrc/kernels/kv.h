@@ -35,10 +35,11 @@ struct KvElem<ORN_KV_E4M3> {
     {
         return __builtin_amdgcn_cvt_f32_fp8((int)x, 0);
     }
-    // inv: 1 / scale; clamped by comparisons, which leave a NaN one
-    static __device__ __forceinline__ T put(float x, float inv)
+    // the quotient in fp32 (a rounded 1 / scale would round twice, and move values
+    // next to a middle of two); clamped by comparisons, which leave a NaN one
+    static __device__ __forceinline__ T put(float x, float scale)
     {
-        x *= inv;
+        x /= scale;
         x = x > 448.0f ? 448.0f : x < -448.0f ? -448.0f : x;
         return (T)(__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false) & 0xff);
     }

@@ -39,18 +39,18 @@ __global__ void __launch_bounds__(128) k_rope_append_any(ornk_kv_pages p, ornk_r
         float *y = part == 0 ? a.q_out : part == 1 ? a.k_out : nullptr;
         if (y) y += ((size_t)t * heads + head) * hd;
         typename E::T *c = nullptr;
-        float inv = 1.0f;
+        float scale = 1.0f;
         if (part && a.slots) {
             const int slot = kv_slot(p, a.slots, t);
             if (slot >= 0) {
                 c = static_cast<typename E::T *>(part == 1 ? p.k : p.v) +
                     kv_at(p, slot >> p.page_log2, head, slot & (p.page - 1));
-                inv = 1.0f / (part == 1 ? p.k_scale : p.v_scale);
+                scale = part == 1 ? p.k_scale : p.v_scale;
             }
         }
         auto put = [&](int i, float v) {
             if (y) y[i] = v;
-            if (c) c[i] = E::put(v, inv);
+            if (c) c[i] = E::put(v, scale);
         };
         const int n_rot = part == 2 ? 0 : R;
         for (int i = tid; i < hd - n_rot; i += 128) {
@@ -70,13 +70,13 @@ __global__ void __launch_bounds__(128) k_rope_append_any(ornk_kv_pages p, ornk_r
 
 // Four elements rounded to the cache's type, in one store.
 template <int TYPE>
-__device__ __forceinline__ void put4(typename KvElem<TYPE>::T *c, v4f x, float inv)
+__device__ __forceinline__ void put4(typename KvElem<TYPE>::T *c, v4f x, float scale)
 {
     typedef typename KvElem<TYPE>::T T;
     typedef T vec __attribute__((ext_vector_type(4)));
     vec v;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = KvElem<TYPE>::put(x[i], inv);
+    for (int i = 0; i < 4; ++i) v[i] = KvElem<TYPE>::put(x[i], scale);
     *reinterpret_cast<vec *>(c) = v;
 }
 
@@ -127,7 +127,6 @@ __global__ void __launch_bounds__(RT, 8) k_rope_append(ornk_kv_pages p, ornk_rop
         it.x = *reinterpret_cast<const v4f *>(x + it.c);
         if (it.two) it.y = *reinterpret_cast<const v4f *>(x + it.c + R);
     };
-    const float k_inv = 1.0f / p.k_scale, v_inv = 1.0f / p.v_scale;
     for (long long at = blockIdx.x; at < a.T; at += gridDim.x) {
         const int t = (int)at;
         Item it;
@@ -170,8 +169,8 @@ __global__ void __launch_bounds__(RT, 8) k_rope_append(ornk_kv_pages p, ornk_rop
                 const bool key = kvh < a.kv;
                 T *c = static_cast<T *>(key ? p.k : p.v) +
                        kv_at(p, slot >> p.page_log2, key ? kvh : kvh - a.kv, slot & (p.page - 1)) + it.c;
-                put4<TYPE>(c, x, key ? k_inv : v_inv);
-                if (it.two) put4<TYPE>(c + R, y, k_inv);
+                put4<TYPE>(c, x, key ? p.k_scale : p.v_scale);
+                if (it.two) put4<TYPE>(c + R, y, p.k_scale);
             }
         }
         __syncthreads();  // the token's angles are consumed

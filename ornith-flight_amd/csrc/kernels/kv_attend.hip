@@ -538,7 +538,9 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
 #pragma unroll
     for (int i = 0; i < HD / 64; ++i) {
         const int at = tid + 64 * WAVES * i;
-        Path::put_q(lds, at / (HD / 4), at % (HD / 4) * 4, q[i] * (a.scale * p.k_scale * 1.44269504088896341f));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[i][e] = q[i][e] * (a.scale * 1.44269504088896341f) * p.k_scale;
+        Path::put_q(lds, at / (HD / 4), at % (HD / 4) * 4, q[i]);
     }
     __syncthreads();
 
@@ -725,14 +727,16 @@ __device__ bool attend_segment(const ornk_kv_pages &p, const ornk_attend_args &a
         if (slot < 0) {  // the whole pair
             const size_t at = (size_t)sg.b * a.heads + sg.j0 + row;
             float *out = a.out + at * hd + c;
-            const float f = Path::shares ? p.v_scale : L != 0.0f ? p.v_scale / L : 0.0f;
-            if (L == 0.0f) acc = (v4f){0.0f, 0.0f, 0.0f, 0.0f};  // no weight, also of an infinity
+            const float f = Path::shares ? 1.0f : 1.0f / L;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)  // (no weight: zeros, also of an infinity)
+                acc[e] = L != 0.0f ? acc[e] * f * p.v_scale : 0.0f;
             if (hd % 4 == 0) {
-                if (c < hd) *reinterpret_cast<v4f *>(out) = acc * f;
+                if (c < hd) *reinterpret_cast<v4f *>(out) = acc;
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (c + e < hd) out[e] = acc[e] * f;
+                    if (c + e < hd) out[e] = acc[e];
             }
             ml = w.ml ? w.ml + at : nullptr;
         } else {
@@ -951,8 +955,7 @@ __device__ __forceinline__ void join_pair(const ornk_kv_pages &p, const ornk_att
     __syncthreads();
     if (sub || row >= rows) return;
     for (int i = 1; i < JS; ++i) add(sm[i][x], sl[i][x], so[i][x]);
-    const float f = l != 0.0f ? p.v_scale / l : 0.0f;
-    o *= f;
+    o *= l != 0.0f ? 1.0f / l : 0.0f;
     if (l == 0.0f) {
         o = (v4f){0.0f, 0.0f, 0.0f, 0.0f};  // no weight, also of an infinity
     } else if (o[0] * 0.0f + o[1] * 0.0f + o[2] * 0.0f + o[3] * 0.0f != 0.0f) {
@@ -970,12 +973,11 @@ __device__ __forceinline__ void join_pair(const ornk_kv_pages &p, const ornk_att
             const float share = (ml.y < 0.0f ? -ml.y : 1.0f) * weight_from(ml.x, m) / l;
             o += *reinterpret_cast<const v4f *>(w.part_o + slot * w.row + c) * share;
         }
-        o *= p.v_scale;
     }
     float *out = a.out + ((size_t)b * a.heads + j0 + row) * hd + c;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        if (c + e < hd) out[e] = o[e];
+        if (c + e < hd) out[e] = o[e] * p.v_scale;
 }
 
 __device__ __forceinline__ void sum_weights(const ornk_kv_pages &p, const ornk_attend_args &a,

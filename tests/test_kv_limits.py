@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_kv_ops import (Cache, attend, attend64, ctx, i32, om, tables)  # noqa: F401
+from test_kv_ops import (Cache, Call, attend, attend64, ctx, host, i32, om, tables)  # noqa: F401
 
 
 # ------------------------------------------------------------ values near the largest
@@ -119,4 +119,92 @@ def test_attend_no_weight_at_all_is_zero(om, ctx, type, D, n):
     k, v = c.rows(table[1], n)
     want, _, tol, _ = attend64(q[1], k, v, 1 / math.sqrt(D))
     assert np.abs(out[1] - want).max() <= tol
+    c.free()
+
+
+# ------------------------------------------------------------ scales of the 8-bit type
+@pytest.mark.parametrize("what", ["append", "attend", "evict"])
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+def test_host_takes_scales_with_a_reciprocal(host, what, which):
+    c = Call(host, what)
+    c.pages.type = host.om.KV_TYPES["e4m3"]
+    for scale in (2.0 ** -126, 1e-20, 0.3, 1e20, 2.0 ** 126):
+        setattr(c.pages, which, scale)
+        assert c() == (0, 1), scale
+    for scale in (1e-45, 1e-39, float(np.nextafter(np.float32(2.0 ** -126), np.float32(0))),
+                  float(np.nextafter(np.float32(2.0 ** 126), np.float32(np.inf))), 3e38):
+        setattr(c.pages, which, scale)
+        assert c() == (-1, 0), scale
+    c.pages.type = host.om.KV_TYPES["f16"]  # has no scales
+    assert c() == (0, 1)
+
+
+E4M3 = np.arange(256, dtype=np.uint8)
+E4M3 = torch.from_numpy(E4M3).view(torch.float8_e4m3fn).float().numpy()
+E4M3 = np.sort(E4M3[np.isfinite(E4M3) & (E4M3 >= 0)])  # 0 twice
+
+
+@pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore::RuntimeWarning")  # 449 x 2^126
+@pytest.mark.parametrize("scale", [0.3, 1.0, 3.0, 0.0123, 1e-20, 7e15, 2.0 ** -126, 2.0 ** 126, 3.3e-38])
+@pytest.mark.parametrize("rotated", [False, True])
+def test_append_rounds_the_quotient(om, ctx, scale, rotated):
+    """x is stored as x / scale of 32 bits, rounded to nearest: at the middles between two
+    values of the type and beside them, at zeros, and past the largest."""
+    scale = float(np.float32(scale))
+    mid = ((E4M3[1:].astype(np.float64) + E4M3[:-1]) / 2 * scale).astype(np.float32)
+    x, d = [mid], mid
+    for _ in range(4):
+        d = np.nextafter(d, np.float32(np.inf))
+        x.append(d)
+    d = mid
+    for _ in range(4):
+        d = np.nextafter(d, np.float32(0))
+        x.append(d)
+    x = np.concatenate(x + [np.zeros(64, np.float32), (E4M3 * np.float64(scale)).astype(np.float32),
+                            np.array([449, 480, 600, 1e6], np.float64).astype(np.float32) * np.float32(scale)])
+    x = np.concatenate([x, -x])
+    D = 64 if not rotated else 66  # 66: rows that are no whole float4s
+    T = -(-x.size // D)
+    x = np.concatenate([x, np.zeros(T * D - x.size, np.float32)]).reshape(T, 1, D)
+    n_pages = -(-T // 16)
+    c = Cache(om, ctx, "e4m3", n_pages, 16, 1, D, seed=1, ks=scale, vs=scale)
+    bufs = [ctx.upload(y) for y in (x, i32(np.arange(T)), i32(np.zeros(T)))]
+    rope = om.rope_axes([8], 1e4) if rotated else None  # at position 0: nothing turns
+    om.kv_append(ctx, c.pages, bufs[0], bufs[0], T, bufs[1], None, None, 0, bufs[2] if rope else None, rope)
+    for got, turned in zip(c.read(), (rotated, False)):
+        y = x[:, 0].copy()
+        if turned:  # cos 1, sin 0; an infinity (past the largest 2^126) makes its pair NaN
+            u, v = x[:, 0, 0:16:2], x[:, 0, 1:16:2]
+            with np.errstate(invalid="ignore"):
+                y[:, 0:16:2], y[:, 1:16:2] = u - v * np.float32(0), u * np.float32(0) + v
+        y = torch.from_numpy((y / np.float32(scale)).clip(-448, 448)).to(torch.float8_e4m3fn).float()
+        got = got.float().transpose(1, 2).reshape(-1, D)[:T]
+        assert torch.isnan(got).sum() == (torch.isnan(got) & torch.isnan(y)).sum() == torch.isnan(y).sum()
+        assert torch.isnan(y).sum() == 0 or scale > 1e37
+        assert ((got != y) & ~torch.isnan(y)).sum() == 0
+    for b in bufs:
+        b.free()
+    c.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vs", [2.0 ** -126, 1e-30, 0.3, 1e30])
+@pytest.mark.parametrize("n", [40, 5000])
+def test_attend_scales_keep_their_digits(om, ctx, vs, n):
+    """out is v_scale times the mean of what is stored, to fp32's rounding, at the ends of the
+    scales, too: 1 / sum and v_scale are not formed as one small number."""
+    rng = np.random.default_rng(n)
+    n_pages = -(-n // 64)
+    vs = float(np.float32(vs))
+    c = Cache(om, ctx, "e4m3", n_pages, 64, 1, 128, seed=n, vs=vs, ks=0.3)
+    c.k[:] = 0  # the scores are exact: what is left is the sum's rounding
+    c.v.copy_((c.v.float().abs() * 16 + 64).clamp(max=448).to(c.v.dtype))
+    c.write()
+    table = tables(rng, [n], 64, n_pages, n_pages)
+    q = rng.standard_normal((1, 4, 128)).astype(np.float32)
+    out = attend(om, ctx, c, q, [n], table)
+    k, v = c.rows(table[0], n)
+    want, _, tol, _ = attend64(q[0], k, v, 1 / math.sqrt(128))
+    assert np.abs(out[0] - want).max() <= tol + 2.0 ** -24 * np.abs(want).max()
     c.free()
