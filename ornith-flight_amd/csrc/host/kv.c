@@ -373,7 +373,7 @@ int gpu_kv_evict(gpu_context *ctx, const ornith_kv_pages *kv, int n_seqs, const 
     if (!score || !dst_table || !dst_lens || !kept || dst_pages < 0)
         return orn_set_err(ctx, ORN_EINVAL, "%s: bad arguments", who);
     const int most = opts->keep < bound ? opts->keep : bound; /* the longest result */
-    if (most > 1 << 27) /* work groups of 256 threads to 16 rows or more, 2^32 threads a launch */
+    if (most > 1 << 27) /* 2^25 stretches of 4 rows: 32 launches of the mover */
         return orn_set_err(ctx, ORN_EUNSUPPORTED, "%s: %d tokens kept (at most 2^27)", who, most);
     if ((long long)dst_pages * p.page < most || !holds(dst_table, span(n_seqs, dst_pages, 1, 1, 4)))
         return orn_set_err(ctx, ORN_EINVAL, "%s: dst_table has no room for %d tokens", who, most);

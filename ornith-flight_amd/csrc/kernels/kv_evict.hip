@@ -156,7 +156,8 @@ __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict
 // of one kv head, sequence and K or V, a stretch at a time: the rows' places go
 // through LDS, then every thread has up to MB words in flight.
 //
-// Into other pages, each group takes one stretch of whole rows.  Within a
+// Into other pages, each group takes one stretch of whole rows, up to MAX_GROUPS of
+// them a launch (rows of 129 words and more have stretches of 4).  Within a
 // sequence's own pages (IN_PLACE) a row moves towards the front or stays: a
 // group takes every row, one stretch after the other, of SLICE bytes of the
 // columns; a stretch is read whole before any of it is written, and no later
@@ -168,6 +169,7 @@ __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict
 // table and row.  The words are a vector type of the compiler: a struct of four
 // was put into LDS with a wait after each load (17 us).
 constexpr int MT = 256, MB = 4, SLICE = 64;
+constexpr int MAX_GROUPS = 1 << 20;  // of a launch's x: 2^28 threads
 
 // Rows of a stretch, of `words` words each (at most MT): MB for every thread.
 __host__ __device__ inline int stretch_rows(int words)
@@ -177,7 +179,8 @@ __host__ __device__ inline int stretch_rows(int words)
 }
 
 template <class WORD, bool IN_PLACE>
-__global__ void __launch_bounds__(MT) k_evict_move(ornk_kv_pages p, ornk_evict_args a, int row_bytes)
+__global__ void __launch_bounds__(MT) k_evict_move(ornk_kv_pages p, ornk_evict_args a, int row_bytes,
+                                                    int group0)
 {
     constexpr int WB = sizeof(WORD);
     __shared__ size_t from[MT], to[MT];  // bytes into the pages; NONE: the row stays where it is
@@ -191,7 +194,7 @@ __global__ void __launch_bounds__(MT) k_evict_move(ornk_kv_pages p, ornk_evict_a
     const int pass = MT / words, mr = stretch_rows(words);
     const int r0 = tid / words < pass ? tid / words : MT, col = tid % words * WB;
     uint8_t *pool = static_cast<uint8_t *>(blockIdx.y >= p.kv ? p.v : p.k) + c0;
-    for (int j0 = IN_PLACE ? 0 : blockIdx.x * mr; j0 < most; j0 += mr) {
+    for (int j0 = IN_PLACE ? 0 : (group0 + blockIdx.x) * mr; j0 < most; j0 += mr) {
         const int rows = min(mr, most - j0);
         int some = 0;  // (kept is -1 past the sequence's last)
         if (tid < rows) {
@@ -239,12 +242,14 @@ void move(const ornk_kv_pages &p, const ornk_evict_args &a, int row_bytes, hipSt
     const unsigned y = 2 * p.kv, z = a.n_seqs;
     if (a.in_place) {
         hipLaunchKernelGGL((k_evict_move<WORD, true>), dim3((row_bytes + SLICE - 1) / SLICE, y, z),
-                           dim3(MT), 0, s, p, a, row_bytes);
+                           dim3(MT), 0, s, p, a, row_bytes, 0);
         return;
     }
     const int mr = stretch_rows(row_bytes / (int)sizeof(WORD));
-    hipLaunchKernelGGL((k_evict_move<WORD, false>), dim3(most ? (most + mr - 1) / mr : 1, y, z),
-                       dim3(MT), 0, s, p, a, row_bytes);
+    const int x = most ? (most + mr - 1) / mr : 1;
+    for (int x0 = 0; x0 < x; x0 += MAX_GROUPS)
+        hipLaunchKernelGGL((k_evict_move<WORD, false>), dim3(x - x0 < MAX_GROUPS ? x - x0 : MAX_GROUPS, y, z),
+                           dim3(MT), 0, s, p, a, row_bytes, x0);
 }
 
 }  // namespace

@@ -3,12 +3,14 @@ of 32 bits, scales of the 8-bit type, sizes of a launch, bits of a product, a
 workspace that grows.  Definitions and tolerances are those of test_kv_ops.py.
 """
 import math
+import os
+import subprocess
 
 import numpy as np
 import pytest
 import torch
 
-from test_kv_ops import (Cache, Call, attend, attend64, ctx, host, i32, om, tables)  # noqa: F401
+from test_kv_ops import (HERE, Cache, Call, attend, attend64, ctx, host, i32, om, tables)  # noqa: F401
 
 
 # ------------------------------------------------------------ values near the largest
@@ -208,3 +210,91 @@ def test_attend_scales_keep_their_digits(om, ctx, vs, n):
     want, _, tol, _ = attend64(q[0], k, v, 1 / math.sqrt(128))
     assert np.abs(out[0] - want).max() <= tol + 2.0 ** -24 * np.abs(want).max()
     c.free()
+
+
+# ------------------------------------------------------------ sizes of the launches
+@pytest.fixture(scope="module")
+def grids(tmp_path_factory):
+    """The launches (x, y, z, threads) of calls, by the kernels' own host side."""
+    hipcc = "/opt/rocm/bin/hipcc"
+    if not os.path.exists(hipcc):
+        pytest.skip("no hipcc")
+    root = os.path.dirname(HERE)
+    d = tmp_path_factory.mktemp("grids")
+    flags = ["-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-I" + os.path.join(root, "include")]
+    kernels = os.path.join(root, "ornith-flight_amd", "csrc", "kernels")
+    for f in ("kv", "kv_attend", "kv_evict"):
+        subprocess.run([hipcc, "--offload-host-only", "-O1", "--offload-arch=gfx950", "-std=c++17", *flags[2:],
+                        "-c", os.path.join(kernels, f + ".hip"), "-o", str(d / (f + ".o"))], check=True)
+    subprocess.run(["gcc", "-std=gnu99", *flags, "-c", os.path.join(HERE, "kv_grids.c"), "-o", str(d / "main.o")],
+                   check=True)
+    subprocess.run(["g++", "-no-pie", "-Wl,--unresolved-symbols=ignore-all", "-o", str(d / "grids"),
+                    *[str(d / (f + ".o")) for f in ("main", "kv", "kv_attend", "kv_evict")]], check=True)
+
+    def run(cases):
+        text = "\n".join(" ".join(map(str, c)) for c in cases)
+        out = subprocess.run([str(d / "grids")], input=text, capture_output=True, text=True, check=True,
+                             timeout=300).stdout.splitlines()
+        assert len(out) == len(cases)
+        return [np.array(line.split(), np.int64).reshape(-1, 4) for line in out]
+    return run
+
+
+def within_the_limits(cases, launches):
+    """A dimension has fewer than 2^32 threads, and y and z at most 65535 groups."""
+    for c, g in zip(cases, launches):
+        assert len(g) >= 1 and (g >= 1).all(), c
+        assert (g[:, 0] * g[:, 3] < 1 << 32).all() and (g[:, 1:3] <= 65535).all(), (c, g.tolist())
+
+
+@pytest.mark.parametrize("in_place", [0, 1])
+@pytest.mark.parametrize("type", [0, 1, 2, 3])
+def test_an_evictions_launches_fit(grids, type, in_place):
+    """Up to the most that a call may keep, whatever words the rows are moved in."""
+    most = 1 << 27
+    cases = [("e", hd, type, kv, n, length, keep, in_place) for hd in (1, 8, 33, 64, 129, 130, 192, 250, 255, 256)
+             for kv, n in ((1, 1), (8, 3), (32767, 65535))
+             for length, keep in ((most, most), (2 ** 31 - 2 ** 16, most), (most, 2 ** 31 - 1), (1 << 26, 1 << 26),
+                                  (5000, 700), (1, 1), (0, 1))]
+    within_the_limits(cases, grids(cases))
+
+
+def test_an_attentions_and_a_rotations_launches_fit(grids):
+    cases = [("a", hd, type, kv, n, length, heads, score) for hd in (1, 64, 100, 256) for type in range(4)
+             for kv, n, heads in ((1, 1, 65535), (32, 65535, 32), (1, 65535, 512), (32767, 64, 32767))
+             for length in (1, 5000, 2 ** 31 - 2 ** 16) for score in (0, 1)]
+    cases += [("r", hd, R, halves, kv, T, heads, slots) for hd, R in ((1, 0), (64, 32), (66, 33), (4096, 256))
+              for halves in (0, 1) for kv, heads in ((1, 0), (8, 64), (65535, 65535))
+              for T in (1, 4097, 2 ** 31 - 1) for slots in (0, 1)]
+    within_the_limits(cases, grids(cases))
+
+
+@pytest.mark.gpu
+def test_evict_more_stretches_than_a_launch_takes(om, ctx):
+    """Rows of 129 bytes are moved by stretches of 4, and more than 2^20 stretches by more than one
+    launch.  Equal scores keep the first tokens, in order."""
+    D, page, n, keep = 129, 1024, 4_400_000, 4_300_000
+    new, old = -(-keep // page), -(-n // page)
+    rng = np.random.default_rng(2)
+    nbytes = (new + old) * page * D
+    K, V = ctx.alloc(nbytes), ctx.alloc(nbytes)
+    pages = om.kv_pages(K, V, "e4m3", new + old, page, 1, D)
+    x = rng.integers(0, 256, nbytes, np.uint8)
+    for b in (K, V):
+        om.lib().gpu_copy_to_device(ctx.ptr, b.ptr, om._p(x), nbytes)
+        x = x[::-1].copy()
+    table, dst = i32(new + np.arange(old))[None], i32(rng.permutation(new))[None]
+    bufs = [ctx.upload(a) for a in (table, i32([n]), np.zeros(n, np.float32), dst, i32([0]), np.zeros(keep, np.int32))]
+    tb, lb, sb, db, dl, kb = bufs
+    om.kv_evict(ctx, pages, 1, tb, old, lb, sb, n, db, new, dl, None, 0, kb, om.evict_opts(keep, max_len=n))
+    assert ctx.download(dl, np.int32, (1,))[0] == keep
+    assert np.array_equal(ctx.download(kb, np.int32, (keep,)), np.arange(keep))
+    for b in (K, V):
+        got = ctx.download(b, np.uint8, (new, page, D))[dst[0]].reshape(-1, D)
+        src = x.reshape(-1, page, D)
+        assert np.array_equal(got[:keep], src[new:].reshape(-1, D)[:keep])
+        last = src[:new][dst[0]].reshape(-1, D)
+        assert np.array_equal(got[keep:], last[keep:])  # places past the last are as they were
+        x = x[::-1].copy()
+    for b in bufs + [K, V]:
+        b.free()
