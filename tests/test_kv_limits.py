@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_kv_ops import (HERE, Cache, Call, attend, attend64, ctx, host, i32, om, tables)  # noqa: F401
+from test_kv_ops import (DTYPE, HERE, Cache, Call, attend, attend64, ctx, host, i32, om, tables, value)  # noqa: F401
 
 
 # ------------------------------------------------------------ values near the largest
@@ -298,3 +298,70 @@ def test_evict_more_stretches_than_a_launch_takes(om, ctx):
         x = x[::-1].copy()
     for b in bufs + [K, V]:
         b.free()
+
+
+# ------------------------------------------------------------ bits of the products
+def sharp(type, D, seed, bits=24):
+    """Queries of a few dimensions and keys whose scores lie up to 40 apart (three heads) and up
+    to 0.8 (three more), V's column j the indicator of token j (so out_j is its weight) and its
+    last column 1.  Returns q, k, v, the weights in 64 bits and what each may be off, relative
+    to itself.
+
+    A score is the sum of 4 products of positive numbers: 12 products of parts and their sums,
+    each rounded once, and the scale's two roundings in the query: 16 e of itself, for the
+    token's score and for the largest; the exponential and the share 8 e, the sum's chain
+    6 sqrt(n) e.  With bits = 16 the query and the weights are cut to 16 bits, as two parts of
+    8 would hold them."""
+    rng = np.random.default_rng(seed)
+    n = 12
+    q = np.zeros((6, D), np.float32)
+    dims = rng.permutation(D)[:4]
+    q[:, dims] = rng.uniform(2, 4, (6, 4)).astype(np.float32) * math.sqrt(D)
+    q[3:] *= 0.02
+    k = torch.zeros(n, D)
+    level = torch.linspace(-1.5, 1.5, n)[torch.from_numpy(rng.permutation(n))]
+    k[:, dims] = level[:, None] * torch.from_numpy(rng.uniform(0.9, 1.1, (n, 4)).astype(np.float32))
+    v = torch.zeros(n, D)
+    v[torch.arange(n), torch.arange(n)] = 1.0
+    v[:, D - 1] = 1.0
+    k, v = k.to(DTYPE[type]), v.to(DTYPE[type])
+
+    def cut(x):
+        return (x.astype(np.float32).view(np.uint32) & np.uint32(2 ** 32 - 2 ** (24 - bits))).view(np.float32)
+    qs = cut(q) if bits < 24 else q
+    s = qs.astype(np.float64) @ value(k).T / math.sqrt(D)
+    e = np.exp(s - s.max(1, keepdims=True))
+    w = (cut(e).astype(np.float64) if bits < 24 else e) / e.sum(1, keepdims=True)
+    size = np.abs(s) + np.abs(s).max(1, keepdims=True)
+    tol = (16 * size + 8 + 6 * math.sqrt(n)) * 2.0 ** -24
+    one = (8 + 6 * math.sqrt(n)) * 2.0 ** -24  # the column of ones: scores do not count
+    return q, k, v, w, tol, one
+
+
+SHARP = [(type, D) for type in DTYPE for D in (64, 80, 128, 250, 256)]
+
+
+@pytest.mark.parametrize("type,D", SHARP)
+def test_16_bits_are_too_few_for_the_next_test(type, D):
+    for seed in range(4):
+        _, _, _, w, tol, one = sharp(type, D, seed)
+        _, _, _, w16, _, _ = sharp(type, D, seed, bits=16)
+        assert (np.abs(w16 - w) > 2 * tol * w)[:3].any()
+        assert (np.abs(w16.sum(1) - 1) > 2 * one)[3:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type,D", SHARP)
+def test_attend_keeps_24_bits(om, ctx, type, D):
+    for seed in range(4):
+        q, k, v, w, tol, one = sharp(type, D, seed)
+        n = k.shape[0]
+        c = Cache(om, ctx, type, 1, 16, 1, D)
+        c.k[0, 0, :n], c.v[0, 0, :n] = k, v
+        c.write()
+        score = np.zeros((1, 1, 16), np.float32)
+        out, sc = attend(om, ctx, c, q[None], [n], i32([[0]]), score=score)
+        assert (np.abs(out[0, :, :n] - w) <= tol * w).all()
+        assert (np.abs(out[0, :, D - 1] - 1) <= one).all()
+        assert (np.abs(sc[0, 0, :n] - w.sum(0)) <= (tol * w).sum(0) + 4 * 2.0 ** -24 * w.sum(0)).all()
+        c.free()
