@@ -365,3 +365,59 @@ def test_attend_keeps_24_bits(om, ctx, type, D):
         assert (np.abs(out[0, :, D - 1] - 1) <= one).all()
         assert (np.abs(sc[0, 0, :n] - w.sum(0)) <= (tol * w).sum(0) + 4 * 2.0 ** -24 * w.sum(0)).all()
         c.free()
+
+
+# ------------------------------------------------------------ a workspace that grows
+def test_a_growing_workspace_waits_before_it_frees(tmp_path):
+    exe = tmp_path / "kv_growth"
+    r = subprocess.run(["gcc", "-std=gnu99", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-no-pie",
+                        "-Wl,--unresolved-symbols=ignore-all", "-o", str(exe), os.path.join(HERE, "kv_growth.c"),
+                        "-lm"], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-3000:]
+    out = subprocess.run([str(exe), "100", "50", "100", "1000", "999", "1", "100000"], capture_output=True,
+                         text=True, timeout=60, check=True).stdout.split("\n")
+    assert out[0] in ("m", "wm") and out[1:7] == ["", "", "wfm", "", "", "wfm"]
+
+
+@pytest.mark.gpu
+def test_calls_in_a_row_on_a_growing_workspace(om):
+    """Asynchronous calls of a fresh context, each asking for more room than the ones before or
+    for less, with an eviction between: each gives what it gives alone."""
+    rng = np.random.default_rng(19)
+    one, two = om.Context(), om.Context()
+    c = Cache(om, one, "bf16", 600, 16, 2, 128, seed=10)
+    jobs, want = [], []
+    for B, n, score in ((1, 40, False), (2, 900, True), (1, 4000, False), (3, 30, True), (2, 4000, True),
+                        (1, 300, True), (9, 600, False), (4, 2000, True), (1, 5, False)):
+        lens = [n] + [int(x) for x in rng.integers(0, n + 1, B - 1)]
+        table = i32(rng.integers(0, 300, (B, 250)))  # of the first half: pages that only the attention reads
+        q = rng.standard_normal((B, 8, 128)).astype(np.float32)
+        s = rng.uniform(0, 1, (B, 2, n)).astype(np.float32) if score else None
+        want.append(attend(om, two, c, q, lens, table, score=s, max_len=n))
+        b = [one.upload(x) for x in (q, np.zeros_like(q), table, i32(lens))]
+        o = dict(max_len=n, flags=om.KV_ASYNC)
+        if score:
+            b += [one.upload(s), one.upload(np.full_like(s, -9.0))]
+            o.update(score_in=b[4], score_out=b[5], score_stride=n)
+        jobs.append((B, b, om.attend_opts(**o)))
+    # an eviction of many sequences of two tokens each, in the second half's pages
+    N = 300
+    ev = [one.upload(x) for x in (i32(300 + np.arange(N))[:, None], i32([2] * N),
+                                  rng.uniform(0, 1, (N, 2, 16)).astype(np.float32), np.zeros((N, 2, 1), np.int32))]
+    score = one.download(ev[2], np.float32, (N, 2, 16))
+    for i, (B, b, o) in enumerate(jobs):
+        om.kv_attend(one, c.pages, b[1], b[0], B, 8, b[2], 250, b[3], o)
+        if i == 4:
+            om.kv_evict(one, c.pages, N, ev[0], 1, ev[1], ev[2], 16, ev[0], 1, ev[1], None, 0, ev[3],
+                        om.evict_opts(1, flags=om.KV_ASYNC))
+    assert om.lib().gpu_kv_check(one.ptr) == 0
+    for (B, b, _), w in zip(jobs, want):
+        out, sc = w if isinstance(w, tuple) else (w, None)
+        assert np.array_equal(one.download(b[1], np.float32, out.shape), out)
+        if sc is not None:
+            assert np.array_equal(one.download(b[5], np.float32, sc.shape), sc)
+    assert np.array_equal(one.download(ev[3], np.int32, (N, 2, 1))[..., 0], score[:, :, :2].argmax(2))
+    assert (one.download(ev[1], np.int32, (N,)) == 1).sum() == N
+    c.free()
+    for x in (one, two):
+        x.close()
