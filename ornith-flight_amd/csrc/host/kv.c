@@ -84,12 +84,17 @@ static int leave(gpu_context *ctx, int rc, unsigned flags, int prev, const char 
     return rc;
 }
 
-int gpu_kv_check(gpu_context *ctx)
+/* A call with nothing of its own to do. */
+static int idle(gpu_context *ctx, unsigned flags, const char *who)
 {
-    if (!ctx) return ORN_EINVAL;
     int prev;
     const int rc = enter(ctx, &prev);
-    return rc ? rc : leave(ctx, ORN_OK, 0, prev, "gpu_kv_check");
+    return rc ? rc : leave(ctx, ORN_OK, flags, prev, who);
+}
+
+int gpu_kv_check(gpu_context *ctx)
+{
+    return ctx ? idle(ctx, 0, "gpu_kv_check") : ORN_EINVAL;
 }
 
 static int elem_bytes(int type)
@@ -211,7 +216,7 @@ int gpu_rope_axes(gpu_context *ctx, gpu_buffer *q_out, gpu_buffer *k_out, const 
     if ((Q && (q_out == K || q_out == k_out)) || (K && k_out == Q) || q_out == positions ||
         k_out == positions)
         return orn_set_err(ctx, ORN_EINVAL, "%s: an output aliases another argument", who);
-    if (!n_tokens || !(n_heads + n_kv_heads)) return ORN_OK;
+    if (!n_tokens || !(n_heads + n_kv_heads)) return idle(ctx, flags, who);
     a.q = Q ? (const float *)Q->dev : NULL;
     a.q_out = Q ? (float *)q_out->dev : NULL;
     a.k = K ? (const float *)K->dev : NULL;
@@ -254,7 +259,7 @@ int gpu_kv_append(gpu_context *ctx, const ornith_kv_pages *kv, const gpu_buffer 
             return orn_set_err(ctx, ORN_EINVAL, "%s: an output aliases another argument", who);
     if (q_out && (q_out == kv->K || q_out == kv->V))
         return orn_set_err(ctx, ORN_EINVAL, "%s: q_out is the cache", who);
-    if (!n_tokens) return ORN_OK;
+    if (!n_tokens) return idle(ctx, flags, who);
     a.q = Q ? (const float *)Q->dev : NULL;
     a.q_out = Q ? (float *)q_out->dev : NULL;
     a.k = (const float *)K->dev;
@@ -327,7 +332,7 @@ int gpu_kv_attend(gpu_context *ctx, const ornith_kv_pages *kv, gpu_buffer *out,
         if (in[i] && (in[i] == out || (in[i] == o->score_out && i < 5)))
             return orn_set_err(ctx, ORN_EINVAL, "%s: an output aliases another argument", who);
     if (out == o->score_out) return orn_set_err(ctx, ORN_EINVAL, "%s: out is score_out", who);
-    if (!n_seqs) return ORN_OK;
+    if (!n_seqs) return idle(ctx, o->flags, who);
     ornk_attend_args a;
     memset(&a, 0, sizeof a);
     a.q = (const float *)Q->dev;
@@ -394,7 +399,7 @@ int gpu_kv_evict(gpu_context *ctx, const ornith_kv_pages *kv, int n_seqs, const 
             if (all[i] && all[i] == all[j] && !(i == 2 && j == 5) && !(i == 3 && j == 6) &&
                 !(i == 4 && j == 7))
                 return orn_set_err(ctx, ORN_EINVAL, "%s: two arguments are one buffer", who);
-    if (!n_seqs) return ORN_OK;
+    if (!n_seqs) return idle(ctx, opts->flags, who);
     ornk_evict_args a;
     memset(&a, 0, sizeof a);
     a.table = (const int *)table->dev;

@@ -2,6 +2,7 @@
 of 32 bits, scales of the 8-bit type, sizes of a launch, bits of a product, a
 workspace that grows.  Definitions and tolerances are those of test_kv_ops.py.
 """
+import ctypes as C
 import math
 import os
 import subprocess
@@ -139,6 +140,28 @@ def test_host_takes_scales_with_a_reciprocal(host, what, which):
         assert c() == (-1, 0), scale
     c.pages.type = host.om.KV_TYPES["f16"]  # has no scales
     assert c() == (0, 1)
+
+
+
+# ------------------------------------------------------------ calls with nothing to do
+@pytest.mark.parametrize("what", ["rope", "append", "attend", "evict"])
+def test_host_an_empty_call_waits_and_reports(host, what):
+    """A synchronous call ends what was queued before it and reports what it met, also where it has
+    no tokens or sequences itself; an asynchronous one does neither."""
+    def empty(flags):
+        c = Call(host, what)
+        c.args["T" if "T" in c.args else "B"] = 0
+        if "flags" in c.args:
+            c.args["flags"] = flags
+        else:
+            c.opts.flags = flags
+        return c()
+    syncs = C.c_int.in_dll(host.L, "kv_syncs")
+    host.L.kv_test_mark(host.ctx, 0, 2)
+    n = syncs.value
+    assert empty(host.om.KV_ASYNC) == (0, 0) and syncs.value == n
+    assert empty(0) == (-1, 0) and syncs.value == n + 1 and "row 2" in host.error()
+    assert empty(0) == (0, 0)
 
 
 E4M3 = np.arange(256, dtype=np.uint8)
