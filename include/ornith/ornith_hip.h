@@ -110,9 +110,9 @@ typedef struct {
 
 /* q_out = Q [n_tokens][n_heads][head_dim] and k_out = K [n_tokens]
  * [n_kv_heads][head_dim] rotated (head_dim up to 4096); positions
- * [n_axes][n_tokens].  Angles are formed in 64 bits, so that far positions keep
- * their digits.  q_out may be Q and k_out may be K; a pair of NULLs with 0 heads
- * leaves one side out. */
+ * [n_axes][n_tokens].  Angles are formed and reduced in 64 bits, so that far
+ * positions keep their digits; the sine and cosine of the rest are of 32.  q_out
+ * may be Q and k_out may be K; a pair of NULLs with 0 heads leaves one side out. */
 int gpu_rope_axes(gpu_context *ctx, gpu_buffer *q_out, gpu_buffer *k_out, const gpu_buffer *Q,
                   const gpu_buffer *K, int n_tokens, int n_heads, int n_kv_heads, int head_dim,
                   const gpu_buffer *positions, const ornith_rope_axes *rope, unsigned flags);
@@ -146,7 +146,8 @@ int gpu_kv_append(gpu_context *ctx, const ornith_kv_pages *kv, const gpu_buffer 
  * whatever it holds. */
 typedef struct {
     float scale;  /* 0: 1 / sqrt(head_dim) */
-    int max_len;  /* no length is larger; 0: the table's width.  Sizes the workspace and
+    int max_len;  /* no length is larger; 0: the table's width.  Sizes the workspace (with
+                   * score_out about 4.5 * n_seqs * n_heads * max_len bytes) and
                    * the launches: a near bound is faster than a far one. */
     unsigned flags;
     const gpu_buffer *score_in;
@@ -169,8 +170,9 @@ int gpu_kv_attend(gpu_context *ctx, const ornith_kv_pages *kv, gpu_buffer *out,
  *
  * dst_table == table (then dst_pages == max_pages) moves them within their own
  * pages, each of which is then one sequence's, once; else no page of dst_table is
- * read as one of table, and none is listed twice.  dst_lens may be lens, dst_score may be score (with
- * dst_stride == score_stride). */
+ * read as one of table, and none is listed twice (faster: rows that may lie in each
+ * other's way are moved one stretch after the other).  dst_lens may be lens, dst_score
+ * may be score (with dst_stride == score_stride). */
 typedef struct {
     int keep;         /* >= 1, >= sink + recent; at most 2^27, or max_len is */
     int sink, recent; /* >= 0 */

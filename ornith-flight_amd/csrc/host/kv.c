@@ -158,7 +158,8 @@ static int err_words(gpu_context *ctx, int **err)
 
 /* The rotation checked; every pair's axis, and its revolutions per position:
  * base^(-p/R) / 2 pi, in 64 bits.  Each frequency is the one before it times
- * base^(-1/R), so pair p's is within p roundings of 2^-53. */
+ * base^(-1/R), so pair p's is off by p roundings of 2^-53 and p times the rounding of
+ * base^(-1/R) itself, about 2 p in all. */
 static int rope_ok(gpu_context *ctx, const ornith_rope_axes *r, int hd, ornk_rope_args *a,
                    const char *who)
 {

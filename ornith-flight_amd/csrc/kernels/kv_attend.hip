@@ -12,10 +12,11 @@
 //   M = max m_i, L = sum l_i 2^(m_i - M), out = sum O_i 2^(m_i - M) / L.
 // (Exponents are base 2: log2 e is in the query's scale.)  The parts' places and
 // the order of their sums depend on the lengths alone: equal calls give equal bits.
+// Stretches whose sums are not finite are done once more (Shares).
 //
 // Bound by the reading of K and V where the cache is large: 64 sequences of up to
-// 8192 tokens, 32 heads over 8 of 128, 1.1 GB of bf16 in 202 us (5.5 TB/s; a
-// streaming read 6.3, a copy 4.7), of f16 in 220; one of 131,071, 16 heads over 2 of
+// 8192 tokens, 32 heads over 8 of 128, 1.04 GB of bf16 in 192 us (5.4 TB/s; a
+// streaming read 6.3, a copy 4.7), of f16 in 205; one of 131,071, 16 heads over 2 of
 // 256 in bf16, 268 MB in 52 us and 6 more for the joining; 32 of up to 16,384, 64
 // heads over 4 of 128 in e4m3, 280 MB in 61 + 6 us (of a CU's cycles vector
 // instructions take half there, mostly unpacking, and MFMA a fifth; in f16 44% and
@@ -38,7 +39,9 @@ constexpr int MAX_SEGMENTS = (1 << (LINE_LOG2 - 8)) + 32;  // of one of 2^8 grou
 // wave's per SIMD at 256 columns (two groups with tiles of 16 keys: 131,071
 // tokens of bf16 64 us instead of 52), and two waves' at 128 (four spill: 209 ->
 // 393 us); the fp32 path of 64 columns leaves room for four (5 x 2047 tokens of
-// 12 kv heads 20.0 -> 18.2 us), the others of 64 do not (126 -> 144 us).
+// 12 kv heads 20.0 -> 18.2 us), the others of 64 do not (126 -> 144 us).  What spills
+// is fp32 of fewer than 64 columns, 6 registers of the 128, and 56 where its rows are
+// not whole 16-byte words.
 constexpr int groups_log2(int type, int HD)
 {
     return HD == 256 ? 0 : HD == 64 && type == ORN_KV_F32 ? 2 : 1;
@@ -259,7 +262,9 @@ struct Exact {
 // infinity or a NaN, which Parts' operands cannot be; and weights relative to a
 // maximum that still grows, up to 2^6 each, whose sums with values near the largest
 // number pass it though the mean does not.  So the maximum and the sum are found
-// first (the scores are formed twice), and O is the sum of shares of it.
+// first (the scores are formed twice), and O is the sum of shares of it.  An infinite
+// value takes the call of 131,071 tokens from 51 to 237 us, and in every sequence the
+// batch of 64 from 244 to 800.
 template <int TYPE, int HD, bool VEC, bool FULL>
 struct Shares : Exact<TYPE, HD, VEC, FULL> {
     static constexpr bool shares = true, ahead = false;

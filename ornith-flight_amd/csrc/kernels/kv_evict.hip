@@ -26,7 +26,7 @@ __device__ __forceinline__ uint32_t order_key(float f)
 //
 // Up to 4096 tokens bound by latency: lengths, scores, then a dozen barriers, 7 us
 // for one sequence or 64; beyond by the instructions of one CU, about 30 per score
-// and round (one sequence, with the move of few tokens: 4096 11 us, 8192 14, 16,384
+// and round (one sequence, with the move of few tokens into other pages: 4096 11 us, 8192 14, 16,384
 // 20, 32,768 33, 131,072 97).  PER 4 up to 4096 tokens (8: 12 us) and 8 beyond (4:
 // 8192 15 us; 16 and 32 hold longer sequences, for 19.5 and 31.5 us at 16,384 and
 // 32,768, but take 16 and 21 us at 8192, as what is unrolled is run).
@@ -166,8 +166,11 @@ __global__ void __launch_bounds__(CT) k_evict_choose(ornk_kv_pages p, ornk_evict
 // Bound by memory: 32 sequences' up to 4096 rows of 8 kv heads of 128 in f16, 0.94
 // GB read and written, take 198 us (4.75 TB/s; a copy 4.72); 2048 rows of 2 heads
 // of 256 in bf16, 8.4 MB, 4.4 us, most of them the start and the chain of kept,
-// table and row.  The words are a vector type of the compiler: a struct of four
-// was put into LDS with a wait after each load (17 us).
+// table and row.  IN_PLACE it is bound by that chain, one stretch after the other in
+// few groups: with the choice, the 32 sequences take 275 us (into other pages 218),
+// 2048 rows of 2 heads of 256 24 (12), 16,384 rows 168 (43), 65,536 rows 640 (159).
+// The words are a vector type of the compiler: a struct of four was put into LDS with
+// a wait after each load (17 us).
 constexpr int MT = 256, MB = 4, SLICE = 64;
 constexpr int MAX_GROUPS = 1 << 20;  // of a launch's x: 2^28 threads
 
