@@ -128,6 +128,30 @@ int gpu_kv_append(gpu_context *ctx, const ornith_kv_pages *kv, const gpu_buffer 
                   const gpu_buffer *Q, int n_heads, const gpu_buffer *positions,
                   const ornith_rope_axes *rope, unsigned flags);
 
+/* Norms of the heads, taken before the rotation: a row x of head_dim becomes
+ * w x / sqrt(mean(x^2) + eps) (ORN_NORM_RMS) or w x / sqrt(sum(x^2) + eps)
+ * (ORN_NORM_L2), with 32-bit sums.  Weights are [head_dim] for all heads, or
+ * [heads][head_dim] with per_head; NULL: 1. */
+enum { ORN_NORM_RMS = 0, ORN_NORM_L2 = 1 };
+typedef struct {
+    int kind;  /* ORN_NORM_* */
+    float eps; /* >= 0 */
+    const gpu_buffer *q_weight, *k_weight;
+    int per_head;
+} ornith_head_norm;
+
+/* gpu_rope_axes and gpu_kv_append with the norms of Q and K in the same pass; V is
+ * stored as it is.  rope and positions may be NULL: no rotation (Q may be given). */
+int gpu_norm_rope_axes(gpu_context *ctx, gpu_buffer *q_out, gpu_buffer *k_out, const gpu_buffer *Q,
+                       const gpu_buffer *K, int n_tokens, int n_heads, int n_kv_heads, int head_dim,
+                       const ornith_head_norm *norm, const gpu_buffer *positions,
+                       const ornith_rope_axes *rope, unsigned flags);
+int gpu_norm_kv_append(gpu_context *ctx, const ornith_kv_pages *kv, const gpu_buffer *K,
+                       const gpu_buffer *V, int n_tokens, const gpu_buffer *slots,
+                       gpu_buffer *q_out, const gpu_buffer *Q, int n_heads,
+                       const ornith_head_norm *norm, const gpu_buffer *positions,
+                       const ornith_rope_axes *rope, unsigned flags);
+
 /* out [n_seqs][n_heads][head_dim]: the attention of one query per sequence, Q
  * [n_seqs][n_heads][head_dim], over the first lens[b] tokens of its row of the
  * table, w = softmax(scale * q.k); n_heads is a multiple of n_kv_heads, head j
@@ -185,9 +209,82 @@ int gpu_kv_evict(gpu_context *ctx, const ornith_kv_pages *kv, int n_seqs, const 
                  gpu_buffer *dst_score, int dst_stride, gpu_buffer *kept,
                  const ornith_evict_opts *opts);
 
+/* Linear attention with a decay for each head, the other kind of layer of a hybrid
+ * stack: gpu_deltanet_step_gated for many heads, sequences and tokens.  With the
+ * state S [key_dim][value_dim] of a sequence's head,
+ *   S_t = a_t S_(t-1) + b_t k_t v_t^T,   out_t = scale * q_t S_t,   a_t = exp(decay),
+ * b_t = 1, or 1 - a_t with `complement` (the gated step's).  A decay is a logarithm,
+ * so that factors near 1 keep their digits: 0 keeps the state, -infinity clears it.
+ *
+ * Q [n_tokens][q_heads][key_dim], K [n_tokens][k_heads][key_dim], V
+ * [n_tokens][v_heads][value_dim], out [n_tokens][n_heads][value_dim]: the head
+ * counts divide n_heads, head h reads head h / (n_heads / q_heads) of Q, and so on.
+ * decay [n_heads], or [n_tokens][n_heads] with `per_token`.
+ *
+ * Sequence b has the tokens starts[b] to starts[b + 1] - 1 (none: it leaves the state
+ * it came with); rows of out that are no sequence's stay as they are.  starts NULL:
+ * one token for each of n_seqs = n_tokens sequences.  It goes on from the state in
+ * slot slots_in[b] and leaves its own in slots_out[b]; -1, or a NULL buffer: from
+ * zeros, and nowhere.  Both may be one buffer.  No slot is written twice in a call,
+ * and none that another sequence starts from is written; sequences may start from
+ * one slot.
+ *
+ * Sums and states are of 32 bits; a prompt's tokens are taken together in chunks,
+ * whose decays are summed in 64.  What a token holds has no effect on those before
+ * it, NaN and infinities included.  A slot outside [-1, n_slots), or tokens outside
+ * [0, n_tokens) or more than max_len, leave their sequence out (gpu_kv_check). */
+typedef struct {
+    gpu_buffer *S; /* [n_slots][n_heads][key_dim][value_dim] fp32; NULL without slots */
+    int n_slots;
+    int n_heads;            /* 1 to 65535 */
+    int key_dim, value_dim; /* 1 to 256 */
+} ornith_linear_states;
+typedef struct {
+    float scale;    /* 0: 1 / sqrt(key_dim) */
+    int per_token;
+    int complement;
+    int max_len;    /* no sequence is longer; 0: n_tokens.  Sizes the launches and the
+                     * workspace: a near bound is faster than a far one. */
+    unsigned flags; /* ORN_KV_ASYNC */
+} ornith_linear_opts;
+int gpu_linear_attend(gpu_context *ctx, const ornith_linear_states *st, gpu_buffer *out,
+                      const gpu_buffer *Q, const gpu_buffer *K, const gpu_buffer *V, int q_heads,
+                      int k_heads, int v_heads, int n_tokens, const gpu_buffer *decay, int n_seqs,
+                      const gpu_buffer *starts, const gpu_buffer *slots_in,
+                      const gpu_buffer *slots_out, const ornith_linear_opts *opts);
+
 /* Waits for the context's stream; ORN_EINVAL (once) if a call of this group met
  * a number out of range since the last report. */
 int gpu_kv_check(gpu_context *ctx);
+
+/* The step's end: a token for each row of logits, tokens [n_rows] int32, from the
+ * random number u [n_rows] in [0, 1) (fp32) and the row's request.  Row r's logits are
+ * the n_vocab floats at r * row_stride (0: n_vocab).
+ *
+ * With p = softmax(logits / temperature), the tokens in descending order (ties: the
+ * lowest first) and S the sum over the top_k first, those are kept that are among the
+ * top_k first, before which the sum is less than top_p * S, and whose p is at least
+ * min_p times the largest; the first always.  The token is the first, in that order,
+ * up to which the kept tokens' sum is more than u times their whole.  Temperature 0
+ * takes the first.  Every p is rounded to a multiple of 2^-42 or less of the largest,
+ * sums of these are exact, and so results do not vary from run to run.  A NaN counts as -infinity, which is never taken: a
+ * row of nothing else gives token -1.  prob [n_rows] (may be NULL): the token's share
+ * of the kept sum.
+ *
+ * A request outside its bounds or a u outside [0, 1) gives token -1, prob 0 and
+ * ORN_EINVAL (after ORN_KV_ASYNC by gpu_kv_check). */
+typedef struct {
+    float temperature; /* finite, >= 0 */
+    int top_k;         /* <= 0: all */
+    float top_p;       /* 0 to 1; 1: all */
+    float min_p;       /* 0 to 1; 0: all */
+} ornith_sample_request;
+#define ORN_SAMPLE_MAX_VOCAB (1 << 20)
+/* requests: [n_rows] ornith_sample_request.  n_rows up to 65535, n_vocab up to
+ * ORN_SAMPLE_MAX_VOCAB.  flags: ORN_KV_ASYNC. */
+int gpu_sample(gpu_context *ctx, gpu_buffer *tokens, gpu_buffer *prob, const gpu_buffer *logits,
+               int n_rows, int n_vocab, int row_stride, const gpu_buffer *requests,
+               const gpu_buffer *u, unsigned flags);
 
 /* Device address of a buffer (for interop and tests). */
 void *gpu_device_ptr(gpu_context *ctx, gpu_buffer *buf);

@@ -7,23 +7,11 @@
  * kernels: a word of pinned host memory per kind of mistake, which stays
  * untouched by correct calls and is looked at after the stream has ended.
  */
-#include "internal.h"
+#include "call.h"
 
 #include <math.h>
 #include <stdio.h>
 #include <string.h>
-
-/* a * b * c * d * elem bytes, SIZE_MAX where that passes 64 bits */
-static size_t span(size_t a, size_t b, size_t c, size_t d, size_t elem)
-{
-    size_t n = a;
-    if (__builtin_mul_overflow(n, b, &n) || __builtin_mul_overflow(n, c, &n) ||
-        __builtin_mul_overflow(n, d, &n) || __builtin_mul_overflow(n, elem, &n))
-        return SIZE_MAX;
-    return n;
-}
-
-static int holds(const gpu_buffer *b, size_t bytes) { return b && b->dev && bytes <= b->size; }
 
 void *orn_kv_ws_get(gpu_context *ctx, size_t bytes)
 {
@@ -42,54 +30,6 @@ void *orn_kv_ws_get(gpu_context *ctx, size_t bytes)
     }
     w->bytes = want;
     return w->base;
-}
-
-/* Calls run on the context's device, whichever is current. */
-static int enter(gpu_context *ctx, int *prev)
-{
-    *prev = ctx->device;
-    int rc = orn_hip_check(ctx, hipGetDevice(prev), "hipGetDevice");
-    if (!rc && *prev != ctx->device)
-        rc = orn_hip_check(ctx, hipSetDevice(ctx->device), "hipSetDevice");
-    return rc;
-}
-
-static int report(gpu_context *ctx, const char *who)
-{
-    static const char *const what[ORNK_KV_ERR_WORDS] = {
-        "a page number of row %d is outside the pages", "slot of token %d is outside the pages",
-        "the length of sequence %d is outside its bounds"};
-    int rc = ORN_OK;
-    for (int i = 0; i < ORNK_KV_ERR_WORDS; ++i) {
-        volatile int *w = ctx->ctl_host + ORN_CTL_KV + i;
-        const int at = *w;
-        if (!at) continue;
-        *w = 0;
-        if (rc) continue;
-        char msg[96];
-        snprintf(msg, sizeof msg, what[i], at - 1);
-        rc = orn_set_err(ctx, ORN_EINVAL, "%s: %s (this call or an earlier asynchronous one)", who,
-                         msg);
-    }
-    return rc;
-}
-
-static int leave(gpu_context *ctx, int rc, unsigned flags, int prev, const char *who)
-{
-    if (!rc && !(flags & ORN_KV_ASYNC)) {
-        rc = orn_hip_check(ctx, hipStreamSynchronize(ctx->stream), who);
-        if (!rc) rc = report(ctx, who);
-    }
-    if (prev != ctx->device) (void)hipSetDevice(prev);
-    return rc;
-}
-
-/* A call with nothing of its own to do. */
-static int idle(gpu_context *ctx, unsigned flags, const char *who)
-{
-    int prev;
-    const int rc = enter(ctx, &prev);
-    return rc ? rc : leave(ctx, ORN_OK, flags, prev, who);
 }
 
 int gpu_kv_check(gpu_context *ctx)
@@ -147,15 +87,6 @@ static int pages_ok(gpu_context *ctx, const ornith_kv_pages *kv, ornk_kv_pages *
     return ORN_OK;
 }
 
-static int err_words(gpu_context *ctx, int **err)
-{
-    void *d = NULL;
-    const int rc = orn_hip_check(ctx, hipHostGetDevicePointer(&d, ctx->ctl_host, 0),
-                                 "hipHostGetDevicePointer");
-    *err = (int *)d + ORN_CTL_KV;
-    return rc;
-}
-
 /* The rotation checked; every pair's axis, and its revolutions per position:
  * base^(-p/R) / 2 pi, in 64 bits.  Each frequency is the one before it times
  * base^(-1/R), so pair p's is off by p roundings of 2^-53 and p times the rounding of
@@ -193,13 +124,34 @@ static int rope_ok(gpu_context *ctx, const ornith_rope_axes *r, int hd, ornk_rop
     return ORN_OK;
 }
 
-int gpu_rope_axes(gpu_context *ctx, gpu_buffer *q_out, gpu_buffer *k_out, const gpu_buffer *Q,
-                  const gpu_buffer *K, int n_tokens, int n_heads, int n_kv_heads, int head_dim,
-                  const gpu_buffer *positions, const ornith_rope_axes *rope, unsigned flags)
+/* The heads' norms checked. */
+static int norm_ok(gpu_context *ctx, const ornith_head_norm *n, int heads, int kv, int hd,
+                   ornk_rope_args *a, const char *who)
 {
-    static const char who[] = "gpu_rope_axes";
+    if (n->kind != ORN_NORM_RMS && n->kind != ORN_NORM_L2)
+        return orn_set_err(ctx, ORN_EUNSUPPORTED, "%s: norm %d", who, n->kind);
+    if (!(n->eps >= 0.0f && n->eps < INFINITY))
+        return orn_set_err(ctx, ORN_EINVAL, "%s: eps %g", who, (double)n->eps);
+    const int each = n->per_head != 0;
+    if ((n->q_weight && heads && !holds(n->q_weight, span(each ? heads : 1, hd, 1, 1, 4))) ||
+        (n->k_weight && kv && !holds(n->k_weight, span(each ? kv : 1, hd, 1, 1, 4))))
+        return orn_set_err(ctx, ORN_EINVAL, "%s: weights too small", who);
+    a->norm = 1 + n->kind;
+    a->per_head = each;
+    a->eps = n->eps;
+    a->qw = n->q_weight && heads ? (const float *)n->q_weight->dev : NULL;
+    a->kw = n->k_weight && kv ? (const float *)n->k_weight->dev : NULL;
+    return ORN_OK;
+}
+
+/* gpu_rope_axes, and with a norm gpu_norm_rope_axes, where rope may be NULL. */
+static int rope_axes(gpu_context *ctx, gpu_buffer *q_out, gpu_buffer *k_out, const gpu_buffer *Q,
+                     const gpu_buffer *K, int n_tokens, int n_heads, int n_kv_heads, int head_dim,
+                     const ornith_head_norm *norm, const gpu_buffer *positions,
+                     const ornith_rope_axes *rope, unsigned flags, const char *who)
+{
     if (!ctx) return ORN_EINVAL;
-    if (!positions || !rope || n_tokens < 0 || n_heads < 0 || n_kv_heads < 0 || n_heads > 65535 ||
+    if (!positions != !rope || (!rope && !norm) || n_tokens < 0 || n_heads < 0 || n_kv_heads < 0 || n_heads > 65535 ||
         n_kv_heads > 65535 || head_dim < 1 || !Q != !n_heads || !q_out != !n_heads ||
         !K != !n_kv_heads || !k_out != !n_kv_heads)
         return orn_set_err(ctx, ORN_EINVAL, "%s: bad arguments", who);
@@ -207,22 +159,27 @@ int gpu_rope_axes(gpu_context *ctx, gpu_buffer *q_out, gpu_buffer *k_out, const 
         return orn_set_err(ctx, ORN_EUNSUPPORTED, "%s: head_dim %d > 4096", who, head_dim);
     ornk_rope_args a;
     memset(&a, 0, sizeof a);
-    int rc = rope_ok(ctx, rope, head_dim, &a, who);
-    if (rc) return rc;
+    int rc = ORN_OK;
+    if ((rope && (rc = rope_ok(ctx, rope, head_dim, &a, who))) ||
+        (norm && (rc = norm_ok(ctx, norm, n_heads, n_kv_heads, head_dim, &a, who))))
+        return rc;
     const size_t nq = span(n_tokens, n_heads, head_dim, 1, 4);
     const size_t nk = span(n_tokens, n_kv_heads, head_dim, 1, 4);
-    if (!holds(positions, span(rope->n_axes, n_tokens, 1, 1, 4)) ||
+    if ((rope && !holds(positions, span(rope->n_axes, n_tokens, 1, 1, 4))) ||
         (Q && (!holds(Q, nq) || !holds(q_out, nq))) || (K && (!holds(K, nk) || !holds(k_out, nk))))
         return orn_set_err(ctx, ORN_EINVAL, "%s: buffer too small", who);
-    if ((Q && (q_out == K || q_out == k_out)) || (K && k_out == Q) || q_out == positions ||
-        k_out == positions)
+    const gpu_buffer *in[] = {positions, norm ? norm->q_weight : NULL, norm ? norm->k_weight : NULL};
+    for (int i = 0; i < 3; ++i)
+        if (in[i] && (in[i] == q_out || in[i] == k_out))
+            return orn_set_err(ctx, ORN_EINVAL, "%s: an output aliases another argument", who);
+    if ((Q && (q_out == K || q_out == k_out)) || (K && k_out == Q))
         return orn_set_err(ctx, ORN_EINVAL, "%s: an output aliases another argument", who);
     if (!n_tokens || !(n_heads + n_kv_heads)) return idle(ctx, flags, who);
     a.q = Q ? (const float *)Q->dev : NULL;
     a.q_out = Q ? (float *)q_out->dev : NULL;
     a.k = K ? (const float *)K->dev : NULL;
     a.k_out = K ? (float *)k_out->dev : NULL;
-    a.pos = (const int *)positions->dev;
+    a.pos = rope ? (const int *)positions->dev : NULL;
     a.T = n_tokens;
     a.heads = n_heads;
     a.kv = n_kv_heads;
@@ -233,29 +190,52 @@ int gpu_rope_axes(gpu_context *ctx, gpu_buffer *q_out, gpu_buffer *k_out, const 
     return leave(ctx, rc, flags, prev, who);
 }
 
-int gpu_kv_append(gpu_context *ctx, const ornith_kv_pages *kv, const gpu_buffer *K,
-                  const gpu_buffer *V, int n_tokens, const gpu_buffer *slots, gpu_buffer *q_out,
-                  const gpu_buffer *Q, int n_heads, const gpu_buffer *positions,
-                  const ornith_rope_axes *rope, unsigned flags)
+int gpu_rope_axes(gpu_context *ctx, gpu_buffer *q_out, gpu_buffer *k_out, const gpu_buffer *Q,
+                  const gpu_buffer *K, int n_tokens, int n_heads, int n_kv_heads, int head_dim,
+                  const gpu_buffer *positions, const ornith_rope_axes *rope, unsigned flags)
 {
-    static const char who[] = "gpu_kv_append";
+    return rope_axes(ctx, q_out, k_out, Q, K, n_tokens, n_heads, n_kv_heads, head_dim, NULL,
+                     positions, rope, flags, "gpu_rope_axes");
+}
+
+int gpu_norm_rope_axes(gpu_context *ctx, gpu_buffer *q_out, gpu_buffer *k_out, const gpu_buffer *Q,
+                       const gpu_buffer *K, int n_tokens, int n_heads, int n_kv_heads, int head_dim,
+                       const ornith_head_norm *norm, const gpu_buffer *positions,
+                       const ornith_rope_axes *rope, unsigned flags)
+{
+    static const char who[] = "gpu_norm_rope_axes";
+    if (ctx && !norm) return orn_set_err(ctx, ORN_EINVAL, "%s: no norm", who);
+    return rope_axes(ctx, q_out, k_out, Q, K, n_tokens, n_heads, n_kv_heads, head_dim, norm,
+                     positions, rope, flags, who);
+}
+
+/* gpu_kv_append, and with a norm gpu_norm_kv_append, whose queries need no rotation. */
+static int kv_append(gpu_context *ctx, const ornith_kv_pages *kv, const gpu_buffer *K,
+                     const gpu_buffer *V, int n_tokens, const gpu_buffer *slots, gpu_buffer *q_out,
+                     const gpu_buffer *Q, int n_heads, const ornith_head_norm *norm,
+                     const gpu_buffer *positions, const ornith_rope_axes *rope, unsigned flags,
+                     const char *who)
+{
     if (!ctx) return ORN_EINVAL;
     ornk_kv_pages p;
     int rc = pages_ok(ctx, kv, &p, who);
     if (rc) return rc;
     if (!K || !V || !slots || n_tokens < 0 || n_heads < 0 || n_heads > 65535 || !Q != !n_heads ||
-        !q_out != !n_heads || !rope != !positions || (Q && !rope))
+        !q_out != !n_heads || !rope != !positions || (Q && !rope && !norm))
         return orn_set_err(ctx, ORN_EINVAL, "%s: bad arguments", who);
     ornk_rope_args a;
     memset(&a, 0, sizeof a);
-    if (rope && (rc = rope_ok(ctx, rope, p.hd, &a, who))) return rc;
+    if ((rope && (rc = rope_ok(ctx, rope, p.hd, &a, who))) ||
+        (norm && (rc = norm_ok(ctx, norm, n_heads, p.kv, p.hd, &a, who))))
+        return rc;
     const size_t nq = span(n_tokens, n_heads, p.hd, 1, 4), nk = span(n_tokens, p.kv, p.hd, 1, 4);
     if (!holds(K, nk) || !holds(V, nk) || !holds(slots, span(n_tokens, 1, 1, 1, 4)) ||
         (Q && (!holds(Q, nq) || !holds(q_out, nq))) ||
         (rope && !holds(positions, span(rope->n_axes, n_tokens, 1, 1, 4))))
         return orn_set_err(ctx, ORN_EINVAL, "%s: buffer too small", who);
-    const gpu_buffer *in[] = {K, V, Q, slots, positions};
-    for (int i = 0; i < 5; ++i)
+    const gpu_buffer *in[] = {K, V, Q, slots, positions, norm ? norm->q_weight : NULL,
+                              norm ? norm->k_weight : NULL};
+    for (int i = 0; i < 7; ++i)
         if (in[i] && (in[i] == kv->K || in[i] == kv->V || (in[i] == q_out && i != 2)))
             return orn_set_err(ctx, ORN_EINVAL, "%s: an output aliases another argument", who);
     if (q_out && (q_out == kv->K || q_out == kv->V))
@@ -276,6 +256,27 @@ int gpu_kv_append(gpu_context *ctx, const ornith_kv_pages *kv, const gpu_buffer 
     if (!(rc = err_words(ctx, &p.err)))
         rc = orn_hip_check(ctx, (hipError_t)ornk_rope_append(&p, &a, ctx->stream), who);
     return leave(ctx, rc, flags, prev, who);
+}
+
+int gpu_kv_append(gpu_context *ctx, const ornith_kv_pages *kv, const gpu_buffer *K,
+                  const gpu_buffer *V, int n_tokens, const gpu_buffer *slots, gpu_buffer *q_out,
+                  const gpu_buffer *Q, int n_heads, const gpu_buffer *positions,
+                  const ornith_rope_axes *rope, unsigned flags)
+{
+    return kv_append(ctx, kv, K, V, n_tokens, slots, q_out, Q, n_heads, NULL, positions, rope, flags,
+                     "gpu_kv_append");
+}
+
+int gpu_norm_kv_append(gpu_context *ctx, const ornith_kv_pages *kv, const gpu_buffer *K,
+                       const gpu_buffer *V, int n_tokens, const gpu_buffer *slots,
+                       gpu_buffer *q_out, const gpu_buffer *Q, int n_heads,
+                       const ornith_head_norm *norm, const gpu_buffer *positions,
+                       const ornith_rope_axes *rope, unsigned flags)
+{
+    static const char who[] = "gpu_norm_kv_append";
+    if (ctx && !norm) return orn_set_err(ctx, ORN_EINVAL, "%s: no norm", who);
+    return kv_append(ctx, kv, K, V, n_tokens, slots, q_out, Q, n_heads, norm, positions, rope, flags,
+                     who);
 }
 
 /* The sequences' table and lengths; *bound: the largest length there may be. */

@@ -6,19 +6,6 @@
 
 namespace {
 
-// cos and sin of pair i's angle at token t.  The turn is formed in 64 bits and
-// reduced before it is rounded, so far positions keep their digits.  The reduced turn,
-// its cosine and its sine are fp32: an output is off by 1.3 times what it is with
-// these in 64 bits, too (of 4099 tokens 5.4e-8 of the whole instead of 4.2e-8), which
-// took 7 % longer there (28.4 us) and 5 % with 8190 tokens' append (71.0 us).
-__device__ __forceinline__ float2 rope_cs(const ornk_rope_args &a, int t, int i)
-{
-    const double turn = (double)a.pos[(size_t)a.axis[i] * a.T + t] * a.turns[i];
-    float2 r;
-    sincospif(2.0f * (float)(turn - rint(turn)), &r.y, &r.x);
-    return r;
-}
-
 // Heads whose pairs are not whole float4s: one work group per token and row
 // (query heads, key heads, value heads), an element or a pair per thread.  Bound by the
 // angles, formed again for every head: 4099 tokens of 32 + 8 heads of 66 in halves 68 us,
@@ -71,18 +58,6 @@ __global__ void __launch_bounds__(128) k_rope_append_any(ornk_kv_pages p, ornk_r
             put(i1, u * cs.y + v * cs.x);
         }
     }
-}
-
-// Four elements rounded to the cache's type, in one store.
-template <int TYPE>
-__device__ __forceinline__ void put4(typename KvElem<TYPE>::T *c, v4f x, float scale)
-{
-    typedef typename KvElem<TYPE>::T T;
-    typedef T vec __attribute__((ext_vector_type(4)));
-    vec v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = KvElem<TYPE>::put(x[i], scale);
-    *reinterpret_cast<vec *>(c) = v;
 }
 
 // Work groups (token, share of its items): an item is a float4 of a row, with
@@ -210,6 +185,7 @@ int launch(const ornk_kv_pages &p, const ornk_rope_args &a, hipStream_t s)
 
 extern "C" int ornk_rope_append(const ornk_kv_pages *pp, const ornk_rope_args *a, hipStream_t s)
 {
+    if (a->norm) return ornk_norm_append(pp, a, s);
     ornk_kv_pages p = {};
     if (pp) p = *pp;
     switch (p.type) {

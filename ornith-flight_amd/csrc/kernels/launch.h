@@ -67,7 +67,10 @@ int ornk_kv_append(float *Kc, float *Vc, const float *Kn, const float *Vn, int p
 #define ORNK_KV_ERR_PAGE 0
 #define ORNK_KV_ERR_SLOT 1
 #define ORNK_KV_ERR_LEN 2
-#define ORNK_KV_ERR_WORDS 3
+#define ORNK_KV_ERR_STATE 3
+#define ORNK_KV_ERR_START 4
+#define ORNK_KV_ERR_SAMPLE 5
+#define ORNK_KV_ERR_WORDS 6
 typedef struct {
     void *k, *v;
     int type, n_pages, page, page_log2, kv, hd;
@@ -83,8 +86,14 @@ typedef struct {
     int T, heads, kv, hd, R, halves;
     double turns[256];      /* per pair, revolutions per position */
     uint8_t axis[256];
+    int norm;               /* 0: none, 1: by the mean square, 2: by the sum of squares */
+    int per_head;
+    float eps;
+    const float *qw, *kw;   /* NULL: ones */
 } ornk_rope_args;
 int ornk_rope_append(const ornk_kv_pages *p, const ornk_rope_args *a, hipStream_t s);
+/* The same with a norm (norm.hip); ornk_rope_append calls it where a->norm is set. */
+int ornk_norm_append(const ornk_kv_pages *p, const ornk_rope_args *a, hipStream_t s);
 
 typedef struct {
     const float *q;
@@ -112,6 +121,34 @@ typedef struct {
     int *counts; /* [n_seqs] work buffer */
 } ornk_evict_args;
 int ornk_kv_evict(const ornk_kv_pages *p, const ornk_evict_args *a, hipStream_t s);
+
+/* ---- linear attention with decays (linear.hip) ------------------------------- */
+typedef struct {
+    const float *q, *k, *v, *decay;
+    float *out, *S;
+    const int *starts, *in, *out_slots; /* NULL: one token each; zeros; nowhere */
+    int n_seqs, n_tokens, n_slots, heads, qh, kh, vh, dk, dv, max_len, per_token, complement;
+    float scale;
+    int *err; /* as ornk_kv_pages' */
+    void *ws;
+} ornk_linear_args;
+size_t ornk_linear_ws(const ornk_linear_args *a);
+int ornk_linear(const ornk_linear_args *a, hipStream_t s);
+
+/* ---- sampling (sample.hip) --------------------------------------------------- */
+typedef struct {
+    const float *logits, *u;
+    const void *requests; /* [rows] ornith_sample_request */
+    int *tokens;
+    float *prob; /* may be NULL */
+    int rows, n;
+    size_t stride;
+    double unit; /* 2^bits, n * 2^bits < 2^62 */
+    int *err;
+    void *ws;
+} ornk_sample_args;
+size_t ornk_sample_ws(const ornk_sample_args *a);
+int ornk_sample(const ornk_sample_args *a, hipStream_t s);
 
 /* ---- fixed scratch of the forward that allocates nothing (scratch.hip) ---- */
 /* Size of the per-device scratch array; equals ORN_NOALLOC_SCRATCH_BYTES of

@@ -27,6 +27,9 @@ GPU_BUF_DEFAULT, GPU_BUF_SHARED, GPU_BUF_CONSTANT = 0, 1, 2
 Q4K_BYTES, Q6K_BYTES = 144, 210
 KV_ASYNC = 1
 KV_TYPES = {"f32": 0, "f16": 1, "bf16": 2, "e4m3": 3}
+NORMS = {"rms": 0, "l2": 1}
+SAMPLE_REQUEST = np.dtype([("temperature", np.float32), ("top_k", np.int32), ("top_p", np.float32),
+                           ("min_p", np.float32)])  # ornith_sample_request
 
 # Every symbol the public headers declare (include/ornith/gpu.h, ornith_hip.h).
 EXPORTED = [
@@ -58,6 +61,7 @@ EXPORTED = [
     "gpu_deltanet_step_gated", "gpu_kv_cache_append",
     "gpu_moe_store_prefetch", "gpu_moe_store_pin", "gpu_moe_store_cache_stats",
     "gpu_rope_axes", "gpu_kv_append", "gpu_kv_attend", "gpu_kv_evict", "gpu_kv_check",
+    "gpu_norm_rope_axes", "gpu_norm_kv_append", "gpu_linear_attend", "gpu_sample",
 ]
 
 
@@ -134,6 +138,24 @@ class EvictOpts(C.Structure):
     """ornith_evict_opts."""
     _fields_ = [("keep", C.c_int), ("sink", C.c_int), ("recent", C.c_int), ("max_len", C.c_int),
                 ("flags", C.c_uint)]
+
+
+class HeadNorm(C.Structure):
+    """ornith_head_norm: norms of the query and key heads."""
+    _fields_ = [("kind", C.c_int), ("eps", C.c_float), ("q_weight", C.c_void_p),
+                ("k_weight", C.c_void_p), ("per_head", C.c_int)]
+
+
+class LinearStates(C.Structure):
+    """ornith_linear_states: the states of one layer's linear attention."""
+    _fields_ = [("S", C.c_void_p), ("n_slots", C.c_int), ("n_heads", C.c_int),
+                ("key_dim", C.c_int), ("value_dim", C.c_int)]
+
+
+class LinearOpts(C.Structure):
+    """ornith_linear_opts."""
+    _fields_ = [("scale", C.c_float), ("per_token", C.c_int), ("complement", C.c_int),
+                ("max_len", C.c_int), ("flags", C.c_uint)]
 
 
 _lib = None
@@ -227,6 +249,13 @@ def lib():
         "gpu_kv_evict": (i, [vp, C.POINTER(KVPages), i, vp, i, vp, vp, i, vp, i, vp, vp, i, vp,
                              C.POINTER(EvictOpts)]),
         "gpu_kv_check": (i, [vp]),
+        "gpu_norm_rope_axes": (i, [vp, vp, vp, vp, vp, i, i, i, i, C.POINTER(HeadNorm), vp,
+                                   C.POINTER(RopeAxes), C.c_uint]),
+        "gpu_norm_kv_append": (i, [vp, C.POINTER(KVPages), vp, vp, i, vp, vp, vp, i,
+                                   C.POINTER(HeadNorm), vp, C.POINTER(RopeAxes), C.c_uint]),
+        "gpu_linear_attend": (i, [vp, C.POINTER(LinearStates), vp, vp, vp, vp, i, i, i, i, vp, i, vp,
+                                  vp, vp, C.POINTER(LinearOpts)]),
+        "gpu_sample": (i, [vp, vp, vp, vp, i, i, i, vp, vp, C.c_uint]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -547,6 +576,58 @@ def kv_evict(ctx, pages, n_seqs, table, max_pages, lens, score, score_stride, ds
                                  score.ptr, score_stride, dst_table.ptr, dst_pages, dst_lens.ptr,
                                  _ptr(dst_score), dst_stride, kept.ptr, C.byref(opts)),
               "gpu_kv_evict")
+
+
+# ---------------------------------------------------------------- norms, linear attention, sampling
+def _ref(struct):
+    return C.byref(struct) if struct is not None else None
+
+
+def head_norm(kind="rms", eps=1e-6, q_weight=None, k_weight=None, per_head=False):
+    """kind: "rms" or "l2"; weights [head_dim], or [heads][head_dim] with per_head."""
+    n = HeadNorm(NORMS[kind], eps, _ptr(q_weight), _ptr(k_weight), int(per_head))
+    n.buffers = (q_weight, k_weight)
+    return n
+
+
+def norm_rope_axes(ctx, q_out, k_out, Q, K, T, heads, kv_heads, head_dim, norm, positions=None,
+                   rope=None, flags=0):
+    ctx.check(lib().gpu_norm_rope_axes(ctx.ptr, _ptr(q_out), _ptr(k_out), _ptr(Q), _ptr(K), T, heads,
+                                       kv_heads, head_dim, C.byref(norm), _ptr(positions), _ref(rope),
+                                       flags), "gpu_norm_rope_axes")
+
+
+def norm_kv_append(ctx, pages, K, V, T, slots, q_out, Q, heads, norm, positions=None, rope=None,
+                   flags=0):
+    ctx.check(lib().gpu_norm_kv_append(ctx.ptr, C.byref(pages), K.ptr, V.ptr, T, slots.ptr,
+                                       _ptr(q_out), _ptr(Q), heads, C.byref(norm), _ptr(positions),
+                                       _ref(rope), flags), "gpu_norm_kv_append")
+
+
+def linear_states(S, n_slots, n_heads, key_dim, value_dim):
+    """The states [n_slots][n_heads][key_dim][value_dim] in the buffer S (None without slots)."""
+    s = LinearStates(_ptr(S), n_slots, n_heads, key_dim, value_dim)
+    s.buffers = (S,)
+    return s
+
+
+def linear_opts(scale=0.0, per_token=False, complement=False, max_len=0, flags=0):
+    return LinearOpts(scale, int(per_token), int(complement), max_len, flags)
+
+
+def linear_attend(ctx, states, out, Q, K, V, q_heads, k_heads, v_heads, T, decay, n_seqs, starts=None,
+                  slots_in=None, slots_out=None, opts=None):
+    """starts None: one token of each sequence."""
+    ctx.check(lib().gpu_linear_attend(ctx.ptr, C.byref(states), out.ptr, Q.ptr, K.ptr, V.ptr, q_heads,
+                                      k_heads, v_heads, T, decay.ptr, n_seqs, _ptr(starts),
+                                      _ptr(slots_in), _ptr(slots_out), _ref(opts)),
+              "gpu_linear_attend")
+
+
+def sample(ctx, tokens, prob, logits, rows, vocab, requests, u, stride=0, flags=0):
+    """requests: a buffer of `rows` SAMPLE_REQUESTs."""
+    ctx.check(lib().gpu_sample(ctx.ptr, tokens.ptr, _ptr(prob), logits.ptr, rows, vocab, stride,
+                               requests.ptr, u.ptr, flags), "gpu_sample")
 
 
 def profile(ctx: Context):
