@@ -28,6 +28,8 @@ int gpu_linear_attend(gpu_context *ctx, const ornith_linear_states *st, gpu_buff
     if (q_heads < 1 || k_heads < 1 || v_heads < 1 || H % q_heads || H % k_heads || H % v_heads)
         return orn_set_err(ctx, ORN_EINVAL, "%s: %d, %d and %d heads for %d", who, q_heads, k_heads,
                            v_heads, H);
+    if (n_tokens > 0x7fff0000) /* indexes a chunk past the end fit an int */
+        return orn_set_err(ctx, ORN_EUNSUPPORTED, "%s: %d tokens (at most 2^31 - 2^16)", who, n_tokens);
     if (!isfinite(o->scale)) return orn_set_err(ctx, ORN_EINVAL, "%s: scale", who);
     if (!holds(Q, span(n_tokens, q_heads, dk, 1, 4)) || !holds(K, span(n_tokens, k_heads, dk, 1, 4)) ||
         !holds(V, span(n_tokens, v_heads, dv, 1, 4)) || !holds(out, span(n_tokens, H, dv, 1, 4)) ||
