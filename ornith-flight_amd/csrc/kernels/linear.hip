@@ -97,15 +97,16 @@ __global__ void __launch_bounds__(256) k_linear_steps(ornk_linear_args a)
 //   o_i = scale (2^G_i q_i S + sum_(j <= i) 2^(G_i - G_j) b_j P_ij v_j)
 //   S  <- 2^G_C S + sum_j 2^(G_C - G_j) b_j k_j v_j^T
 // Exponents are differences of tokens in order, so no factor overflows before the
-// formula does.  A group of 4 waves takes a head's 64 CB columns of V, a wave 16 CB of
-// them, in its lanes' order: lane 16 g + c holds column CB c + j of its wave in
-// register j, and the accumulators' rows 4 g + r.  So S's accumulators are the second
-// operand of q S as they are, P's (formed as K Q^T) the first of P V, and V never
-// leaves its registers.  K and Q are in LDS; each wave forms P over its share of the
-// key's dimensions, and the shares meet in LDS.
+// formula does.  A group of 4 waves takes 64 CB columns of a head's V, a wave 16 CB of
+// them: lane 16 g + c has columns CB c + j, and rows 4 g + r of a block of 16 in its
+// registers [r][j].  So S's accumulators are the second operand of q S as they are, P's
+// (formed as K Q^T) the first of P V, and V never leaves its registers.  K and Q are in
+// LDS.  P has three blocks of 16 x 16 (keys and queries of the first half, first and
+// second, of the second), one for each of three waves; the fourth sums the next chunk's
+// decays meanwhile.
 constexpr int C = 32;
 
-struct Decays {
+struct alignas(16) Decays {
     double G[C];
     float q[C];  // 2^G_i scale
     float k[C];  // 2^(G_C - G_j) b_j
@@ -124,11 +125,20 @@ __device__ __forceinline__ float exp2_of(double x)
 
 // Token i's decay of a chunk in base 2: 0 behind its n tokens.  Where 2^x is 0 a
 // smaller x changes nothing but the sums' digits.
-__device__ __forceinline__ double decay2(const ornk_linear_args &a, size_t t, int h, bool on)
+__device__ __forceinline__ double decay2(float decay, bool on)
 {
-    if (!on) return 0.0;
-    const double x = (double)a.decay[a.per_token ? t * a.heads + h : h] * 1.4426950408889634;
-    return x < -16384.0 ? -16384.0 : x;
+    const double x = (double)decay * 1.4426950408889634;
+    return !on ? 0.0 : x < -16384.0 ? -16384.0 : x;
+}
+
+// x of the lane that a DPP step names, 0 where there is none or its row takes none
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp(double x)
+{
+    const uint64_t u = __double_as_longlong(x);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
+    return __longlong_as_double((uint64_t)hi << 32 | lo);
 }
 
 // One wave, lanes i and i + 32 alike: the chunk's sums and factors.
@@ -136,11 +146,11 @@ __device__ __forceinline__ double fill_decays(const ornk_linear_args &a, Decays 
 {
     const int i = threadIdx.x & (C - 1);
     double G = x;
-#pragma unroll
-    for (int o = 1; o < C; o <<= 1) {
-        const double y = __shfl_up(G, o, C);
-        if (i >= o) G += y;
-    }
+    G += dpp<0x111, 0xf>(G);  // row_shr:1
+    G += dpp<0x112, 0xf>(G);
+    G += dpp<0x114, 0xf>(G);
+    G += dpp<0x118, 0xf>(G);
+    G += dpp<0x142, 0xa>(G);  // row_bcast:15, the second row of each half
     const double end = __shfl(G, C - 1, C);
     const float b = !on ? 0.0f : a.complement ? -expm1f((float)(x * 0.6931471805599453)) : 1.0f;
     d.G[i] = G;
@@ -159,27 +169,108 @@ struct Cut {
     float *decays;     // [n_seqs][heads][segs]: what a part leaves of a state
 };
 
-// SUMS: only what a part adds to a state that begins with zeros.
+// N floats at p, 0 from `left` on; VEC: they are whole, or there are none
+template <int N, bool VEC>
+__device__ __forceinline__ void load(float (&x)[N], const float *p, int left)
+{
+    typedef float vec __attribute__((ext_vector_type(N)));
+    if (VEC) {
+        vec y = 0.0f;
+        if (left > 0) y = *reinterpret_cast<const vec *>(p);
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = ((const float *)&y)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = i < left ? p[i] : 0.0f;
+    }
+}
+
+template <int N, bool VEC>
+__device__ __forceinline__ void store(float *p, const float (&x)[N], int left)
+{
+    typedef float vec __attribute__((ext_vector_type(N)));
+    if (VEC) {
+        vec y;
+#pragma unroll
+        for (int i = 0; i < N; ++i) ((float *)&y)[i] = x[i];
+        if (left > 0) *reinterpret_cast<vec *>(p) = y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < left) p[i] = x[i];
+    }
+}
+
+// O += P V within a block of 16 tokens, one key after the other: for values that are
+// not finite, which the matrix cores would carry to tokens before them as 0 times
+// themselves.
+template <int CB>
+__device__ __forceinline__ void add_in_order(v4f (&O)[CB], v4f P, const float (&v)[4][CB])
+{
+    const int g = (threadIdx.x & 63) >> 4, c = threadIdx.x & 15;
+#pragma unroll 1
+    for (int key = 0; key < 16; ++key) {
+        const int kr = key & 3, at = 16 * (key >> 2);
+        const float ps = kr == 0 ? P[0] : kr == 1 ? P[1] : kr == 2 ? P[2] : P[3];
+        float vs[CB];
+#pragma unroll
+        for (int j = 0; j < CB; ++j)
+            vs[j] = __shfl(kr == 0 ? v[0][j] : kr == 1 ? v[1][j] : kr == 2 ? v[2][j] : v[3][j], at + c, 64);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float pr = __shfl(ps, at + 4 * g + r, 64);
+#pragma unroll
+            for (int j = 0; j < CB; ++j)
+                if (4 * g + r >= key) O[j][r] = fmaf(pr, vs[j], O[j][r]);
+        }
+    }
+}
+
+// The sequence of rank `rank` by length, the longest first: groups that start late are
+// then short ones.  Up to 256 sequences; of more the order makes little difference.
+__device__ __forceinline__ int by_length(const ornk_linear_args &a, int rank, int *lens)
+{
+    if (!a.starts || a.n_seqs > 256) return rank;
+    const int i = threadIdx.x;
+    if (i < a.n_seqs) lens[i] = a.starts[i + 1] - a.starts[i];
+    __syncthreads();
+    int before = 0;
+    if (i < a.n_seqs) {
+        const int n = lens[i];
+        for (int j = 0; j < a.n_seqs; ++j) before += lens[j] > n || (lens[j] == n && j < i);
+    }
+    __syncthreads();
+    if (i < a.n_seqs && before == rank) lens[0] = i;
+    __syncthreads();
+    return lens[0];
+}
+
+// SUMS: only what a part adds to a state that begins with zeros.  VEC: rows of K and Q
+// are whole float4s, those of V whole vectors of CB.
 template <int KB, int CB, bool VEC, bool SUMS>
 __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cut cut)
 {
-    constexpr int LD = 16 * KB + 4;          // floats of a row in LDS
-    constexpr int NL = C * 4 * KB / 256 > 0 ? C * 4 * KB / 256 : 1;  // float4s of a chunk per thread
-    __shared__ __align__(16) float Ks[C][LD];
+    constexpr int LD = 16 * KB + 4;    // floats of a row in LDS
+    constexpr int RS = 64 / KB;        // rows that the threads load at a time, a float4 each
+    constexpr int NL = C / RS;
+    constexpr int NK = KB > 8 ? 1 : 2; // K of the next chunk beside this one's where two groups still fit a CU
+    __shared__ __align__(16) float Ks[NK][C][LD];
     __shared__ __align__(16) float Qs[SUMS ? 1 : C][LD];
-    __shared__ __align__(16) v4f part[SUMS ? 1 : 4][3][64];
-    __shared__ Decays dec[2];
+    __shared__ __align__(16) v4f Ps[SUMS ? 1 : 3][64];
+    __shared__ __align__(16) Decays dec[2];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
-    const int b = blockIdx.x, h = blockIdx.y;
     const int blocks = (a.dv + 64 * CB - 1) / (64 * CB);
-    const int sg = blockIdx.z / blocks, col0 = (blockIdx.z - sg * blocks) * 64 * CB + w * 16 * CB + c * CB;
+    const int rest = blockIdx.x / a.heads, h = blockIdx.x - rest * a.heads;
+    const int sg = rest / blocks, block = rest - sg * blocks;
+    const int col0 = block * 64 * CB + w * 16 * CB + c * CB, cols = a.dv - col0;
+    const int b = cut.segs > 1 ? blockIdx.y : by_length(a, blockIdx.y, (int *)&Ks[0][0][0]);
     const Seq seq = seq_of(a, b);
     const int first = sg * cut.len;
     if (seq.n < 0 || (sg && first >= seq.n)) return;
     if (SUMS && first + cut.len >= seq.n) return;  // nothing begins behind it
     const int last = min(seq.n, first + cut.len);
     const int hq = h / (a.heads / a.qh), hk = h / (a.heads / a.kh), hv = h / (a.heads / a.vh);
-    const bool busy = col0 - c * CB < a.dv;  // the wave has columns
+    const bool busy = block * 64 * CB + w * 16 * CB < a.dv;  // the wave has columns
     const size_t size = (size_t)a.dk * a.dv;
     float *const mine = cut.segs > 1 ? cut.states + (((size_t)b * a.heads + h) * cut.segs + sg) * size : nullptr;
 
@@ -190,150 +281,145 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * kb + 4 * g + r;
+            for (int j = 0; j < CB; ++j) S[kb][j] = v4f{0, 0, 0, 0};
+        if (from && cols > 0) {
 #pragma unroll
-                for (int j = 0; j < CB; ++j)
-                    S[kb][j][r] = from && row < a.dk && col0 + j < a.dv ? from[(size_t)row * a.dv + col0 + j] : 0.0f;
-            }
-    }
-
-    v4f kn[NL], qn[SUMS ? 1 : NL];  // the next chunk's rows of K and Q on their way
-    float vn[2][4][CB];
-    double xn = 0.0;
-    bool on_n = false;
-    auto fetch = [&](int t) {  // the chunk from token t of the sequence on
-        const size_t row0 = (size_t)seq.t0 + t;
-        const int n = last - t;
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const int at = tid + 256 * i, row = at / (4 * KB), col = 4 * (at - row * 4 * KB);
-            v4f x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-            if (row < C && row < n) {
-                const float *kp = a.k + ((row0 + row) * a.kh + hk) * a.dk + col;
-                const float *qp = a.q + ((row0 + row) * a.qh + hq) * a.dk + col;
-                if (VEC) {
-                    if (col < a.dk) {
-                        x = *reinterpret_cast<const v4f *>(kp);
-                        if (!SUMS) y = *reinterpret_cast<const v4f *>(qp);
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (col + e < a.dk) {
-                            x[e] = kp[e];
-                            if (!SUMS) y[e] = qp[e];
-                        }
-                }
-            }
-            kn[i] = x;
-            if (!SUMS) qn[i] = y;
-        }
-        if (busy) {
-#pragma unroll
-            for (int tb = 0; tb < 2; ++tb)
+            for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * tb + 4 * g + r;
-                    const float *vp = a.v + ((row0 + row) * a.vh + hv) * a.dv + col0;
+                    const int row = 16 * kb + 4 * g + r;
+                    float x[CB];
+                    load<CB, VEC>(x, from + (size_t)row * a.dv + col0, row < a.dk ? cols : 0);
 #pragma unroll
-                    for (int j = 0; j < CB; ++j) vn[tb][r][j] = row < n && col0 + j < a.dv ? vp[j] : 0.0f;
+                    for (int j = 0; j < CB; ++j) S[kb][j][r] = x[j];
                 }
         }
-        if (w == 3) {
-            const int i = lane & (C - 1);
-            on_n = i < n;
-            xn = decay2(a, row0 + i, h, on_n);
-        }
-    };
-    double left = 0.0;  // wave 3: the part's decays
-    auto stage = [&](int p) {
+    }
+
+    // rows of a chunk: uniform addresses, and each lane's place in them
+    const size_t ks = (size_t)a.kh * a.dk, qs = (size_t)a.qh * a.dk, vs = (size_t)a.vh * a.dv,
+                 os = (size_t)a.heads * a.dv;
+    const int lr = tid / (4 * KB), lc = 4 * (tid - lr * 4 * KB), left_k = a.dk - lc;
+    float kn[NL][4], qn[SUMS ? 1 : NL][4], v[2][4][CB];
+    auto fetch = [&](int t) {  // K and Q of the chunk from token t of the sequence on
+        const int n = last - t;
+        const float *kp = a.k + ((size_t)seq.t0 + t) * ks + hk * a.dk, *qp = a.q + ((size_t)seq.t0 + t) * qs + hq * a.dk;
+        const uint32_t ko = lr * (uint32_t)ks + lc, qo = lr * (uint32_t)qs + lc;
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-            const int at = tid + 256 * i, row = at / (4 * KB), col = 4 * (at - row * 4 * KB);
-            if (row < C) {
-                *reinterpret_cast<v4f *>(&Ks[row][col]) = kn[i];
-                if (!SUMS) *reinterpret_cast<v4f *>(&Qs[row][col]) = qn[i];
-            }
+            const int left = n >= C || lr + i * RS < n ? left_k : 0;
+            load<4, VEC>(kn[i], kp + i * RS * ks + ko, left);
+            if (!SUMS) load<4, VEC>(qn[i], qp + i * RS * qs + qo, left);
         }
+    };
+    auto fetch_v = [&](int t) {
+        const int n = last - t;
+        const float *vp = a.v + ((size_t)seq.t0 + t) * vs + hv * a.dv;
+        const uint32_t vo = 4 * g * (uint32_t)vs + col0;
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                load<CB, VEC>(v[tb][r], vp + (16 * tb + r) * vs + vo,
+                              n >= C || 16 * tb + 4 * g + r < n ? cols : 0);
+    };
+    float xn = 0.0f;     // wave 3: a decay of the chunk that it sums next
+    double left = 0.0;   // and the part's sum
+    auto fetch_decays = [&](int t) {
+        const int i = lane & (C - 1);
+        const size_t tok = (size_t)seq.t0 + t + (i < last - t ? i : 0);
+        xn = a.decay[a.per_token ? tok * a.heads + h : h];
+    };
+    auto fill = [&](int p, int t) {
+        const bool on = (lane & (C - 1)) < last - t;
+        left += fill_decays(a, dec[p], decay2(xn, on), on);
+        if (t + C < last) fetch_decays(t + C);
+    };
+    auto stage_k = [&](int p) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+            *reinterpret_cast<v4f *>(&Ks[p & (NK - 1)][lr + i * RS][lc]) = v4f{kn[i][0], kn[i][1], kn[i][2], kn[i][3]};
+    };
+    auto stage_q = [&] {
+#pragma unroll
+        for (int i = 0; i < (SUMS ? 0 : NL); ++i)
+            *reinterpret_cast<v4f *>(&Qs[lr + i * RS][lc]) = v4f{qn[i][0], qn[i][1], qn[i][2], qn[i][3]};
     };
 
     int p = 0;
     if (first < last) {
         fetch(first);
-        if (w == 3) left += fill_decays(a, dec[0], xn, on_n);
-        stage(0);
+        if (w == 3) fetch_decays(first);
+        fetch_v(first);
+        if (w == 3) fill(0, first);
+        if (cut.segs < 2) __syncthreads();  // by_length's lens are read
+        stage_k(0);
+        stage_q();
     }
     for (int t = first; t < last; t += C, p ^= 1) {
+        const bool more = t + C < last;
+        const float(*const K)[LD] = Ks[p & (NK - 1)];
         __syncthreads();
-        float v[2][4][CB];
-#pragma unroll
-        for (int tb = 0; tb < 2; ++tb)
+        if (more) fetch(t + C);
+        const Decays &d = dec[p];
+        v4f O[2][CB];
+        if (w == 3) {
+            if (more) fill(p ^ 1, t + C);
+        } else if (!SUMS) {
+            const int i = w, query = 16 * (i > 0) + c, key = 16 * (i > 1) + 4 * g;
+            const float *kr = K[16 * (i > 1) + c], *qr = Qs[16 * (i > 0) + c];
+            v4f P0 = {0, 0, 0, 0}, P1 = {0, 0, 0, 0}, f;
+            const double G = d.G[query];
 #pragma unroll
             for (int r = 0; r < 4; ++r)
+                f[r] = query >= key + r ? exp2_of(G - d.G[key + r]) * d.b[key + r] : 0.0f;
 #pragma unroll
-                for (int j = 0; j < CB; ++j) v[tb][r][j] = vn[tb][r][j];
-        if (t + C < last) fetch(t + C);
-        const Decays &d = dec[p];
-        if (!SUMS) {
-            // P over this wave's dimensions: keys jb x queries ib
-            v4f P[3] = {};
+            for (int x = 0; x < KB; x += 2) {
+                const int at = 16 * x + 4 * g;
+                const v4f k0 = *reinterpret_cast<const v4f *>(kr + at), q0 = *reinterpret_cast<const v4f *>(qr + at);
+                const v4f k1 = *reinterpret_cast<const v4f *>(kr + at + 16), q1 = *reinterpret_cast<const v4f *>(qr + at + 16);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    P0 = MFMA4(k0[r], q0[r], P0);
+                    P1 = MFMA4(k1[r], q1[r], P1);
+                }
+            }
+            P0 += P1;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) P0[r] = query >= key + r ? P0[r] * f[r] : 0.0f;
+            Ps[i][lane] = P0;
+        }
+        if (!SUMS && busy) {  // q S
+#pragma unroll
+            for (int ib = 0; ib < 2; ++ib)
+#pragma unroll
+                for (int j = 0; j < CB; ++j) O[ib][j] = v4f{0, 0, 0, 0};
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
-                if ((kb & 3) != w) continue;
                 const int at = 16 * kb + 4 * g;
-                const v4f k0 = *reinterpret_cast<const v4f *>(&Ks[c][at]);
-                const v4f k1 = *reinterpret_cast<const v4f *>(&Ks[16 + c][at]);
                 const v4f q0 = *reinterpret_cast<const v4f *>(&Qs[c][at]);
                 const v4f q1 = *reinterpret_cast<const v4f *>(&Qs[16 + c][at]);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    P[0] = MFMA4(k0[r], q0[r], P[0]);
-                    P[1] = MFMA4(k0[r], q1[r], P[1]);
-                    P[2] = MFMA4(k1[r], q1[r], P[2]);
-                }
-            }
+                for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int i = 0; i < 3; ++i) part[w][i][lane] = P[i];
-            // q S
-            v4f O[2][CB] = {};
-            if (busy) {
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb) {
-                    const int at = 16 * kb + 4 * g;
-                    const v4f q0 = *reinterpret_cast<const v4f *>(&Qs[c][at]);
-                    const v4f q1 = *reinterpret_cast<const v4f *>(&Qs[16 + c][at]);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-#pragma unroll
-                        for (int j = 0; j < CB; ++j) {
-                            O[0][j] = MFMA4(q0[r], S[kb][j][r], O[0][j]);
-                            O[1][j] = MFMA4(q1[r], S[kb][j][r], O[1][j]);
-                        }
-                }
-#pragma unroll
-                for (int ib = 0; ib < 2; ++ib) {
-                    const v4f f = *reinterpret_cast<const v4f *>(&d.q[16 * ib + 4 * g]);
-#pragma unroll
-                    for (int j = 0; j < CB; ++j) O[ib][j] *= f;
-                }
-            }
-            __syncthreads();
-            if (busy) {
-#pragma unroll
-                for (int i = 0; i < 3; ++i) {
-                    const int ib = i > 0, jb = i > 1;
-                    P[i] = (part[0][i][lane] + part[1][i][lane]) + (part[2][i][lane] + part[3][i][lane]);
-                    const double Gi = d.G[16 * ib + c];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int j = 4 * g + r;
-                        const float f = exp2_of(Gi - d.G[16 * jb + j]) * d.b[16 * jb + j];
-                        P[i][r] = ib != jb || c >= j ? P[i][r] * f : 0.0f;
+                    for (int j = 0; j < CB; ++j) {
+                        O[0][j] = MFMA4(q0[r], S[kb][j][r], O[0][j]);
+                        O[1][j] = MFMA4(q1[r], S[kb][j][r], O[1][j]);
                     }
-                }
-                // A value that is not finite would reach tokens before it, as 0 times itself:
-                // those of a diagonal block are added one by one.
+            }
+#pragma unroll
+            for (int ib = 0; ib < 2; ++ib) {
+                const v4f f = *reinterpret_cast<const v4f *>(&d.q[16 * ib + 4 * g]);
+#pragma unroll
+                for (int j = 0; j < CB; ++j) O[ib][j] *= f;
+            }
+        }
+        __syncthreads();
+        stage_q();
+        if (NK > 1) stage_k(p ^ 1);
+        if (busy) {
+            if (!SUMS) {
+                const v4f P0 = Ps[0][lane], P1 = Ps[1][lane], P2 = Ps[2][lane];
                 float z = 0.0f;
 #pragma unroll
                 for (int tb = 0; tb < 2; ++tb)
@@ -341,57 +427,36 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
                     for (int r = 0; r < 4; ++r)
 #pragma unroll
                         for (int j = 0; j < CB; ++j) z = fmaf(v[tb][r][j], 0.0f, z);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int j = 0; j < CB; ++j) O[1][j] = MFMA4(P1[r], v[0][r][j], O[1][j]);
                 if (!__any(z != z)) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
 #pragma unroll
                         for (int j = 0; j < CB; ++j) {
-                            O[0][j] = MFMA4(P[0][r], v[0][r][j], O[0][j]);
-                            O[1][j] = MFMA4(P[1][r], v[0][r][j], O[1][j]);
-                            O[1][j] = MFMA4(P[2][r], v[1][r][j], O[1][j]);
+                            O[0][j] = MFMA4(P0[r], v[0][r][j], O[0][j]);
+                            O[1][j] = MFMA4(P2[r], v[1][r][j], O[1][j]);
                         }
                 } else {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-#pragma unroll
-                        for (int j = 0; j < CB; ++j) O[1][j] = MFMA4(P[1][r], v[0][r][j], O[1][j]);
-                    for (int key = 0; key < 16; ++key) {
-                        const int at = 16 * (key >> 2), kr = key & 3;
-#pragma unroll
-                        for (int ib = 0; ib < 2; ++ib) {
-                            const v4f pk = P[2 * ib];
-                            const float ps = kr == 0 ? pk[0] : kr == 1 ? pk[1] : kr == 2 ? pk[2] : pk[3];
-                            float vs[CB];
-#pragma unroll
-                            for (int j = 0; j < CB; ++j) {
-                                const float x = kr == 0 ? v[ib][0][j] : kr == 1 ? v[ib][1][j]
-                                                : kr == 2 ? v[ib][2][j] : v[ib][3][j];
-                                vs[j] = __shfl(x, at + c, 64);
-                            }
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                const float pr = __shfl(ps, at + 4 * g + r, 64);
-#pragma unroll
-                                for (int j = 0; j < CB; ++j)
-                                    if (4 * g + r >= key) O[ib][j][r] = fmaf(pr, vs[j], O[ib][j][r]);
-                            }
-                        }
-                    }
+                    add_in_order(O[0], P0, v[0]);
+                    add_in_order(O[1], P2, v[1]);
                 }
+                const int n = last - t;
+                float *const op = a.out + ((size_t)seq.t0 + t) * os + h * a.dv;
+                const uint32_t oo = 4 * g * (uint32_t)os + col0;
 #pragma unroll
                 for (int ib = 0; ib < 2; ++ib)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const int row = 16 * ib + 4 * g + r;
-                        if (t + row >= last) continue;
-                        float *op = a.out + (((size_t)seq.t0 + t + row) * a.heads + h) * a.dv + col0;
+                        float x[CB];
 #pragma unroll
-                        for (int j = 0; j < CB; ++j)
-                            if (col0 + j < a.dv) op[j] = O[ib][j][r];
+                        for (int j = 0; j < CB; ++j) x[j] = O[ib][j][r];
+                        store<CB, VEC>(op + (16 * ib + r) * os + oo, x,
+                                       n >= C || 16 * ib + 4 * g + r < n ? cols : 0);
                     }
             }
-        }
-        if (busy) {
             const float all = d.all;
 #pragma unroll
             for (int tb = 0; tb < 2; ++tb) {
@@ -409,36 +474,36 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
                 for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float k = Ks[16 * tb + 4 * g + r][16 * kb + c];
+                        const float k = K[16 * tb + 4 * g + r][16 * kb + c];
 #pragma unroll
                         for (int j = 0; j < CB; ++j) S[kb][j] = MFMA4(k, v[tb][r][j], S[kb][j]);
                     }
             }
+            if (more) fetch_v(t + C);
         }
-        if (t + C < last) {
-            if (w == 3) left += fill_decays(a, dec[p ^ 1], xn, on_n);
+        if (NK == 1) {
             __syncthreads();
-            stage(p ^ 1);
+            stage_k(0);
         }
     }
 
     float *to = nullptr;
     if (SUMS) {
         to = mine;
-        if (tid == 192 && blockIdx.z == sg * blocks)
-            cut.decays[((size_t)b * a.heads + h) * cut.segs + sg] = exp2_of(left);
+        if (tid == 192 && !block) cut.decays[((size_t)b * a.heads + h) * cut.segs + sg] = exp2_of(left);
     } else if (last == seq.n && seq.out >= 0) {
         to = a.S + ((size_t)seq.out * a.heads + h) * size;
     }
-    if (!to || !busy) return;
+    if (!to || cols <= 0) return;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int row = 16 * kb + 4 * g + r;
+            float x[CB];
 #pragma unroll
-            for (int j = 0; j < CB; ++j)
-                if (row < a.dk && col0 + j < a.dv) to[(size_t)row * a.dv + col0 + j] = S[kb][j][r];
+            for (int j = 0; j < CB; ++j) x[j] = S[kb][j][r];
+            store<CB, VEC>(to + (size_t)row * a.dv + col0, x, row < a.dk ? cols : 0);
         }
 }
 
@@ -474,13 +539,14 @@ Cut cut_of(const ornk_linear_args &a, int cb)
     return c;
 }
 
-int columns(const ornk_linear_args &a) { return a.dv > 64 && a.dk <= 128 ? 2 : 1; }
+// Blocks of 16 columns of a wave.  Two need a state of 256 registers beyond 128 rows.
+int blocks_of(const ornk_linear_args &a) { return a.dv > 64 && a.dk <= 128 ? 2 : 1; }
 
 template <int KB, int CB, bool VEC>
 void launch(const ornk_linear_args &a, const Cut &cut, hipStream_t s)
 {
     const int blocks = (a.dv + 64 * CB - 1) / (64 * CB);
-    const dim3 grid(a.n_seqs, a.heads, cut.segs * blocks);
+    const dim3 grid((unsigned)a.heads * cut.segs * blocks, a.n_seqs);
     if (cut.segs > 1) {
         hipLaunchKernelGGL((k_linear_chunks<KB, CB, VEC, true>), grid, dim3(256), 0, s, a, cut);
         hipLaunchKernelGGL(k_linear_join, dim3(a.n_seqs, a.heads, (a.dk * a.dv + 255) / 256), dim3(256), 0, s,
@@ -492,7 +558,7 @@ void launch(const ornk_linear_args &a, const Cut &cut, hipStream_t s)
 template <int KB, int CB>
 void launch(const ornk_linear_args &a, const Cut &cut, hipStream_t s)
 {
-    if (a.dk % 4) launch<KB, CB, false>(a, cut, s);
+    if (a.dk % 4 || a.dv % CB) launch<KB, CB, false>(a, cut, s);
     else launch<KB, CB, true>(a, cut, s);
 }
 
@@ -500,7 +566,7 @@ void launch(const ornk_linear_args &a, const Cut &cut, hipStream_t s)
 
 extern "C" size_t ornk_linear_ws(const ornk_linear_args *a)
 {
-    const Cut c = cut_of(*a, columns(*a));
+    const Cut c = cut_of(*a, blocks_of(*a));
     return c.segs < 2 ? 0 : sizeof(float) * a->n_seqs * a->heads * c.segs * ((size_t)a->dk * a->dv + 1);
 }
 
@@ -510,7 +576,7 @@ extern "C" int ornk_linear(const ornk_linear_args *a, hipStream_t s)
         hipLaunchKernelGGL(k_linear_steps, dim3(a->n_seqs, a->heads, (a->dv + 63) / 64), dim3(256), 0, s, *a);
         return hipGetLastError();
     }
-    const int cb = columns(*a);
+    const int cb = blocks_of(*a);
     Cut c = cut_of(*a, cb);
     c.states = static_cast<float *>(a->ws);
     if (c.segs > 1) c.decays = c.states + (size_t)a->n_seqs * a->heads * c.segs * a->dk * a->dv;
