@@ -120,7 +120,7 @@ __device__ __forceinline__ float exp2_of(double x)
 {
     const float hi = (float)x, lo = (float)(x - (double)hi);
     const float e = __builtin_amdgcn_exp2f(hi);
-    return hi == lo ? e : fmaf(e, lo * 0.693147181f, e);
+    return fmaf(e, lo * 0.693147181f, e);
 }
 
 // Token i's decay of a chunk in base 2: 0 behind its n tokens.  Where 2^x is 0 a
@@ -169,14 +169,13 @@ struct Cut {
     float *decays;     // [n_seqs][heads][segs]: what a part leaves of a state
 };
 
-// N floats at p, 0 from `left` on; VEC: they are whole, or there are none
+// N floats at p; without VEC only those before `left`, and 0 for the others.
 template <int N, bool VEC>
-__device__ __forceinline__ void load(float (&x)[N], const float *p, int left)
+__device__ __forceinline__ void load(float (&x)[N], const float *p, int left = N)
 {
     typedef float vec __attribute__((ext_vector_type(N)));
     if (VEC) {
-        vec y = 0.0f;
-        if (left > 0) y = *reinterpret_cast<const vec *>(p);
+        const vec y = *reinterpret_cast<const vec *>(p);
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = ((const float *)&y)[i];
     } else {
@@ -193,7 +192,7 @@ __device__ __forceinline__ void store(float *p, const float (&x)[N], int left)
         vec y;
 #pragma unroll
         for (int i = 0; i < N; ++i) ((float *)&y)[i] = x[i];
-        if (left > 0) *reinterpret_cast<vec *>(p) = y;
+        *reinterpret_cast<vec *>(p) = y;
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -289,39 +288,66 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
                 for (int r = 0; r < 4; ++r) {
                     const int row = 16 * kb + 4 * g + r;
                     float x[CB];
-                    load<CB, VEC>(x, from + (size_t)row * a.dv + col0, row < a.dk ? cols : 0);
+                    load<CB, VEC>(x, from + (size_t)min(row, a.dk - 1) * a.dv + col0, cols);
 #pragma unroll
-                    for (int j = 0; j < CB; ++j) S[kb][j][r] = x[j];
+                    for (int j = 0; j < CB; ++j) S[kb][j][r] = row < a.dk ? x[j] : 0.0f;
                 }
         }
     }
 
-    // rows of a chunk: uniform addresses, and each lane's place in them
+    // Rows of a chunk: uniform addresses, and each lane's place in them.  Where every load
+    // is whole (VEC), lanes without columns load others' and rows behind the end the last
+    // one, and what they get is dropped.
     const size_t ks = (size_t)a.kh * a.dk, qs = (size_t)a.qh * a.dk, vs = (size_t)a.vh * a.dv,
                  os = (size_t)a.heads * a.dv;
     const int lr = tid / (4 * KB), lc = 4 * (tid - lr * 4 * KB), left_k = a.dk - lc;
+    const float *kp = a.k + ((size_t)seq.t0 + first) * ks + hk * a.dk, *qp = a.q + ((size_t)seq.t0 + first) * qs + hq * a.dk,
+                *vp = a.v + ((size_t)seq.t0 + first) * vs + hv * a.dv;
+    float *op = a.out + ((size_t)seq.t0 + first) * os + h * a.dv;
+    const uint32_t lcv = VEC && left_k <= 0 ? 0 : lc, colv = VEC && cols <= 0 ? 0 : col0;
     float kn[NL][4], qn[SUMS ? 1 : NL][4], v[2][4][CB];
-    auto fetch = [&](int t) {  // K and Q of the chunk from token t of the sequence on
-        const int n = last - t;
-        const float *kp = a.k + ((size_t)seq.t0 + t) * ks + hk * a.dk, *qp = a.q + ((size_t)seq.t0 + t) * qs + hq * a.dk;
-        const uint32_t ko = lr * (uint32_t)ks + lc, qo = lr * (uint32_t)qs + lc;
+    auto fetch = [&](int n) {  // K and Q of the next chunk, of which n tokens are left
+        const uint32_t ko = lr * (uint32_t)ks + lcv, qo = lr * (uint32_t)qs + lcv;
+        if (VEC && n >= C) {
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const int left = n >= C || lr + i * RS < n ? left_k : 0;
-            load<4, VEC>(kn[i], kp + i * RS * ks + ko, left);
-            if (!SUMS) load<4, VEC>(qn[i], qp + i * RS * qs + qo, left);
+            for (int i = 0; i < NL; ++i) {
+                load<4, true>(kn[i], kp + i * RS * ks + ko);
+                if (!SUMS) load<4, true>(qn[i], qp + i * RS * qs + qo);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const int row = min(lr + i * RS, n - 1);
+                load<4, VEC>(kn[i], kp + row * ks + lcv, left_k);
+                if (!SUMS) load<4, VEC>(qn[i], qp + row * qs + lcv, left_k);
+                if (lr + i * RS >= n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) kn[i][e] = 0.0f;
+            }
         }
+        kp += C * ks;
+        qp += C * qs;
     };
-    auto fetch_v = [&](int t) {
-        const int n = last - t;
-        const float *vp = a.v + ((size_t)seq.t0 + t) * vs + hv * a.dv;
-        const uint32_t vo = 4 * g * (uint32_t)vs + col0;
+    auto fetch_v = [&](int n) {
+        const uint32_t vo = 4 * g * (uint32_t)vs + colv;
+        if (VEC && n >= C) {
 #pragma unroll
-        for (int tb = 0; tb < 2; ++tb)
+            for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                load<CB, VEC>(v[tb][r], vp + (16 * tb + r) * vs + vo,
-                              n >= C || 16 * tb + 4 * g + r < n ? cols : 0);
+                for (int r = 0; r < 4; ++r) load<CB, true>(v[tb][r], vp + (16 * tb + r) * vs + vo);
+        } else {
+#pragma unroll
+            for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = 16 * tb + 4 * g + r;
+                    load<CB, VEC>(v[tb][r], vp + min(row, n - 1) * vs + colv, cols);
+                    if (row >= n)
+#pragma unroll
+                        for (int j = 0; j < CB; ++j) v[tb][r][j] = 0.0f;
+                }
+        }
+        vp += C * vs;
     };
     float xn = 0.0f;     // wave 3: a decay of the chunk that it sums next
     double left = 0.0;   // and the part's sum
@@ -336,11 +362,13 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
         if (t + C < last) fetch_decays(t + C);
     };
     auto stage_k = [&](int p) {
+        if (left_k <= 0) return;
 #pragma unroll
         for (int i = 0; i < NL; ++i)
             *reinterpret_cast<v4f *>(&Ks[p & (NK - 1)][lr + i * RS][lc]) = v4f{kn[i][0], kn[i][1], kn[i][2], kn[i][3]};
     };
     auto stage_q = [&] {
+        if (SUMS || left_k <= 0) return;
 #pragma unroll
         for (int i = 0; i < (SUMS ? 0 : NL); ++i)
             *reinterpret_cast<v4f *>(&Qs[lr + i * RS][lc]) = v4f{qn[i][0], qn[i][1], qn[i][2], qn[i][3]};
@@ -348,11 +376,19 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
 
     int p = 0;
     if (first < last) {
-        fetch(first);
+        fetch(last - first);
         if (w == 3) fetch_decays(first);
-        fetch_v(first);
+        fetch_v(last - first);
         if (w == 3) fill(0, first);
         if (cut.segs < 2) __syncthreads();  // by_length's lens are read
+        if (left_k <= 0) {  // columns behind the key's dimensions stay 0
+            const v4f z = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                for (int k = 0; k < NK; ++k) *reinterpret_cast<v4f *>(&Ks[k][lr + i * RS][lc]) = z;
+                if (!SUMS) *reinterpret_cast<v4f *>(&Qs[lr + i * RS][lc]) = z;
+            }
+        }
         stage_k(0);
         stage_q();
     }
@@ -360,7 +396,7 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
         const bool more = t + C < last;
         const float(*const K)[LD] = Ks[p & (NK - 1)];
         __syncthreads();
-        if (more) fetch(t + C);
+        if (more) fetch(last - t - C);
         const Decays &d = dec[p];
         v4f O[2][CB];
         if (w == 3) {
@@ -373,15 +409,23 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 f[r] = query >= key + r ? exp2_of(G - d.G[key + r]) * d.b[key + r] : 0.0f;
+            v4f kq[2][4];
+            auto read = [&](v4f (&y)[4], int x) {
+                y[0] = *reinterpret_cast<const v4f *>(kr + 16 * x + 4 * g);
+                y[1] = *reinterpret_cast<const v4f *>(qr + 16 * x + 4 * g);
+                y[2] = *reinterpret_cast<const v4f *>(kr + 16 * x + 4 * g + 16);
+                y[3] = *reinterpret_cast<const v4f *>(qr + 16 * x + 4 * g + 16);
+            };
+            read(kq[0], 0);
 #pragma unroll
             for (int x = 0; x < KB; x += 2) {
-                const int at = 16 * x + 4 * g;
-                const v4f k0 = *reinterpret_cast<const v4f *>(kr + at), q0 = *reinterpret_cast<const v4f *>(qr + at);
-                const v4f k1 = *reinterpret_cast<const v4f *>(kr + at + 16), q1 = *reinterpret_cast<const v4f *>(qr + at + 16);
+                if (x + 2 < KB) read(kq[x / 2 + 1 & 1], x + 2);
+                __builtin_amdgcn_sched_barrier(0);
+                const v4f(&y)[4] = kq[x / 2 & 1];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    P0 = MFMA4(k0[r], q0[r], P0);
-                    P1 = MFMA4(k1[r], q1[r], P1);
+                    P0 = MFMA4(y[0][r], y[1][r], P0);
+                    P1 = MFMA4(y[2][r], y[3][r], P1);
                 }
             }
             P0 += P1;
@@ -394,17 +438,22 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
             for (int ib = 0; ib < 2; ++ib)
 #pragma unroll
                 for (int j = 0; j < CB; ++j) O[ib][j] = v4f{0, 0, 0, 0};
+            v4f q[2][2];
+            auto read = [&](v4f (&y)[2], int kb) {
+                y[0] = *reinterpret_cast<const v4f *>(&Qs[c][16 * kb + 4 * g]);
+                y[1] = *reinterpret_cast<const v4f *>(&Qs[16 + c][16 * kb + 4 * g]);
+            };
+            read(q[0], 0);
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
-                const int at = 16 * kb + 4 * g;
-                const v4f q0 = *reinterpret_cast<const v4f *>(&Qs[c][at]);
-                const v4f q1 = *reinterpret_cast<const v4f *>(&Qs[16 + c][at]);
+                if (kb + 1 < KB) read(q[kb + 1 & 1], kb + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
 #pragma unroll
                     for (int j = 0; j < CB; ++j) {
-                        O[0][j] = MFMA4(q0[r], S[kb][j][r], O[0][j]);
-                        O[1][j] = MFMA4(q1[r], S[kb][j][r], O[1][j]);
+                        O[0][j] = MFMA4(q[kb & 1][0][r], S[kb][j][r], O[0][j]);
+                        O[1][j] = MFMA4(q[kb & 1][1][r], S[kb][j][r], O[1][j]);
                     }
             }
 #pragma unroll
@@ -444,18 +493,24 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
                     add_in_order(O[1], P2, v[1]);
                 }
                 const int n = last - t;
-                float *const op = a.out + ((size_t)seq.t0 + t) * os + h * a.dv;
                 const uint32_t oo = 4 * g * (uint32_t)os + col0;
+                auto put = [&](int ib, int r) {
+                    float x[CB];
 #pragma unroll
-                for (int ib = 0; ib < 2; ++ib)
+                    for (int j = 0; j < CB; ++j) x[j] = O[ib][j][r];
+                    store<CB, VEC>(op + (16 * ib + r) * os + oo, x, cols);
+                };
+                if (cols > 0) {
+                    if (n >= C) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        float x[CB];
+                        for (int i = 0; i < 8; ++i) put(i >> 2, i & 3);
+                    } else {
 #pragma unroll
-                        for (int j = 0; j < CB; ++j) x[j] = O[ib][j][r];
-                        store<CB, VEC>(op + (16 * ib + r) * os + oo, x,
-                                       n >= C || 16 * ib + 4 * g + r < n ? cols : 0);
+                        for (int i = 0; i < 8; ++i)
+                            if (16 * (i >> 2) + 4 * g + (i & 3) < n) put(i >> 2, i & 3);
                     }
+                }
+                op += C * os;
             }
             const float all = d.all;
 #pragma unroll
@@ -479,7 +534,7 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
                         for (int j = 0; j < CB; ++j) S[kb][j] = MFMA4(k, v[tb][r][j], S[kb][j]);
                     }
             }
-            if (more) fetch_v(t + C);
+            if (more) fetch_v(last - t - C);
         }
         if (NK == 1) {
             __syncthreads();
@@ -503,7 +558,7 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
             float x[CB];
 #pragma unroll
             for (int j = 0; j < CB; ++j) x[j] = S[kb][j][r];
-            store<CB, VEC>(to + (size_t)row * a.dv + col0, x, row < a.dk ? cols : 0);
+            if (row < a.dk) store<CB, VEC>(to + (size_t)row * a.dv + col0, x, cols);
         }
 }
 
