@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
                 *vp = a.v + ((size_t)seq.t0 + first) * vs + hv * a.dv;
     float *op = a.out + ((size_t)seq.t0 + first) * os + h * a.dv;
     const uint32_t lcv = VEC && left_k <= 0 ? 0 : lc, colv = VEC && cols <= 0 ? 0 : col0;
-    float kn[NL][4], qn[SUMS ? 1 : NL][4], v[2][4][CB];
+    float kn[NL][4], qn[SUMS ? 1 : NL][4], v[2][4][CB], vn[2][4][CB];
     auto fetch = [&](int n) {  // K and Q of the next chunk, of which n tokens are left
         const uint32_t ko = lr * (uint32_t)ks + lcv, qo = lr * (uint32_t)qs + lcv;
         if (VEC && n >= C) {
@@ -334,17 +334,17 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
 #pragma unroll
             for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) load<CB, true>(v[tb][r], vp + (16 * tb + r) * vs + vo);
+                for (int r = 0; r < 4; ++r) load<CB, true>(vn[tb][r], vp + (16 * tb + r) * vs + vo);
         } else {
 #pragma unroll
             for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int row = 16 * tb + 4 * g + r;
-                    load<CB, VEC>(v[tb][r], vp + min(row, n - 1) * vs + colv, cols);
+                    load<CB, VEC>(vn[tb][r], vp + min(row, n - 1) * vs + colv, cols);
                     if (row >= n)
 #pragma unroll
-                        for (int j = 0; j < CB; ++j) v[tb][r][j] = 0.0f;
+                        for (int j = 0; j < CB; ++j) vn[tb][r][j] = 0.0f;
                 }
         }
         vp += C * vs;
@@ -396,7 +396,12 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
         const bool more = t + C < last;
         const float(*const K)[LD] = Ks[p & (NK - 1)];
         __syncthreads();
-        if (more) fetch(last - t - C);
+#pragma unroll
+        for (int i = 0; i < 8 * CB; ++i) (&v[0][0][0])[i] = (&vn[0][0][0])[i];
+        if (more) {
+            fetch(last - t - C);
+            fetch_v(last - t - C);
+        }
         const Decays &d = dec[p];
         v4f O[2][CB];
         if (w == 3) {
@@ -534,7 +539,6 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
                         for (int j = 0; j < CB; ++j) S[kb][j] = MFMA4(k, v[tb][r][j], S[kb][j]);
                     }
             }
-            if (more) fetch_v(last - t - C);
         }
         if (NK == 1) {
             __syncthreads();
@@ -581,12 +585,12 @@ __global__ void __launch_bounds__(256) k_linear_join(ornk_linear_args a, Cut cut
 }
 
 // Sequences are cut where their heads and columns leave CUs idle: into parts of at
-// least 256 tokens, until there are two groups for each CU.
+// least 128 tokens, until there are two groups for each CU.
 Cut cut_of(const ornk_linear_args &a, int cb)
 {
     const long long groups = (long long)a.n_seqs * a.heads * ((a.dv + 64 * cb - 1) / (64 * cb));
     long long segs = 512 / groups;
-    if (segs > a.max_len / 256) segs = a.max_len / 256;
+    if (segs > a.max_len / 128) segs = a.max_len / 128;
     Cut c = {1, a.max_len, nullptr, nullptr};
     if (segs < 2) return c;
     c.len = (int)(((a.max_len + segs - 1) / segs + C - 1) / C * C);
@@ -594,8 +598,13 @@ Cut cut_of(const ornk_linear_args &a, int cb)
     return c;
 }
 
-// Blocks of 16 columns of a wave.  Two need a state of 256 registers beyond 128 rows.
-int blocks_of(const ornk_linear_args &a) { return a.dv > 64 && a.dk <= 128 ? 2 : 1; }
+// Blocks of 16 columns of a wave: two, where there is then a group for each CU, and the
+// state's registers leave room for another group.
+int blocks_of(const ornk_linear_args &a)
+{
+    if (a.dv <= 64 || a.dk > 128) return 1;
+    return (long long)a.n_seqs * a.heads * ((a.dv + 127) / 128) * cut_of(a, 2).segs >= 256 ? 2 : 1;
+}
 
 template <int KB, int CB, bool VEC>
 void launch(const ornk_linear_args &a, const Cut &cut, hipStream_t s)
