@@ -56,6 +56,8 @@ struct Row {
     double per;        // log2(e) / temperature
     double unit;       // weights are whole multiples of 1 / unit; n of them fit 62 bits
     float scale;       // bins per logit
+    float reach;       // tokens farther below the largest take no part in the order
+    bool by_rank;      // the top_k are few: all of them are put in order, and bins only count
     uint32_t cut, ties;  // by passes: kept are keys above `cut`, and the first `ties` of it
 };
 
@@ -96,17 +98,38 @@ __device__ __forceinline__ Row row_of(const ornk_sample_args &a, int row)
     return r;
 }
 
-// The row's largest and least logits known: what the weights and bins need.  Weights
-// below 2^-53 of the largest are 0, so bins end there.
+// The row's largest and least logits known: what the weights and bins need, and how far
+// below the largest a border of the choice may lie, which is where the bins end:
+// - a weight below 2^-53 of the largest is 0;
+// - the tokens below (1 - top_p) / 2 n are less than half of what top_p leaves out;
+// - min_p leaves out what is below it.
+// Where the top_k are few the first alone holds; where they are many, too, since their
+// own border may lie anywhere.
 __device__ __forceinline__ void scale_row(Row &r, uint32_t top, uint32_t low)
 {
     r.top_key = top;
     r.top = logit_of(top);
-    r.per = 1.4426950408889634 / (double)r.q.temperature;
-    const float all = r.top - logit_of(low), most = 37.0f * r.q.temperature;
-    const float range = all < most ? all : most;
+    const double T = r.q.temperature;
+    r.per = 1.4426950408889634 / T;
+    r.by_rank = r.q.top_k > 0 && r.q.top_k <= CAP / 2;
+    r.reach = 37.0f * r.q.temperature;
+    if (r.q.top_k <= 0 || r.q.top_k >= r.n) {
+        r.by_rank = false;
+        if (r.q.top_p < 1.0f)
+            r.reach = fminf(r.reach, (float)(-log((1.0 - (double)r.q.top_p) / (2.0 * r.n)) * T));
+        if (r.q.min_p > 0.0f) r.reach = fminf(r.reach, (float)(-log((double)r.q.min_p) * T * 1.0001));
+    }
+    const float all = r.top - logit_of(low);
+    const float range = all < r.reach ? all : r.reach;
     const float s = (float)NB / range;
     r.scale = range > 0.0f ? s < 1e30f ? s : 1e30f : 0.0f;
+}
+
+// A logit's distance below the largest; a NaN counts as far.
+__device__ __forceinline__ float below(const Row &r, float x) { return x == r.top ? 0.0f : r.top - x; }
+__device__ __forceinline__ bool within(const Row &r, float x)
+{
+    return below(r, x) <= r.reach && x > -INFINITY;
 }
 
 __device__ __forceinline__ void put_result(const ornk_sample_args &a, int row, int token, float prob)
@@ -246,6 +269,11 @@ __device__ __forceinline__ void mark_bins(const Row &r, Bins &s)
     uint64_t lo = all, hi = all;
     s.by_k = r.q.top_k > 0 && (uint32_t)r.q.top_k < s.c[NB];
     __syncthreads();
+    if (r.by_rank) {
+        mark(s, 0, s.by_k ? find<NT, uint32_t>(s, s.c, (uint32_t)r.q.top_k - 1) : NB - 1);
+        __syncthreads();
+        return;
+    }
     if (s.by_k) {
         const int b = find<NT, uint32_t>(s, s.c, (uint32_t)r.q.top_k - 1);
         mark(s, b, b);
@@ -332,13 +360,13 @@ __device__ __forceinline__ void choose(const ornk_sample_args &a, int row, const
         if (lane >= o) before += y;
     }
     if (lane == 63) s.tmp[tid >> 6] = before;
-    if (!tid) {
-        s.whole = b.w[NB];
-        s.by_min = r.q.min_p > 0.0f ? b.w[b.min_lo] : ~0ull;
-    }
     __syncthreads();
     before -= sum;
     for (int i = 0; i < tid >> 6; ++i) before += s.tmp[i];
+    if (tid == RT - 1) {
+        s.whole = r.by_rank ? before + sum : b.w[NB];
+        s.by_min = r.q.min_p == 0.0f ? ~0ull : r.by_rank ? 0 : b.w[b.min_lo];
+    }
     uint64_t run = before;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -356,7 +384,8 @@ __device__ __forceinline__ void choose(const ornk_sample_args &a, int row, const
         for (int i = 0; i < PER; ++i) {
             const int at = tid * per + i;
             if (i >= per || at >= m) continue;
-            f(i, b.w[bin[i]] + (run - s.first_w[bin[i]]), b.c[bin[i]] + (at - s.first[bin[i]]));
+            if (r.by_rank) f(i, run, (uint32_t)at);
+            else f(i, b.w[bin[i]] + (run - s.first_w[bin[i]]), b.c[bin[i]] + (at - s.first[bin[i]]));
             run += w[i];
         }
     };
@@ -366,17 +395,17 @@ __device__ __forceinline__ void choose(const ornk_sample_args &a, int row, const
         });
         __syncthreads();
     }
+    if (!tid) s.end = s.whole;  // also where top_p's border lies behind min_p's
+    __syncthreads();
     if (r.q.top_p < 1.0f) {
         const uint64_t least = least_of(r, s.whole);
         each([&](int i, uint64_t at, uint32_t) {
             if (at < least && least <= at + w[i]) s.end = at + w[i];
         });
-    } else if (!tid) {
-        s.end = s.whole;
     }
     if (r.q.min_p > 0.0f)
         each([&](int i, uint64_t at, uint32_t) {
-            if (bin[i] >= b.min_lo && bin[i] <= b.min_hi && e[i] >= (double)r.q.min_p)
+            if ((r.by_rank || (bin[i] >= b.min_lo && bin[i] <= b.min_hi)) && e[i] >= (double)r.q.min_p)
                 atomicMax((unsigned long long *)&s.by_min, (unsigned long long)(at + w[i]));
         });
     __syncthreads();
@@ -544,36 +573,48 @@ __device__ __forceinline__ Ends ends_of(const float *x, int i0, int end)
     return e;
 }
 
+// Into the bins of w and c, which are in LDS.  What is out of reach belongs to the sum
+// that top_p is a share of, behind all bins' tokens.
 template <int NT>
 __device__ __forceinline__ void fill_bins(const Row &r, int i0, int end, uint64_t *w, uint32_t *c)
 {
+    uint64_t rest = 0;
 #pragma unroll 2
     for (int i = i0 + 4 * (int)threadIdx.x; i < end; i += 4 * NT) {
         const v4f y = load4(r.x, end, i);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+            const bool in = within(r, y[j]);
+            if (r.by_rank) {
+                if (in) atomicAdd(&c[bin_of(r, y[j])], 1u);
+                continue;
+            }
+            if (!in && r.q.top_p == 1.0f) continue;
             const uint64_t v = fixed(r, weight(r, y[j]));
-            if (!v) continue;
-            const int bin = bin_of(r, y[j]);
-            atomicAdd((unsigned long long *)&w[bin], (unsigned long long)v);
-            if (r.q.top_k > 0) atomicAdd(&c[bin], 1u);
+            if (in) {
+                const int bin = bin_of(r, y[j]);
+                atomicAdd((unsigned long long *)&w[bin], (unsigned long long)v);
+                if (r.q.top_k > 0) atomicAdd(&c[bin], 1u);
+            } else {
+                rest += v;
+            }
         }
     }
+    if (r.by_rank || r.q.top_p == 1.0f) return;
+    for (int o = 32; o; o >>= 1) rest += __shfl_xor(rest, o, 64);
+    if (!(threadIdx.x & 63) && rest) atomicAdd((unsigned long long *)&w[NB - 1], (unsigned long long)rest);
 }
 
-// Those in marked bins to the list; *count goes on past CAP.
-template <int NT>
-__device__ __forceinline__ void gather(const Row &r, const Bins &b, int i0, int end, uint64_t *list, uint32_t *count)
+// Those in marked bins: f(token's place in the order).
+template <int NT, class F>
+__device__ __forceinline__ void gather(const Row &r, const Bins &b, int i0, int end, F f)
 {
 #pragma unroll 2
     for (int i = i0 + 4 * (int)threadIdx.x; i < end; i += 4 * NT) {
         const v4f y = load4(r.x, end, i);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (!(y[j] > -INFINITY) || !is_marked(b, bin_of(r, y[j])) || !fixed(r, weight(r, y[j]))) continue;
-            const uint32_t at = atomicAdd(count, 1u);
-            if (at < CAP) list[at] = (uint64_t)~key_of(y[j]) << 32 | (uint32_t)(i + j);
-        }
+        for (int j = 0; j < 4; ++j)
+            if (within(r, y[j]) && is_marked(b, bin_of(r, y[j]))) f((uint64_t)~key_of(y[j]) << 32 | (uint32_t)(i + j));
     }
 }
 
@@ -602,7 +643,10 @@ __global__ void __launch_bounds__(RT) k_sample_row(ornk_sample_args a)
     __syncthreads();
     sums_before<RT>(b);
     mark_bins<RT>(r, b);
-    gather<RT>(r, b, 0, r.n, s.c.list, &s.c.count);
+    gather<RT>(r, b, 0, r.n, [&](uint64_t t) {
+        const uint32_t at = atomicAdd(&s.c.count, 1u);
+        if (at < CAP) s.c.list[at] = t;
+    });
     __syncthreads();
     const uint32_t m = s.c.count;
     __syncthreads();
@@ -674,11 +718,10 @@ __global__ void __launch_bounds__(SL) k_sample_bins(ornk_sample_args a, Slices s
     __syncthreads();
     fill_bins<SL>(r, i0, min(i0 + s.len, a.n), w, c);
     __syncthreads();
-    for (int i = tid; i < NB; i += SL)
-        if (w[i]) {
-            atomicAdd((unsigned long long *)&s.w[(size_t)row * NB + i], (unsigned long long)w[i]);
-            if (r.q.top_k > 0) atomicAdd(&s.c[(size_t)row * NB + i], c[i]);
-        }
+    for (int i = tid; i < NB; i += SL) {
+        if (w[i]) atomicAdd((unsigned long long *)&s.w[(size_t)row * NB + i], (unsigned long long)w[i]);
+        if (c[i]) atomicAdd(&s.c[(size_t)row * NB + i], c[i]);
+    }
 }
 
 template <int NT>
@@ -693,17 +736,37 @@ __device__ __forceinline__ void load_bins(const Slices &s, int row, const Row &r
     mark_bins<NT>(r, b);
 }
 
-// The marked tokens to the row's list.
+// The marked tokens to the row's list: those of a group together, as long as LDS holds
+// them (an atomic of its own for each token took 110 us for 16 rows of 2000).
 __global__ void __launch_bounds__(SL) k_sample_gather(ornk_sample_args a, Slices s)
 {
+    constexpr int MINE = 1024;
     __shared__ Bins b;
     __shared__ Ends tmp[MAX_SLICES / 64];
+    __shared__ uint64_t mine[MINE];
+    __shared__ uint32_t count, base;
     const int row = blockIdx.y, tid = threadIdx.x, i0 = blockIdx.x * s.len;
     Row r;
     Ends e;
     if (!row_ready(a, s, row, r, e, tmp)) return;
+    if (!tid) count = 0;
     load_bins<SL>(s, row, r, b);
-    gather<SL>(r, b, i0, min(i0 + s.len, a.n), s.list + (size_t)row * CAP, &s.count[row]);
+    uint64_t *list = s.list + (size_t)row * CAP;
+    gather<SL>(r, b, i0, min(i0 + s.len, a.n), [&](uint64_t t) {
+        const uint32_t at = atomicAdd(&count, 1u);
+        if (at < MINE) {
+            mine[at] = t;
+        } else {
+            const uint32_t to = atomicAdd(&s.count[row], 1u);
+            if (to < CAP) list[to] = t;
+        }
+    });
+    __syncthreads();
+    const uint32_t m = count < MINE ? count : MINE;
+    if (!tid && m) base = atomicAdd(&s.count[row], m);
+    __syncthreads();
+    for (uint32_t i = tid; i < m; i += SL)
+        if (base + i < CAP) list[base + i] = mine[i];
 }
 
 __global__ void __launch_bounds__(RT) k_sample_choose(ornk_sample_args a, Slices s)

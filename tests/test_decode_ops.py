@@ -688,14 +688,14 @@ def test_linear_reports_bad_numbers(om, ctx):
 
 # ---------------------------------------- sampling
 def _choices(x, temperature, top_k, top_p, min_p, u):
-    """The tokens that 64-bit sums allow: more than one next to a border only."""
+    """The tokens that 64-bit sums allow, and their shares: more than one next to a border only."""
     x = np.where(np.isnan(x), -np.inf, x.astype(np.float64))
     on = int((x > -np.inf).sum())
     if not on:
-        return {-1: 0.0}
+        return {-1: [0.0]}
     order = np.lexsort((np.arange(x.size), -x))[:on]
     if temperature == 0:
-        return {int(order[0]): 1.0}
+        return {int(order[0]): [1.0]}
     top = x[order[0]]
     with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
         w = np.where(x[order] == top, 1.0, np.exp((x[order] - top) / float(np.float32(temperature))))
@@ -713,7 +713,7 @@ def _choices(x, temperature, top_k, top_p, min_p, u):
         for s in (-1.0, 1.0):
             i = int(np.searchsorted(c, float(np.float32(u)) * c[-1] + s * off, side="right"))
             i = min(i, len(kept) - 1)
-            found[int(order[i])] = kept[i] / c[-1]
+            found.setdefault(int(order[i]), []).append(kept[i] / c[-1])
     return found
 
 
@@ -744,7 +744,7 @@ def _check_sample(om, ctx, x, requests, u):
         ok = _choices(row, *q, u[i])
         several += len(ok) > 1
         assert int(t[i]) in ok, (i, q, u[i], int(t[i]), ok)
-        want = ok[int(t[i])]
+        want = min(ok[int(t[i])], key=lambda w: abs(p[i] - w))
         assert abs(p[i] - want) <= want * (EPS + 2 * x.shape[1] * 2.0 ** -45), (i, q, p[i], want)
     assert several <= len(requests) // 8  # the borders are seldom near
 
@@ -790,6 +790,30 @@ def test_sample_of_equal_logits(om, ctx):
     assert err is None
     assert t.tolist() == [2500, 250, 0, 4999, 37, 0]
     assert np.allclose(p, [1 / 5000, 1 / 1000, 1 / 2500, 1 / 5000, 1 / 50, 1.0], rtol=2e-7, atol=0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [9000, 40000])
+def test_sample_of_many_equal_logits(om, ctx, n):
+    """More of them next to a border than are put in order, and others above and below."""
+    g = np.random.default_rng(n)
+    x = np.zeros((2 * len(REQUESTS), n), np.float32)
+    x[::3, g.integers(0, n, 50)] = 1.5
+    x[1::2, g.integers(0, n, 50)] = -2.0
+    x[::4, g.integers(0, n, 3000)] = -np.inf
+    u = (g.random(len(x)) * 0.999).astype(np.float32)
+    requests = REQUESTS + [(1.0, 5000, 0.9, 0.0), (1.0, 8500, 1.0, 0.0), (2.0, 8999, 0.5, 0.1)] + REQUESTS[3:]
+    _check_sample(om, ctx, x, requests, u)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [20000, 60000])
+def test_sample_with_a_large_top_k(om, ctx, n):
+    g = np.random.default_rng(n)
+    requests = [(1.0, k, p, m) for k in (1, 2, 64, 4096, 4097, 12000, n - 1, n, 2 ** 31 - 1)
+                for p, m in ((1.0, 0.0), (0.9, 0.0), (0.999, 0.001))]
+    x = (g.standard_normal((len(requests), n)) * 2).astype(np.float32)
+    _check_sample(om, ctx, x, requests, g.random(len(x)).astype(np.float32))
 
 
 @pytest.mark.gpu
