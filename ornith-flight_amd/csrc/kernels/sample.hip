@@ -233,13 +233,14 @@ __device__ __forceinline__ void mark(Bins &s, int lo, int hi)
 }
 
 // Every sum below is known up to the bins marked, so those of the next border are.
-__device__ __forceinline__ void mark_bins(const Row &r, Bins &s)
+// counted: only that the bins hold the top_k is known.  min_bin: min_p's.
+__device__ __forceinline__ void mark_bins(const Row &r, Bins &s, bool counted, int min_bin)
 {
     if (threadIdx.x < NB / 32) s.marked[threadIdx.x] = 0;
     if (!threadIdx.x) s.last = 0;
     __syncthreads();
     const bool by_k = r.q.top_k > 0 && (uint32_t)r.q.top_k < s.c[NB];
-    if (r.by_rank) {
+    if (counted) {
         mark(s, 0, by_k ? find<uint32_t>(s, s.c, (uint32_t)r.q.top_k - 1) : NB - 1);
         __syncthreads();
         return;
@@ -252,9 +253,8 @@ __device__ __forceinline__ void mark_bins(const Row &r, Bins &s)
         hi = s.w[b + 1];
     }
     if (r.q.min_p > 0.0f) {
-        const int b = bin_at(r, -logf(r.q.min_p) * r.q.temperature);
-        s.min_lo = b > 0 ? b - 1 : 0;  // the logarithm's rounding may move the border to the next bin
-        s.min_hi = b < NB - 1 ? b + 1 : b;
+        s.min_lo = min_bin > 0 ? min_bin - 1 : 0;  // the logarithm's rounding may move it to the next bin
+        s.min_hi = min_bin < NB - 1 ? min_bin + 1 : min_bin;
         mark(s, s.min_lo, s.min_hi);
     }
 #pragma unroll 1
@@ -271,6 +271,8 @@ __device__ __forceinline__ void mark_bins(const Row &r, Bins &s)
     }
     __syncthreads();
 }
+
+__device__ __forceinline__ float min_below(const Row &r) { return -logf(r.q.min_p) * r.q.temperature; }
 
 __device__ __forceinline__ bool is_marked(const Bins &s, int bin) { return s.marked[bin >> 5] >> (bin & 31) & 1; }
 
@@ -307,10 +309,12 @@ __device__ __forceinline__ float share(const Row &r, uint32_t key, uint64_t all)
 }
 
 // At most CT tokens: each finds its place by counting those before it.
-__device__ __forceinline__ void choose_few(const ornk_sample_args &a, int row, const Row &r, const Bins &b, Choice &s, int m)
+template <class F>
+__device__ __forceinline__ void choose_few(const ornk_sample_args &a, int row, const Row &r, const Bins &b, Choice &s, int m,
+                                           bool binned, F place_of)
 {
     const int tid = threadIdx.x, lane = tid & 63;
-    const bool binned = !r.by_rank, on = tid < m;
+    const bool on = tid < m;
     auto order = [&](int i) { return s.list[i] ^ 0xffffffffu; };  // the key, then the least index
     int place = 0;
     if (on) {
@@ -325,7 +329,7 @@ __device__ __forceinline__ void choose_few(const ornk_sample_args &a, int row, c
     const uint32_t key = (uint32_t)(token >> 32);
     const double e = on ? weight(r, logit_of(key)) : 0.0;
     const uint64_t w = on ? fixed(r, e) : 0, run = wave_scan(w);
-    const int bin = binned && on ? bin_of(r, logit_of(key)) : -1;
+    const int bin = binned && on ? place_of(logit_of(key)) : -1;
     if (lane == 63) s.tmp[0][tid >> 6] = run;
     __syncthreads();
     uint64_t lo = run - w, all = 0;  // the sum before it
@@ -337,7 +341,7 @@ __device__ __forceinline__ void choose_few(const ornk_sample_args &a, int row, c
     if (binned) {
         uint64_t *first_w = s.w + CT;                                       // of a bin's tokens in the list
         uint32_t *first = reinterpret_cast<uint32_t *>(s.w + CT + NB);
-        if (on && (!tid || bin_of(r, logit_of((uint32_t)(s.w[tid - 1] >> 32))) != bin)) first_w[bin] = lo, first[bin] = tid;
+        if (on && (!tid || place_of(logit_of((uint32_t)(s.w[tid - 1] >> 32))) != bin)) first_w[bin] = lo, first[bin] = tid;
         __syncthreads();
         if (on) {
             lo = b.w[bin] + lo - first_w[bin];
@@ -379,10 +383,12 @@ __device__ __forceinline__ void choose_few(const ornk_sample_args &a, int row, c
 // More: every border is the first key, from the largest down, up to which a sum (of
 // tokens, or of their weights) passes a limit, found by passes over the tokens, 8 bits of
 // the keys' distance from the least each.
-__device__ __forceinline__ void choose_many(const ornk_sample_args &a, int row, const Row &r, Bins &b, Choice &s, uint32_t m)
+template <class F>
+__device__ __forceinline__ void choose_many(const ornk_sample_args &a, int row, const Row &r, Bins &b, Choice &s, uint32_t m,
+                                            bool binned, F place_of)
 {
     const int tid = threadIdx.x, lane = tid & 63;
-    const bool listed = m <= CAP, binned = listed && !r.by_rank;
+    const bool listed = m <= CAP;
     const int n = listed ? (int)m : r.n;
     // f(key, index, weight) of every token that has a weight
     auto each = [&](auto f) {
@@ -410,7 +416,7 @@ __device__ __forceinline__ void choose_many(const ornk_sample_args &a, int row, 
         sum[0] += v;
         ++sum[2];
         if (r.q.min_p == 0.0f || weight(r, logit_of(key)) < (double)r.q.min_p) return;
-        const int bin = binned ? bin_of(r, logit_of(key)) : 0;
+        const int bin = binned ? place_of(logit_of(key)) : 0;
         if (!binned || (bin >= b.min_lo && bin <= b.min_hi)) sum[1] += v;
     });
 #pragma unroll
@@ -465,7 +471,7 @@ __device__ __forceinline__ void choose_many(const ornk_sample_args &a, int row, 
         // there may be, less theirs
         auto those = [&](auto f) {
             each([&](uint32_t k, uint32_t index, uint64_t v) {
-                if (bin >= 0 && bin_of(r, logit_of(k)) != bin) return;
+                if (bin >= 0 && place_of(logit_of(k)) != bin) return;
                 if (stage == INDEX) {
                     if (k != key) return;
                     k = ORN_SAMPLE_MAX_VOCAB - 1 - index;
@@ -544,10 +550,86 @@ __device__ __forceinline__ void choose_many(const ornk_sample_args &a, int row, 
     }
 }
 
-__device__ __forceinline__ void choose(const ornk_sample_args &a, int row, const Row &r, Bins &b, Choice &s, uint32_t m)
+// Which part of a bin: the marked bins (without bins: all of the reach) in as many equal
+// stretches as NB allows.
+struct Fine {
+    int parts;       // of a bin; 1: the bins are as they were
+    uint32_t before[NB / 32];
+};
+
+__device__ __forceinline__ int fine_at(const Row &r, const Bins &b, const Fine &f, float below)
 {
-    if (m <= CT) choose_few(a, row, r, b, s, (int)m);
-    else choose_many(a, row, r, b, s, m);
+    const int bin = bin_at(r, below), in = (int)((below * r.scale - (float)bin) * (float)f.parts);
+    const uint32_t word = b.marked[bin >> 5];
+    return (int)(f.before[bin >> 5] + __popc(word & ((1u << (bin & 31)) - 1))) * f.parts + (in < f.parts ? in : f.parts - 1);
+}
+
+// The choice from a list.  A longer one is divided once more, by finer bins.
+__device__ __forceinline__ void choose(const ornk_sample_args &a, int row, const Row &r, Bins &b, Bins &c, Fine &f,
+                                       Choice &s, uint32_t m)
+{
+    const int tid = threadIdx.x, lane = tid & 63;
+    bool binned = !r.by_rank;
+    const bool fine = m > CT && m <= CAP;
+    if (fine) {
+        if (r.by_rank) {  // the list's own bins
+            if (tid < NB / 32) b.marked[tid] = ~0u;
+            for (int i = tid; i <= NB; i += CT) b.w[i] = b.c[i] = 0;
+        }
+        for (int i = tid; i < NB; i += CT) c.w[i] = c.c[i] = 0;
+        if (!tid) s.count = 0;
+        __syncthreads();
+        if (tid < 64) {
+            const uint32_t n = lane < NB / 32 ? __popc(b.marked[lane]) : 0;
+            const uint32_t to = (uint32_t)wave_scan(n);
+            if (lane < NB / 32) f.before[lane] = to - n;
+            if (lane == NB / 32 - 1) f.parts = NB / (int)to;
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int i = tid; i < (int)m; i += CT) {
+            const float x = logit_of((uint32_t)(s.list[i] >> 32));
+            const int bin = fine_at(r, b, f, below(r, x));
+            atomicAdd((unsigned long long *)&c.w[bin], (unsigned long long)fixed(r, weight(r, x)));
+            atomicAdd(&c.c[bin], 1u);
+        }
+        __syncthreads();
+        sums_before(c);
+        if (binned) {
+            // from the list's sums to the row's: what lies between marked bins
+            uint64_t *dw = s.w;
+            uint32_t *dc = reinterpret_cast<uint32_t *>(s.w + NB);
+            for (int bin = tid; bin < NB; bin += CT) {
+                if (!is_marked(b, bin)) continue;
+                const int o = (int)(f.before[bin >> 5] + __popc(b.marked[bin >> 5] & ((1u << (bin & 31)) - 1)));
+                dw[o] = b.w[bin] - c.w[o * f.parts];
+                dc[o] = b.c[bin] - c.c[o * f.parts];
+            }
+            __syncthreads();
+            const int used = (int)(f.before[NB / 32 - 1] + __popc(b.marked[NB / 32 - 1])) * f.parts;
+            for (int i = tid; i <= NB; i += CT) {
+                c.w[i] = i < used ? c.w[i] + dw[i / f.parts] : b.w[NB];
+                c.c[i] = i < used ? c.c[i] + dc[i / f.parts] : b.c[NB];
+            }
+            __syncthreads();
+        }
+        binned = true;
+        mark_bins(r, c, false, r.q.min_p > 0.0f ? fine_at(r, b, f, min_below(r)) : 0);
+#pragma unroll 1
+        for (int i = tid; i < (int)m; i += CT) {
+            const uint64_t t = s.list[i];
+            if (!is_marked(c, fine_at(r, b, f, below(r, logit_of((uint32_t)(t >> 32)))))) continue;
+            const uint32_t at = atomicAdd(&s.count, 1u);
+            s.w[at] = t;
+        }
+        __syncthreads();
+        m = s.count;
+        for (int i = tid; i < (int)m; i += CT) s.list[i] = s.w[i];
+        __syncthreads();
+    }
+    auto place_of = [&](float x) { return fine ? fine_at(r, b, f, below(r, x)) : bin_of(r, x); };
+    if (m <= CT) choose_few(a, row, r, fine ? c : b, s, (int)m, binned, place_of);
+    else choose_many(a, row, r, fine ? c : b, s, m, binned && m <= CAP, place_of);
 }
 
 // ---- passes over logits, tokens i0 to end - 1 of a row by a group ------------------
@@ -689,7 +771,8 @@ __device__ __forceinline__ void first_of(const Row &r, float top, int i0, int en
 // ---- shorter rows: a group each, in one launch -------------------------------------
 __global__ void __launch_bounds__(ST) k_sample_row(ornk_sample_args a)
 {
-    __shared__ Bins b;
+    __shared__ Bins b, fine;
+    __shared__ Fine parts;
     __shared__ Choice s;
     __shared__ Ends ends[ST / 64];
     const int row = blockIdx.x, tid = threadIdx.x;
@@ -726,14 +809,16 @@ __global__ void __launch_bounds__(ST) k_sample_row(ornk_sample_args a)
         fill_bins(r, 0, r.n, b.w, b.c);
         __syncthreads();
         sums_before(b);
-        mark_bins(r, b);
+        mark_bins(r, b, r.by_rank, bin_at(r, min_below(r)));
     }
     gather(r, bound ? nullptr : &b, 0, r.n, [&](uint64_t t) {
         const uint32_t at = atomicAdd(&s.count, 1u);
         if (at < CAP) s.list[at] = t;
     });
     __syncthreads();
-    if (tid < CT) choose(a, row, r, b, s, s.count);
+    const uint32_t m = s.count;
+    __syncthreads();
+    if (tid < CT) choose(a, row, r, b, fine, parts, s, m);
 }
 
 // ---- longer rows: in slices ------------------------------------------------------
@@ -849,7 +934,7 @@ struct OwnBins {
         }
         __syncthreads();
         sums_before(b);
-        mark_bins(r, b);
+        mark_bins(r, b, r.by_rank, bin_at(r, min_below(r)));
     }
 };
 
@@ -902,14 +987,15 @@ __global__ void __launch_bounds__(ST) k_sample_gather(ornk_sample_args a, Slices
 // of its steps.
 __global__ void __launch_bounds__(CT) k_sample_choose(ornk_sample_args a, Slices s)
 {
-    __shared__ Bins b;
+    __shared__ Bins b, fine;
+    __shared__ Fine parts;
     __shared__ Choice k;
     __shared__ Ends tmp[MAX_SLICES / 64];
     const int row = blockIdx.x, tid = threadIdx.x;
     Row r = row_of(a, row);
     const Ends own = own_ends(s, row);
     const OwnBins<CT> bins(s, row);
-    const uint32_t m = s.count[row], first = s.first[row];
+    const uint32_t m = s.count[row], first = s.first[row], bound = s.bound[row];
     const uint64_t *list = s.list + (size_t)row * CAP;
     const uint64_t mine = list[tid];
     const Ends e = row_ends(own, tmp);
@@ -920,12 +1006,12 @@ __global__ void __launch_bounds__(CT) k_sample_choose(ornk_sample_args a, Slices
         put_result(a, row, none ? -1 : (int)first, none ? 0.0f : 1.0f);
         return;
     }
-    scale_row(r, e, 0);
+    scale_row(r, e, r.by_rank ? bound : 0);
     k.list[tid] = mine;
     for (int i = tid + CT; i < min((int)m, CAP); i += CT) k.list[i] = list[i];
     if (!r.by_rank) bins.put(r, b);
     __syncthreads();
-    choose(a, row, r, b, k, m);
+    choose(a, row, r, b, fine, parts, k, m);
 }
 
 constexpr int ROW_MAX = 32768;  // tokens of a row that one group takes
@@ -933,7 +1019,7 @@ constexpr int ROW_MAX = 32768;  // tokens of a row that one group takes
 Slices slices_of(const ornk_sample_args &a)
 {
     constexpr int UNIT = 4 * ST;
-    const long long want = ((long long)a.rows * a.n / 768 + UNIT - 1) / UNIT;  // for 768 groups
+    const long long want = ((long long)a.rows * a.n / 1536 + UNIT - 1) / UNIT;  // for 1536 groups
     const long long least = ((long long)a.n + UNIT * MAX_SLICES - 1) / (UNIT * MAX_SLICES);
     long long k = want < 1 ? 1 : want > 8 ? 8 : want;
     if (k > a.n / (8 * UNIT)) k = a.n / (8 * UNIT);  // 8 slices: parts for CAP / 2 of the top_k
