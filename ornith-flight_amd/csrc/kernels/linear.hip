@@ -38,57 +38,83 @@ __device__ __forceinline__ Seq seq_of(const ornk_linear_args &a, int b)
     return s;
 }
 
-// Token by token: a group of 4 waves holds 64 columns of a head's state, a wave a
-// quarter of its rows.
-__global__ void __launch_bounds__(256) k_linear_steps(ornk_linear_args a)
+// One token of each sequence (or none): V columns per lane, L lanes to a row of the
+// state, 256 / L rows at a time and up to 16 of them in flight per thread.  q and k come
+// through LDS, and the row groups' shares of q S meet there.
+template <int V, int L>
+__global__ void __launch_bounds__(256) k_linear_step(ornk_linear_args a)
 {
-    __shared__ float q[256], k[256], part[4][64];
-    const int b = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
-    const int w = tid >> 6, col = blockIdx.z * 64 + (tid & 63);
+    typedef float vec __attribute__((ext_vector_type(V)));
+    constexpr int G = 256 / L, R = 16;
+    __shared__ float q[256], k[256];
+    __shared__ vec part[G][L];
+    const int blocks = (a.dv + V * L - 1) / (V * L), tid = threadIdx.x, g = tid / L;
+    const int b = blockIdx.y, h = blockIdx.x / blocks;
+    const int col = V * ((blockIdx.x - h * blocks) * L + tid - g * L);
     const Seq seq = seq_of(a, b);
     if (seq.n < 0) return;
+    const size_t t = seq.t0, size = (size_t)a.dk * a.dv;
+    const float *from = seq.in >= 0 ? a.S + ((size_t)seq.in * a.heads + h) * size + col : nullptr;
+    float *to = seq.out >= 0 ? a.S + ((size_t)seq.out * a.heads + h) * size + col : nullptr;
     const bool on = col < a.dv;
-    const int hq = h / (a.heads / a.qh), hk = h / (a.heads / a.kh), hv = h / (a.heads / a.vh);
-    const size_t size = (size_t)a.dk * a.dv;
-    float s[64];
-#pragma unroll
-    for (int i = 0; i < 64; ++i) {
-        const int r = 4 * i + w;
-        s[i] = on && r < a.dk && seq.in >= 0
-                   ? a.S[((size_t)seq.in * a.heads + h) * size + (size_t)r * a.dv + col]
-                   : 0.0f;
-    }
-    for (int j = 0; j < seq.n; ++j) {
-        const size_t t = (size_t)seq.t0 + j;
-        __syncthreads();
+    float f = 1.0f;
+    vec v = 0.0f, o = 0.0f;
+    if (!seq.n && tid < a.dk) q[tid] = k[tid] = 0.0f;
+    if (seq.n) {
         if (tid < a.dk) {
-            q[tid] = a.q[(t * a.qh + hq) * a.dk + tid] * a.scale;
-            k[tid] = a.k[(t * a.kh + hk) * a.dk + tid];
+            q[tid] = a.q[(t * a.qh + h / (a.heads / a.qh)) * a.dk + tid] * a.scale;
+            k[tid] = a.k[(t * a.kh + h / (a.heads / a.kh)) * a.dk + tid];
         }
-        __syncthreads();
-        const float g = a.decay[a.per_token ? t * a.heads + h : h];
-        const float f = expf(g);
-        float v = on ? a.v[(t * a.vh + hv) * a.dv + col] : 0.0f, o = 0.0f;
-        if (a.complement) v *= -expm1f(g);
+        if (on) v = *reinterpret_cast<const vec *>(a.v + (t * a.vh + h / (a.heads / a.vh)) * a.dv + col);
+        const float decay = a.decay[a.per_token ? t * a.heads + h : h];
+        f = expf(decay);
+        if (a.complement) v *= -expm1f(decay);
+    }
+    vec s[R];
+    auto load = [&](int r0) {
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {
-            const int r = 4 * i + w;
+        for (int i = 0; i < R; ++i) {
+            const int r = r0 + G * i;
+            s[i] = 0.0f;
+            if (from && on && r < a.dk) s[i] = *reinterpret_cast<const vec *>(from + (size_t)r * a.dv);
+        }
+    };
+    load(g);
+    __syncthreads();
+    for (int r0 = 0;; load(r0 + g)) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int r = r0 + g + G * i;
             if (r < a.dk) {
-                s[i] = fmaf(k[r], v, f * s[i]);
-                o = fmaf(q[r], s[i], o);
+                const float kr = k[r], qr = q[r];
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    s[i][e] = fmaf(kr, v[e], f * s[i][e]);
+                    o[e] = fmaf(qr, s[i][e], o[e]);
+                }
+                if (to && on) *reinterpret_cast<vec *>(to + (size_t)r * a.dv) = s[i];
             }
         }
-        part[w][tid & 63] = o;
-        __syncthreads();
-        if (w == 0 && on)
-            a.out[(t * a.heads + h) * a.dv + col] = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
+        r0 += G * R;
+        if (r0 >= a.dk) break;
     }
-    if (seq.out < 0 || !on) return;
-#pragma unroll
-    for (int i = 0; i < 64; ++i) {
-        const int r = 4 * i + w;
-        if (r < a.dk) a.S[((size_t)seq.out * a.heads + h) * size + (size_t)r * a.dv + col] = s[i];
+    if (!seq.n) return;
+    part[g][tid - g * L] = o;
+    __syncthreads();
+    if (tid < L && on) {
+        vec sum = part[0][tid];
+        for (int i = 1; i < G; ++i) sum += part[i][tid];
+        *reinterpret_cast<vec *>(a.out + (t * a.heads + h) * a.dv + col) = sum;
     }
+}
+
+// Whole heads in a group (64 KB of state at 128 x 128) where that gives every CU two of
+// them, else in groups of 32 columns.
+template <int V, int L>
+void launch_step(const ornk_linear_args &a, hipStream_t s)
+{
+    const int blocks = (a.dv + V * L - 1) / (V * L);
+    hipLaunchKernelGGL((k_linear_step<V, L>), dim3((unsigned)a.heads * blocks, a.n_seqs), dim3(256), 0, s, a);
 }
 
 // ---- chunks ------------------------------------------------------------------
@@ -637,7 +663,9 @@ extern "C" size_t ornk_linear_ws(const ornk_linear_args *a)
 extern "C" int ornk_linear(const ornk_linear_args *a, hipStream_t s)
 {
     if (a->max_len <= 1) {
-        hipLaunchKernelGGL(k_linear_steps, dim3(a->n_seqs, a->heads, (a->dv + 63) / 64), dim3(256), 0, s, *a);
+        if (a->dv % 4) launch_step<1, 32>(*a, s);
+        else if ((long long)a->n_seqs * a->heads >= 512 && a->dv > 32) launch_step<4, 32>(*a, s);
+        else launch_step<4, 8>(*a, s);
         return hipGetLastError();
     }
     const int cb = blocks_of(*a);
