@@ -49,12 +49,25 @@ __device__ __forceinline__ Row row_of(const ornk_kv_pages &p, const ornk_rope_ar
     return r;
 }
 
-// What a row is multiplied by: 1 / sqrt(sum or mean of squares + eps).
-__device__ __forceinline__ float factor(const ornk_rope_args &a, float ss)
-{
-    if (a.norm == 1) ss /= (float)a.hd;
-    return 1.0f / sqrtf(ss + a.eps);
-}
+// What a row is divided by: sqrt(sum or mean of squares + eps).
+struct Norm {
+    float s, per;  // per = 1 / s
+    bool exact;    // the quotient's remainder is a number
+    __device__ __forceinline__ Norm(const ornk_rope_args &a, float ss)
+    {
+        if (a.norm == 1) ss /= (float)a.hd;
+        s = sqrtf(ss + a.eps);
+        per = 1.0f / s;
+        exact = s < INFINITY && per < INFINITY;
+    }
+    // x / s; the product with 1 / s alone rounds once more (of 4099 tokens' heads of 128
+    // 4.9e-8 of the whole instead of 4.2e-8)
+    __device__ __forceinline__ float operator()(float x) const
+    {
+        const float q = x * per;
+        return exact ? fmaf(fmaf(-q, s, x), per, q) : q;
+    }
+};
 
 // Rows that are no whole float4s (or halves of pairs that are not four): a wave per
 // row, an element or a pair per lane.  The token's angles are formed once, in LDS.
@@ -73,16 +86,14 @@ __global__ void __launch_bounds__(NT) k_norm_append_any(ornk_kv_pages p, ornk_ro
         __syncthreads();
         for (int i = r0 + (threadIdx.x >> 6); i < r1; i += NT / 64) {
             const Row r = row_of<TYPE>(p, a, t, slot, i);
-            float f = 1.0f;
-            if (r.norm) {
-                float ss = 0.0f;
+            float ss = 0.0f;
+            if (r.norm)
                 for (int d = lane; d < hd; d += 64) ss = fmaf(r.x[d], r.x[d], ss);
-                f = factor(a, orn_wave_sum(ss));
-            }
+            const Norm norm(a, orn_wave_sum(ss));
             auto get = [&](int d) {
                 const float x = r.x[d];
                 if (!r.norm) return x;
-                return r.w ? x * f * r.w[d] : x * f;
+                return r.w ? norm(x) * r.w[d] : norm(x);
             };
             auto put = [&](int d, float x) {
                 if (r.out) r.out[d] = x;
@@ -147,14 +158,17 @@ __global__ void __launch_bounds__(NT, 8) k_norm_append(ornk_kv_pages p, ornk_rop
                 for (int e = 0; e < 4; ++e) ss = fmaf(y[e], y[e], fmaf(x[e], x[e], ss));
             }
             for (int o = G >> 1; o; o >>= 1) ss += __shfl_xor(ss, o, 64);
-            const float f = factor(a, ss);
+            const Norm norm(a, ss);
             for (int it = li; it < items; it += G) {
                 if (items > G) load(it);
                 bool two;
                 const int c = column(it, two);
                 if (r.norm) {
-                    x *= f;
-                    y *= f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        x[e] = norm(x[e]);
+                        y[e] = norm(y[e]);
+                    }
                     if (r.w) {
                         x *= *reinterpret_cast<const v4f *>(r.w + c);
                         if (two) y *= *reinterpret_cast<const v4f *>(r.w + c + R);
