@@ -300,9 +300,12 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
     float *const mine = cut.segs > 1 ? cut.states + (((size_t)b * a.heads + h) * cut.segs + sg) * size : nullptr;
 
     v4f S[KB][CB];
+    bool zero;  // the state is, still
+    const bool stored = SUMS || (last == seq.n && seq.out >= 0);  // it is, in the end
     {
         const float *from = SUMS ? nullptr : cut.segs > 1 ? mine
                             : seq.in >= 0 ? a.S + ((size_t)seq.in * a.heads + h) * size : nullptr;
+        zero = !from;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -469,6 +472,8 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
             for (int ib = 0; ib < 2; ++ib)
 #pragma unroll
                 for (int j = 0; j < CB; ++j) O[ib][j] = v4f{0, 0, 0, 0};
+        }
+        if (!SUMS && busy && !zero) {
             v4f q[2][2];
             auto read = [&](v4f (&y)[2], int kb) {
                 y[0] = *reinterpret_cast<const v4f *>(&Qs[c][16 * kb + 4 * g]);
@@ -543,6 +548,8 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
                 }
                 op += C * os;
             }
+        }
+        if (busy && (more || stored)) {
             const float all = d.all;
 #pragma unroll
             for (int tb = 0; tb < 2; ++tb) {
@@ -566,20 +573,16 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
                     }
             }
         }
+        zero = false;
         if (NK == 1) {
             __syncthreads();
             stage_k(0);
         }
     }
 
-    float *to = nullptr;
-    if (SUMS) {
-        to = mine;
-        if (tid == 192 && !block) cut.decays[((size_t)b * a.heads + h) * cut.segs + sg] = exp2_of(left);
-    } else if (last == seq.n && seq.out >= 0) {
-        to = a.S + ((size_t)seq.out * a.heads + h) * size;
-    }
-    if (!to || cols <= 0) return;
+    if (SUMS && tid == 192 && !block) cut.decays[((size_t)b * a.heads + h) * cut.segs + sg] = exp2_of(left);
+    if (!stored || cols <= 0) return;
+    float *const to = SUMS ? mine : a.S + ((size_t)seq.out * a.heads + h) * size;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -611,7 +614,8 @@ __global__ void __launch_bounds__(256) k_linear_join(ornk_linear_args a, Cut cut
 }
 
 // Sequences are cut where their heads and columns leave CUs idle: into parts of at
-// least 128 tokens, until there are two groups for each CU.
+// least 128 tokens, until there are two groups for each CU (one prompt of 8191 tokens, 16
+// heads of 128: 176 us; with one group 196).
 Cut cut_of(const ornk_linear_args &a, int cb)
 {
     const long long groups = (long long)a.n_seqs * a.heads * ((a.dv + 64 * cb - 1) / (64 * cb));
