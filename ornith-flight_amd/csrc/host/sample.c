@@ -41,8 +41,8 @@ int gpu_sample(gpu_context *ctx, gpu_buffer *tokens, gpu_buffer *prob, const gpu
     a.n = n_vocab;
     a.stride = stride;
     /* a token's weight relative to the largest in as many bits as leave 62 for the sum,
-     * and no more than a double has */
-    int bits = 52;
+     * and no more than a double's sum with 2^52 has */
+    int bits = 51;
     while ((size_t)n_vocab > (size_t)1 << (62 - bits)) --bits; /* 42 at the largest */
     a.unit = (double)((uint64_t)1 << bits);
     int prev, rc;

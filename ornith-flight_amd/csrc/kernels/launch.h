@@ -143,7 +143,7 @@ typedef struct {
     float *prob; /* may be NULL */
     int rows, n;
     size_t stride;
-    double unit; /* 2^bits, n * 2^bits < 2^62 */
+    double unit; /* at most 2^51, n * unit at most 2^62 */
     int *err;
     void *ws;
 } ornk_sample_args;

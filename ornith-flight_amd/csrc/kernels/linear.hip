@@ -620,7 +620,7 @@ Cut cut_of(const ornk_linear_args &a, int cb)
 {
     const long long groups = (long long)a.n_seqs * a.heads * ((a.dv + 64 * cb - 1) / (64 * cb));
     long long segs = 512 / groups;
-    if (segs > a.max_len / 128) segs = a.max_len / 128;
+    if (segs > a.max_len / 64) segs = a.max_len / 64;
     Cut c = {1, a.max_len, nullptr, nullptr};
     if (segs < 2) return c;
     c.len = (int)(((a.max_len + segs - 1) / segs + C - 1) / C * C);

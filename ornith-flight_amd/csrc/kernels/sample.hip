@@ -97,12 +97,16 @@ __device__ __forceinline__ int bin_of(const Row &r, float x) { return bin_at(r, 
 // A token's weight, exp((x - largest) / temperature), as a whole number of units.
 __device__ __forceinline__ double weight(const Row &r, float x)
 {
-    if (x == r.top) return 1.0;
+    if (r.top == INFINITY) return x == INFINITY ? 1.0 : 0.0;
     const double y = ((double)x - (double)r.top) * r.per;
     return y > -60.0 ? exp2_of(y) : 0.0;  // also where x is a NaN
 }
 
-__device__ __forceinline__ uint64_t fixed(const Row &r, double w) { return (uint64_t)(w * r.unit + 0.5); }
+// To the nearest whole number, which is at most 2^51: the low bits of its sum with 2^52.
+__device__ __forceinline__ uint64_t fixed(const Row &r, double w)
+{
+    return __double_as_longlong(fma(w, r.unit, 0x1p52)) & 0xfffffffffffffull;
+}
 
 // top_p's share of a sum, as a number of units that the kept tokens reach
 __device__ __forceinline__ uint64_t least_of(const Row &r, uint64_t all)
@@ -1008,7 +1012,15 @@ __global__ void __launch_bounds__(CT) k_sample_choose(ornk_sample_args a, Slices
     }
     scale_row(r, e, r.by_rank ? bound : 0);
     k.list[tid] = mine;
-    for (int i = tid + CT; i < min((int)m, CAP); i += CT) k.list[i] = list[i];
+#pragma unroll 1
+    for (int i = tid + CT; i < min((int)m, CAP); i += 8 * CT) {
+        uint64_t t[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = list[min(i + CT * j, CAP - 1)];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (i + CT * j < CAP) k.list[i + CT * j] = t[j];
+    }
     if (!r.by_rank) bins.put(r, b);
     __syncthreads();
     choose(a, row, r, b, fine, parts, k, m);

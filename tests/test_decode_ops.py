@@ -239,7 +239,7 @@ def test_host_sample(host):
         return h.call("gpu_sample", a)
 
     h.L.decode_unit.restype = C.c_double
-    assert call() == (0, 1) and h.L.decode_unit() == 2.0 ** 52
+    assert call() == (0, 1) and h.L.decode_unit() == 2.0 ** 51
     assert call(prob=None) == (0, 1)
     assert call(rows=0) == (0, 0)
     assert call(rows=4, stride=120) == (0, 1)
@@ -258,7 +258,7 @@ def test_host_sample(host):
     for vocab in (1, 1023, 1024, 1025, 248320, 1 << 20):
         assert call(rows=1, vocab=vocab, logits=h.buf(vocab * 4)) == (0, 1)
         assert vocab * h.L.decode_unit() <= 2.0 ** 62
-        assert h.L.decode_unit() == 2.0 ** 52 or vocab * h.L.decode_unit() >= 2.0 ** 61
+        assert h.L.decode_unit() == 2.0 ** 51 or vocab * h.L.decode_unit() >= 2.0 ** 61
 
 
 def test_host_reports_and_keeps_the_device(host, om):
