@@ -60,8 +60,8 @@ struct Row {
     float top;     // the largest logit
     double per;    // log2(e) / temperature
     double unit;   // weights are whole multiples of 1 / unit; n of them fit 62 bits
-    float scale;   // bins per logit
-    float reach;   // tokens farther below the largest are behind every border
+    float scale;   // bins to `below`
+    float reach;   // tokens farther below are behind every border
     bool by_rank;  // the top_k are few: all of them are listed
 };
 
@@ -79,11 +79,12 @@ __device__ __forceinline__ Row row_of(const ornk_sample_args &a, int row)
     return r;
 }
 
-// How far below a row's largest logit another lies; for a NaN a NaN.
+// Half of how far below a row's largest logit another lies (the whole may pass the largest
+// number); for a NaN a NaN.
 __device__ __forceinline__ float below(const Row &r, float x)
 {
     if (r.top == INFINITY) return x == INFINITY ? 0.0f : INFINITY;
-    return r.top - x;
+    return fmaf(-0.5f, x, 0.5f * r.top);
 }
 
 __device__ __forceinline__ int bin_at(const Row &r, float below)
@@ -142,7 +143,7 @@ __device__ __forceinline__ Ends wave_ends(Ends e)
 
 // What the weights and bins need, and how far below the largest a border of the choice
 // may lie, which is where the bins end:
-// - a weight below 2^-53 of the largest is 0;
+// - a weight below 2^-53 of the largest (37 temperatures) is 0;
 // - the tokens below (1 - top_p) / 2 n are less than half of what top_p leaves out;
 // - min_p leaves out what is below it.
 // Where the top_k are few, `bound` is a key that as many tokens have or pass (0: none is
@@ -152,12 +153,12 @@ __device__ __forceinline__ void scale_row(Row &r, Ends e, uint32_t bound)
     const float T = r.q.temperature;
     r.top = e.top;
     r.per = 1.4426950408889634 / (double)T;
-    r.reach = fminf(37.0f * T, 3.4028234e38f);
+    r.reach = fminf(18.5f * T, 3.4028234e38f);
     if (r.by_rank) {
         if (bound) r.reach = fminf(r.reach, below(r, logit_of(bound)));
     } else if (r.q.top_k <= 0 || r.q.top_k >= r.n) {
-        if (r.q.top_p < 1.0f) r.reach = fminf(r.reach, -logf((1.0f - r.q.top_p) / (2.0f * r.n)) * T * 1.0001f);
-        if (r.q.min_p > 0.0f) r.reach = fminf(r.reach, -logf(r.q.min_p) * T * 1.0001f);
+        if (r.q.top_p < 1.0f) r.reach = fminf(r.reach, -logf((1.0f - r.q.top_p) / (2.0f * r.n)) * T * 0.50005f);
+        if (r.q.min_p > 0.0f) r.reach = fminf(r.reach, -logf(r.q.min_p) * T * 0.50005f);
     }
     const float range = fminf(below(r, e.low), r.reach), s = (float)NB / range;
     r.scale = range > 0.0f ? fminf(s, 1e30f) : 0.0f;
@@ -276,7 +277,7 @@ __device__ __forceinline__ void mark_bins(const Row &r, Bins &s, bool counted, i
     __syncthreads();
 }
 
-__device__ __forceinline__ float min_below(const Row &r) { return -logf(r.q.min_p) * r.q.temperature; }
+__device__ __forceinline__ float min_below(const Row &r) { return -logf(r.q.min_p) * r.q.temperature * 0.5f; }
 
 __device__ __forceinline__ bool is_marked(const Bins &s, int bin) { return s.marked[bin >> 5] >> (bin & 31) & 1; }
 
@@ -594,7 +595,9 @@ __device__ __forceinline__ void choose(const ornk_sample_args &a, int row, const
         for (int i = tid; i < (int)m; i += CT) {
             const float x = logit_of((uint32_t)(s.list[i] >> 32));
             const int bin = fine_at(r, b, f, below(r, x));
-            atomicAdd((unsigned long long *)&c.w[bin], (unsigned long long)fixed(r, weight(r, x)));
+            const uint64_t v = fixed(r, weight(r, x));
+            if (!v) continue;
+            atomicAdd((unsigned long long *)&c.w[bin], (unsigned long long)v);
             atomicAdd(&c.c[bin], 1u);
         }
         __syncthreads();
@@ -695,8 +698,12 @@ __device__ __forceinline__ void fill_bins(const Row &r, int i0, int end, uint64_
         r, i0, end,
         [&](float x, int) {
             const int bin = bin_of(r, x);
+            if (!r.by_rank) {
+                const uint64_t v = fixed(r, weight(r, x));
+                if (!v) return;
+                atomicAdd((unsigned long long *)&w[bin], (unsigned long long)v);
+            }
             if (r.q.top_k > 0) atomicAdd(&c[bin], 1u);
-            if (!r.by_rank) atomicAdd((unsigned long long *)&w[bin], (unsigned long long)fixed(r, weight(r, x)));
         },
         [&](float x) {
             if (sums) rest += fixed(r, weight(r, x));

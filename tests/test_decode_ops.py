@@ -817,6 +817,22 @@ def test_sample_with_a_large_top_k(om, ctx, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [9000, 40000])
+def test_sample_where_weights_end(om, ctx, n):
+    """More tokens of the top_k than have a weight; logits farther apart than the largest number."""
+    g = np.random.default_rng(n)
+    x = np.full((6, n), -80.0, np.float32)
+    x[:, 0] = 0.0
+    x[:4, 10:1000] = -30.0 - 0.001 * g.random((4, 990))
+    x[:4, 1000:8000] = -36.6 - 0.1 * g.random((4, 7000))  # 2^-53 of the largest
+    x[4] = np.where(g.random(n) < 0.5, -3e38, 3e38)
+    x[5] = np.linspace(-3.4e38, 3.4e38, n)
+    requests = [(1.0, 3000, 1.0, 0.0), (1.0, 300, 0.9999999, 0.0), (1.0, 0, 1.0, 0.0), (1.0, 1000, 0.9, 0.0),
+                (1e38, 0, 1.0, 0.0), (2e38, 0, 0.9, 0.01)]
+    _check_sample(om, ctx, x, requests, np.array([0.3, 0.99, 0.999999, 0.5, 0.999, 0.9], np.float32))
+
+
+@pytest.mark.gpu
 def test_sample_of_special_rows(om, ctx):
     n = 300
     g = np.random.default_rng(3)
@@ -884,3 +900,206 @@ def test_sample_repeats(om, ctx):
     for _ in range(3):
         again = _sample(om, ctx, x, REQUESTS, u)
         assert np.array_equal(first[0], again[0]) and np.array_equal(first[1], again[1])
+
+
+# ---------------------------------------- together, and at the limits
+def _unit(x, eps=1e-6):
+    return _norm64(x, None, "l2", eps)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("flags", ["sync", "async"])
+def test_decode_loop(om, ctx, flags):
+    """A hybrid stack's loop: prompts and then tokens through a linear layer (unit queries and
+    keys, states in slots) and an attention layer (normed, rotated and appended; attended),
+    the LM head's product and a sampled token for each sequence, whose row of an embedding is the
+    next input.  Against 64 bits, the tokens being the device's own."""
+    F = om.KV_ASYNC if flags == "async" else 0
+    g = torch.Generator().manual_seed(11)
+    B, H, kv, D, V, page, steps = 3, 4, 2, 32, 400, 8, 5
+    lens = [37, 5, 70]
+    W = H * D
+    emb, head = torch.randn(V, W, generator=g), torch.randn(W, V, generator=g) * 0.3
+    qw, kw = 1 + 0.2 * torch.randn(1, D, generator=g), 1 + 0.2 * torch.randn(1, D, generator=g)
+    rate = -torch.rand(H, generator=g)
+    width = -(-(max(lens) + steps) // page)
+    table = torch.randperm(B * width, generator=g).view(B, width).to(torch.int32)
+    kp, vp, S = (ctx.alloc(B * width * kv * page * D * 4), ctx.alloc(B * width * kv * page * D * 4),
+                 ctx.alloc((B + 1) * H * D * D * 4))
+    pages = om.kv_pages(kp, vp, "f32", B * width, page, kv, D)
+    states = om.linear_states(S, B + 1, H, D, D)
+    rope = om.rope_axes([12], 1e4, halves=True)
+    slots = torch.tensor([3, 0, 2], dtype=torch.int32)
+    none = torch.full((B,), -1, dtype=torch.int32)
+    tb, qwb, kwb, rb, slb, nb, headb = _up(ctx, table, qw, kw, rate, slots, none, head)
+    norm, unit = om.head_norm("rms", 1e-6, qwb, kwb), om.head_norm("l2", 1e-6)
+    requests = np.array([(0.8, 40, 0.95, 0.0), (1.0, 0, 0.9, 0.02), (0.0, 0, 1.0, 0.0)], om.SAMPLE_REQUEST)
+    reqb = ctx.upload(requests)
+
+    # 64 bits: a sequence's own state and cache
+    S64 = torch.zeros(B, H, D, D, dtype=torch.float64)
+    K64, V64 = [torch.zeros(0, kv, D, dtype=torch.float64) for _ in range(B)], [torch.zeros(0, kv, D, dtype=torch.float64) for _ in range(B)]
+
+    tokens = [torch.randint(0, V, (n,), generator=g) for n in lens]
+    done = [0] * B
+    for step in range(steps):
+        x = torch.cat([emb[t] for t in tokens]).view(-1, H, D)  # the layers' projections
+        n = [len(t) for t in tokens]
+        T = sum(n)
+        pos = torch.cat([torch.arange(d, d + m) for d, m in zip(done, n)]).to(torch.int32)
+        at = torch.cat([table[b, (torch.arange(d, d + m) // page)] * page + torch.arange(d, d + m) % page
+                        for b, (d, m) in enumerate(zip(done, n))]).to(torch.int32)
+        starts = torch.tensor([sum(n[:b]) for b in range(B + 1)], dtype=torch.int32)
+        k2 = x[:, :kv].contiguous()
+        xb, k2b, pb, ab, stb, lb = _up(ctx, x, k2, pos, at, starts,
+                                       torch.tensor([d + m for d, m in zip(done, n)], dtype=torch.int32))
+        uq, uk, lin, q2 = (ctx.alloc(T * W * 4) for _ in range(4))
+        om.norm_rope_axes(ctx, uq, uk, xb, xb, T, H, H, D, unit, flags=F)
+        om.linear_attend(ctx, states, lin, uq, uk, xb, H, H, H, T, rb, B, stb if step == 0 else None,
+                         nb if step == 0 else slb, slb, om.linear_opts(max_len=max(n), flags=F))
+        om.norm_kv_append(ctx, pages, k2b, k2b, T, ab, q2, xb, H, norm, pb, rope, flags=F)
+        last = starts[1:].long() - 1
+        if step == 0:  # the last token's query of each prompt
+            ctx.check(om.lib().gpu_kv_check(ctx.ptr), "check")
+            qb = _up(ctx, _down(ctx, q2, (T, H, D))[last])[0]
+        else:
+            qb = q2
+        att, logits, tok, prob = ctx.alloc(B * W * 4), ctx.alloc(B * V * 4), ctx.alloc(B * 4), ctx.alloc(B * 4)
+        om.kv_attend(ctx, pages, att, qb, B, H, tb, width, lb, om.attend_opts(flags=F))
+        ctx.check(om.lib().gpu_kv_check(ctx.ptr), "check")
+        y = _down(ctx, lin, (T, H, D))[last] + _down(ctx, att, (B, H, D))
+        yb = _up(ctx, y)[0]
+        om.lib().gpu_matmul(ctx.ptr, logits.ptr, yb.ptr, headb.ptr, B, V, W, 0, 0)
+        u = torch.rand(B, generator=g)
+        ub = _up(ctx, u)[0]
+        om.sample(ctx, tok, prob, logits, B, V, reqb, ub, flags=F)
+        ctx.check(om.lib().gpu_kv_check(ctx.ptr), "check")
+        got = _down(ctx, tok, (B,), torch.int32)
+
+        # the same in 64 bits
+        x64 = x.double()
+        uq64 = _unit(x64)
+        lin64 = torch.zeros(T, H, D, dtype=torch.float64)
+        qn, _ = _rope64(_norm64(x, qw, "rms", 1e-6), [12], 1e4, True, pos[None], 0)
+        kn, _ = _rope64(_norm64(k2, kw, "rms", 1e-6), [12], 1e4, True, pos[None], 0)
+        att64 = torch.zeros(B, H, D, dtype=torch.float64)
+        for b in range(B):
+            for t in range(int(starts[b]), int(starts[b + 1])):
+                S64[b] = S64[b] * torch.exp(rate.double())[:, None, None] + uq64[t][:, :, None] * x64[t][:, None]
+                lin64[t] = (S64[b] * uq64[t][:, :, None]).sum(1) / math.sqrt(D)
+            rows = slice(int(starts[b]), int(starts[b + 1]))
+            K64[b], V64[b] = torch.cat([K64[b], kn[rows]]), torch.cat([V64[b], k2[rows].double()])
+            for h in range(H):
+                w = torch.softmax(K64[b][:, h // 2] @ qn[last[b], h] / math.sqrt(D), 0)
+                att64[b, h] = w @ V64[b][:, h // 2]
+        # each part's own bound (of heads of 32, up to 75 tokens; values of a few units)
+        assert (y.double() - (lin64[last] + att64)).abs().max() < 2e-5
+        shown = _down(ctx, logits, (B, V)).numpy()
+        for b in range(B):
+            assert int(got[b]) in _choices(shown[b], *[r.item() for r in requests[b]], u[b].item())
+        done = [d + m for d, m in zip(done, n)]
+        tokens = [got[b:b + 1].long() for b in range(B)]
+    ends = _down(ctx, S, (B + 1, H, D, D))[slots.long()]
+    assert (ends.double() - S64).abs().max() < 2e-5
+
+
+@pytest.mark.gpu
+def test_two_contexts_at_once(om, ctx):
+    """Calls of two contexts in flight together, each with its own workspace."""
+    other = om.Context()
+    try:
+        H, D, L, n = 4, 64, 1500, 50000
+        g, q, k, v, decay = _linear_inputs([L], H, H, H, H, D, D, "token", 21)
+        x = torch.randn(4, n, generator=g)
+        u = torch.rand(4, generator=g)
+        requests = np.array([REQUESTS[i] for i in (0, 1, 3, 5)], om.SAMPLE_REQUEST)
+        results = []
+        for together in (False, True):
+            got = []
+            work = []
+            for c in (ctx, other):
+                b = _up(c, q, k, v, decay, x, u) + [c.upload(requests)]
+                work.append((c, b, c.alloc(L * H * D * 4), c.alloc(16), c.alloc(16)))
+            for rep in range(3):
+                for c, b, out, tok, prob in work:
+                    F = om.KV_ASYNC if together else 0
+                    om.linear_attend(c, om.linear_states(None, 0, H, D, D), out, *b[:3], H, H, H, L, b[3], 1,
+                                     _up(c, torch.tensor([0, L], dtype=torch.int32))[0], None, None,
+                                     om.linear_opts(per_token=True, flags=F))
+                    om.sample(c, tok, prob, b[4], 4, n, b[6], b[5], flags=F)
+            for c, b, out, tok, prob in work:
+                c.check(om.lib().gpu_kv_check(c.ptr), "check")
+                got.append((_down(c, out, (L, H, D)), _down(c, tok, (4,), torch.int32), _down(c, prob, (4,))))
+            results += got
+        for r in results[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(results[0], r))
+    finally:
+        other.close()
+
+
+@pytest.mark.gpu
+def test_many_sequences_and_rows(om, ctx):
+    """More sequences than are ordered by length, as many as there may be, as many rows."""
+    _check_linear(om, ctx, [(b * 37) % 70 for b in range(300)], 1, 1, 1, 1, 16, 16, seed=1)
+    B = 65535
+    q, k, v = (torch.arange(B, dtype=torch.float32).view(B, 1, 1) % m for m in (7, 5, 3))
+    bufs = _up(ctx, q, k, v, torch.zeros(1))
+    out = ctx.alloc(B * 4)
+    om.linear_attend(ctx, om.linear_states(None, 0, 1, 1, 1), out, *bufs[:3], 1, 1, 1, B, bufs[3], B,
+                     opts=om.linear_opts(scale=1.0))
+    assert torch.equal(_down(ctx, out, (B, 1, 1)), q * k * v)
+    x = (torch.arange(B * 5) % 7).float().view(B, 5)
+    r = np.zeros(B, om.SAMPLE_REQUEST)
+    r["top_p"] = 1.0
+    xb, ub, rb, tok = ctx.upload(x.numpy()), ctx.alloc(B * 4), ctx.upload(r), ctx.alloc(B * 4)
+    om.sample(ctx, tok, None, xb, B, 5, rb, ub)
+    assert torch.equal(_down(ctx, tok, (B,), torch.int32).long(), x.argmax(1))
+
+
+@pytest.mark.gpu
+def test_more_tokens_than_groups(om, ctx):
+    """Heads of more tokens than a launch has groups."""
+    T = (1 << 20) + 77
+    x = torch.randn(T, 1, 4, generator=torch.Generator().manual_seed(3))
+    xb = _up(ctx, x)[0]
+    out = ctx.alloc(T * 16)
+    om.norm_rope_axes(ctx, out, None, xb, None, T, 1, 0, 4, om.head_norm("rms"))
+    want = _norm64(x, None, "rms", 1e-6)
+    _close(_down(ctx, out, x.shape), want, want.abs() * (4 / 64 + 16) * EPS)
+
+
+@pytest.mark.gpu
+def test_states_and_logits_past_4_gb(om, ctx):
+    H, D = 64, 256
+    n_slots = (5 << 30) // (H * D * D * 4)
+    S = ctx.alloc(n_slots * H * D * D * 4)
+    for L in (1, 40):
+        g, q, k, v, decay = _linear_inputs([L], H, 1, 1, 1, D, D, "head", L)
+        ib, ob = _up(ctx, torch.tensor([n_slots - 1], dtype=torch.int32), torch.tensor([n_slots - 2], dtype=torch.int32))
+        bufs = _up(ctx, q, k, v, decay)
+        out = ctx.alloc(L * H * D * 4)
+        om.linear_attend(ctx, om.linear_states(S, n_slots, H, D, D), out, *bufs[:3], 1, 1, 1, L, bufs[3], 1,
+                         _up(ctx, torch.tensor([0, L], dtype=torch.int32))[0], ib, ob)
+        want, bound, ends, _ = _linear64(q, k, v, decay, [0, L], torch.zeros(1, H, D, D), D ** -0.5, False)
+        c = (8 + 6 * math.sqrt(2 * L + D)) * EPS
+        _close(_down(ctx, out, (L, H, D)), want, bound * c + 1e-37)
+        # the state, seen by another token that starts from it
+        one = torch.zeros(1, 1, D)
+        qb, kb = _up(ctx, q[:1], one)
+        out = ctx.alloc(H * D * 4)
+        om.linear_attend(ctx, om.linear_states(S, n_slots, H, D, D), out, qb, kb, kb, 1, 1, 1, 1,
+                         _up(ctx, torch.zeros(H))[0], 1, None, ob, None)
+        got = _down(ctx, out, (1, H, D))
+        want = (ends[0] * q[0].double()[:, :, None]).sum(1) * D ** -0.5
+        _close(got[0], want, (ends[0].abs() * q[0].double().abs()[:, :, None]).sum(1) * D ** -0.5 * 2 * c + 1e-37)
+    S.free()
+    rows, stride = 1200, 1 << 20
+    xb = ctx.alloc(rows * stride * 4)  # zeros
+    r = np.zeros(rows, om.SAMPLE_REQUEST)
+    r["temperature"], r["top_p"] = 1.0, 1.0
+    u = np.linspace(0, 0.999, rows).astype(np.float32)
+    rb, ub, tok = ctx.upload(r), ctx.upload(u), ctx.alloc(rows * 4)
+    om.sample(ctx, tok, None, xb, rows, 1000, rb, ub, stride=stride)
+    xb.free()
+    got = ctx.download(tok, np.int32, (rows,))
+    assert np.abs(got - u.astype(np.float64) * 1000).max() <= 1.0 and (got == np.floor(u.astype(np.float64) * 1000)).mean() > 0.99
