@@ -40,7 +40,9 @@ __device__ __forceinline__ Seq seq_of(const ornk_linear_args &a, int b)
 
 // One token of each sequence (or none): V columns per lane, L lanes to a row of the
 // state, 256 / L rows at a time and up to 16 of them in flight per thread.  q and k come
-// through LDS, and the row groups' shares of q S meet there.
+// through LDS, and the row groups' shares of q S meet there.  Bound by memory, the state in
+// and out: 64 sequences of 32 heads of 128 x 128 move 272 MB in 59 us (4.6 TB/s; a copy 5.1),
+// one 6.7 us.
 template <int V, int L>
 __global__ void __launch_bounds__(256) k_linear_step(ornk_linear_args a)
 {
@@ -108,8 +110,8 @@ __global__ void __launch_bounds__(256) k_linear_step(ornk_linear_args a)
     }
 }
 
-// Whole heads in a group (64 KB of state at 128 x 128) where that gives every CU two of
-// them, else in groups of 32 columns.
+// Groups of 128 columns where that gives every CU two of them, else of 32 (one sequence of
+// 32 heads of 128: 11.0 us in groups of 64 columns, 6.7).
 template <int V, int L>
 void launch_step(const ornk_linear_args &a, hipStream_t s)
 {
@@ -130,6 +132,13 @@ void launch_step(const ornk_linear_args &a, hipStream_t s)
 // LDS.  P has three blocks of 16 x 16 (keys and queries of the first half, first and
 // second, of the second), one for each of three waves; the fourth sums the next chunk's
 // decays meanwhile.
+//
+// Bound by the matrix cores, which take 15 ns for an fp32 16x16x4 product of a SIMD (140
+// TFLOP/s; vector instructions beside it wait for it) and are busy 68 % of the time: 24 x
+// up to 1501 tokens, 32 heads of 128 (18,210 tokens in all) 432 us, 89 TFLOP/s of the
+// recurrence's and 104 of what is computed; C = 32 costs 19 % more than the recurrence
+// (P, P V), 64 would cost 50 % and save no wait that a second group does not hide.  Eight
+// waves of 16 columns instead of four of 32: 703 us then, against 557.
 constexpr int C = 32;
 
 struct alignas(16) Decays {
@@ -252,7 +261,8 @@ __device__ __forceinline__ void add_in_order(v4f (&O)[CB], v4f P, const float (&
 }
 
 // The sequence of rank `rank` by length, the longest first: groups that start late are
-// then short ones.  Up to 256 sequences; of more the order makes little difference.
+// then short ones (24 x up to 1501 tokens 557 -> 449 us).  Up to 256 sequences; of more the
+// order makes little difference.
 __device__ __forceinline__ int by_length(const ornk_linear_args &a, int rank, int *lens)
 {
     if (!a.starts || a.n_seqs > 256) return rank;
@@ -595,7 +605,8 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
         }
 }
 
-// From what each part adds to what each part begins with, an element per thread.
+// From what each part adds to what each part begins with, an element per thread (16 heads
+// of 128 x 128 in 32 parts 15 us, 67 MB).
 __global__ void __launch_bounds__(256) k_linear_join(ornk_linear_args a, Cut cut)
 {
     const int b = blockIdx.x, h = blockIdx.y, e = blockIdx.z * 256 + threadIdx.x;
@@ -614,8 +625,11 @@ __global__ void __launch_bounds__(256) k_linear_join(ornk_linear_args a, Cut cut
 }
 
 // Sequences are cut where their heads and columns leave CUs idle: into parts of at
-// least 128 tokens, until there are two groups for each CU (one prompt of 8191 tokens, 16
-// heads of 128: 176 us; with one group 196).
+// least 64 tokens, until there are two groups for each CU.  What the parts add to a state
+// is formed first, and their tokens after that from what they begin with, which takes 1.4
+// times the products.  One prompt of 8191 tokens, 16 heads of 128: 176 us (sums 57, joining
+// 15, tokens 115); with one group for each CU 196.  5 x 333, 12 heads of 96 x 80: 45; with
+// parts of 128 tokens 50.
 Cut cut_of(const ornk_linear_args &a, int cb)
 {
     const long long groups = (long long)a.n_seqs * a.heads * ((a.dv + 64 * cb - 1) / (64 * cb));
@@ -629,7 +643,9 @@ Cut cut_of(const ornk_linear_args &a, int cb)
 }
 
 // Blocks of 16 columns of a wave: two, where there is then a group for each CU, and the
-// state's registers leave room for another group.
+// state's registers leave room for another group.  Two share a group's P and its waits (one
+// prompt of 8191 tokens, 16 heads of 128: 176 us, with one block 198); one gives twice the
+// groups (5 x 333, 12 heads of 96 x 80: 53, with two 74).
 int blocks_of(const ornk_linear_args &a)
 {
     if (a.dv <= 64 || a.dk > 128) return 1;
