@@ -17,7 +17,7 @@ namespace {
 
 constexpr int NB = 1024;   // bins of a row's logits
 constexpr int CAP = 4096;  // tokens of a row that are listed
-constexpr int ST = 1024;   // threads of a group that goes over logits
+constexpr int ST = 1024;   // threads of a group that has a row
 constexpr int CT = 256;    // those of them that work on bins and on a list: with more waves
                            // the same steps wait for each other's instructions
 
@@ -652,11 +652,12 @@ __device__ __forceinline__ v4f load4(const float *x, int n, int i)
     return y;
 }
 
+template <int NT>
 __device__ __forceinline__ Ends ends_of(const float *x, int i0, int end)
 {
     Ends e = {-INFINITY, INFINITY};
 #pragma unroll 4
-    for (int i = i0 + 4 * (int)threadIdx.x; i < end; i += 4 * ST) {
+    for (int i = i0 + 4 * (int)threadIdx.x; i < end; i += 4 * NT) {
         const v4f y = load4(x, end, i);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -669,16 +670,16 @@ __device__ __forceinline__ Ends ends_of(const float *x, int i0, int end)
 
 // f(logit, token) of those within reach, g(logit) of the others; one copy of each in a
 // loop, the next float4 on its way.
-template <class F, class G>
+template <int NT, class F, class G>
 __device__ __forceinline__ void each_token(const Row &r, int i0, int end, F f, G g)
 {
     int i = i0 + 4 * (int)threadIdx.x;
     if (i >= end) return;
     v4f next = load4(r.x, end, i);
 #pragma unroll 1
-    for (; i < end; i += 4 * ST) {
+    for (; i < end; i += 4 * NT) {
         v4f y = next;
-        if (i + 4 * ST < end) next = load4(r.x, end, i + 4 * ST);
+        if (i + 4 * NT < end) next = load4(r.x, end, i + 4 * NT);
 #pragma unroll 1
         for (int j = 0; j < 4; ++j) {
             if (below(r, y[0]) <= r.reach) f(y[0], i + j);
@@ -690,11 +691,12 @@ __device__ __forceinline__ void each_token(const Row &r, int i0, int end, F f, G
 
 // Into the bins of w and c, which are in LDS.  What is out of reach belongs to the sum
 // that top_p is a share of, behind all bins' tokens.
+template <int NT>
 __device__ __forceinline__ void fill_bins(const Row &r, int i0, int end, uint64_t *w, uint32_t *c)
 {
     uint64_t rest = 0;
     const bool sums = !r.by_rank && r.q.top_p < 1.0f;
-    each_token(
+    each_token<NT>(
         r, i0, end,
         [&](float x, int) {
             const int bin = bin_of(r, x);
@@ -714,11 +716,11 @@ __device__ __forceinline__ void fill_bins(const Row &r, int i0, int end, uint64_
 }
 
 // Those in marked bins, or (b is NULL) all within reach: f(key << 32 | token).
-template <class F>
+template <int NT, class F>
 __device__ __forceinline__ void gather(const Row &r, const Bins *b, int i0, int end, F f)
 {
     const float last = b && b->last < NB - 1 ? (float)(b->last + 1) : INFINITY;
-    each_token(
+    each_token<NT>(
         r, i0, end,
         [&](float x, int i) {
             if (!b || (below(r, x) * r.scale < last && is_marked(*b, bin_of(r, x))))
@@ -769,10 +771,11 @@ __device__ __forceinline__ uint32_t kth_largest(const uint32_t (&key)[P], uint32
 }
 
 // The first token that has the largest logit.
+template <int NT>
 __device__ __forceinline__ void first_of(const Row &r, float top, int i0, int end, uint32_t *first)
 {
 #pragma unroll 1
-    for (int i = i0 + (int)threadIdx.x; i < end; i += ST)
+    for (int i = i0 + (int)threadIdx.x; i < end; i += NT)
         if (r.x[i] == top) {
             atomicMin(first, (uint32_t)i);
             return;
@@ -792,7 +795,7 @@ __global__ void __launch_bounds__(ST) k_sample_row(ornk_sample_args a)
         if (!tid) *(volatile int *)(a.err + ORNK_KV_ERR_SAMPLE) = 1 + row, put_result(a, row, -1, 0.0f);
         return;
     }
-    const Ends own = ends_of(r.x, 0, r.n);
+    const Ends own = ends_of<ST>(r.x, 0, r.n);
     Ends e = wave_ends(own);
     if (!(tid & 63)) ends[tid >> 6] = e;
     if (!tid) s.count = r.q.temperature == 0.0f ? ~0u : 0;
@@ -803,7 +806,7 @@ __global__ void __launch_bounds__(ST) k_sample_row(ornk_sample_args a)
         return;
     }
     if (r.q.temperature == 0.0f) {
-        first_of(r, e.top, 0, r.n, &s.count);
+        first_of<ST>(r, e.top, 0, r.n, &s.count);
         __syncthreads();
         if (!tid) put_result(a, row, (int)s.count, 1.0f);
         return;
@@ -817,12 +820,12 @@ __global__ void __launch_bounds__(ST) k_sample_row(ornk_sample_args a)
     if (!bound) {
         for (int i = tid; i < NB; i += ST) b.w[i] = 0, b.c[i] = 0;
         __syncthreads();
-        fill_bins(r, 0, r.n, b.w, b.c);
+        fill_bins<ST>(r, 0, r.n, b.w, b.c);
         __syncthreads();
         sums_before(b);
         mark_bins(r, b, r.by_rank, bin_at(r, min_below(r)));
     }
-    gather(r, bound ? nullptr : &b, 0, r.n, [&](uint64_t t) {
+    gather<ST>(r, bound ? nullptr : &b, 0, r.n, [&](uint64_t t) {
         const uint32_t at = atomicAdd(&s.count, 1u);
         if (at < CAP) s.list[at] = t;
     });
@@ -833,12 +836,13 @@ __global__ void __launch_bounds__(ST) k_sample_row(ornk_sample_args a)
 }
 
 // ---- longer rows: in slices ------------------------------------------------------
+constexpr int SL = 512;  // threads of a slice's group: 64 rows of 248,320 take 68 us, with 1024 or 256 73
 constexpr int MAX_SLICES = 256;
 constexpr int MAX_TOPS = 4096;
 
 // Work buffers of a row.
 struct Slices {
-    int n, len;       // number of a row's slices, their tokens (a multiple of 4 * ST)
+    int n, len;       // number of a row's slices, their tokens (a multiple of 4 * SL)
     int per;          // parts of a slice whose largest keys are kept: 1 << per threads have one
     Ends *ends;       // [rows][n]
     uint64_t *w;      // [rows][NB]
@@ -851,24 +855,24 @@ struct Slices {
 };
 
 // The slices' ends and largest keys; the row's bins and list emptied.
-__global__ void __launch_bounds__(ST) k_sample_ends(ornk_sample_args a, Slices s)
+__global__ void __launch_bounds__(SL) k_sample_ends(ornk_sample_args a, Slices s)
 {
-    __shared__ Ends tmp[ST / 64];
+    __shared__ Ends tmp[SL / 64];
     const int row = blockIdx.y, tid = threadIdx.x, i0 = blockIdx.x * s.len;
-    for (int i = blockIdx.x * ST + tid; i < NB; i += s.n * ST) {
+    for (int i = blockIdx.x * SL + tid; i < NB; i += s.n * SL) {
         s.w[(size_t)row * NB + i] = 0;
         s.c[(size_t)row * NB + i] = 0;
     }
     if (!blockIdx.x && !tid) s.count[row] = 0, s.first[row] = ~0u;
-    const Ends own = ends_of(a.logits + (size_t)row * a.stride, i0, min(i0 + s.len, a.n));
+    const Ends own = ends_of<SL>(a.logits + (size_t)row * a.stride, i0, min(i0 + s.len, a.n));
     float top = own.top;
     for (int o = 1; o < 1 << s.per; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
     if (!(tid & ((1 << s.per) - 1)))
-        s.tops[(size_t)row * MAX_TOPS + blockIdx.x * (ST >> s.per) + (tid >> s.per)] = key_of(top);
+        s.tops[(size_t)row * MAX_TOPS + blockIdx.x * (SL >> s.per) + (tid >> s.per)] = key_of(top);
     Ends e = wave_ends(own);
     if (!(tid & 63)) tmp[tid >> 6] = e;
     __syncthreads();
-    for (int i = 0; i < ST / 64; ++i) e = join(e, tmp[i]);
+    for (int i = 0; i < SL / 64; ++i) e = join(e, tmp[i]);
     if (!tid) s.ends[(size_t)row * s.n + blockIdx.x] = e;
 }
 
@@ -890,7 +894,7 @@ __device__ __forceinline__ Ends row_ends(Ends e, Ends *tmp)
     return e;
 }
 
-__global__ void __launch_bounds__(ST) k_sample_bins(ornk_sample_args a, Slices s)
+__global__ void __launch_bounds__(SL) k_sample_bins(ornk_sample_args a, Slices s)
 {
     __shared__ uint64_t w[NB];
     __shared__ uint32_t c[NB];
@@ -899,13 +903,13 @@ __global__ void __launch_bounds__(ST) k_sample_bins(ornk_sample_args a, Slices s
     Row r = row_of(a, row);
     const Ends own = own_ends(s, row);
     if (!r.valid || r.q.temperature == 0.0f) return;
-    const int tops = s.n * (ST >> s.per);
+    const int tops = s.n * (SL >> s.per);
     uint32_t bound = 0;
     if (r.by_rank && r.q.top_k <= tops) {
-        uint32_t key[MAX_TOPS / ST];
+        uint32_t key[MAX_TOPS / SL];
 #pragma unroll
-        for (int i = 0; i < MAX_TOPS / ST; ++i)
-            key[i] = tid + ST * i < tops ? s.tops[(size_t)row * MAX_TOPS + tid + ST * i] : 0;
+        for (int i = 0; i < MAX_TOPS / SL; ++i)
+            key[i] = tid + SL * i < tops ? s.tops[(size_t)row * MAX_TOPS + tid + SL * i] : 0;
         bound = kth_largest(key, r.q.top_k, c);
     }
     if (!blockIdx.x && !tid) s.bound[row] = bound;
@@ -913,11 +917,11 @@ __global__ void __launch_bounds__(ST) k_sample_bins(ornk_sample_args a, Slices s
     const Ends e = row_ends(own, tmp);
     if (!(e.top > -INFINITY)) return;
     scale_row(r, e, 0);
-    for (int i = tid; i < NB; i += ST) w[i] = 0, c[i] = 0;
+    for (int i = tid; i < NB; i += SL) w[i] = 0, c[i] = 0;
     __syncthreads();
-    fill_bins(r, i0, min(i0 + s.len, a.n), w, c);
+    fill_bins<SL>(r, i0, min(i0 + s.len, a.n), w, c);
     __syncthreads();
-    for (int i = tid; i < NB; i += ST) {
+    for (int i = tid; i < NB; i += SL) {
         if (w[i]) atomicAdd((unsigned long long *)&s.w[(size_t)row * NB + i], (unsigned long long)w[i]);
         if (c[i]) atomicAdd(&s.c[(size_t)row * NB + i], c[i]);
     }
@@ -952,7 +956,7 @@ struct OwnBins {
 // The tokens in marked bins, or those that pass the bound, to the row's list: those of a
 // group together, as long as LDS holds them (an atomic of its own for each token took 110
 // us for 16 rows of 2000).
-__global__ void __launch_bounds__(ST) k_sample_gather(ornk_sample_args a, Slices s)
+__global__ void __launch_bounds__(SL) k_sample_gather(ornk_sample_args a, Slices s)
 {
     constexpr int MINE = 1024;
     __shared__ Bins b;
@@ -962,13 +966,13 @@ __global__ void __launch_bounds__(ST) k_sample_gather(ornk_sample_args a, Slices
     const int row = blockIdx.y, tid = threadIdx.x, i0 = blockIdx.x * s.len, end = min(i0 + s.len, a.n);
     Row r = row_of(a, row);
     const Ends own = own_ends(s, row);
-    const OwnBins<ST> bins(s, row);
+    const OwnBins<SL> bins(s, row);
     const uint32_t bound = s.bound[row];
     if (!r.valid) return;
     const Ends e = row_ends(own, tmp);
     if (!(e.top > -INFINITY)) return;
     if (r.q.temperature == 0.0f) {
-        if (s.ends[(size_t)row * s.n + blockIdx.x].top == e.top) first_of(r, e.top, i0, end, &s.first[row]);
+        if (s.ends[(size_t)row * s.n + blockIdx.x].top == e.top) first_of<SL>(r, e.top, i0, end, &s.first[row]);
         return;
     }
     scale_row(r, e, r.by_rank ? bound : 0);
@@ -977,7 +981,7 @@ __global__ void __launch_bounds__(ST) k_sample_gather(ornk_sample_args a, Slices
     if (binned) bins.put(r, b);
     __syncthreads();
     uint64_t *list = s.list + (size_t)row * CAP;
-    gather(r, binned ? &b : nullptr, i0, end, [&](uint64_t t) {
+    gather<SL>(r, binned ? &b : nullptr, i0, end, [&](uint64_t t) {
         const uint32_t at = atomicAdd(&count, 1u);
         if (at < MINE) {
             mine[at] = t;
@@ -990,7 +994,7 @@ __global__ void __launch_bounds__(ST) k_sample_gather(ornk_sample_args a, Slices
     const uint32_t m = count < MINE ? count : MINE;
     if (!tid && m) base = atomicAdd(&s.count[row], m);
     __syncthreads();
-    for (uint32_t i = tid; i < m; i += ST)
+    for (uint32_t i = tid; i < m; i += SL)
         if (base + i < CAP) list[base + i] = mine[i];
 }
 
@@ -1037,16 +1041,18 @@ constexpr int ROW_MAX = 32768;  // tokens of a row that one group takes
 
 Slices slices_of(const ornk_sample_args &a)
 {
-    constexpr int UNIT = 4 * ST;
-    const long long want = ((long long)a.rows * a.n / 1536 + UNIT - 1) / UNIT;  // for 1536 groups
+    // 4096 to 32768 tokens each, for 1536 groups: shorter slices add more bins than they
+    // count (16 rows of 100,000 in slices of 2048 take 61 us, of 4096 53).
+    constexpr int UNIT = 4 * SL;
+    const long long want = ((long long)a.rows * a.n / 1536 + UNIT - 1) / UNIT;
     const long long least = ((long long)a.n + UNIT * MAX_SLICES - 1) / (UNIT * MAX_SLICES);
-    long long k = want < 1 ? 1 : want > 8 ? 8 : want;
-    if (k > a.n / (8 * UNIT)) k = a.n / (8 * UNIT);  // 8 slices: parts for CAP / 2 of the top_k
+    long long k = want < 4096 / UNIT ? 4096 / UNIT : want > 32768 / UNIT ? 32768 / UNIT : want;
+    if (k > a.n / (8 * UNIT)) k = a.n / (8 * UNIT);  // 8 slices: parts for a top_k of CAP
     if (k < least) k = least;
     Slices s = {};
     s.len = (int)k * UNIT;
     s.n = (a.n + s.len - 1) / s.len;
-    while (s.n * (ST >> s.per) > MAX_TOPS) ++s.per;
+    while (s.n * (SL >> s.per) > MAX_TOPS) ++s.per;
     return s;
 }
 
@@ -1076,9 +1082,9 @@ extern "C" int ornk_sample(const ornk_sample_args *a, hipStream_t st)
     s.first = s.count + R;
     s.bound = s.first + R;
     const dim3 grid(s.n, a->rows);
-    hipLaunchKernelGGL(k_sample_ends, grid, dim3(ST), 0, st, *a, s);
-    hipLaunchKernelGGL(k_sample_bins, grid, dim3(ST), 0, st, *a, s);
-    hipLaunchKernelGGL(k_sample_gather, grid, dim3(ST), 0, st, *a, s);
+    hipLaunchKernelGGL(k_sample_ends, grid, dim3(SL), 0, st, *a, s);
+    hipLaunchKernelGGL(k_sample_bins, grid, dim3(SL), 0, st, *a, s);
+    hipLaunchKernelGGL(k_sample_gather, grid, dim3(SL), 0, st, *a, s);
     hipLaunchKernelGGL(k_sample_choose, dim3(a->rows), dim3(CT), 0, st, *a, s);
     return hipGetLastError();
 }
