@@ -35,6 +35,18 @@ __device__ __forceinline__ float logit_of(uint32_t key)
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
+typedef float v4u __attribute__((ext_vector_type(4), aligned(4)));
+
+// A float4 of the row from token i on; -infinity behind its end.
+__device__ __forceinline__ v4f load4(const float *x, int n, int i)
+{
+    if (i + 4 <= n) return *reinterpret_cast<const v4u *>(x + i);
+    v4f y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = i + e < n ? x[i + e] : -INFINITY;
+    return y;
+}
+
 // 2^x for x <= 0 in 64 bits: the series of 2^f on [-1/2, 1/2], whose first term left
 // out is below 2^-52.
 __device__ __forceinline__ double exp2_of(double x)
@@ -217,6 +229,13 @@ __device__ __forceinline__ void sums_before(Bins &s)
     __syncthreads();
 }
 
+// Whether the k-th of the parts' largest logits is a bound of the top_k: of tokens in any
+// order about parts * ln(parts / (parts - k)) pass it, which have to fit the list.
+__device__ __forceinline__ bool is_bound(const Row &r, int parts)
+{
+    return r.by_rank && r.q.top_k < parts && -logf(1.0f - (float)r.q.top_k / (float)parts) * (float)parts < 0.75f * CAP;
+}
+
 // The bin in which a sum passes `limit`, which is below the whole.  All threads.
 template <class T>
 __device__ __forceinline__ int find(Bins &s, const T *sum, T limit)
@@ -281,6 +300,76 @@ __device__ __forceinline__ float min_below(const Row &r) { return -logf(r.q.min_
 
 __device__ __forceinline__ bool is_marked(const Bins &s, int bin) { return s.marked[bin >> 5] >> (bin & 31) & 1; }
 
+__device__ __forceinline__ uint64_t wave_sum(uint64_t v)
+{
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+// ---- passes over logits, tokens i0 to end - 1 of a row by a group ------------------
+template <int NT>
+__device__ __forceinline__ Ends ends_of(const float *x, int i0, int end)
+{
+    Ends e = {-INFINITY, INFINITY};
+#pragma unroll 4
+    for (int i = i0 + 4 * (int)threadIdx.x; i < end; i += 4 * NT) {
+        const v4f y = load4(x, end, i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            e.top = fmaxf(e.top, y[j]);  // which a NaN leaves as it is
+            e.low = y[j] > -INFINITY ? fminf(e.low, y[j]) : e.low;
+        }
+    }
+    return e;
+}
+
+// f(logit, token) of those within reach, g(logit) of the others; one copy of each in a
+// loop, the next float4 on its way.
+template <int NT, class F, class G>
+__device__ __forceinline__ void each_token(const Row &r, int i0, int end, F f, G g)
+{
+    int i = i0 + 4 * (int)threadIdx.x;
+    if (i >= end) return;
+    v4f next = load4(r.x, end, i);
+#pragma unroll 1
+    for (; i < end; i += 4 * NT) {
+        v4f y = next;
+        if (i + 4 * NT < end) next = load4(r.x, end, i + 4 * NT);
+#pragma unroll 1
+        for (int j = 0; j < 4; ++j) {
+            if (below(r, y[0]) <= r.reach) f(y[0], i + j);
+            else g(y[0]);
+            y = v4f{y[1], y[2], y[3], y[0]};
+        }
+    }
+}
+
+// Into the bins of w and c, which are in LDS.  What is out of reach belongs to the sum
+// that top_p is a share of, behind all bins' tokens.
+template <int NT>
+__device__ __forceinline__ void fill_bins(const Row &r, int i0, int end, uint64_t *w, uint32_t *c)
+{
+    uint64_t rest = 0;
+    const bool sums = !r.by_rank && r.q.top_p < 1.0f;
+    each_token<NT>(
+        r, i0, end,
+        [&](float x, int) {
+            const int bin = bin_of(r, x);
+            if (!r.by_rank) {
+                const uint64_t v = fixed(r, weight(r, x));
+                if (!v) return;
+                atomicAdd((unsigned long long *)&w[bin], (unsigned long long)v);
+            }
+            if (r.q.top_k > 0) atomicAdd(&c[bin], 1u);
+        },
+        [&](float x) {
+            if (sums) rest += fixed(r, weight(r, x));
+        });
+    if (!sums) return;
+    rest = wave_sum(rest);
+    if (!(threadIdx.x & 63) && rest) atomicAdd((unsigned long long *)&w[NB - 1], (unsigned long long)rest);
+}
+
 // ---- the choice ------------------------------------------------------------------
 // By CT threads, of a list in LDS, or (where more than CAP tokens lie next to a border: a
 // great many logits alike) of the whole row.  Loops stay loops: a group runs this once,
@@ -292,12 +381,6 @@ struct Choice {
     uint32_t keys[2][CT / 64];
     uint32_t count;
 };
-
-__device__ __forceinline__ uint64_t wave_sum(uint64_t v)
-{
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
-}
 
 __device__ __forceinline__ uint64_t wave_scan(uint64_t v)
 {
@@ -386,76 +469,81 @@ __device__ __forceinline__ void choose_few(const ornk_sample_args &a, int row, c
 }
 
 // More: every border is the first key, from the largest down, up to which a sum (of
-// tokens, or of their weights) passes a limit, found by passes over the tokens, 8 bits of
-// the keys' distance from the least each.
+// tokens, or of their weights) passes a limit.  Its bin is known; the key is found by passes
+// over the bin's tokens, 8 bits of the keys' distance from the least each.  Of the whole row
+// (m > CAP) a bin's tokens are listed first, if they are few; the many of one that does not
+// fit are mostly alike, and need one pass for a border and one for the index.  64 rows of
+// 248,320 logits and a top_p: 373 us where all are equal, 461 where they are multiples of 1/4.
 template <class F>
 __device__ __forceinline__ void choose_many(const ornk_sample_args &a, int row, const Row &r, Bins &b, Choice &s, uint32_t m,
-                                            bool binned, F place_of)
+                                            F place_of)
 {
     const int tid = threadIdx.x, lane = tid & 63;
-    const bool listed = m <= CAP;
-    const int n = listed ? (int)m : r.n;
-    // f(key, index, weight) of every token that has a weight
+    bool listed = m <= CAP;
+    int n = listed ? (int)m : r.n;
+    // f(key, index, place in the list) of the list's tokens, or of the row's within reach
     auto each = [&](auto f) {
+        const int step = listed ? 1 : 4;
+        v4f x, next;
+        if (!listed) next = load4(r.x, n, 4 * tid);
 #pragma unroll 1
-        for (int i = tid; i < n; i += CT) {
-            uint32_t key, index = i;
-            uint64_t v;
-            if (listed) {
-                key = (uint32_t)(s.list[i] >> 32);
-                index = (uint32_t)s.list[i];
-                v = s.w[i];
-            } else {
-                key = key_of(r.x[i]);
-                v = fixed(r, weight(r, logit_of(key)));
+        for (int i = step * tid; i < n; i += step * CT) {
+            if (!listed) x = next, next = load4(r.x, n, i + 4 * CT);
+#pragma unroll 1
+            for (int j = 0; j < step; ++j) {
+                const uint64_t t = listed ? s.list[i] : (uint64_t)key_of(x[0]) << 32 | (i + j);
+                if (listed || below(r, x[0]) <= r.reach) f((uint32_t)(t >> 32), (uint32_t)t, i);
+                if (!listed) x = __builtin_shufflevector(x, x, 1, 2, 3, 0);
             }
-            if (v) f(key, index, v);
         }
     };
-    if (listed) {
+    uint32_t seen = 0;  // of a row's tokens the last key, which many may share, and its weight
+    uint64_t seen_units = 0;
+    auto units = [&](uint32_t key, int at) {
+        if (listed) return s.w[at];
+        if (key != seen) seen = key, seen_units = fixed(r, weight(r, logit_of(key)));
+        return seen_units;
+    };
+    auto weigh = [&] {  // the list
 #pragma unroll 1
         for (int i = tid; i < n; i += CT) s.w[i] = fixed(r, weight(r, logit_of((uint32_t)(s.list[i] >> 32))));
+    };
+    if (listed) weigh();
+    auto group_sum = [&](uint64_t v) {
+        v = wave_sum(v);
+        if (!lane) s.tmp[1][tid >> 6] = v;
+        __syncthreads();
+        v = 0;
+        for (int i = 0; i < CT / 64; ++i) v += s.tmp[1][i];
+        __syncthreads();
+        return v;
+    };
+    uint64_t by_min = ~0ull;
+    if (r.q.min_p > 0.0f) {
+        uint64_t sum = 0;
+        each([&](uint32_t key, uint32_t, int at) {
+            const int bin = place_of(logit_of(key));
+            if (bin >= b.min_lo && bin <= b.min_hi && weight(r, logit_of(key)) >= (double)r.q.min_p) sum += units(key, at);
+        });
+        by_min = b.w[b.min_lo] + group_sum(sum);
     }
-    uint64_t sum[3] = {0, 0, 0};  // weights, those of at least min_p, tokens
-    each([&](uint32_t key, uint32_t, uint64_t v) {
-        sum[0] += v;
-        ++sum[2];
-        if (r.q.min_p == 0.0f || weight(r, logit_of(key)) < (double)r.q.min_p) return;
-        const int bin = binned ? place_of(logit_of(key)) : 0;
-        if (!binned || (bin >= b.min_lo && bin <= b.min_hi)) sum[1] += v;
-    });
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        sum[i] = wave_sum(sum[i]);
-        if (!lane) s.tmp[i][tid >> 6] = sum[i];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        sum[i] = 0;
-        for (int j = 0; j < CT / 64; ++j) sum[i] += s.tmp[i][j];
-    }
-    uint64_t whole = binned ? b.w[NB] : sum[0], end = whole;
-    const uint64_t by_min = r.q.min_p == 0.0f ? ~0ull : (binned ? b.w[b.min_lo] : 0) + sum[1];
-    const uint64_t count = binned ? b.c[NB] : sum[2];
+    uint64_t whole = b.w[NB], end = whole;
 
     enum { TOP_K, TOP_P, TARGET, INDEX };
     uint64_t all = 0;   // of the kept
     uint32_t key = 0;   // the token's
     uint64_t rank = 0;  // and its place among those of the same key
+    int bin = 0;
 #pragma unroll 1
     for (int stage = TOP_K; stage <= INDEX; ++stage) {
         uint64_t limit, base = 0;
-        int bin = -1;
         if (stage == TOP_K) {
-            if (r.q.top_k <= 0 || (uint64_t)r.q.top_k >= count) continue;
-            limit = r.q.top_k - 1;
-            if (binned) {
-                bin = find<uint32_t>(b, b.c, (uint32_t)limit);
-                limit -= b.c[bin];
-            }
+            if (r.q.top_k <= 0 || (uint32_t)r.q.top_k >= b.c[NB]) continue;
+            bin = find<uint32_t>(b, b.c, (uint32_t)r.q.top_k - 1);
+            limit = r.q.top_k - 1 - b.c[bin];
         } else if (stage == INDEX) {
             limit = rank;
+            if (!listed) break;
         } else {
             if (stage == TOP_P) {
                 end = whole;
@@ -466,29 +554,54 @@ __device__ __forceinline__ void choose_many(const ornk_sample_args &a, int row, 
                 all = end < by_min ? end : by_min;
                 limit = target_of(r, all);
             }
-            if (binned) {
-                bin = find<uint64_t>(b, b.w, limit);
-                base = b.w[bin];
-                limit -= base;
-            }
+            bin = find<uint64_t>(b, b.w, limit);
+            base = b.w[bin];
+            limit -= base;
         }
         // f(key, weight) of this stage's tokens; of INDEX the keys are the largest index
         // there may be, less theirs
         auto those = [&](auto f) {
-            each([&](uint32_t k, uint32_t index, uint64_t v) {
-                if (bin >= 0 && place_of(logit_of(k)) != bin) return;
-                if (stage == INDEX) {
-                    if (k != key) return;
-                    k = ORN_SAMPLE_MAX_VOCAB - 1 - index;
-                }
-                f(k, v);
+            each([&](uint32_t k, uint32_t index, int at) {
+                if (stage == INDEX ? k != key : place_of(logit_of(k)) != bin) return;
+                const uint64_t v = units(k, at);
+                if (v) f(stage == INDEX ? ORN_SAMPLE_MAX_VOCAB - 1 - index : k, v);
             });
         };
         uint32_t low = ~0u, high = 0;
-        those([&](uint32_t k, uint64_t) {
-            low = k < low ? k : low;
-            high = k > high ? k : high;
-        });
+        const bool fill = m > CAP && stage != INDEX;
+        if (fill) {
+            listed = false;
+            n = r.n;
+            if (!tid) s.count = 0;
+            __syncthreads();
+            v4f next = load4(r.x, n, 4 * tid);
+#pragma unroll 1
+            for (int i = 4 * tid; i < n; i += 4 * CT) {
+                const v4f x = next;
+                next = load4(r.x, n, i + 4 * CT);
+                int in = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t k = key_of(x[j]);
+                    const bool on = below(r, x[j]) <= r.reach && bin_of(r, x[j]) == bin;
+                    in |= on << j;
+                    low = on && k < low ? k : low;
+                    high = on && k > high ? k : high;
+                }
+                if (!in || *(volatile uint32_t *)&s.count > CAP) continue;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (!(in >> j & 1)) continue;
+                    const uint32_t at = atomicAdd(&s.count, 1u);
+                    if (at < CAP) s.list[at] = (uint64_t)key_of(x[j]) << 32 | (i + j);
+                }
+            }
+        } else {
+            those([&](uint32_t k, uint64_t) {
+                low = k < low ? k : low;
+                high = k > high ? k : high;
+            });
+        }
         for (int o = 32; o; o >>= 1) {
             const uint32_t x = __shfl_xor(low, o, 64), y = __shfl_xor(high, o, 64);
             low = x < low ? x : low;
@@ -500,10 +613,16 @@ __device__ __forceinline__ void choose_many(const ornk_sample_args &a, int row, 
             low = s.keys[0][i] < low ? s.keys[0][i] : low;
             high = s.keys[1][i] > high ? s.keys[1][i] : high;
         }
+        if (fill && s.count <= CAP) {
+            listed = true;
+            n = (int)s.count;
+            weigh();
+            __syncthreads();
+        }
         // the border: a key's distance from the least, and the sum above it
         uint32_t found = 0;
         uint64_t above = 0;
-        int known = 32 - __clz((int)((high - low) | 1));  // bits from this one on are known
+        int known = low == high ? 0 : 32 - __clz((int)(high - low));  // bits from this one on are known
 #pragma unroll 1
         while (known > 0) {
             const int shift = known > 8 ? known - 8 : 0;
@@ -532,27 +651,67 @@ __device__ __forceinline__ void choose_many(const ornk_sample_args &a, int row, 
         found += low;
         if (stage == INDEX) {
             if (!tid) put_result(a, row, ORN_SAMPLE_MAX_VOCAB - 1 - found, share(r, key, all));
-            break;
+            return;
         }
         const uint64_t w = fixed(r, weight(r, logit_of(found)));
         if (stage == TOP_K) {
             uint64_t more = 0;
-            those([&](uint32_t k, uint64_t v) {
-                if (k > found) more += v;
-            });
-            more = wave_sum(more);
-            if (!lane) s.tmp[1][tid >> 6] = more;
-            __syncthreads();
-            whole = (bin < 0 ? 0 : b.w[bin]) + (limit + 1 - above) * w;
-            for (int j = 0; j < CT / 64; ++j) whole += s.tmp[1][j];
-            end = whole;
+            if (low != high)
+                those([&](uint32_t k, uint64_t v) {
+                    if (k > found) more += v;
+                });
+            whole = end = b.w[bin] + group_sum(more) + (limit + 1 - above) * w;
         } else if (stage == TOP_P) {
             end = base + above + ((limit - above) / w + 1) * w;
         } else {
             key = found;
             rank = (limit - above) / w;
         }
+        __syncthreads();
     }
+
+    // The index in a row: each wave counts the key's tokens in stretches of 256, one of which
+    // has the rank.
+    uint32_t *counts = reinterpret_cast<uint32_t *>(s.w);
+    constexpr int PER = ORN_SAMPLE_MAX_VOCAB / 256 / CT;
+    for (int i = 0; i < PER; ++i) counts[CT * i + tid] = 0;
+    __syncthreads();
+    v4f next = load4(r.x, r.n, 4 * tid), after = load4(r.x, r.n, 4 * tid + 4 * CT);
+#pragma unroll 1
+    for (int i0 = 0; i0 < r.n; i0 += 4 * CT) {
+        const v4f x = next;
+        next = after;
+        after = load4(r.x, r.n, i0 + 4 * tid + 8 * CT);
+        int c = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c += __popcll(__ballot(key_of(x[j]) == key));
+        if (!lane) counts[(i0 >> 8) + (tid >> 6)] = c;
+    }
+    __syncthreads();
+    uint32_t mine = 0;
+    for (int i = 0; i < PER; ++i) mine += counts[PER * tid + i];
+    uint64_t run = wave_scan(mine);
+    if (lane == 63) s.tmp[0][tid >> 6] = run;
+    __syncthreads();
+    run -= mine;
+    for (int i = 0; i < tid >> 6; ++i) run += s.tmp[0][i];
+    if (run <= rank && rank < run + mine) {
+        int i = PER * tid;
+        for (; rank >= run + counts[i]; ++i) run += counts[i];
+        s.found[0] = i;
+        s.found[1] = run;
+    }
+    __syncthreads();
+    if (tid >= 64) return;
+    const int i = 256 * (int)s.found[0] + 4 * lane;
+    const v4f x = load4(r.x, r.n, i);
+    int in = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) in += key_of(x[j]) == key;
+    run = s.found[1] + wave_scan(in) - in;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (key_of(x[j]) == key && run++ == rank) put_result(a, row, i + j, share(r, key, all));
 }
 
 // Which part of a bin: the marked bins (without bins: all of the reach) in as many equal
@@ -569,9 +728,10 @@ __device__ __forceinline__ int fine_at(const Row &r, const Bins &b, const Fine &
     return (int)(f.before[bin >> 5] + __popc(word & ((1u << (bin & 31)) - 1))) * f.parts + (in < f.parts ? in : f.parts - 1);
 }
 
-// The choice from a list.  A longer one is divided once more, by finer bins.
-__device__ __forceinline__ void choose(const ornk_sample_args &a, int row, const Row &r, Bins &b, Bins &c, Fine &f,
-                                       Choice &s, uint32_t m)
+// The choice from a list.  A longer one is divided once more, by finer bins.  Where too many
+// tokens pass the bound of the top_k, the bins are filled after all.
+__device__ __forceinline__ void choose(const ornk_sample_args &a, int row, Row &r, const Ends &e, Bins &b, Bins &c,
+                                       Fine &f, Choice &s, uint32_t m)
 {
     const int tid = threadIdx.x, lane = tid & 63;
     bool binned = !r.by_rank;
@@ -634,87 +794,22 @@ __device__ __forceinline__ void choose(const ornk_sample_args &a, int row, const
         for (int i = tid; i < (int)m; i += CT) s.list[i] = s.w[i];
         __syncthreads();
     }
+    if (m > CAP && r.by_rank) {
+        r.by_rank = false;
+        scale_row(r, e, 0);
+        for (int i = tid; i < NB; i += CT) b.w[i] = b.c[i] = 0;
+        __syncthreads();
+        fill_bins<CT>(r, 0, r.n, b.w, b.c);
+        __syncthreads();
+        sums_before(b);
+        mark_bins(r, b, false, bin_at(r, min_below(r)));
+    }
     auto place_of = [&](float x) { return fine ? fine_at(r, b, f, below(r, x)) : bin_of(r, x); };
     if (m <= CT) choose_few(a, row, r, fine ? c : b, s, (int)m, binned, place_of);
-    else choose_many(a, row, r, fine ? c : b, s, m, binned && m <= CAP, place_of);
+    else choose_many(a, row, r, fine ? c : b, s, m, place_of);
 }
 
-// ---- passes over logits, tokens i0 to end - 1 of a row by a group ------------------
-typedef float v4u __attribute__((ext_vector_type(4), aligned(4)));
-
-// A float4 of the row from token i on; -infinity behind its end.
-__device__ __forceinline__ v4f load4(const float *x, int n, int i)
-{
-    if (i + 4 <= n) return *reinterpret_cast<const v4u *>(x + i);
-    v4f y;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = i + e < n ? x[i + e] : -INFINITY;
-    return y;
-}
-
-template <int NT>
-__device__ __forceinline__ Ends ends_of(const float *x, int i0, int end)
-{
-    Ends e = {-INFINITY, INFINITY};
-#pragma unroll 4
-    for (int i = i0 + 4 * (int)threadIdx.x; i < end; i += 4 * NT) {
-        const v4f y = load4(x, end, i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            e.top = fmaxf(e.top, y[j]);  // which a NaN leaves as it is
-            e.low = y[j] > -INFINITY ? fminf(e.low, y[j]) : e.low;
-        }
-    }
-    return e;
-}
-
-// f(logit, token) of those within reach, g(logit) of the others; one copy of each in a
-// loop, the next float4 on its way.
-template <int NT, class F, class G>
-__device__ __forceinline__ void each_token(const Row &r, int i0, int end, F f, G g)
-{
-    int i = i0 + 4 * (int)threadIdx.x;
-    if (i >= end) return;
-    v4f next = load4(r.x, end, i);
-#pragma unroll 1
-    for (; i < end; i += 4 * NT) {
-        v4f y = next;
-        if (i + 4 * NT < end) next = load4(r.x, end, i + 4 * NT);
-#pragma unroll 1
-        for (int j = 0; j < 4; ++j) {
-            if (below(r, y[0]) <= r.reach) f(y[0], i + j);
-            else g(y[0]);
-            y = v4f{y[1], y[2], y[3], y[0]};
-        }
-    }
-}
-
-// Into the bins of w and c, which are in LDS.  What is out of reach belongs to the sum
-// that top_p is a share of, behind all bins' tokens.
-template <int NT>
-__device__ __forceinline__ void fill_bins(const Row &r, int i0, int end, uint64_t *w, uint32_t *c)
-{
-    uint64_t rest = 0;
-    const bool sums = !r.by_rank && r.q.top_p < 1.0f;
-    each_token<NT>(
-        r, i0, end,
-        [&](float x, int) {
-            const int bin = bin_of(r, x);
-            if (!r.by_rank) {
-                const uint64_t v = fixed(r, weight(r, x));
-                if (!v) return;
-                atomicAdd((unsigned long long *)&w[bin], (unsigned long long)v);
-            }
-            if (r.q.top_k > 0) atomicAdd(&c[bin], 1u);
-        },
-        [&](float x) {
-            if (sums) rest += fixed(r, weight(r, x));
-        });
-    if (!sums) return;
-    rest = wave_sum(rest);
-    if (!(threadIdx.x & 63) && rest) atomicAdd((unsigned long long *)&w[NB - 1], (unsigned long long)rest);
-}
-
+// ---- lists ----------------------------------------------------------------------
 // Those in marked bins, or (b is NULL) all within reach: f(key << 32 | token).
 template <int NT, class F>
 __device__ __forceinline__ void gather(const Row &r, const Bins *b, int i0, int end, F f)
@@ -812,7 +907,7 @@ __global__ void __launch_bounds__(ST) k_sample_row(ornk_sample_args a)
         return;
     }
     uint32_t bound = 0;
-    if (r.by_rank && r.q.top_k <= ST) {
+    if (is_bound(r, min(ST, r.n / 4))) {
         const uint32_t key[1] = {key_of(own.top)};
         bound = kth_largest(key, r.q.top_k, b.c);
     }
@@ -832,7 +927,7 @@ __global__ void __launch_bounds__(ST) k_sample_row(ornk_sample_args a)
     __syncthreads();
     const uint32_t m = s.count;
     __syncthreads();
-    if (tid < CT) choose(a, row, r, b, fine, parts, s, m);
+    if (tid < CT) choose(a, row, r, e, b, fine, parts, s, m);
 }
 
 // ---- longer rows: in slices ------------------------------------------------------
@@ -905,7 +1000,7 @@ __global__ void __launch_bounds__(SL) k_sample_bins(ornk_sample_args a, Slices s
     if (!r.valid || r.q.temperature == 0.0f) return;
     const int tops = s.n * (SL >> s.per);
     uint32_t bound = 0;
-    if (r.by_rank && r.q.top_k <= tops) {
+    if (is_bound(r, tops)) {
         uint32_t key[MAX_TOPS / SL];
 #pragma unroll
         for (int i = 0; i < MAX_TOPS / SL; ++i)
@@ -954,14 +1049,12 @@ struct OwnBins {
 };
 
 // The tokens in marked bins, or those that pass the bound, to the row's list: those of a
-// group together, as long as LDS holds them (an atomic of its own for each token took 110
-// us for 16 rows of 2000).
+// group together (an atomic of its own for each token took 110 us for 16 rows of 2000).
 __global__ void __launch_bounds__(SL) k_sample_gather(ornk_sample_args a, Slices s)
 {
-    constexpr int MINE = 1024;
     __shared__ Bins b;
     __shared__ Ends tmp[MAX_SLICES / 64];
-    __shared__ uint64_t mine[MINE];
+    __shared__ uint32_t mine[CAP];
     __shared__ uint32_t count, base;
     const int row = blockIdx.y, tid = threadIdx.x, i0 = blockIdx.x * s.len, end = min(i0 + s.len, a.n);
     Row r = row_of(a, row);
@@ -980,22 +1073,17 @@ __global__ void __launch_bounds__(SL) k_sample_gather(ornk_sample_args a, Slices
     const bool binned = !(r.by_rank && bound);
     if (binned) bins.put(r, b);
     __syncthreads();
-    uint64_t *list = s.list + (size_t)row * CAP;
     gather<SL>(r, binned ? &b : nullptr, i0, end, [&](uint64_t t) {
         const uint32_t at = atomicAdd(&count, 1u);
-        if (at < MINE) {
-            mine[at] = t;
-        } else {
-            const uint32_t to = atomicAdd(&s.count[row], 1u);
-            if (to < CAP) list[to] = t;
-        }
+        if (at < CAP) mine[at] = (uint32_t)t;
     });
     __syncthreads();
-    const uint32_t m = count < MINE ? count : MINE;
+    const uint32_t m = count;
     if (!tid && m) base = atomicAdd(&s.count[row], m);
     __syncthreads();
-    for (uint32_t i = tid; i < m; i += SL)
-        if (base + i < CAP) list[base + i] = mine[i];
+    if (m > CAP || base >= CAP) return;
+    uint64_t *list = s.list + (size_t)row * CAP + base;
+    for (uint32_t i = tid; i < min(m, CAP - base); i += SL) list[i] = (uint64_t)key_of(r.x[mine[i]]) << 32 | mine[i];
 }
 
 // All that the choice needs is loaded at once: each wait for memory is longer than most
@@ -1034,7 +1122,7 @@ __global__ void __launch_bounds__(CT) k_sample_choose(ornk_sample_args a, Slices
     }
     if (!r.by_rank) bins.put(r, b);
     __syncthreads();
-    choose(a, row, r, b, fine, parts, k, m);
+    choose(a, row, r, e, b, fine, parts, k, m);
 }
 
 constexpr int ROW_MAX = 32768;  // tokens of a row that one group takes

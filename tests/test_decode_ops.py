@@ -817,6 +817,28 @@ def test_sample_with_a_large_top_k(om, ctx, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [7001, 30000, 32769, 90001])
+@pytest.mark.parametrize("what", ["sorted", "one bin", "few values", "two bins"])
+def test_sample_of_crowded_rows(om, ctx, n, what):
+    """The largest beside each other; more tokens between two borders than are put in order."""
+    g = np.random.default_rng(n + len(what))
+    requests = [(T, k, p, m) for T, p, m in ((1.0, 0.9, 0.0), (50.0, 0.7, 0.0), (40.0, 1.0, 0.0), (30.0, 0.999, 0.2))
+                for k in (0, 1000, 2048, 6000)]
+    x = g.standard_normal((len(requests), n)) * 2
+    if what == "sorted":
+        x = -np.sort(-x, axis=1)
+    elif what == "few values":
+        x = np.round(x)
+    else:  # what lies far below makes the bins wide
+        x *= 0.01
+        x[:, g.integers(0, n, 7)] = -500.0
+        if what == "two bins":
+            x[:, n // 2:] -= 40.0
+    x = x.astype(np.float32)
+    _check_sample(om, ctx, x, requests, (g.random(len(x)) * 0.999).astype(np.float32))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [9000, 40000])
 def test_sample_where_weights_end(om, ctx, n):
     """More tokens of the top_k than have a weight; logits farther apart than the largest number."""
