@@ -50,7 +50,8 @@ int gpu_kv_cache_append(gpu_context *ctx, gpu_buffer *K_cache, gpu_buffer *V_cac
  * sequence, and the eviction that bounds the cache.  The reference keeps one
  * contiguous fp32 cache of 256 positions (inference.c:15) and attends one head
  * at a time; these calls take a batch of sequences, query heads that share kv
- * heads, and narrower cache types.
+ * heads, and narrower cache types.  Beside them stands the rest of a hybrid
+ * stack's step: norms of the heads, linear attention, the choice of a token.
  *
  * Activations are fp32, lengths, positions, slots and page numbers int32, all
  * in buffers of the context; a call takes up to 65535 sequences and as many
@@ -214,7 +215,9 @@ int gpu_kv_evict(gpu_context *ctx, const ornith_kv_pages *kv, int n_seqs, const 
  * state S [key_dim][value_dim] of a sequence's head,
  *   S_t = a_t S_(t-1) + b_t k_t v_t^T,   out_t = scale * q_t S_t,   a_t = exp(decay),
  * b_t = 1, or 1 - a_t with `complement` (the gated step's).  A decay is a logarithm,
- * so that factors near 1 keep their digits: 0 keeps the state, -infinity clears it.
+ * so that factors near 1 keep their digits: 0 keeps the state, -infinity clears a
+ * finite one.  Above 0 a state grows; where factors' products pass the largest number
+ * the results they take part in are infinite or NaN.
  *
  * Q [n_tokens][q_heads][key_dim], K [n_tokens][k_heads][key_dim], V
  * [n_tokens][v_heads][value_dim], out [n_tokens][n_heads][value_dim]: the head
@@ -267,9 +270,9 @@ int gpu_kv_check(gpu_context *ctx);
  * min_p times the largest; the first always.  The token is the first, in that order,
  * up to which the kept tokens' sum is more than u times their whole.  Temperature 0
  * takes the first.  Every p is rounded to a multiple of 2^-42 or less of the largest,
- * sums of these are exact, and so results do not vary from run to run.  A NaN counts as -infinity, which is never taken: a
- * row of nothing else gives token -1.  prob [n_rows] (may be NULL): the token's share
- * of the kept sum.
+ * sums of these are exact, and so results do not vary from run to run; one rounded to 0
+ * is not taken.  A NaN counts as -infinity, which is never taken: a row of nothing else
+ * gives token -1.  prob [n_rows] (may be NULL): the token's share of the kept sum.
  *
  * A request outside its bounds or a u outside [0, 1) gives token -1, prob 0 and
  * ORN_EINVAL (after ORN_KV_ASYNC by gpu_kv_check). */

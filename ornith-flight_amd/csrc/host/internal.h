@@ -41,8 +41,9 @@ struct gpu_context {
     size_t used_memory;
     char err[256];
     orn_workspace ws;
-    /* the same for the paged cache's calls: apart, because the MoE forward's
-     * logits and counters stay readable in `ws` and its graphs record it */
+    /* the same for the decode step's calls (kv.c, linear.c, sample.c): apart, because
+     * the MoE forward's logits and counters stay readable in `ws` and its graphs
+     * record it */
     orn_workspace kv_ws;
     /* this device's fixed scratch, resolved by the first
      * gpu_moe_forward_noalloc call on the context (NULL until then) */
