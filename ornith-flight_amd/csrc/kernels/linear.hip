@@ -200,7 +200,9 @@ __device__ __forceinline__ double fill_decays(const ornk_linear_args &a, Decays 
 
 struct Cut {
     int segs, len;     // parts of a sequence that are done side by side, and their tokens
-    float *states;     // [n_seqs][heads][segs][dk][dv]: what a part adds, then what it begins with
+    bool joined;       // by a launch of its own; else each part joins those before it
+    float *states;     // [n_seqs][heads][segs][dk][dv]: what a part adds, then (joined) what it
+                       // begins with; of the last part what the sequence begins with
     float *decays;     // [n_seqs][heads][segs]: what a part leaves of a state
 };
 
@@ -302,35 +304,65 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
     const Seq seq = seq_of(a, b);
     const int first = sg * cut.len;
     if (seq.n < 0 || (sg && first >= seq.n)) return;
-    if (SUMS && first + cut.len >= seq.n) return;  // nothing begins behind it
     const int last = min(seq.n, first + cut.len);
     const int hq = h / (a.heads / a.qh), hk = h / (a.heads / a.kh), hv = h / (a.heads / a.vh);
     const bool busy = block * 64 * CB + w * 16 * CB < a.dv;  // the wave has columns
     const size_t size = (size_t)a.dk * a.dv;
-    float *const mine = cut.segs > 1 ? cut.states + (((size_t)b * a.heads + h) * cut.segs + sg) * size : nullptr;
+    const size_t part = ((size_t)b * a.heads + h) * cut.segs;  // its first
+    float *const mine = cut.segs > 1 ? cut.states + (part + sg) * size : nullptr;
+    const float *const begin = seq.in >= 0 ? a.S + ((size_t)seq.in * a.heads + h) * size : nullptr;
+    if (SUMS && first + cut.len >= seq.n) {  // nothing begins behind it
+        if (!cut.joined && begin && cols > 0) {  // its slot may be written before all parts have begun
+            for (int row = g; row < a.dk; row += 4) {
+                float x[CB];
+                load<CB, VEC>(x, begin + (size_t)row * a.dv + col0, cols);
+                store<CB, VEC>(mine + (size_t)row * a.dv + col0, x, cols);
+            }
+        }
+        return;
+    }
 
     v4f S[KB][CB];
     bool zero;  // the state is, still
     const bool stored = SUMS || (last == seq.n && seq.out >= 0);  // it is, in the end
     {
-        const float *from = SUMS ? nullptr : cut.segs > 1 ? mine
-                            : seq.in >= 0 ? a.S + ((size_t)seq.in * a.heads + h) * size : nullptr;
+        const float *from = SUMS ? nullptr : cut.segs < 2 || !begin ? begin
+                            : cut.states + (part + (seq.n ? (seq.n - 1) / cut.len : 0)) * size;
+        if (!SUMS && cut.segs > 1 && cut.joined) from = mine;
         zero = !from;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int j = 0; j < CB; ++j) S[kb][j] = v4f{0, 0, 0, 0};
-        if (from && cols > 0) {
+        auto add = [&](const float *p, float keep) {  // all loads on their way at once
+            float x[KB][4][CB];
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * kb + 4 * g + r;
-                    float x[CB];
-                    load<CB, VEC>(x, from + (size_t)min(row, a.dk - 1) * a.dv + col0, cols);
+                for (int r = 0; r < 4; ++r)
+                    load<CB, VEC>(x[kb][r], p + (size_t)min(16 * kb + 4 * g + r, a.dk - 1) * a.dv + col0, cols);
 #pragma unroll
-                    for (int j = 0; j < CB; ++j) S[kb][j][r] = row < a.dk ? x[j] : 0.0f;
-                }
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int j = 0; j < CB; ++j) S[kb][j][r] = fmaf(keep, S[kb][j][r], x[kb][r][j]);
+        };
+        if (from && cols > 0) add(from, 0.0f);
+        if (!SUMS && cut.segs > 1 && !cut.joined) {
+#pragma unroll 1
+            for (int i = 0; i < sg; ++i)
+                if (cols > 0) add(cut.states + (part + i) * size, cut.decays[part + i]);
+            zero = zero && !sg;
+        }
+        if (a.dk < 16 * KB) {  // rows behind the key's dimensions stay 0
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int j = 0; j < CB; ++j)
+                        if (16 * kb + 4 * g + r >= a.dk) S[kb][j][r] = 0.0f;
         }
     }
 
@@ -590,7 +622,7 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
         }
     }
 
-    if (SUMS && tid == 192 && !block) cut.decays[((size_t)b * a.heads + h) * cut.segs + sg] = exp2_of(left);
+    if (SUMS && tid == 192 && !block) cut.decays[part + sg] = exp2_of(left);
     if (!stored || cols <= 0) return;
     float *const to = SUMS ? mine : a.S + ((size_t)seq.out * a.heads + h) * size;
 #pragma unroll
@@ -624,21 +656,26 @@ __global__ void __launch_bounds__(256) k_linear_join(ornk_linear_args a, Cut cut
     }
 }
 
+// Parts of a sequence that join those before them by themselves, which saves a launch (4 x
+// 2000, 16 heads of 128: 167 -> 158 us); more would read too much.
+constexpr int JOIN = 8;
+
 // Sequences are cut where their heads and columns leave CUs idle: into parts of at
 // least 64 tokens, until there are two groups for each CU.  What the parts add to a state
 // is formed first, and their tokens after that from what they begin with, which takes 1.4
 // times the products.  One prompt of 8191 tokens, 16 heads of 128: 176 us (sums 57, joining
-// 15, tokens 115); with one group for each CU 196.  5 x 333, 12 heads of 96 x 80: 45; with
-// parts of 128 tokens 50.
+// 15, tokens 115); with one group for each CU 196.  5 x 333, 12 heads of 96 x 80: 42; with
+// parts of 128 tokens 50 (of 64 45 then).
 Cut cut_of(const ornk_linear_args &a, int cb)
 {
     const long long groups = (long long)a.n_seqs * a.heads * ((a.dv + 64 * cb - 1) / (64 * cb));
     long long segs = 512 / groups;
     if (segs > a.max_len / 64) segs = a.max_len / 64;
-    Cut c = {1, a.max_len, nullptr, nullptr};
+    Cut c = {1, a.max_len, false, nullptr, nullptr};
     if (segs < 2) return c;
     c.len = (int)(((a.max_len + segs - 1) / segs + C - 1) / C * C);
     c.segs = (a.max_len - 1) / c.len + 1;
+    c.joined = c.segs > JOIN;
     return c;
 }
 
@@ -659,8 +696,9 @@ void launch(const ornk_linear_args &a, const Cut &cut, hipStream_t s)
     const dim3 grid((unsigned)a.heads * cut.segs * blocks, a.n_seqs);
     if (cut.segs > 1) {
         hipLaunchKernelGGL((k_linear_chunks<KB, CB, VEC, true>), grid, dim3(256), 0, s, a, cut);
-        hipLaunchKernelGGL(k_linear_join, dim3(a.n_seqs, a.heads, (a.dk * a.dv + 255) / 256), dim3(256), 0, s,
-                           a, cut);
+        if (cut.joined)
+            hipLaunchKernelGGL(k_linear_join, dim3(a.n_seqs, a.heads, (a.dk * a.dv + 255) / 256), dim3(256), 0,
+                               s, a, cut);
     }
     hipLaunchKernelGGL((k_linear_chunks<KB, CB, VEC, false>), grid, dim3(256), 0, s, a, cut);
 }
