@@ -279,92 +279,136 @@ __device__ __forceinline__ int by_length(const ornk_linear_args &a, int rank, in
     __syncthreads();
     if (i < a.n_seqs && before == rank) lens[0] = i;
     __syncthreads();
-    return lens[0];
+    const int b = lens[0];
+    __syncthreads();
+    return b;
 }
 
-// SUMS: only what a part adds to a state that begins with zeros.  VEC: rows of K and Q
-// are whole float4s, those of V whole vectors of CB.
-template <int KB, int CB, bool VEC, bool SUMS>
-__global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cut cut)
-{
-    constexpr int LD = 16 * KB + 4;    // floats of a row in LDS
-    constexpr int RS = 64 / KB;        // rows that the threads load at a time, a float4 each
-    constexpr int NL = C / RS;
-    constexpr int NK = KB > 8 ? 1 : 2; // K of the next chunk beside this one's where two groups still fit a CU
-    __shared__ __align__(16) float Ks[NK][C][LD];
-    __shared__ __align__(16) float Qs[SUMS ? 1 : C][LD];
-    __shared__ __align__(16) v4f Ps[SUMS ? 1 : 3][64];
-    __shared__ __align__(16) Decays dec[2];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
-    const int blocks = (a.dv + 64 * CB - 1) / (64 * CB);
-    const int rest = blockIdx.x / a.heads, h = blockIdx.x - rest * a.heads;
-    const int sg = rest / blocks, block = rest - sg * blocks;
-    const int col0 = block * 64 * CB + w * 16 * CB + c * CB, cols = a.dv - col0;
-    const int b = cut.segs > 1 ? blockIdx.y : by_length(a, blockIdx.y, (int *)&Ks[0][0][0]);
-    const Seq seq = seq_of(a, b);
-    const int first = sg * cut.len;
-    if (seq.n < 0 || (sg && first >= seq.n)) return;
-    const int last = min(seq.n, first + cut.len);
-    const int hq = h / (a.heads / a.qh), hk = h / (a.heads / a.kh), hv = h / (a.heads / a.vh);
-    const bool busy = block * 64 * CB + w * 16 * CB < a.dv;  // the wave has columns
-    const size_t size = (size_t)a.dk * a.dv;
-    const size_t part = ((size_t)b * a.heads + h) * cut.segs;  // its first
-    float *const mine = cut.segs > 1 ? cut.states + (part + sg) * size : nullptr;
-    const float *const begin = seq.in >= 0 ? a.S + ((size_t)seq.in * a.heads + h) * size : nullptr;
-    if (SUMS && first + cut.len >= seq.n) {  // nothing begins behind it
-        if (!cut.joined && begin && cols > 0) {  // its slot may be written before all parts have begun
-            for (int row = g; row < a.dk; row += 4) {
-                float x[CB];
-                load<CB, VEC>(x, begin + (size_t)row * a.dv + col0, cols);
-                store<CB, VEC>(mine + (size_t)row * a.dv + col0, x, cols);
-            }
-        }
-        return;
-    }
+// What a group has: a part of a sequence, and 64 CB columns of a head.
+struct Part {
+    Seq seq;
+    int h, sg, block, first, last;  // tokens first to last - 1 of the sequence
+    size_t at;                      // of the head's parts in the work buffers, the first
+};
 
-    v4f S[KB][CB];
-    bool zero;  // the state is, still
-    const bool stored = SUMS || (last == seq.n && seq.out >= 0);  // it is, in the end
-    {
-        const float *from = SUMS ? nullptr : cut.segs < 2 || !begin ? begin
-                            : cut.states + (part + (seq.n ? (seq.n - 1) / cut.len : 0)) * size;
-        if (!SUMS && cut.segs > 1 && cut.joined) from = mine;
-        zero = !from;
+template <int CB>
+__device__ __forceinline__ Part part_of(const ornk_linear_args &a, const Cut &cut, int *lens)
+{
+    Part p;
+    const int blocks = (a.dv + 64 * CB - 1) / (64 * CB), rest = blockIdx.x / a.heads;
+    p.h = blockIdx.x - rest * a.heads;
+    p.sg = rest / blocks;
+    p.block = rest - p.sg * blocks;
+    const int b = cut.segs > 1 ? blockIdx.y : by_length(a, blockIdx.y, lens);
+    p.seq = seq_of(a, b);
+    p.first = p.sg * cut.len;
+    p.last = min(p.seq.n, p.first + cut.len);
+    p.at = ((size_t)b * a.heads + p.h) * cut.segs;
+    return p;
+}
+
+// The state that a part begins with; whether it is known to be 0.
+template <int KB, int CB, bool VEC, bool SUMS>
+__device__ __forceinline__ bool begin_state(const ornk_linear_args &a, const Cut &cut, const Part &p, int col0,
+                                            v4f (&S)[KB][CB])
+{
+    const int g = (threadIdx.x & 63) >> 4, cols = a.dv - col0;
+    const size_t size = (size_t)a.dk * a.dv;
+    const float *from = p.seq.in >= 0 ? a.S + ((size_t)p.seq.in * a.heads + p.h) * size : nullptr;
+    if (SUMS) from = nullptr;
+    else if (cut.segs > 1 && cut.joined) from = cut.states + (p.at + p.sg) * size;
+    else if (cut.segs > 1 && from) from = cut.states + (p.at + (p.seq.n ? (p.seq.n - 1) / cut.len : 0)) * size;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int j = 0; j < CB; ++j) S[kb][j] = v4f{0, 0, 0, 0};
+    auto add = [&](const float *y, float keep) {  // all loads on their way at once
+        float x[KB][4][CB];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int j = 0; j < CB; ++j) S[kb][j] = v4f{0, 0, 0, 0};
-        auto add = [&](const float *p, float keep) {  // all loads on their way at once
-            float x[KB][4][CB];
+            for (int r = 0; r < 4; ++r)
+                load<CB, VEC>(x[kb][r], y + (size_t)min(16 * kb + 4 * g + r, a.dk - 1) * a.dv + col0, cols);
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    load<CB, VEC>(x[kb][r], p + (size_t)min(16 * kb + 4 * g + r, a.dk - 1) * a.dv + col0, cols);
+            for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int j = 0; j < CB; ++j) S[kb][j][r] = fmaf(keep, S[kb][j][r], x[kb][r][j]);
-        };
-        if (from && cols > 0) add(from, 0.0f);
-        if (!SUMS && cut.segs > 1 && !cut.joined) {
+                for (int j = 0; j < CB; ++j) S[kb][j][r] = fmaf(keep, S[kb][j][r], x[kb][r][j]);
+    };
+    if (from && cols > 0) add(from, 0.0f);
+    const bool joins = !SUMS && cut.segs > 1 && !cut.joined;
+    if (joins) {
 #pragma unroll 1
-            for (int i = 0; i < sg; ++i)
-                if (cols > 0) add(cut.states + (part + i) * size, cut.decays[part + i]);
-            zero = zero && !sg;
-        }
-        if (a.dk < 16 * KB) {  // rows behind the key's dimensions stay 0
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int j = 0; j < CB; ++j)
-                        if (16 * kb + 4 * g + r >= a.dk) S[kb][j][r] = 0.0f;
-        }
+        for (int i = 0; i < p.sg; ++i)
+            if (cols > 0) add(cut.states + (p.at + i) * size, cut.decays[p.at + i]);
     }
+    if (a.dk < 16 * KB) {  // rows behind the key's dimensions stay 0
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int j = 0; j < CB; ++j)
+                    if (16 * kb + 4 * g + r >= a.dk) S[kb][j][r] = 0.0f;
+    }
+    return !from && !(joins && p.sg);
+}
+
+template <int KB, int CB, bool VEC>
+__device__ __forceinline__ void end_state(const ornk_linear_args &a, float *to, int col0, const v4f (&S)[KB][CB])
+{
+    const int g = (threadIdx.x & 63) >> 4, cols = a.dv - col0;
+    if (cols <= 0) return;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = 16 * kb + 4 * g + r;
+            float x[CB];
+#pragma unroll
+            for (int j = 0; j < CB; ++j) x[j] = S[kb][j][r];
+            if (row < a.dk) store<CB, VEC>(to + (size_t)row * a.dv + col0, x, cols);
+        }
+}
+
+template <bool SUMS>
+__device__ __forceinline__ float *state_of(const ornk_linear_args &a, const Cut &cut, const Part &p)
+{
+    const size_t size = (size_t)a.dk * a.dv;
+    return SUMS ? cut.states + (p.at + p.sg) * size : a.S + ((size_t)p.seq.out * a.heads + p.h) * size;
+}
+
+template <int KB, bool SUMS>
+struct Exact {
+    static constexpr int LD = 16 * KB + 4;    // floats of a row in LDS
+    static constexpr int NK = KB > 8 ? 1 : 2; // K of the next chunk beside this one's where two groups still fit a CU
+    __align__(16) float Ks[NK][C][LD];
+    __align__(16) float Qs[SUMS ? 1 : C][LD];
+    __align__(16) v4f Ps[SUMS ? 1 : 3][64];
+    __align__(16) Decays dec[2];
+};
+
+// With fp32 operands: what 32-bit arithmetic gives, infinities and NaN included.
+template <int KB, int CB, bool VEC, bool SUMS>
+__device__ __forceinline__ void exact_chunks(const ornk_linear_args &a, const Cut &cut, const Part &part, Exact<KB, SUMS> &lds)
+{
+    constexpr int LD = Exact<KB, SUMS>::LD, NK = Exact<KB, SUMS>::NK;
+    constexpr int RS = 64 / KB;        // rows that the threads load at a time, a float4 each
+    constexpr int NL = C / RS;
+    auto &Ks = lds.Ks;
+    auto &Qs = lds.Qs;
+    auto &Ps = lds.Ps;
+    auto &dec = lds.dec;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
+    const Seq &seq = part.seq;
+    const int h = part.h, first = part.first, last = part.last, block = part.block;
+    const int col0 = block * 64 * CB + w * 16 * CB + c * CB, cols = a.dv - col0;
+    const int hq = h / (a.heads / a.qh), hk = h / (a.heads / a.kh), hv = h / (a.heads / a.vh);
+    const bool busy = block * 64 * CB + w * 16 * CB < a.dv;  // the wave has columns
+    const bool stored = SUMS || (last == seq.n && seq.out >= 0);  // the state is, in the end
+    v4f S[KB][CB];
+    bool zero = begin_state<KB, CB, VEC, SUMS>(a, cut, part, col0, S);  // the state is, still
 
     // Rows of a chunk: uniform addresses, and each lane's place in them.  Where every load
     // is whole (VEC), lanes without columns load others' and rows behind the end the last
@@ -451,7 +495,6 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
         if (w == 3) fetch_decays(first);
         fetch_v(last - first);
         if (w == 3) fill(0, first);
-        if (cut.segs < 2) __syncthreads();  // by_length's lens are read
         if (left_k <= 0) {  // columns behind the key's dimensions stay 0
             const v4f z = {0, 0, 0, 0};
 #pragma unroll
@@ -622,19 +665,382 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
         }
     }
 
-    if (SUMS && tid == 192 && !block) cut.decays[part + sg] = exp2_of(left);
-    if (!stored || cols <= 0) return;
-    float *const to = SUMS ? mine : a.S + ((size_t)seq.out * a.heads + h) * size;
+    if (SUMS && tid == 192 && !block) cut.decays[part.at + part.sg] = exp2_of(left);
+    if (stored) end_state<KB, CB, VEC>(a, state_of<SUMS>(a, cut, part), col0, S);
+}
+
+// With operands of three bf16 parts, which hold the 24 bits of an fp32 number, and the six
+// products of parts that are not below its last bit: 16 x the rate, so 2.7 x the speed.
+// Parts of an infinity are no numbers, so whatever is not finite shows in the results, and
+// the part is done again with fp32 operands.
+template <int KB, bool SUMS>
+struct Split {
+    // [part][row][pair of dimensions]: of 32 dimensions those that a lane group of the
+    // state's rows has, 4 g + r and 16 + 4 g + r, side by side; a row's 16 bytes turned by its number
+    __align__(16) uint32_t K[SUMS ? 1 : 3][C][8 * KB];
+    __align__(16) uint32_t Q[SUMS ? 1 : 3][C][8 * KB];
+    // [part][four dimensions][a dimension's pairs of tokens], tokens in the same order
+    __align__(16) uint32_t T[SUMS ? 2 : 1][3][4 * KB][64 + 4];
+    __align__(16) uint2 P[SUMS ? 1 : 3][3][64];
+    __align__(16) Decays dec[2];
+};
+
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+
+// x without its first part of 8 bits
+__device__ __forceinline__ float rest_of(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+// the first parts of two
+__device__ __forceinline__ uint32_t firsts(float x, float y)
+{
+    return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+}
+
+// Eight numbers as three operands of the matrix cores.
+__device__ __forceinline__ void split8(u4 (&o)[3], const float (&x)[8])
+{
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
+    for (int i = 0; i < 4; ++i) {
+        const float r0 = rest_of(x[2 * i]), r1 = rest_of(x[2 * i + 1]);
+        o[0][i] = firsts(x[2 * i], x[2 * i + 1]);
+        o[1][i] = firsts(r0, r1);
+        o[2][i] = firsts(rest_of(r0), rest_of(r1));
+    }
+}
+
+__device__ __forceinline__ v4f mfma(u4 a, u4 b, v4f c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), c, 0, 0, 0);
+}
+
+// The parts of a product, the small ones first.
+#define PRODUCTS(F) F(0, 2) F(2, 0) F(1, 1) F(0, 1) F(1, 0) F(0, 0)
+
+// false: something was not finite, and nothing of the state is stored.
+template <int KB, int CB, bool SUMS>
+__device__ __forceinline__ bool split_chunks(const ornk_linear_args &a, const Cut &cut, const Part &part, Split<KB, SUMS> &lds)
+{
+    constexpr int M = 2 * KB - 1;  // 16-byte words of a row, less one
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, g = lane >> 4, c = lane & 15;
+    const Seq &seq = part.seq;
+    const int h = part.h, first = part.first, last = part.last, block = part.block;
+    const int col0 = block * 64 * CB + w * 16 * CB + c * CB, cols = a.dv - col0;
+    const int hq = h / (a.heads / a.qh), hk = h / (a.heads / a.kh), hv = h / (a.heads / a.vh);
+    const bool busy = block * 64 * CB + w * 16 * CB < a.dv;
+    const bool stored = SUMS || (last == seq.n && seq.out >= 0);
+    v4f S[KB][CB];
+    bool zero = begin_state<KB, CB, true, SUMS>(a, cut, part, col0, S);
+
+    // a thread has four dimensions of four tokens of K and Q
+    const int lr = tid / (4 * KB), ld = tid - lr * 4 * KB;
+    const bool loads = lr < C / 4;
+    const bool filled = 4 * ld < a.dk;
+    const size_t ks = (size_t)a.kh * a.dk, qs = (size_t)a.qh * a.dk, vs = (size_t)a.vh * a.dv,
+                 os = (size_t)a.heads * a.dv;
+    const float *kp = a.k + ((size_t)seq.t0 + first) * ks + hk * a.dk, *qp = a.q + ((size_t)seq.t0 + first) * qs + hq * a.dk,
+                *vp = a.v + ((size_t)seq.t0 + first) * vs + hv * a.dv;
+    float *op = a.out + ((size_t)seq.t0 + first) * os + h * a.dv;
+    const uint32_t lcv = filled ? 4 * ld : 0, colv = cols <= 0 ? 0 : col0;
+    float kn[4][4], qn[SUMS ? 1 : 4][4], v[2][4][CB], vn[2][4][CB];
+    auto fetch = [&](int n) {
+        if (loads) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int row = 16 * kb + 4 * g + r;
-            float x[CB];
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t row = min(4 * lr + e, n - 1);
+                load<4, true>(kn[e], kp + (row * (uint32_t)ks + lcv));
+                if (!SUMS) load<4, true>(qn[e], qp + (row * (uint32_t)qs + lcv));
+            }
+            if (n < C || !filled) {
 #pragma unroll
-            for (int j = 0; j < CB; ++j) x[j] = S[kb][j][r];
-            if (row < a.dk) store<CB, VEC>(to + (size_t)row * a.dv + col0, x, cols);
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (4 * lr + e >= n || !filled) kn[e][i] = 0.0f;
+                        if (!SUMS && !filled) qn[e][i] = 0.0f;
+                    }
+            }
         }
+        kp += C * ks;
+        qp += C * qs;
+    };
+    auto fetch_v = [&](int n) {
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t row = min(16 * tb + 4 * g + r, n - 1);
+                load<CB, true>(vn[tb][r], vp + (row * (uint32_t)vs + colv));
+            }
+        if (n < C) {
+#pragma unroll
+            for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int j = 0; j < CB; ++j)
+                        if (16 * tb + 4 * g + r >= n) vn[tb][r][j] = 0.0f;
+        }
+        vp += C * vs;
+    };
+    float xn = 0.0f;
+    double left = 0.0;
+    auto fetch_decays = [&](int t) {
+        const int i = lane & (C - 1);
+        const size_t tok = (size_t)seq.t0 + t + (i < last - t ? i : 0);
+        xn = a.decay[a.per_token ? tok * a.heads + h : h];
+    };
+    auto fill = [&](int p, int t) {
+        const bool on = (lane & (C - 1)) < last - t;
+        left += fill_decays(a, lds.dec[p], decay2(xn, on), on);
+        if (t + C < last) fetch_decays(t + C);
+    };
+    auto stage = [&](int p) {
+        if (!loads) return;
+        const int word = (4 * (ld >> 3) + (ld & 3)), half = ld >> 2 & 1;
+        auto rows = [&](uint32_t (&to)[SUMS ? 1 : 3][C][8 * KB], const float (&x)[4][4], int part) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int row = 4 * lr + e;
+                *reinterpret_cast<uint2 *>(&to[part][row][4 * (word ^ (row & M)) + 2 * half]) =
+                    uint2{firsts(x[e][0], x[e][1]), firsts(x[e][2], x[e][3])};
+            }
+        };
+#pragma unroll
+        for (int part = 0; part < 3; ++part) {
+            if (part) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        kn[e][i] = rest_of(kn[e][i]);
+                        if (!SUMS) qn[e][i] = rest_of(qn[e][i]);
+                    }
+            }
+            if (!SUMS) {
+                rows(lds.K, kn, part);
+                if constexpr (!SUMS) rows(lds.Q, qn, part);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<uint2 *>(&lds.T[SUMS ? p : 0][part][ld][16 * i + 4 * (lr & 3) + 2 * (lr >> 2)]) =
+                    uint2{firsts(kn[0][i], kn[1][i]), firsts(kn[2][i], kn[3][i])};
+        }
+    };
+    auto row_of = [&](const uint32_t (&from)[SUMS ? 1 : 3][C][8 * KB], int part, int row, int x) {
+        return *reinterpret_cast<const u4 *>(&from[part][row][4 * ((4 * x + g) ^ (row & M))]);
+    };
+
+    float bad = 0.0f;  // 0, or a NaN
+    int p = 0;
+    if (first < last) {
+        fetch(last - first);
+        if (w == 3) fetch_decays(first);
+        fetch_v(last - first);
+        if (w == 3) fill(0, first);
+    }
+    for (int t = first; t < last; t += C, p ^= 1) {
+        const bool more = t + C < last;
+        stage(p);
+#pragma unroll
+        for (int i = 0; i < 8 * CB; ++i) (&v[0][0][0])[i] = (&vn[0][0][0])[i];
+        __syncthreads();
+        if (more) {
+            fetch(last - t - C);
+            fetch_v(last - t - C);
+        }
+        const Decays &d = lds.dec[p];
+        v4f O[2][CB];
+        if (w == 3) {
+            if (more) fill(p ^ 1, t + C);
+        } else if constexpr (!SUMS) {
+            const int i = w, query = 16 * (i > 0) + c, key = 16 * (i > 1) + 4 * g, kr = 16 * (i > 1) + c;
+            v4f P0 = {0, 0, 0, 0}, P1 = {0, 0, 0, 0};
+#pragma unroll
+            for (int x = 0; x < KB / 2; ++x) {
+                u4 k[3], q[3];
+#pragma unroll
+                for (int y = 0; y < 3; ++y) {
+                    k[y] = row_of(lds.K, y, kr, x);
+                    q[y] = row_of(lds.Q, y, query, x);
+                }
+                v4f &P = x & 1 ? P1 : P0;
+#define F(A, B) P = mfma(k[A], q[B], P);
+                PRODUCTS(F)
+#undef F
+            }
+            P0 += P1;
+            const double G = d.G[query];
+            float y[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                y[r] = query >= key + r ? P0[r] * (exp2_of(G - d.G[key + r]) * d.b[key + r]) : 0.0f;
+#pragma unroll
+            for (int z = 0; z < 3; ++z) {
+                lds.P[i][z][lane] = uint2{firsts(y[0], y[1]), firsts(y[2], y[3])};
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[r] = rest_of(y[r]);
+            }
+        }
+        if constexpr (!SUMS) {
+#pragma unroll
+            for (int ib = 0; ib < 2; ++ib)
+#pragma unroll
+                for (int j = 0; j < CB; ++j) O[ib][j] = v4f{0, 0, 0, 0};
+            if (busy && !zero) {  // q S
+#pragma unroll
+                for (int x = 0; x < KB / 2; ++x) {
+                    u4 q[2][3], s[CB][3];
+#pragma unroll
+                    for (int y = 0; y < 3; ++y) {
+                        q[0][y] = row_of(lds.Q, y, c, x);
+                        q[1][y] = row_of(lds.Q, y, 16 + c, x);
+                    }
+#pragma unroll
+                    for (int j = 0; j < CB; ++j) {
+                        float y[8];
+#pragma unroll
+                        for (int r = 0; r < 8; ++r) y[r] = S[2 * x + (r >> 2)][j][r & 3];
+                        split8(s[j], y);
+                    }
+#define F(A, B)                                                                     \
+    _Pragma("unroll") for (int j = 0; j < CB; ++j)                                  \
+    {                                                                               \
+        O[0][j] = mfma(q[0][A], s[j][B], O[0][j]);                                  \
+        O[1][j] = mfma(q[1][A], s[j][B], O[1][j]);                                  \
+    }
+                    PRODUCTS(F)
+#undef F
+                }
+#pragma unroll
+                for (int ib = 0; ib < 2; ++ib) {
+                    const v4f f = *reinterpret_cast<const v4f *>(&d.q[16 * ib + 4 * g]);
+#pragma unroll
+                    for (int j = 0; j < CB; ++j) O[ib][j] *= f;
+                }
+            }
+            __syncthreads();
+            if (busy) {
+                u4 m[2][3];
+#pragma unroll
+                for (int z = 0; z < 3; ++z) {
+                    const uint2 x0 = lds.P[0][z][lane], x1 = lds.P[1][z][lane], x2 = lds.P[2][z][lane];
+                    m[0][z] = u4{x0.x, x0.y, 0, 0};
+                    m[1][z] = u4{x1.x, x1.y, x2.x, x2.y};
+                }
+                u4 s[CB][3];
+#pragma unroll
+                for (int j = 0; j < CB; ++j) {
+                    float y[8];
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) y[r] = v[r >> 2][r & 3][j];
+                    split8(s[j], y);
+                }
+#define F(A, B)                                                                     \
+    _Pragma("unroll") for (int j = 0; j < CB; ++j)                                  \
+    {                                                                               \
+        O[0][j] = mfma(m[0][A], s[j][B], O[0][j]);                                  \
+        O[1][j] = mfma(m[1][A], s[j][B], O[1][j]);                                  \
+    }
+                PRODUCTS(F)
+#undef F
+                const int n = last - t;
+                const uint32_t oo = 4 * g * (uint32_t)os + col0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int ib = i >> 2, r = i & 3;
+                    float x[CB];
+#pragma unroll
+                    for (int j = 0; j < CB; ++j) {
+                        x[j] = O[ib][j][r];
+                        bad = fmaf(x[j], 0.0f, bad);
+                    }
+                    if (cols > 0 && 16 * ib + 4 * g + r < n) store<CB, true>(op + (16 * ib + r) * os + oo, x, cols);
+                }
+                op += C * os;
+            }
+        }
+        if (busy && (more || stored)) {
+            const float all = d.all;
+            u4 s[CB][3];
+#pragma unroll
+            for (int j = 0; j < CB; ++j) {
+                float y[8];
+#pragma unroll
+                for (int tb = 0; tb < 2; ++tb) {
+                    const v4f f = *reinterpret_cast<const v4f *>(&d.k[16 * tb + 4 * g]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) y[4 * tb + r] = v[tb][r][j] * f[r];
+                }
+                split8(s[j], y);
+            }
+#pragma unroll
+            for (int kb = 0; kb < KB; kb += 2) {
+                u4 k[2][3];
+#pragma unroll
+                for (int z = 0; z < 3; ++z)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        k[i][z] = *reinterpret_cast<const u4 *>(
+                            &lds.T[SUMS ? p : 0][z][4 * (kb + i) + (c >> 2)][16 * (c & 3) + 4 * g]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < CB; ++j) S[kb + i][j] *= all;
+#define F(A, B)                                                                     \
+    _Pragma("unroll") for (int i = 0; i < 2; ++i)                                   \
+        _Pragma("unroll") for (int j = 0; j < CB; ++j)                              \
+            S[kb + i][j] = mfma(k[i][A], s[j][B], S[kb + i][j]);
+                PRODUCTS(F)
+#undef F
+            }
+        }
+        zero = false;
+        if (!SUMS) __syncthreads();
+    }
+    if (stored && busy) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int j = 0; j < CB; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) bad = fmaf(S[kb][j][r], 0.0f, bad);
+    }
+    if (__syncthreads_or(bad != bad)) return false;
+    if (SUMS && tid == 192 && !block) cut.decays[part.at + part.sg] = exp2_of(left);
+    if (stored) end_state<KB, CB, true>(a, state_of<SUMS>(a, cut, part), col0, S);
+    return true;
+}
+#undef PRODUCTS
+
+// SUMS: only what a part adds to a state that begins with zeros.  VEC: rows of K and Q
+// are whole float4s, those of V whole vectors of CB.
+template <int KB, int CB, bool VEC, bool SUMS>
+__global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cut cut)
+{
+    constexpr bool FAST = VEC && KB <= 8;
+    __shared__ union Lds {
+        int lens[256];
+        Exact<KB, SUMS> exact;
+        Split<FAST ? KB : 1, SUMS> split;
+        __device__ Lds() {}
+    } lds;
+    const Part part = part_of<CB>(a, cut, lds.lens);
+    if (part.seq.n < 0 || (part.sg && part.first >= part.seq.n)) return;
+    if (SUMS && part.first + cut.len >= part.seq.n) {
+        // Nothing begins behind it; but where each part joins those before it, its place
+        // holds what the sequence begins with, whose slot may be written before all have begun.
+        if (cut.joined || part.seq.in < 0) return;
+        const size_t size = (size_t)a.dk * a.dv;
+        const float *from = a.S + ((size_t)part.seq.in * a.heads + part.h) * size;
+        float *to = cut.states + (part.at + part.sg) * size;
+        const int col = part.block * 64 * CB + (threadIdx.x & 63), n = min(a.dv, (part.block + 1) * 64 * CB);
+        for (int row = threadIdx.x >> 6; row < a.dk; row += 4)
+            for (int i = col; i < n; i += 64) to[(size_t)row * a.dv + i] = from[(size_t)row * a.dv + i];
+        return;
+    }
+    if constexpr (FAST)
+        if (split_chunks<KB, CB, SUMS>(a, cut, part, lds.split)) return;
+    exact_chunks<KB, CB, VEC, SUMS>(a, cut, part, lds.exact);
 }
 
 // From what each part adds to what each part begins with, an element per thread (16 heads
