@@ -233,8 +233,10 @@ int gpu_kv_evict(gpu_context *ctx, const ornith_kv_pages *kv, int n_seqs, const 
  * one slot.
  *
  * Sums and states are of 32 bits; a prompt's tokens are taken together in chunks,
- * whose decays are summed in 64.  What a token holds has no effect on those before
- * it, NaN and infinities included.  A slot outside [-1, n_slots), or tokens outside
+ * whose decays are summed in 64 and whose products are of operands of 24 bits (fewer
+ * below 2^-110).  What a token holds has no effect on those before it, NaN and
+ * infinities included, but for their last digits: a stretch with a result that is not
+ * finite is done with other instructions.  A slot outside [-1, n_slots), or tokens outside
  * [0, n_tokens) or more than max_len, leave their sequence out (gpu_kv_check). */
 typedef struct {
     gpu_buffer *S; /* [n_slots][n_heads][key_dim][value_dim] fp32; NULL without slots */

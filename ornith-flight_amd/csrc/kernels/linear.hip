@@ -1,6 +1,8 @@
 // SPDX-License-Identifier: MIT
 //
 // Linear attention with a decay for each head (ornith_hip.h).
+#include <type_traits>
+
 #include "common.h"
 #include "launch.h"
 
@@ -120,7 +122,7 @@ void launch_step(const ornk_linear_args &a, hipStream_t s)
 }
 
 // ---- chunks ------------------------------------------------------------------
-// C tokens at a time, on the fp32 matrix cores.  With G_i the sum of a chunk's decays
+// C tokens at a time, on the matrix cores.  With G_i the sum of a chunk's decays
 // up to token i (base 2, in 64 bits), S the state before it and P_ij = q_i k_j:
 //   o_i = scale (2^G_i q_i S + sum_(j <= i) 2^(G_i - G_j) b_j P_ij v_j)
 //   S  <- 2^G_C S + sum_j 2^(G_C - G_j) b_j k_j v_j^T
@@ -133,12 +135,13 @@ void launch_step(const ornk_linear_args &a, hipStream_t s)
 // second, of the second), one for each of three waves; the fourth sums the next chunk's
 // decays meanwhile.
 //
-// Bound by the matrix cores, which take 15 ns for an fp32 16x16x4 product of a SIMD (140
-// TFLOP/s; vector instructions beside it wait for it) and are busy 68 % of the time: 24 x
-// up to 1501 tokens, 32 heads of 128 (18,210 tokens in all) 432 us, 89 TFLOP/s of the
-// recurrence's and 104 of what is computed; C = 32 costs 19 % more than the recurrence
-// (P, P V), 64 would cost 50 % and save no wait that a second group does not hide.  Eight
-// waves of 16 columns instead of four of 32: 703 us then, against 557.
+// With fp32 operands it was bound by the matrix cores, which take 15 ns for a 16x16x4
+// product of a SIMD (140 TFLOP/s): 24 x up to 1501 tokens, 32 heads of 128 (18,210 tokens in
+// all) 431 us.  With three bf16 parts (8 ns for 16x16x32, six products) it takes 342: 1.27 GB
+// are moved at 3.7 TB/s, and each wave's 240 matrix instructions and 1100 others of a chunk
+// wait for three barriers, with one other group on the CU.  C = 32 costs 19 % more than the recurrence (P, P V).
+// Later loads of V, K and Q staged before S's products, and heads that share K and Q on one
+// XCD made no difference.
 constexpr int C = 32;
 
 struct alignas(16) Decays {
@@ -669,10 +672,11 @@ __device__ __forceinline__ void exact_chunks(const ornk_linear_args &a, const Cu
     if (stored) end_state<KB, CB, VEC>(a, state_of<SUMS>(a, cut, part), col0, S);
 }
 
-// With operands of three bf16 parts, which hold the 24 bits of an fp32 number, and the six
-// products of parts that are not below its last bit: 16 x the rate, so 2.7 x the speed.
-// Parts of an infinity are no numbers, so whatever is not finite shows in the results, and
-// the part is done again with fp32 operands.
+// With operands of three bf16 parts, which hold the 24 bits of an fp32 number (of those
+// below 2^-110 fewer), and the six products of parts that reach its last bit: what is left
+// out is at most 2^-22 of a product.  16 x the rate, so 2.7 x the speed.  Parts of an
+// infinity are no numbers, so whatever is not finite shows in the results, and the part is
+// done again with fp32 operands.
 template <int KB, bool SUMS>
 struct Split {
     // [part][row][pair of dimensions]: of 32 dimensions those that a lane group of the
@@ -688,24 +692,38 @@ struct Split {
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 
-// x without its first part of 8 bits
-__device__ __forceinline__ float rest_of(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
-// the first parts of two
-__device__ __forceinline__ uint32_t firsts(float x, float y)
+// Part Z of two numbers, of which the parts before it are taken off, and what it leaves,
+// exactly.  The second is rounded to nearest, so that what the products leave out has either
+// sign; the others are the leading 8 bits (an instruction that issues in half the time: all
+// three rounded 353 us where this takes 342).
+template <int Z>
+__device__ __forceinline__ uint32_t take(float &x, float &y)
 {
-    return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    const uint32_t p = Z == 1 ? __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{x, y}), b2))
+                              : __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+    x -= __uint_as_float(Z == 1 ? p << 16 : __float_as_uint(x) & 0xffff0000u);
+    y -= __uint_as_float(Z == 1 ? p & 0xffff0000u : __float_as_uint(y) & 0xffff0000u);
+    return p;
+}
+
+// F(Z) for each of the parts.
+template <class F>
+__device__ __forceinline__ void each_part(F f)
+{
+    f(std::integral_constant<int, 0>());
+    f(std::integral_constant<int, 1>());
+    f(std::integral_constant<int, 2>());
 }
 
 // Eight numbers as three operands of the matrix cores.
-__device__ __forceinline__ void split8(u4 (&o)[3], const float (&x)[8])
+__device__ __forceinline__ void split8(u4 (&o)[3], float (&x)[8])
 {
+    each_part([&](auto z) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float r0 = rest_of(x[2 * i]), r1 = rest_of(x[2 * i + 1]);
-        o[0][i] = firsts(x[2 * i], x[2 * i + 1]);
-        o[1][i] = firsts(r0, r1);
-        o[2][i] = firsts(rest_of(r0), rest_of(r1));
-    }
+        for (int i = 0; i < 4; ++i) o[z][i] = take<z>(x[2 * i], x[2 * i + 1]);
+    });
 }
 
 __device__ __forceinline__ v4f mfma(u4 a, u4 b, v4f c)
@@ -797,34 +815,29 @@ __device__ __forceinline__ bool split_chunks(const ornk_linear_args &a, const Cu
     auto stage = [&](int p) {
         if (!loads) return;
         const int word = (4 * (ld >> 3) + (ld & 3)), half = ld >> 2 & 1;
-        auto rows = [&](uint32_t (&to)[SUMS ? 1 : 3][C][8 * KB], const float (&x)[4][4], int part) {
+        auto rows = [&](auto z, uint32_t (&to)[SUMS ? 1 : 3][C][8 * KB], float (&x)[4][4]) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int row = 4 * lr + e;
-                *reinterpret_cast<uint2 *>(&to[part][row][4 * (word ^ (row & M)) + 2 * half]) =
-                    uint2{firsts(x[e][0], x[e][1]), firsts(x[e][2], x[e][3])};
+                const uint32_t y0 = take<z>(x[e][0], x[e][1]), y1 = take<z>(x[e][2], x[e][3]);
+                *reinterpret_cast<uint2 *>(&to[z][row][4 * (word ^ (row & M)) + 2 * half]) = uint2{y0, y1};
             }
         };
+        each_part([&](auto z) {
+            if constexpr (!SUMS) {
+                float x[4][4];
 #pragma unroll
-        for (int part = 0; part < 3; ++part) {
-            if (part) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        kn[e][i] = rest_of(kn[e][i]);
-                        if (!SUMS) qn[e][i] = rest_of(qn[e][i]);
-                    }
-            }
-            if (!SUMS) {
-                rows(lds.K, kn, part);
-                if constexpr (!SUMS) rows(lds.Q, qn, part);
+                for (int i = 0; i < 16; ++i) (&x[0][0])[i] = (&kn[0][0])[i];
+                rows(z, lds.K, x);
+                rows(z, lds.Q, qn);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<uint2 *>(&lds.T[SUMS ? p : 0][part][ld][16 * i + 4 * (lr & 3) + 2 * (lr >> 2)]) =
-                    uint2{firsts(kn[0][i], kn[1][i]), firsts(kn[2][i], kn[3][i])};
-        }
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t y0 = take<z>(kn[0][i], kn[1][i]), y1 = take<z>(kn[2][i], kn[3][i]);
+                *reinterpret_cast<uint2 *>(&lds.T[SUMS ? p : 0][z][ld][16 * i + 4 * (lr & 3) + 2 * (lr >> 2)]) =
+                    uint2{y0, y1};
+            }
+        });
     };
     auto row_of = [&](const uint32_t (&from)[SUMS ? 1 : 3][C][8 * KB], int part, int row, int x) {
         return *reinterpret_cast<const u4 *>(&from[part][row][4 * ((4 * x + g) ^ (row & M))]);
@@ -874,12 +887,10 @@ __device__ __forceinline__ bool split_chunks(const ornk_linear_args &a, const Cu
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 y[r] = query >= key + r ? P0[r] * (exp2_of(G - d.G[key + r]) * d.b[key + r]) : 0.0f;
-#pragma unroll
-            for (int z = 0; z < 3; ++z) {
-                lds.P[i][z][lane] = uint2{firsts(y[0], y[1]), firsts(y[2], y[3])};
-#pragma unroll
-                for (int r = 0; r < 4; ++r) y[r] = rest_of(y[r]);
-            }
+            each_part([&](auto z) {
+                const uint32_t y0 = take<z>(y[0], y[1]), y1 = take<z>(y[2], y[3]);
+                lds.P[i][z][lane] = uint2{y0, y1};
+            });
         }
         if constexpr (!SUMS) {
 #pragma unroll
@@ -1062,16 +1073,17 @@ __global__ void __launch_bounds__(256) k_linear_join(ornk_linear_args a, Cut cut
     }
 }
 
-// Parts of a sequence that join those before them by themselves, which saves a launch (4 x
-// 2000, 16 heads of 128: 167 -> 158 us); more would read too much.
-constexpr int JOIN = 8;
+// Parts of a sequence that join those before them by themselves, which saves a launch (5 x
+// 333, 12 heads of 96 x 80: 40 -> 37 us); with 8 of them it takes longer (1 x 512, 32 heads of
+// 128: 48 us, by a launch 38).
+constexpr int JOIN = 4;
 
 // Sequences are cut where their heads and columns leave CUs idle: into parts of at
 // least 64 tokens, until there are two groups for each CU.  What the parts add to a state
 // is formed first, and their tokens after that from what they begin with, which takes 1.4
-// times the products.  One prompt of 8191 tokens, 16 heads of 128: 176 us (sums 57, joining
-// 15, tokens 115); with one group for each CU 196.  5 x 333, 12 heads of 96 x 80: 42; with
-// parts of 128 tokens 50 (of 64 45 then).
+// times the products.  One prompt of 8191 tokens, 16 heads of 128: 140 us (sums 40, joining
+// 15, tokens 92); with one group for each CU 153.  5 x 333, 12 heads of 96 x 80: 37; with
+// parts of 128 tokens 47.
 Cut cut_of(const ornk_linear_args &a, int cb)
 {
     const long long groups = (long long)a.n_seqs * a.heads * ((a.dv + 64 * cb - 1) / (64 * cb));
@@ -1087,8 +1099,8 @@ Cut cut_of(const ornk_linear_args &a, int cb)
 
 // Blocks of 16 columns of a wave: two, where there is then a group for each CU, and the
 // state's registers leave room for another group.  Two share a group's P and its waits (one
-// prompt of 8191 tokens, 16 heads of 128: 176 us, with one block 198); one gives twice the
-// groups (5 x 333, 12 heads of 96 x 80: 53, with two 74).
+// prompt of 8191 tokens, 16 heads of 128: 140 us, with one block 150); one gives twice the
+// groups (1 x 512, 16 heads of 128: 26, with two 36).
 int blocks_of(const ornk_linear_args &a)
 {
     if (a.dv <= 64 || a.dk > 128) return 1;

@@ -16,7 +16,8 @@ GPU: each call against its definition in 64 bits.  With e = 2^-24 (half a step o
           to 2^-40, is off by at most 4 e, products by 4 e in all, and the chains of at most
           2 L + dk sums by independent roundings, whose 6 standard deviations are below
           6 sqrt(2 L + dk) e.  Chains of decays (token by token, or chunk by chunk) round
-          twice for each of L tokens: in that sum.
+          twice for each of L tokens: in that sum.  So is what products of bf16 parts leave
+          out, less than 4 e of each and of either sign (its deviation is below e).
   sample  tokens are equal.  A weight is rounded to 2^-45 of the largest or finer at the sizes
           here (up to 2^17 tokens), a sum of n of them is off by at most n 2^-46, a border (a
           share of one) by as much: where the 64-bit sums come within n 2^-44 of a border of
@@ -634,6 +635,41 @@ def test_linear_keeps_later_tokens_out(om, ctx, dk, dv):
         o, _ = _linear_run(om, ctx, [L], H, 1, 1, 2, dk, dv, q, k, v, d, S, [0], [1])
         assert torch.isfinite(o[:at]).all() and torch.isnan(o[at:, 0]).all()
         assert torch.isfinite(o[:, 1]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("L", [200, 700, 1500])
+@pytest.mark.parametrize("dk,dv", [(128, 128), (64, 40), (96, 80), (33, 47)])
+def test_linear_parts_that_are_not_finite(om, ctx, L, dk, dv):
+    """In a sequence that is cut, in place: what is finite is right beside what is not."""
+    H, at, lens = 2, 130, [L, 90]
+    g, q, k, v, decay = _linear_inputs(lens, H, 1, 2, 2, dk, dv, "token", L + dk)
+    S = torch.randn(2, H, dk, dv, generator=g)
+    want, bound, ends, eb = _linear64(q, k, v, decay, [0, L, L + 90], S, dk ** -0.5, False)
+    c = (8 + 6 * math.sqrt(2 * L + dk)) * EPS
+    v[at, 0, 3], v[at + 1, 0, 5] = math.inf, math.nan
+    o, S1 = _linear_run(om, ctx, lens, H, 1, 2, 2, dk, dv, q, k, v, decay, S, [0, 1], [0, 1], in_place=True)
+    bad = torch.zeros(L + 90, H, dv, dtype=torch.bool)
+    bad[at:L, 0, 3] = bad[at + 1:L, 0, 5] = True
+    assert not torch.isfinite(o[bad]).any() and not torch.isfinite(S1[0, 0][:, [3, 5]]).any()
+    _close(o[~bad], want[~bad], bound[~bad] * c)
+    S1[0, 0][:, [3, 5]] = 0.0
+    ends[0, 0][:, [3, 5]] = 0.0
+    _close(S1, ends, eb * c + 1e-37)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** 100])
+def test_linear_of_small_and_large_values(om, ctx, scale):
+    """V and the state by a power of two: the same digits."""
+    H, L, d = 2, 300, 128
+    g, q, k, v, decay = _linear_inputs([L], H, 2, 2, 2, d, d, "head", 12)
+    S = torch.randn(1, H, d, d, generator=g)
+    want, bound, ends, eb = _linear64(q, k, v * scale, decay, [0, L], S * scale, d ** -0.5, False)
+    c = (8 + 6 * math.sqrt(2 * L + d)) * EPS
+    o, S1 = _linear_run(om, ctx, [L], H, 2, 2, 2, d, d, q, k, v * scale, decay, S * scale, [0], [0], in_place=True)
+    _close(o, want, bound * c)
+    _close(S1, ends, eb * c)
 
 
 @pytest.mark.gpu
