@@ -138,7 +138,7 @@ void launch_step(const ornk_linear_args &a, hipStream_t s)
 // With fp32 operands it was bound by the matrix cores, which take 15 ns for a 16x16x4
 // product of a SIMD (140 TFLOP/s): 24 x up to 1501 tokens, 32 heads of 128 (18,210 tokens in
 // all) 431 us.  With three bf16 parts (8 ns for 16x16x32, six products) it takes 342: 1.27 GB
-// are moved at 3.7 TB/s, and each wave's 240 matrix instructions and 1100 others of a chunk
+// are moved at 3.7 TB/s, and each wave's 232 matrix instructions and 1150 others of a chunk
 // wait for three barriers, with one other group on the CU.  C = 32 costs 19 % more than the recurrence (P, P V).
 // Later loads of V, K and Q staged before S's products, and heads that share K and Q on one
 // XCD made no difference.
