@@ -139,9 +139,9 @@ void launch_step(const ornk_linear_args &a, hipStream_t s)
 // product of a SIMD (140 TFLOP/s): 24 x up to 1501 tokens, 32 heads of 128 (18,210 tokens in
 // all) 431 us.  With three bf16 parts (8 ns for 16x16x32, six products) it takes 342: 1.27 GB
 // are moved at 3.7 TB/s, and each wave's 232 matrix instructions and 1150 others of a chunk
-// wait for three barriers, with one other group on the CU.  C = 32 costs 19 % more than the recurrence (P, P V).
-// Later loads of V, K and Q staged before S's products, and heads that share K and Q on one
-// XCD made no difference.
+// wait for three barriers, with one other group on the CU.  C = 32 costs 19 % more than the
+// recurrence (P, P V).  Later loads of V, addresses of whole chunks kept apart, K and Q
+// staged before S's products, and heads that share K and Q on one XCD made no difference.
 constexpr int C = 32;
 
 struct alignas(16) Decays {
