@@ -234,9 +234,12 @@ int gpu_kv_evict(gpu_context *ctx, const ornith_kv_pages *kv, int n_seqs, const 
  *
  * Sums and states are of 32 bits; a prompt's tokens are taken together in chunks,
  * whose decays are summed in 64 and whose products are of operands of 24 bits (fewer
- * below 2^-110).  What a token holds has no effect on those before it, NaN and
+ * below 2^-110).  What decays leave of a large number keeps its digits however small
+ * the factor is; where none before it passes 2^16, what they take below 2^-88 may be
+ * lost.  q k and q S of a prompt are formed before the decays, and have to be numbers of
+ * 32 bits themselves.  What a token holds has no effect on those before it, NaN and
  * infinities included, but for their last digits: a stretch with a result that is not
- * finite is done with other instructions.  A slot outside [-1, n_slots), or tokens outside
+ * finite, or with large numbers that decay far, is done with other instructions.  A slot outside [-1, n_slots), or tokens outside
  * [0, n_tokens) or more than max_len, leave their sequence out (gpu_kv_check). */
 typedef struct {
     gpu_buffer *S; /* [n_slots][n_heads][key_dim][value_dim] fp32; NULL without slots */

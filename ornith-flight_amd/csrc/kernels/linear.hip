@@ -40,6 +40,38 @@ __device__ __forceinline__ Seq seq_of(const ornk_linear_args &a, int b)
     return s;
 }
 
+// 2^x for x <= 0 (or the formula's overflow): the part of x that fp32 leaves out counts, too.
+// Relative error 2^-23 from 2^-126 on; below it is 0.
+__device__ __forceinline__ float exp2_of(double x)
+{
+    const float hi = (float)x, lo = (float)(x - (double)hi);
+    const float e = __builtin_amdgcn_exp2f(hi);
+    return fmaf(e, lo * 0.693147181f, e);
+}
+
+// 2^x as m 2^e, for what is large enough to leave something below that: e is 0 but for x
+// from -1024 to -126.
+struct Factor {
+    float m;
+    int e;
+};
+
+__device__ __forceinline__ int exponent_of(double x) { return x < -126.0 && x > -1024.0 ? (int)ceil(x) : 0; }
+
+__device__ __forceinline__ Factor factor_of(double x)
+{
+    const int e = exponent_of(x);
+    return {exp2_of(x - e), e};
+}
+
+// Token i's decay of a chunk in base 2: 0 behind its n tokens.  Where 2^x is 0 a
+// smaller x changes nothing but the sums' digits.
+__device__ __forceinline__ double decay2(float decay, bool on)
+{
+    const double x = (double)decay * 1.4426950408889634;
+    return !on ? 0.0 : x < -16384.0 ? -16384.0 : x;
+}
+
 // One token of each sequence (or none): V columns per lane, L lanes to a row of the
 // state, 256 / L rows at a time and up to 16 of them in flight per thread.  q and k come
 // through LDS, and the row groups' shares of q S meet there.  Bound by memory, the state in
@@ -62,6 +94,7 @@ __global__ void __launch_bounds__(256) k_linear_step(ornk_linear_args a)
     float *to = seq.out >= 0 ? a.S + ((size_t)seq.out * a.heads + h) * size + col : nullptr;
     const bool on = col < a.dv;
     float f = 1.0f;
+    int exponent = 0;
     vec v = 0.0f, o = 0.0f;
     if (!seq.n && tid < a.dk) q[tid] = k[tid] = 0.0f;
     if (seq.n) {
@@ -71,7 +104,9 @@ __global__ void __launch_bounds__(256) k_linear_step(ornk_linear_args a)
         }
         if (on) v = *reinterpret_cast<const vec *>(a.v + (t * a.vh + h / (a.heads / a.vh)) * a.dv + col);
         const float decay = a.decay[a.per_token ? t * a.heads + h : h];
-        f = expf(decay);
+        const double x = decay2(decay, true);
+        exponent = __builtin_amdgcn_readfirstlane(exponent_of(x));
+        f = exponent ? exp2_of(x - exponent) : expf(decay);
         if (a.complement) v *= -expm1f(decay);
     }
     vec s[R];
@@ -91,9 +126,14 @@ __global__ void __launch_bounds__(256) k_linear_step(ornk_linear_args a)
             const int r = r0 + g + G * i;
             if (r < a.dk) {
                 const float kr = k[r], qr = q[r];
+                if (exponent)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) s[i][e] = ldexpf(f * s[i][e], exponent);
+                else
+                    s[i] *= f;
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    s[i][e] = fmaf(kr, v[e], f * s[i][e]);
+                    s[i][e] = fmaf(kr, v[e], s[i][e]);
                     o[e] = fmaf(qr, s[i][e], o[e]);
                 }
                 if (to && on) *reinterpret_cast<vec *>(to + (size_t)r * a.dv) = s[i];
@@ -144,30 +184,25 @@ void launch_step(const ornk_linear_args &a, hipStream_t s)
 // staged before S's products, and heads that share K and Q on one XCD made no difference.
 constexpr int C = 32;
 
+// A chunk is far where its decays together are below 2^FAR: factors times small numbers lose
+// digits there, and below 2^-126 they are 0, which shows in what large numbers leave.  So where
+// one of its numbers passes 2^16 (if none does, what is lost is below 2^-94 of each token), its
+// part is done again in chunks that end before they are far: within those no factor is small
+// but the first token's, which the state alone takes, as a mantissa and an exponent.  Looking
+// for large numbers takes 1 to 3 % (4 x 2000, 8 heads of 256 x 256 287 -> 301 us), chunks cut so
+// from the start twice as long where decays are strong (548).
+constexpr double FAR = -64.0;
+constexpr float LARGE = 65536.0f;
+
 struct alignas(16) Decays {
-    double G[C];
-    float q[C];  // 2^G_i scale
+    double G[C]; // behind the chunk's last token as there
+    float q[C];  // 2^G_i scale (in chunks that are cut the mantissa)
     float k[C];  // 2^(G_C - G_j) b_j
     float b[C];  // b_j scale
-    float all;   // 2^G_C
+    float all;   // 2^G_C (or its mantissa)
+    int far;
+    int n;       // tokens
 };
-
-// 2^x for x <= 0 (or the formula's overflow), relative error 2^-23: the part of x that
-// fp32 leaves out counts, too
-__device__ __forceinline__ float exp2_of(double x)
-{
-    const float hi = (float)x, lo = (float)(x - (double)hi);
-    const float e = __builtin_amdgcn_exp2f(hi);
-    return fmaf(e, lo * 0.693147181f, e);
-}
-
-// Token i's decay of a chunk in base 2: 0 behind its n tokens.  Where 2^x is 0 a
-// smaller x changes nothing but the sums' digits.
-__device__ __forceinline__ double decay2(float decay, bool on)
-{
-    const double x = (double)decay * 1.4426950408889634;
-    return !on ? 0.0 : x < -16384.0 ? -16384.0 : x;
-}
 
 // x of the lane that a DPP step names, 0 where there is none or its row takes none
 template <int CTRL, int ROWS>
@@ -179,23 +214,55 @@ __device__ __forceinline__ double dpp(double x)
     return __longlong_as_double((uint64_t)hi << 32 | lo);
 }
 
-// One wave, lanes i and i + 32 alike: the chunk's sums and factors.
-__device__ __forceinline__ double fill_decays(const ornk_linear_args &a, Decays &d, double x, bool on)
+// The sum of x up to each lane's, lanes i and i + 32 alike.
+__device__ __forceinline__ double sums(double x)
+{
+    x += dpp<0x111, 0xf>(x);  // row_shr:1
+    x += dpp<0x112, 0xf>(x);
+    x += dpp<0x114, 0xf>(x);
+    x += dpp<0x118, 0xf>(x);
+    x += dpp<0x142, 0xa>(x);  // row_bcast:15, the second row of each half
+    return x;
+}
+
+__device__ __forceinline__ double lane_of(double x, int lane)
+{
+    const uint64_t u = __double_as_longlong(x);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+    const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+    return __longlong_as_double((uint64_t)hi << 32 | lo);
+}
+
+// One wave, lanes i and i + 32 alike: the sums and factors of a chunk of up to n tokens; with
+// CUT only as many of them as are not far.  The chunk's sum.
+template <bool CUT>
+__device__ __forceinline__ double fill_decays(const ornk_linear_args &a, Decays &d, double x, int &n)
 {
     const int i = threadIdx.x & (C - 1);
-    double G = x;
-    G += dpp<0x111, 0xf>(G);  // row_shr:1
-    G += dpp<0x112, 0xf>(G);
-    G += dpp<0x114, 0xf>(G);
-    G += dpp<0x118, 0xf>(G);
-    G += dpp<0x142, 0xa>(G);  // row_bcast:15, the second row of each half
-    const double end = __shfl(G, C - 1, C);
-    const float b = !on ? 0.0f : a.complement ? -expm1f((float)(x * 0.6931471805599453)) : 1.0f;
+    double G = sums(x), span = G;  // span: without growth, and without what clears any state
+    double end = lane_of(G, C - 1);
+    const bool plain = x <= 0.0 && x > -300.0;
+    bool far = end < FAR;
+    if (__any(!plain)) {
+        span = sums(plain ? x : 0.0);
+        far = lane_of(span, C - 1) < FAR;
+    }
+    if (CUT && far) {
+        const uint32_t near = (uint32_t)__ballot(i == 0 || span - lane_of(span, 0) >= FAR);
+        n = min(n, __builtin_ctzll(~(uint64_t)near));
+        end = lane_of(G, n - 1);
+        if (i >= n) G = end;
+    }
+    const float b = i >= n ? 0.0f : a.complement ? -expm1f((float)(x * 0.6931471805599453)) : 1.0f;
     d.G[i] = G;
-    d.q[i] = exp2_of(G) * a.scale;
+    d.q[i] = (CUT && far ? factor_of(G).m : exp2_of(G)) * a.scale;
     d.k[i] = exp2_of(end - G) * b;
     d.b[i] = b * a.scale;
-    if (!i) d.all = exp2_of(end);
+    if (!i) {
+        d.all = CUT && far ? factor_of(end).m : exp2_of(end);
+        d.far = far;
+        d.n = n;
+    }
     return end;
 }
 
@@ -206,7 +273,7 @@ struct Cut {
     bool joined;       // by a launch of its own; else each part joins those before it
     float *states;     // [n_seqs][heads][segs][dk][dv]: what a part adds, then (joined) what it
                        // begins with; of the last part what the sequence begins with
-    float *decays;     // [n_seqs][heads][segs]: what a part leaves of a state
+    Factor *decays;    // [n_seqs][heads][segs]: what a part leaves of a state
 };
 
 // N floats at p; without VEC only those before `left`, and 0 for the others.
@@ -325,8 +392,15 @@ __device__ __forceinline__ bool begin_state(const ornk_linear_args &a, const Cut
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int j = 0; j < CB; ++j) S[kb][j] = v4f{0, 0, 0, 0};
-    auto add = [&](const float *y, float keep) {  // all loads on their way at once
+    auto add = [&](const float *y, Factor keep) {  // all loads on their way at once
         float x[KB][4][CB];
+        if (__builtin_amdgcn_readfirstlane(keep.e))
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int j = 0; j < CB; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) S[kb][j][r] = ldexpf(S[kb][j][r], keep.e);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -337,9 +411,9 @@ __device__ __forceinline__ bool begin_state(const ornk_linear_args &a, const Cut
 #pragma unroll
             for (int r = 0; r < 4; ++r)
 #pragma unroll
-                for (int j = 0; j < CB; ++j) S[kb][j][r] = fmaf(keep, S[kb][j][r], x[kb][r][j]);
+                for (int j = 0; j < CB; ++j) S[kb][j][r] = fmaf(keep.m, S[kb][j][r], x[kb][r][j]);
     };
-    if (from && cols > 0) add(from, 0.0f);
+    if (from && cols > 0) add(from, {0.0f, 0});
     const bool joins = !SUMS && cut.segs > 1 && !cut.joined;
     if (joins) {
 #pragma unroll 1
@@ -392,9 +466,22 @@ struct Exact {
     __align__(16) Decays dec[2];
 };
 
-// With fp32 operands: what 32-bit arithmetic gives, infinities and NaN included.
-template <int KB, int CB, bool VEC, bool SUMS>
-__device__ __forceinline__ void exact_chunks(const ornk_linear_args &a, const Cut &cut, const Part &part, Exact<KB, SUMS> &lds)
+__device__ __forceinline__ float larger(float most, float x) { return fmaxf(most, fabsf(x)); }
+
+template <int KB, int CB>
+__device__ __forceinline__ float largest(float most, const float (&v)[2][4][CB], const v4f (&S)[KB][CB])
+{
+#pragma unroll
+    for (int i = 0; i < 8 * CB; ++i) most = larger(most, (&v[0][0][0])[i]);
+#pragma unroll
+    for (int i = 0; i < 4 * KB * CB; ++i) most = larger(most, S[i / (4 * CB)][i / 4 % CB][i & 3]);
+    return most;
+}
+
+// With fp32 operands: what 32-bit arithmetic gives, infinities and NaN included.  CUT: chunks
+// end before they are far.  false: they have to, and nothing of the state is stored.
+template <int KB, int CB, bool VEC, bool SUMS, bool CUT>
+__device__ __forceinline__ bool exact_chunks(const ornk_linear_args &a, const Cut &cut, const Part &part, Exact<KB, SUMS> &lds)
 {
     constexpr int LD = Exact<KB, SUMS>::LD, NK = Exact<KB, SUMS>::NK;
     constexpr int RS = 64 / KB;        // rows that the threads load at a time, a float4 each
@@ -424,7 +511,10 @@ __device__ __forceinline__ void exact_chunks(const ornk_linear_args &a, const Cu
     float *op = a.out + ((size_t)seq.t0 + first) * os + h * a.dv;
     const uint32_t lcv = VEC && left_k <= 0 ? 0 : lc, colv = VEC && cols <= 0 ? 0 : col0;
     float kn[NL][4], qn[SUMS ? 1 : NL][4], v[2][4][CB], vn[2][4][CB];
-    auto fetch = [&](int n) {  // K and Q of the next chunk, of which n tokens are left
+    // K and Q of the next chunk, `skip` tokens behind this one's first; n are left from there on
+    auto fetch = [&](int n, int skip) {
+        kp += skip * ks;
+        qp += skip * qs;
         const uint32_t ko = lr * (uint32_t)ks + lcv, qo = lr * (uint32_t)qs + lcv;
         if (VEC && n >= C) {
 #pragma unroll
@@ -443,10 +533,9 @@ __device__ __forceinline__ void exact_chunks(const ornk_linear_args &a, const Cu
                     for (int e = 0; e < 4; ++e) kn[i][e] = 0.0f;
             }
         }
-        kp += C * ks;
-        qp += C * qs;
     };
-    auto fetch_v = [&](int n) {
+    auto fetch_v = [&](int n, int skip) {
+        vp += skip * vs;
         const uint32_t vo = 4 * g * (uint32_t)vs + colv;
         if (VEC && n >= C) {
 #pragma unroll
@@ -465,7 +554,6 @@ __device__ __forceinline__ void exact_chunks(const ornk_linear_args &a, const Cu
                         for (int j = 0; j < CB; ++j) vn[tb][r][j] = 0.0f;
                 }
         }
-        vp += C * vs;
     };
     float xn = 0.0f;     // wave 3: a decay of the chunk that it sums next
     double left = 0.0;   // and the part's sum
@@ -475,12 +563,18 @@ __device__ __forceinline__ void exact_chunks(const ornk_linear_args &a, const Cu
         xn = a.decay[a.per_token ? tok * a.heads + h : h];
     };
     auto fill = [&](int p, int t) {
-        const bool on = (lane & (C - 1)) < last - t;
-        left += fill_decays(a, dec[p], decay2(xn, on), on);
-        if (t + C < last) fetch_decays(t + C);
+        int n = min(C, last - t);
+        const double x = decay2(xn, (lane & (C - 1)) < n);
+        left += fill_decays<CUT>(a, dec[p], x, n);
+        if (t + n < last) fetch_decays(t + n);
     };
+    float own_k = 0.0f;  // the largest of the K staged
     auto stage_k = [&](int p) {
+        own_k = 0.0f;
         if (left_k <= 0) return;
+        if (!CUT)
+#pragma unroll
+            for (int i = 0; i < 4 * NL; ++i) own_k = larger(own_k, kn[i >> 2][i & 3]);
 #pragma unroll
         for (int i = 0; i < NL; ++i)
             *reinterpret_cast<v4f *>(&Ks[p & (NK - 1)][lr + i * RS][lc]) = v4f{kn[i][0], kn[i][1], kn[i][2], kn[i][3]};
@@ -492,11 +586,12 @@ __device__ __forceinline__ void exact_chunks(const ornk_linear_args &a, const Cu
             *reinterpret_cast<v4f *>(&Qs[lr + i * RS][lc]) = v4f{qn[i][0], qn[i][1], qn[i][2], qn[i][3]};
     };
 
-    int p = 0;
+    float most = 0.0f;  // the largest of far chunks' numbers
+    int p = 0, n = C;
     if (first < last) {
-        fetch(last - first);
+        fetch(last - first, 0);
         if (w == 3) fetch_decays(first);
-        fetch_v(last - first);
+        fetch_v(last - first, 0);
         if (w == 3) fill(0, first);
         if (left_k <= 0) {  // columns behind the key's dimensions stay 0
             const v4f z = {0, 0, 0, 0};
@@ -509,20 +604,34 @@ __device__ __forceinline__ void exact_chunks(const ornk_linear_args &a, const Cu
         stage_k(0);
         stage_q();
     }
-    for (int t = first; t < last; t += C, p ^= 1) {
-        const bool more = t + C < last;
-        const float(*const K)[LD] = Ks[p & (NK - 1)];
+    for (int t = first; t < last; t += n, p ^= 1) {
+        float(*const K)[LD] = Ks[p & (NK - 1)];
         __syncthreads();
+        const Decays &d = dec[p];
+        if (CUT) n = __builtin_amdgcn_readfirstlane(d.n);
+        const bool more = t + n < last, far = CUT && __builtin_amdgcn_readfirstlane(d.far);
+        float own = own_k;  // the largest of this chunk's
 #pragma unroll
         for (int i = 0; i < 8 * CB; ++i) (&v[0][0][0])[i] = (&vn[0][0][0])[i];
-        if (more) {
-            fetch(last - t - C);
-            fetch_v(last - t - C);
+        if (CUT && n < C && more) {  // cut: the tokens behind are the next chunk's
+            if (left_k > 0)
+#pragma unroll
+                for (int i = 0; i < NL; ++i)
+                    if (lr + i * RS >= n) *reinterpret_cast<v4f *>(&K[lr + i * RS][lc]) = v4f{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (16 * (i >> 2) + 4 * g + (i & 3) >= n)
+#pragma unroll
+                    for (int j = 0; j < CB; ++j) v[i >> 2][i & 3][j] = 0.0f;
+            __syncthreads();
         }
-        const Decays &d = dec[p];
+        if (more) {
+            fetch(last - t - n, n);
+            fetch_v(last - t - n, n);
+        }
         v4f O[2][CB];
         if (w == 3) {
-            if (more) fill(p ^ 1, t + C);
+            if (more) fill(p ^ 1, t + n);
         } else if (!SUMS) {
             const int i = w, query = 16 * (i > 0) + c, key = 16 * (i > 1) + 4 * g;
             const float *kr = K[16 * (i > 1) + c], *qr = Qs[16 * (i > 0) + c];
@@ -551,6 +660,9 @@ __device__ __forceinline__ void exact_chunks(const ornk_linear_args &a, const Cu
                 }
             }
             P0 += P1;
+            if (!CUT)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) own = larger(own, P0[r]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) P0[r] = query >= key + r ? P0[r] * f[r] : 0.0f;
             Ps[i][lane] = P0;
@@ -583,8 +695,18 @@ __device__ __forceinline__ void exact_chunks(const ornk_linear_args &a, const Cu
 #pragma unroll
             for (int ib = 0; ib < 2; ++ib) {
                 const v4f f = *reinterpret_cast<const v4f *>(&d.q[16 * ib + 4 * g]);
+                if (!CUT)
+#pragma unroll
+                    for (int i = 0; i < 4 * CB; ++i) own = larger(own, O[ib][i >> 2][i & 3]);
 #pragma unroll
                 for (int j = 0; j < CB; ++j) O[ib][j] *= f;
+                if (CUT && far)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int exponent = exponent_of(d.G[16 * ib + 4 * g + r]);
+#pragma unroll
+                        for (int j = 0; j < CB; ++j) O[ib][j][r] = ldexpf(O[ib][j][r], exponent);
+                    }
             }
         }
         __syncthreads();
@@ -616,7 +738,7 @@ __device__ __forceinline__ void exact_chunks(const ornk_linear_args &a, const Cu
                     add_in_order(O[0], P0, v[0]);
                     add_in_order(O[1], P2, v[1]);
                 }
-                const int n = last - t;
+                const int rows = CUT ? n : last - t;
                 const uint32_t oo = 4 * g * (uint32_t)os + col0;
                 auto put = [&](int ib, int r) {
                     float x[CB];
@@ -625,20 +747,32 @@ __device__ __forceinline__ void exact_chunks(const ornk_linear_args &a, const Cu
                     store<CB, VEC>(op + (16 * ib + r) * os + oo, x, cols);
                 };
                 if (cols > 0) {
-                    if (n >= C) {
+                    if (rows >= C) {
 #pragma unroll
                         for (int i = 0; i < 8; ++i) put(i >> 2, i & 3);
                     } else {
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
-                            if (16 * (i >> 2) + 4 * g + (i & 3) < n) put(i >> 2, i & 3);
+                            if (16 * (i >> 2) + 4 * g + (i & 3) < rows) put(i >> 2, i & 3);
                     }
                 }
-                op += C * os;
+                op += n * os;
             }
+        }
+        if (!CUT && __builtin_amdgcn_readfirstlane(d.far)) {
+            if (busy) own = largest(own, v, S);
+            most = fmaxf(most, own);
         }
         if (busy && (more || stored)) {
             const float all = d.all;
+            if (CUT && far) {
+                const int exponent = exponent_of(d.G[C - 1]);
+#pragma unroll
+                for (int i = 0; i < 4 * KB * CB; ++i) {
+                    float y = S[i / (4 * CB)][i / 4 % CB][i & 3];
+                    S[i / (4 * CB)][i / 4 % CB][i & 3] = ldexpf(y, exponent);
+                }
+            }
 #pragma unroll
             for (int tb = 0; tb < 2; ++tb) {
                 const v4f f = *reinterpret_cast<const v4f *>(&d.k[16 * tb + 4 * g]);
@@ -668,15 +802,17 @@ __device__ __forceinline__ void exact_chunks(const ornk_linear_args &a, const Cu
         }
     }
 
-    if (SUMS && tid == 192 && !block) cut.decays[part.at + part.sg] = exp2_of(left);
+    if (!CUT && __syncthreads_or(most > LARGE)) return false;
+    if (SUMS && tid == 192 && !block) cut.decays[part.at + part.sg] = factor_of(left);
     if (stored) end_state<KB, CB, VEC>(a, state_of<SUMS>(a, cut, part), col0, S);
+    return true;
 }
 
 // With operands of three bf16 parts, which hold the 24 bits of an fp32 number (of those
 // below 2^-110 fewer), and the six products of parts that reach its last bit: what is left
 // out is at most 2^-22 of a product.  16 x the rate, so 2.7 x the speed.  Parts of an
 // infinity are no numbers, so whatever is not finite shows in the results, and the part is
-// done again with fp32 operands.
+// done again with fp32 operands, as where a far chunk's numbers are large.
 template <int KB, bool SUMS>
 struct Split {
     // [part][row][pair of dimensions]: of 32 dimensions those that a lane group of the
@@ -734,7 +870,7 @@ __device__ __forceinline__ v4f mfma(u4 a, u4 b, v4f c)
 // The parts of a product, the small ones first.
 #define PRODUCTS(F) F(0, 2) F(2, 0) F(1, 1) F(0, 1) F(1, 0) F(0, 0)
 
-// false: something was not finite, and nothing of the state is stored.
+// false: something was not finite, or large in a far chunk, and nothing of the state is stored.
 template <int KB, int CB, bool SUMS>
 __device__ __forceinline__ bool split_chunks(const ornk_linear_args &a, const Cut &cut, const Part &part, Split<KB, SUMS> &lds)
 {
@@ -808,12 +944,16 @@ __device__ __forceinline__ bool split_chunks(const ornk_linear_args &a, const Cu
         xn = a.decay[a.per_token ? tok * a.heads + h : h];
     };
     auto fill = [&](int p, int t) {
-        const bool on = (lane & (C - 1)) < last - t;
-        left += fill_decays(a, lds.dec[p], decay2(xn, on), on);
+        int n = min(C, last - t);
+        left += fill_decays<false>(a, lds.dec[p], decay2(xn, (lane & (C - 1)) < n), n);
         if (t + C < last) fetch_decays(t + C);
     };
+    float own = 0.0f;  // the largest of this chunk's
     auto stage = [&](int p) {
+        own = 0.0f;
         if (!loads) return;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) own = larger(own, kn[i >> 2][i & 3]);
         const int word = (4 * (ld >> 3) + (ld & 3)), half = ld >> 2 & 1;
         auto rows = [&](auto z, uint32_t (&to)[SUMS ? 1 : 3][C][8 * KB], float (&x)[4][4]) {
 #pragma unroll
@@ -843,7 +983,8 @@ __device__ __forceinline__ bool split_chunks(const ornk_linear_args &a, const Cu
         return *reinterpret_cast<const u4 *>(&from[part][row][4 * ((4 * x + g) ^ (row & M))]);
     };
 
-    float bad = 0.0f;  // 0, or a NaN
+    float bad = 0.0f;   // 0, or a NaN
+    float most = 0.0f;  // the largest of far chunks' numbers
     int p = 0;
     if (first < last) {
         fetch(last - first);
@@ -882,6 +1023,8 @@ __device__ __forceinline__ bool split_chunks(const ornk_linear_args &a, const Cu
 #undef F
             }
             P0 += P1;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) own = larger(own, P0[r]);
             const double G = d.G[query];
             float y[4];
 #pragma unroll
@@ -926,6 +1069,8 @@ __device__ __forceinline__ bool split_chunks(const ornk_linear_args &a, const Cu
                 for (int ib = 0; ib < 2; ++ib) {
                     const v4f f = *reinterpret_cast<const v4f *>(&d.q[16 * ib + 4 * g]);
 #pragma unroll
+                    for (int i = 0; i < 4 * CB; ++i) own = larger(own, O[ib][i >> 2][i & 3]);
+#pragma unroll
                     for (int j = 0; j < CB; ++j) O[ib][j] *= f;
                 }
             }
@@ -969,6 +1114,10 @@ __device__ __forceinline__ bool split_chunks(const ornk_linear_args &a, const Cu
                 }
                 op += C * os;
             }
+        }
+        if (__builtin_amdgcn_readfirstlane(d.far)) {
+            if (busy) own = largest(own, v, S);
+            most = fmaxf(most, own);
         }
         if (busy && (more || stored)) {
             const float all = d.all;
@@ -1016,8 +1165,8 @@ __device__ __forceinline__ bool split_chunks(const ornk_linear_args &a, const Cu
 #pragma unroll
                 for (int r = 0; r < 4; ++r) bad = fmaf(S[kb][j][r], 0.0f, bad);
     }
-    if (__syncthreads_or(bad != bad)) return false;
-    if (SUMS && tid == 192 && !block) cut.decays[part.at + part.sg] = exp2_of(left);
+    if (__syncthreads_or(bad != bad || most > LARGE)) return false;
+    if (SUMS && tid == 192 && !block) cut.decays[part.at + part.sg] = factor_of(left);
     if (stored) end_state<KB, CB, true>(a, state_of<SUMS>(a, cut, part), col0, S);
     return true;
 }
@@ -1051,7 +1200,9 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
     }
     if constexpr (FAST)
         if (split_chunks<KB, CB, SUMS>(a, cut, part, lds.split)) return;
-    exact_chunks<KB, CB, VEC, SUMS>(a, cut, part, lds.exact);
+    if constexpr (!FAST)
+        if (exact_chunks<KB, CB, VEC, SUMS, false>(a, cut, part, lds.exact)) return;
+    exact_chunks<KB, CB, VEC, SUMS, true>(a, cut, part, lds.exact);
 }
 
 // From what each part adds to what each part begins with, an element per thread (16 heads
@@ -1067,9 +1218,10 @@ __global__ void __launch_bounds__(256) k_linear_join(ornk_linear_args a, Cut cut
     for (int i = 0; i == 0 || i * cut.len < seq.n; ++i) {
         float *p = cut.states + (at + i) * size + e;
         const bool more = (i + 1) * cut.len < seq.n;
-        const float add = more ? *p : 0.0f, keep = more ? cut.decays[at + i] : 0.0f;
+        const float add = more ? *p : 0.0f;
+        const Factor keep = more ? cut.decays[at + i] : Factor{0.0f, 0};
         *p = s;
-        s = fmaf(keep, s, add);
+        s = keep.e ? ldexpf(keep.m * s, keep.e) + add : fmaf(keep.m, s, add);
     }
 }
 
@@ -1133,7 +1285,8 @@ void launch(const ornk_linear_args &a, const Cut &cut, hipStream_t s)
 extern "C" size_t ornk_linear_ws(const ornk_linear_args *a)
 {
     const Cut c = cut_of(*a, blocks_of(*a));
-    return c.segs < 2 ? 0 : sizeof(float) * a->n_seqs * a->heads * c.segs * ((size_t)a->dk * a->dv + 1);
+    if (c.segs < 2) return 0;
+    return (size_t)a->n_seqs * a->heads * c.segs * (sizeof(float) * a->dk * a->dv + sizeof(Factor));
 }
 
 extern "C" int ornk_linear(const ornk_linear_args *a, hipStream_t s)
@@ -1147,7 +1300,8 @@ extern "C" int ornk_linear(const ornk_linear_args *a, hipStream_t s)
     const int cb = blocks_of(*a);
     Cut c = cut_of(*a, cb);
     c.states = static_cast<float *>(a->ws);
-    if (c.segs > 1) c.decays = c.states + (size_t)a->n_seqs * a->heads * c.segs * a->dk * a->dv;
+    if (c.segs > 1)
+        c.decays = reinterpret_cast<Factor *>(c.states + (size_t)a->n_seqs * a->heads * c.segs * a->dk * a->dv);
     if (a->dk > 128) launch<16, 1>(*a, c, s);
     else if (cb == 2) a->dk > 64 ? launch<8, 2>(*a, c, s) : launch<4, 2>(*a, c, s);
     else a->dk > 64 ? launch<8, 1>(*a, c, s) : launch<4, 1>(*a, c, s);
