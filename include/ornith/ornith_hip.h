@@ -131,7 +131,8 @@ int gpu_kv_append(gpu_context *ctx, const ornith_kv_pages *kv, const gpu_buffer 
 
 /* Norms of the heads, taken before the rotation: a row x of head_dim becomes
  * w x / sqrt(mean(x^2) + eps) (ORN_NORM_RMS) or w x / sqrt(sum(x^2) + eps)
- * (ORN_NORM_L2), with 32-bit sums.  Weights are [head_dim] for all heads, or
+ * (ORN_NORM_L2), with 32-bit sums; where squares pass the largest number or lose digits
+ * below the least, of a multiple of the row.  Weights are [head_dim] for all heads, or
  * [heads][head_dim] with per_head; NULL: 1. */
 enum { ORN_NORM_RMS = 0, ORN_NORM_L2 = 1 };
 typedef struct {

@@ -49,23 +49,45 @@ __device__ __forceinline__ Row row_of(const ornk_kv_pages &p, const ornk_rope_ar
     return r;
 }
 
-// What a row is divided by: sqrt(sum or mean of squares + eps).
+// What a row is divided by: sqrt(sum or mean of squares + eps).  Where that square is not a
+// 32-bit number, or so small that squares lost digits, it is formed of the row times c,
+// 2^-70 or 2^100: scaled(c) is the sum of the squares of that.
 struct Norm {
-    float s, per;  // per = 1 / s
-    bool exact;    // the quotient's remainder is a number
-    __device__ __forceinline__ Norm(const ornk_rope_args &a, float ss)
+    float s, per, c;  // per = 1 / s
+    template <class F>
+    __device__ __forceinline__ Norm(const ornk_rope_args &a, float ss, bool norm, F scaled)
     {
-        if (a.norm == 1) ss /= (float)a.hd;
-        s = sqrtf(ss + a.eps);
+        const float n = a.norm == 1 ? (float)a.hd : 1.0f;
+        float m = ss / n + a.eps;
+        c = 1.0f;
+        if (norm && !(m >= 0x1p-100f && m < INFINITY)) {
+            c = m < 1.0f ? 0x1p100f : 0x1p-70f;
+            m = scaled(c) / n + a.eps * c * c;
+        }
+        s = sqrtf(m);
         per = 1.0f / s;
-        exact = s < INFINITY && per < INFINITY;
     }
     // x / s; the product with 1 / s alone rounds once more (of 4099 tokens' heads of 128
     // 4.9e-8 of the whole instead of 4.2e-8)
-    __device__ __forceinline__ float operator()(float x) const
+    template <int N, class T>
+    __device__ __forceinline__ void divide(T &x) const
     {
-        const float q = x * per;
-        return exact ? fmaf(fmaf(-q, s, x), per, q) : q;
+        if (c == 1.0f) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float q = x[e] * per;
+                x[e] = fmaf(fmaf(-q, s, x[e]), per, q);
+            }
+            return;
+        }
+        const bool exact = s < INFINITY && per < INFINITY;  // the quotient's remainder is a number
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float y = c > 1.0f ? x[e] * c : x[e];
+            float q = y * per;
+            if (exact) q = fmaf(fmaf(-q, s, y), per, q);
+            x[e] = c < 1.0f ? q * c : q;
+        }
     }
 };
 
@@ -90,11 +112,16 @@ __global__ void __launch_bounds__(NT) k_norm_append_any(ornk_kv_pages p, ornk_ro
             float ss = 0.0f;
             if (r.norm)
                 for (int d = lane; d < hd; d += 64) ss = fmaf(r.x[d], r.x[d], ss);
-            const Norm norm(a, orn_wave_sum(ss));
+            const Norm norm(a, orn_wave_sum(ss), r.norm, [&](float c) {
+                float sum = 0.0f;
+                for (int d = lane; d < hd; d += 64) sum = fmaf(r.x[d] * c, r.x[d] * c, sum);
+                return orn_wave_sum(sum);
+            });
             auto get = [&](int d) {
-                const float x = r.x[d];
-                if (!r.norm) return x;
-                return r.w ? norm(x) * r.w[d] : norm(x);
+                float x[1] = {r.x[d]};
+                if (!r.norm) return x[0];
+                norm.template divide<1>(x);
+                return r.w ? x[0] * r.w[d] : x[0];
             };
             auto put = [&](int d, float x) {
                 if (r.out) r.out[d] = x;
@@ -162,17 +189,23 @@ __global__ void __launch_bounds__(NT, 8) k_norm_append(ornk_kv_pages p, ornk_rop
                 for (int e = 0; e < 4; ++e) ss = fmaf(y[e], y[e], fmaf(x[e], x[e], ss));
             }
             for (int o = G >> 1; o; o >>= 1) ss += __shfl_xor(ss, o, 64);
-            const Norm norm(a, ss);
+            const Norm norm(a, ss, on && r.norm, [&](float c) {
+                float sum = 0.0f;
+                for (int it = li; it < items; it += G) {
+                    if (items > G) load(it);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum = fmaf(y[e] * c, y[e] * c, fmaf(x[e] * c, x[e] * c, sum));
+                }
+                for (int o = G >> 1; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
+                return sum;
+            });
             for (int it = li; it < items; it += G) {
                 if (items > G) load(it);
                 bool two;
                 const int c = column(it, two);
                 if (r.norm) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x[e] = norm(x[e]);
-                        y[e] = norm(y[e]);
-                    }
+                    norm.template divide<4>(x);
+                    if (HALVES) norm.template divide<4>(y);
                     if (r.w) {
                         x *= *reinterpret_cast<const v4f *>(r.w + c);
                         if (two) y *= *reinterpret_cast<const v4f *>(r.w + c + R);
