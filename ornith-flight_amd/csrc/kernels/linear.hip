@@ -394,6 +394,11 @@ __device__ __forceinline__ bool begin_state(const ornk_linear_args &a, const Cut
         for (int j = 0; j < CB; ++j) S[kb][j] = v4f{0, 0, 0, 0};
     auto add = [&](const float *y, Factor keep) {  // all loads on their way at once
         float x[KB][4][CB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                load<CB, VEC>(x[kb][r], y + (size_t)min(16 * kb + 4 * g + r, a.dk - 1) * a.dv + col0, cols);
         if (__builtin_amdgcn_readfirstlane(keep.e))
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
@@ -401,11 +406,6 @@ __device__ __forceinline__ bool begin_state(const ornk_linear_args &a, const Cut
                 for (int j = 0; j < CB; ++j)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) S[kb][j][r] = ldexpf(S[kb][j][r], keep.e);
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                load<CB, VEC>(x[kb][r], y + (size_t)min(16 * kb + 4 * g + r, a.dk - 1) * a.dv + col0, cols);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
