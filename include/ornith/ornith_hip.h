@@ -240,8 +240,14 @@ int gpu_kv_evict(gpu_context *ctx, const ornith_kv_pages *kv, int n_seqs, const 
  * lost.  q k and q S of a prompt are formed before the decays, and have to be numbers of
  * 32 bits themselves.  What a token holds has no effect on those before it, NaN and
  * infinities included, but for their last digits: a stretch with a result that is not
- * finite, or with large numbers that decay far, is done with other instructions.  A slot outside [-1, n_slots), or tokens outside
- * [0, n_tokens) or more than max_len, leave their sequence out (gpu_kv_check). */
+ * finite, or with large numbers that decay far, is done with other instructions.  A slot
+ * outside [-1, n_slots), or tokens outside [0, n_tokens) or more than max_len, leave their
+ * sequence out (gpu_kv_check).
+ *
+ * Single tokens and prompts are best taken in a call each: where one sequence of a call
+ * has more than one token all go by chunks, and how prompts are cut between work groups
+ * goes by max_len for all (8191 tokens beside 63 single ones, 32 heads of 128: 1.46 ms in
+ * one call, 0.29 in two). */
 typedef struct {
     gpu_buffer *S; /* [n_slots][n_heads][key_dim][value_dim] fp32; NULL without slots */
     int n_slots;

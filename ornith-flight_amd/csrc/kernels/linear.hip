@@ -167,9 +167,9 @@ void launch_step(const ornk_linear_args &a, hipStream_t s)
 //   o_i = scale (2^G_i q_i S + sum_(j <= i) 2^(G_i - G_j) b_j P_ij v_j)
 //   S  <- 2^G_C S + sum_j 2^(G_C - G_j) b_j k_j v_j^T
 // Exponents are differences of tokens in order, so no factor overflows before the
-// formula does.  A group of 4 waves takes 64 CB columns of a head's V, a wave 16 CB of
-// them: lane 16 g + c has columns CB c + j, and rows 4 g + r of a block of 16 in its
-// registers [r][j].  So S's accumulators are the second operand of q S as they are, P's
+// formula's own factors together do.  A group of 4 waves takes 64 CB columns of a head's
+// V, a wave 16 CB of them: lane 16 g + c has columns CB c + j, and rows 4 g + r of a block
+// of 16 in its registers [r][j].  So S's accumulators are the second operand of q S as they are, P's
 // (formed as K Q^T) the first of P V, and V never leaves its registers.  K and Q are in
 // LDS.  P has three blocks of 16 x 16 (keys and queries of the first half, first and
 // second, of the second), one for each of three waves; the fourth sums the next chunk's
@@ -177,10 +177,10 @@ void launch_step(const ornk_linear_args &a, hipStream_t s)
 //
 // With fp32 operands it was bound by the matrix cores, which take 15 ns for a 16x16x4
 // product of a SIMD (140 TFLOP/s): 24 x up to 1501 tokens, 32 heads of 128 (18,210 tokens in
-// all) 431 us.  With three bf16 parts (8 ns for 16x16x32, six products) it takes 342: 1.27 GB
-// are moved at 3.7 TB/s, and each wave's 232 matrix instructions and 1150 others of a chunk
-// wait for three barriers, with one other group on the CU.  C = 32 costs 19 % more than the
-// recurrence (P, P V).  Later loads of V, addresses of whole chunks kept apart, K and Q
+// all) 431 us.  With three bf16 parts (8 ns for 16x16x32, six products) it takes 346 to 360, by
+// the run: 1.28 GB are moved at 3.7 TB/s, and each wave's 232 matrix instructions and 1170 others
+// of a chunk wait for three barriers, with one other group on the CU.  C = 32 costs 19 % more
+// than the recurrence (P, P V).  Later loads of V, addresses of whole chunks kept apart, K and Q
 // staged before S's products, and heads that share K and Q on one XCD made no difference.
 constexpr int C = 32;
 
@@ -189,8 +189,9 @@ constexpr int C = 32;
 // one of its numbers passes 2^16 (if none does, what is lost is below 2^-94 of each token), its
 // part is done again in chunks that end before they are far: within those no factor is small
 // but the first token's, which the state alone takes, as a mantissa and an exponent.  Looking
-// for large numbers takes 1 to 3 % (4 x 2000, 8 heads of 256 x 256 287 -> 301 us), chunks cut so
-// from the start twice as long where decays are strong (548).
+// for large numbers takes 1 to 5 % (8191 tokens, 16 heads of 128 142 -> 143 us, 4 x 2000, 8 of
+// 256 x 256 288 -> 301), chunks cut so from the start nearly twice as long where decays are
+// strong (548).
 constexpr double FAR = -64.0;
 constexpr float LARGE = 65536.0f;
 
@@ -831,7 +832,7 @@ typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 // Part Z of two numbers, of which the parts before it are taken off, and what it leaves,
 // exactly.  The second is rounded to nearest, so that what the products leave out has either
 // sign; the others are the leading 8 bits (an instruction that issues in half the time: all
-// three rounded 353 us where this takes 342).
+// three rounded take 3 % longer).
 template <int Z>
 __device__ __forceinline__ uint32_t take(float &x, float &y)
 {
@@ -1206,7 +1207,7 @@ __global__ void __launch_bounds__(256, 2) k_linear_chunks(ornk_linear_args a, Cu
 }
 
 // From what each part adds to what each part begins with, an element per thread (16 heads
-// of 128 x 128 in 32 parts 15 us, 67 MB).
+// of 128 x 128 in 32 parts 16 us, 67 MB).
 __global__ void __launch_bounds__(256) k_linear_join(ornk_linear_args a, Cut cut)
 {
     const int b = blockIdx.x, h = blockIdx.y, e = blockIdx.z * 256 + threadIdx.x;
@@ -1226,16 +1227,16 @@ __global__ void __launch_bounds__(256) k_linear_join(ornk_linear_args a, Cut cut
 }
 
 // Parts of a sequence that join those before them by themselves, which saves a launch (5 x
-// 333, 12 heads of 96 x 80: 40 -> 37 us); with 8 of them it takes longer (1 x 512, 32 heads of
-// 128: 48 us, by a launch 38).
+// 333, 12 heads of 96 x 80: 42 -> 39 us); with 8 of them it takes longer (1 x 512, 32 heads of
+// 128: 51 us, by a launch 42).
 constexpr int JOIN = 4;
 
 // Sequences are cut where their heads and columns leave CUs idle: into parts of at
 // least 64 tokens, until there are two groups for each CU.  What the parts add to a state
 // is formed first, and their tokens after that from what they begin with, which takes 1.4
-// times the products.  One prompt of 8191 tokens, 16 heads of 128: 140 us (sums 40, joining
-// 15, tokens 92); with one group for each CU 153.  5 x 333, 12 heads of 96 x 80: 37; with
-// parts of 128 tokens 47.
+// times the products.  One prompt of 8191 tokens, 16 heads of 128: 143 us (alone, under a
+// profiler, sums 41, joining 16, tokens 93); with one group for each CU 159.  5 x 333, 12
+// heads of 96 x 80: 39; with parts of 128 tokens 50.
 Cut cut_of(const ornk_linear_args &a, int cb)
 {
     const long long groups = (long long)a.n_seqs * a.heads * ((a.dv + 64 * cb - 1) / (64 * cb));
@@ -1251,8 +1252,8 @@ Cut cut_of(const ornk_linear_args &a, int cb)
 
 // Blocks of 16 columns of a wave: two, where there is then a group for each CU, and the
 // state's registers leave room for another group.  Two share a group's P and its waits (one
-// prompt of 8191 tokens, 16 heads of 128: 140 us, with one block 150); one gives twice the
-// groups (1 x 512, 16 heads of 128: 26, with two 36).
+// prompt of 8191 tokens, 16 heads of 128: 143 us, with one block 158); one gives twice the
+// groups (1 x 512, 16 heads of 128: 29, with two 33).
 int blocks_of(const ornk_linear_args &a)
 {
     if (a.dv <= 64 || a.dk > 128) return 1;

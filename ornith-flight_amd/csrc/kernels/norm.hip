@@ -93,7 +93,8 @@ struct Norm {
 
 // Rows that are no whole float4s (or halves of pairs that are not four): a wave per
 // row, an element or a pair per lane, which reads the row a second time after its sum.  The
-// token's angles are formed once, in LDS.
+// token's angles are formed once, in LDS.  Bound by its loads of one element per lane, twice:
+// 4099 tokens of 32 + 8 heads of 66 65 us (87 MB, 17 at the copy's rate).
 template <int TYPE>
 __global__ void __launch_bounds__(NT) k_norm_append_any(ornk_kv_pages p, ornk_rope_args a, int rows)
 {
@@ -146,8 +147,8 @@ __global__ void __launch_bounds__(NT) k_norm_append_any(ornk_kv_pages p, ornk_ro
 // A row by 2^g lanes, an item of it per lane: a float4, with HALVES two of one pair's
 // four (R apart).  A row of more than 64 items is read a second time after its sum.
 // Bound by memory: 8190 tokens of 32 + 8 heads of 128 with the append to f16 move 369 MB in
-// 76 us (4.9 TB/s; a copy 5.1), 4099 of 16 + 16 heads without rotation 134 MB in 32 us.  One
-// token of 16 + 2 heads takes 7.2 us, the launch and the caller's side (kernel 4.9).
+// 75 us (4.9 TB/s; a copy 5.1), 4099 of 16 + 16 heads without rotation 134 MB in 32 us.  One
+// token of 16 + 2 heads takes 7.0 us, the launch and the caller's side (kernel 4.9).
 template <int TYPE, bool HALVES>
 __global__ void __launch_bounds__(NT, 8) k_norm_append(ornk_kv_pages p, ornk_rope_args a, int rows, int g)
 {

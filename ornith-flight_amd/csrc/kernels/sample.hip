@@ -6,8 +6,8 @@
 // fall into bins of equal stretches; a bin's weights are summed as whole numbers, in which
 // the order of the additions does not show.  The bins tell each border of the choice
 // (top_k, top_p, min_p, the random number's) up to one or a few of them; only the tokens
-// there are listed, and the borders found among them.  Rows of which the top_k are asked
-// need no bins: the k-th largest of the largest logits of many parts of a row is a bound
+// there are listed, and the borders found among them.  Rows of which a small top_k is
+// asked need no bins: the k-th largest of the largest logits of many parts of a row is a bound
 // that k tokens reach and few more.
 #include "../../../include/ornith/ornith_hip.h"
 #include "common.h"
@@ -1135,7 +1135,7 @@ Slices slices_of(const ornk_sample_args &a)
     const long long want = ((long long)a.rows * a.n / 1536 + UNIT - 1) / UNIT;
     const long long least = ((long long)a.n + UNIT * MAX_SLICES - 1) / (UNIT * MAX_SLICES);
     long long k = want < 4096 / UNIT ? 4096 / UNIT : want > 32768 / UNIT ? 32768 / UNIT : want;
-    if (k > a.n / (8 * UNIT)) k = a.n / (8 * UNIT);  // 8 slices: parts for a top_k of CAP
+    if (k > a.n / (8 * UNIT)) k = a.n / (8 * UNIT);  // 8 slices at least: parts whose bound a top_k of 1600 has
     if (k < least) k = least;
     Slices s = {};
     s.len = (int)k * UNIT;
