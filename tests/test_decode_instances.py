@@ -115,7 +115,7 @@ def test_the_launches_fit(launches):
 def test_the_slices_of_rows(launches):
     """Their number, for slices of 4096 tokens and of more."""
     cases = {(4, 1 << 20): 4096, (4, (1 << 20) - 1): 4096, (4, 524289): 4096, (70, 200000): 10240, (64, 150001): 8192,
-             (64, 248320): 12288, (256, 248320): 30720, (2, 32769): 4096}
+             (64, 248320): 12288, (128, 248320): 22528, (2, 32769): 4096}
     for ((_, n), length), call in zip(cases.items(), launches([("s", *c, 0, 0, 0) for c in cases])):
         assert call[0][1] == -(-n // length)
 
